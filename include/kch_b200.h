@@ -54,6 +54,8 @@ long long kch_launch_count(int reset);      /* kernels launched by this library 
 #define KCH_STATUS_KDA_STEP 0x6D03       /* status word: the state copy of the one-token KDA step did not arrive */
 #define KCH_STATUS_KDA_CHUNK 0x6D04      /* status word: a chunk record of the fp32 KDA scan did not arrive */
 #define KCH_STATUS_ATTEND_TILES 0x6D05   /* status word: a wait of the attention over key tiles (operands / accumulator) expired */
+#define KCH_STATUS_PAGED_TABLE 0x6D06    /* status word: a block table named no page of the pool, or ended before its sequence did */
+#define KCH_STATUS_PAGED_ATTEND 0x6D07   /* status word: a wait of the attention over pages (operands / accumulator) expired */
 #define KCH_STATUS_INDEXER_DECODE 0x6D02 /* status word: a wait of the one-token indexer (key tiles / accumulator) expired */
 int kch_selftest_bounded_wait(unsigned int limit_polls, unsigned int* polls_out, void* stream);
 
@@ -408,6 +410,68 @@ int kch_cache_store_rows(const float* rows, int64_t n, int c, int B, void* dst, 
  * payload [rows,c], scales [rows,c/64], norms [rows] = max(||dequantised row||, 1e-12). */
 int kch_quantize_rows(const void* x, int64_t ld, void* payload, float* scales, float* norms, int64_t rows,
                       int c, int kind, int dtype, void* stream);
+
+/* ---- paged key / value cache ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose caches hold one batch in lock step.  Keys and values of many sequences in a pool of
+ * pages: k, v [num_pages, n_kv, page_size, c], 16-byte aligned, in the activations' type (`kind` = KCH_F32 / KCH_BF16) or in
+ * 8 bits (KCH_FP8_E4M3, KCH_INT8) with one fp32 scale a row, [num_pages, n_kv, page_size].  c: a multiple of 8 up to 256;
+ * page_size: a power of two from 8 to 256. */
+typedef struct kch_paged_cache {
+  void *k, *v;
+  float *k_scales, *v_scales;  /* 8-bit kinds only */
+  int kind;
+  int64_t num_pages;
+  int page_size, n_kv, c;
+} kch_paged_cache;
+
+/* A ragged batch: rows cu_seqlens[b] .. cu_seqlens[b + 1] of the packed tensors [N, ..] are the positions t0[b], t0[b] + 1, .. of
+ * sequence b, and position p of it lies in page table[b, p / page_size] of the pool, row p % page_size.  All lengths are read on
+ * the device: a captured call replays with other ones.  Entries of the table behind a sequence's last page are not read.  An
+ * entry that is needed and names no page of the pool, or a position behind the table, raises KCH_STATUS_PAGED_TABLE; nothing is
+ * stored for it, and it reads as zeros.  cu_seqlens does not decrease and stays within 0 .. N; rows outside
+ * [cu_seqlens[0], cu_seqlens[B]) belong to no sequence.  Up to 4096 sequences. */
+typedef struct kch_paged_batch {
+  const int32_t* table;      /* [B, max_pages] rows ld_table apart */
+  int64_t ld_table;
+  int max_pages;
+  const int32_t* t0;         /* [B] */
+  const int32_t* cu_seqlens; /* [B + 1] */
+  int B;
+  int64_t N;
+} kch_paged_batch;
+
+/* Writes the packed rows k, v [N, n_kv, c] (tokens ld_k / ld_v elements apart) into their pages.  8-bit kinds: s = max |x| / 448
+ * (e4m3) or / 127 (int8) over the row of a key head, 1 for a row of zeros; stored round(x / s), ties to even.  A row that is not
+ * finite reads back as NaN.  A position that occurs twice in a batch holds either row. */
+int kch_paged_append(const kch_paged_cache* cache, const kch_paged_batch* batch, const void* k, int64_t ld_k, const void* v,
+                     int64_t ld_v, int dtype, void* stream);
+/* Reads the rows of those positions back as packed rows in `dtype`: stored value times scale, rounded once.  Rows of no sequence:
+ * zeros with `zero_rest`, else left as they are. */
+int kch_paged_read(const kch_paged_cache* cache, const kch_paged_batch* batch, void* k, int64_t ld_k, void* v, int64_t ld_v, int dtype,
+                   int zero_rest, void* stream);
+
+/* Attention of the new tokens over the pages, which hold them already: query i of sequence b stands at position t0[b] + i and
+ * sees the keys up to it, the last `sliding_window` of them where that is not 0; query head h reads key head h / (nh / n_kv).
+ * The sink logit of a head (optional) adds to the denominator.  q [N, nh, c] (tokens ld_q elements apart) and out [N, nh, c] in
+ * `dtype`, which is that of the cache's activations.  Rows of no sequence: zeros with `zero_rest`, else left as they are. */
+typedef struct kch_paged_attend_args {
+  kch_paged_cache cache;
+  kch_paged_batch batch;
+  const void* q;
+  int64_t ld_q;
+  int dtype, nh;
+  float scale;
+  int sliding_window;
+  const void* sink;          /* [nh] or NULL */
+  int sink_dtype;
+  void* out;
+  int zero_rest;
+  void* workspace;           /* 256-byte aligned */
+  int64_t workspace_bytes;
+} kch_paged_attend_args;
+int64_t kch_paged_attend_workspace_bytes(const kch_paged_attend_args* args);
+int kch_paged_attend(const kch_paged_attend_args* args, void* stream);
 
 /* ---- whole layers ------------------------------------------------------------------------------------------- */
 

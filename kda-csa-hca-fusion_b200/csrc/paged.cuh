@@ -1,0 +1,239 @@
+// What the kernels of the paged key / value cache share: where a token of a ragged batch lies, and how the attention over the
+// pages is divided over the CTAs.
+//
+// Division.  An item is a block of at most R rows (consecutive (token, head of the group) pairs of one sequence, so that the
+// heads which share a key head also share its tiles) against the key tiles that any of them sees.  The steps of all items
+// form one line: sequence, key head, row block, step.  CTA i of C takes the steps [i, i + 1) * ceil(U / C), whatever items
+// they belong to: a single long sequence is split along its keys, a batch of many short ones gives several items to a CTA, a
+// causal chunk is balanced to one step, and the host needs no length (they stay on the device, so a captured graph replays
+// with other ones).  An item that one CTA has whole is stored by it; the parts of the others go to the workspace (at most two
+// a CTA: the item that its range ends in, and the one that it starts in the middle of) and are joined by a second kernel, in
+// the order of the CTAs, so that the result does not depend on when they ran.
+#pragma once
+#include "kch_common.cuh"
+
+#define PG_MAX_B 4096                  // sequences of a call: their table of steps is kept in shared memory
+#define PG_LOG2E 1.4426950408889634f
+
+unsigned int* kch_status_device_ptr();
+
+struct PgBatch {
+  const int32_t* table; int64_t ld_table;
+  const int32_t *t0, *cu;
+  int B; int64_t N;                    // sequences; rows of the packed tensors
+  int64_t cap;                         // positions that a row of the table covers
+  int64_t num_pages;
+  int shift;                           // log2(page_size)
+  unsigned int* status;
+};
+
+struct PgSeq { int64_t row0; int len; int64_t t0, kv; };      // first packed row, new tokens, tokens before them, keys in all
+
+// (Whatever cu_seqlens and t0 hold, rows stay inside the packed tensors and keys inside the table.)
+__device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
+  PgSeq s;
+  const int64_t lo = min(max((int64_t)__ldg(a.cu + b), (int64_t)0), a.N), hi = min(max((int64_t)__ldg(a.cu + b + 1), lo), a.N);
+  s.row0 = lo;
+  s.len = (int)(hi - lo);
+  s.t0 = max((int64_t)__ldg(a.t0 + b), (int64_t)0);
+  s.kv = min(s.t0 + s.len, a.cap);
+  return s;
+}
+__device__ __forceinline__ void pg_bad(const PgBatch& a) { atomicCAS(a.status, 0u, (unsigned)KCH_STATUS_PAGED_TABLE); }
+// page of `index` pages into sequence b, or -1 (and the status word) where the table holds none
+__device__ __forceinline__ int64_t pg_page(const PgBatch& a, int b, int64_t index) {
+  const int64_t p = __ldg(a.table + b * a.ld_table + index);
+  if (p >= 0 && p < a.num_pages) return p;
+  pg_bad(a);
+  return -1;
+}
+
+// One block of rows of a sequence: which keys its rows see together.
+struct PgSpan { int rows; int64_t first_key; int tiles, steps; };   // tiles of KT keys from first_key (a multiple of KT) on
+// R rows a block, KT keys a tile; HALF: a block of at most R / 2 rows takes two tiles a step
+template <int R, int KT, bool HALF>
+__device__ __forceinline__ PgSpan pg_span(const PgSeq& s, int G, int window, int block) {
+  PgSpan x;
+  const int64_t r0 = (int64_t)block * R, all = (int64_t)s.len * G, r1 = min(r0 + R, all);
+  x.rows = (int)(r1 - r0);
+  const int64_t first = s.t0 + r0 / G, last = s.t0 + (r1 - 1) / G;          // positions of the first and the last query
+  const int64_t lo = window > 0 ? max(first - window + 1, (int64_t)0) : 0, hi = min(last + 1, s.kv);
+  x.first_key = lo / KT * KT;
+  x.tiles = hi > x.first_key ? (int)((hi - x.first_key + KT - 1) / KT) : 0;
+  x.steps = max(HALF && x.rows <= R / 2 ? (x.tiles + 1) / 2 : x.tiles, 1);  // (a row without keys is stored all the same)
+  return x;
+}
+template <int R>
+__device__ __forceinline__ int pg_blocks(const PgSeq& s, int G) { return (int)(((int64_t)s.len * G + R - 1) / R); }
+
+struct PgPlace {                       // where a CTA's range of steps begins
+  int64_t per, left;                   // steps of a CTA; steps of this one
+  int b, h, block, step;
+};
+
+// The whole block calls it; `mem`: PG_PLAN_BYTES(B) of shared memory, free again after the next __syncthreads().
+#define PG_PLAN_BYTES(B) (16 + 8 * ((B) + 1))
+template <int R, int KT, bool HALF>
+__device__ PgPlace pg_plan(const PgBatch& a, int G, int n_kv, int window, void* mem, int cta, int ctas) {
+  int64_t* base = reinterpret_cast<int64_t*>(mem);          // [B + 1] steps before sequence b
+  int* found = reinterpret_cast<int*>(base + a.B + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  // steps of a sequence: a lane each where it is one block (a batch of single tokens), else a warp over its blocks
+  for (int b0 = warp * 32; b0 < a.B; b0 += warps * 32) {
+    const int b = b0 + lane;
+    PgSeq s = {0, 0, 0, 0};
+    if (b < a.B) s = pg_seq(a, b);
+    const int blocks = pg_blocks<R>(s, G);
+    int64_t mine = blocks == 1 ? pg_span<R, KT, HALF>(s, G, window, 0).steps : 0;
+    unsigned many = __ballot_sync(0xffffffffu, blocks > 1);
+    while (many) {
+      const int from = __ffs(many) - 1;
+      many &= many - 1;
+      PgSeq t;
+      t.row0 = 0;
+      t.len = __shfl_sync(0xffffffffu, s.len, from);
+      t.t0 = __shfl_sync(0xffffffffu, s.t0, from);
+      t.kv = __shfl_sync(0xffffffffu, s.kv, from);
+      const int nb = __shfl_sync(0xffffffffu, blocks, from);
+      int64_t sum = 0;
+      for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, HALF>(t, G, window, i).steps;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == from) mine = sum;
+    }
+    if (b < a.B) base[b + 1] = mine * n_kv;
+    if (b < a.B && s.t0 + s.len > a.cap) pg_bad(a);
+  }
+  if (tid == 0) { base[0] = 0; found[0] = -1; }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      int64_t x = b < a.B ? base[b + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (b < a.B) base[b + 1] = run + x;
+      run += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  PgPlace p = {};
+  const int64_t total = base[a.B];
+  p.per = max((total + ctas - 1) / ctas, (int64_t)1);
+  const int64_t start = p.per * cta;
+  p.left = max(min(p.per, total - start), (int64_t)0);
+  if (p.left > 0)
+    for (int b = tid; b < a.B; b += blockDim.x)
+      if (base[b] <= start && start < base[b + 1]) found[0] = b;
+  __syncthreads();
+  if (p.left > 0) {                    // every warp finds the block by itself
+    p.b = found[0];
+    const PgSeq s = pg_seq(a, p.b);
+    const int blocks = pg_blocks<R>(s, G);
+    const int64_t head = (base[p.b + 1] - base[p.b]) / n_kv;
+    p.h = (int)((start - base[p.b]) / head);
+    int64_t rest = start - base[p.b] - p.h * head;
+    for (int i0 = 0; i0 < blocks; i0 += 32) {
+      const int i = i0 + lane;
+      const int64_t n = i < blocks ? pg_span<R, KT, HALF>(s, G, window, i).steps : 0;
+      int64_t x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
+      if (hit) {
+        const int at = __ffs(hit) - 1;
+        p.block = i0 + at;
+        p.step = (int)(rest - __shfl_sync(0xffffffffu, x - n, at));
+        break;
+      }
+      rest -= __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  return p;
+}
+
+// The items of a CTA, one after the other; every role of a kernel walks them by itself.
+template <int R, int KT, bool HALF>
+struct PgWalk {
+  const PgBatch& a;
+  int G, n_kv, window;
+  int b, h, block;                     // the item
+  int first, count;                    // its steps that belong to this CTA
+  PgSeq s;
+  PgSpan x;
+  int64_t left;                        // steps of the CTA behind them
+  __device__ __forceinline__ PgWalk(const PgBatch& a_, int G_, int n_kv_, int window_, const PgPlace& p)
+      : a(a_), G(G_), n_kv(n_kv_), window(window_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), left(p.left) {
+    if (left > 0) {
+      s = pg_seq(a, b);
+      open();
+    }
+  }
+  __device__ __forceinline__ bool valid() const { return count > 0; }
+  __device__ __forceinline__ bool starts() const { return first == 0; }
+  __device__ __forceinline__ bool ends() const { return first + count == x.steps; }
+  __device__ __forceinline__ void next() {
+    first = 0;
+    count = 0;
+    if (left <= 0) return;
+    if (++block == pg_blocks<R>(s, G)) {
+      block = 0;
+      if (++h == n_kv) {
+        h = 0;
+        do { s = pg_seq(a, ++b); } while (s.len == 0);       // (steps are left, so a sequence with rows follows)
+      }
+    }
+    open();
+  }
+
+ private:
+  __device__ __forceinline__ void open() {
+    x = pg_span<R, KT, HALF>(s, G, window, block);
+    count = (int)min((int64_t)(x.steps - first), left);
+    left -= count;
+  }
+};
+
+// Parts of items in the workspace: one record a CTA (the item that starts in its range and ends in another's), then two slots
+// a CTA of R rows: c sums, the row's maximum (base 2) and its sum.
+struct PgRecord { int valid, b, h, block, last, rows; int64_t row0; };       // last: the CTA that has the item's end
+__host__ __device__ __forceinline__ int64_t pg_slot_floats(int R, int c) { return (int64_t)R * (c + 2); }
+__host__ __device__ __forceinline__ int64_t pg_records_bytes(int ctas) { return ((int64_t)ctas * (int64_t)sizeof(PgRecord) + 255) / 256 * 256; }
+static inline int64_t pg_workspace_bytes(int ctas, int R, int c) { return pg_records_bytes(ctas) + 2 * ctas * pg_slot_floats(R, c) * 4; }
+
+struct PgJoinArgs {
+  void* out; int dtype;                // [N, nh, c]
+  int nh, G, c, R;
+  const void* sink; int sink_dtype;
+  const PgRecord* records; const float* slots;
+};
+int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s);
+
+struct PgAttend {                      // what both attention kernels get
+  PgBatch bt;
+  const void *q, *k, *v; const float *ks, *vs;
+  void* out;
+  int64_t ld_q;
+  int n_kv, G, c, page, window, zero_rest;
+  float scale;                         // times log2(e)
+  const void* sink; int sink_dtype;
+  PgRecord* records; float* slots;
+};
+
+// rows behind the last sequence (and before the first), where the caller wants zeros there
+__device__ __forceinline__ void pg_zero_rest(const PgAttend& a, int es, int cta, int ctas) {
+  if (!a.zero_rest) return;
+  const int64_t lo = min(max((int64_t)__ldg(a.bt.cu), (int64_t)0), a.bt.N), hi = min(max((int64_t)__ldg(a.bt.cu + a.bt.B), lo), a.bt.N);
+  const int64_t row = (int64_t)a.n_kv * a.G * a.c * es / 16, words = (lo + a.bt.N - hi) * row;      // 16-byte words of a token
+  for (int64_t i = (int64_t)cta * blockDim.x + threadIdx.x; i < words; i += (int64_t)ctas * blockDim.x) {
+    const int64_t t = i / row, at = (t < lo ? t : hi + t - lo) * row + i % row;
+    reinterpret_cast<uint4*>(a.out)[at] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}

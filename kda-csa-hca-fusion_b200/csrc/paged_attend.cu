@@ -1,0 +1,354 @@
+// Attention of new tokens over a paged cache on CUDA cores, the kernel that joins parts of items, and the entry point.
+//
+//   l_j = scale * <q, k_j>,  o = sum_j 2^(l_j log2 e - m) v_j / (sum_j 2^(l_j log2 e - m) + 2^(sink log2 e - m)),  keys j of the
+//   sequence with pos(q) - window < j <= pos(q);  a row without keys is 0.
+//
+// fp32 (whose products the tensor cores would round) and head widths that the tcgen05 kernel does not have.  An item's ROWS x KT
+// scores are a register tile of 4 (1) x 4 a thread over rows and keys staged in shared memory in fp32 (stored values times their
+// scale), the softmax keeps a running maximum and sum a row, and the sums stay in registers, a row's columns over 16 threads.
+#include <math.h>
+
+#include "paged.cuh"
+
+template <typename P> struct PgStored;            // 8 stored values as floats
+template <> struct PgStored<float> {
+  static constexpr int ES = 4;
+  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>((const float*)p + i)), b = __ldg(reinterpret_cast<const float4*>((const float*)p + i) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+template <> struct PgStored<bf16> {
+  static constexpr int ES = 2;
+  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>((const bf16*)p + i));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u); }
+  }
+};
+template <> struct PgStored<__nv_fp8_e4m3> {
+  static constexpr int ES = 1;
+  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>((const uint8_t*)p + i));
+    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __nv_fp8_e4m3 v;
+      v.__x = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+      x[e] = float(v);
+    }
+  }
+};
+template <> struct PgStored<int8_t> {
+  static constexpr int ES = 1;
+  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>((const uint8_t*)p + i));
+    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3)));
+  }
+};
+
+#define PA_KT 64
+#define PA_THREADS 256
+
+static int pa_smem(int ROWS, int DMAX, int B) {
+  const int need = (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4, plan = PG_PLAN_BYTES(B);
+  return need > plan ? need : plan;
+}
+
+// T: activations; P: stored values; DMAX: widths up to this (columns behind the width are 0)
+template <typename T, typename P, int ROWS, int DMAX>
+__global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend a) {
+  constexpr int LD = DMAX + 4, LS = PA_KT + 4, RT = ROWS / 16, CT = DMAX / 64;
+  extern __shared__ float4 pa_mem[];
+  float* sq = reinterpret_cast<float*>(pa_mem);
+  float *sk = sq + ROWS * LD, *sv = sk + PA_KT * LD, *sp = sv + PA_KT * LD, *sm = sp + ROWS * LS, *sl = sm + ROWS, *sa = sl + ROWS;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, c = a.c, c8 = c >> 3;
+  const PgPlace place = pg_plan<ROWS, PA_KT, false>(a.bt, a.G, a.n_kv, a.window, pa_mem, blockIdx.x, gridDim.x);
+  pg_zero_rest(a, sizeof(T), blockIdx.x, gridDim.x);
+  __syncthreads();
+  for (int i = tid; i < (ROWS + 2 * PA_KT) * LD; i += PA_THREADS) sq[i] = 0.f;      // columns c .. DMAX of all three stay 0
+  PgRecord rec = {};
+  PgWalk<ROWS, PA_KT, false> w(a.bt, a.G, a.n_kv, a.window, place);
+  for (; w.valid(); w.next()) {
+    const int64_t r0 = (int64_t)w.block * ROWS;                // first (token, head) row of the block in its sequence
+    __syncthreads();
+    for (int i = tid; i < ROWS * c8; i += PA_THREADS) {
+      const int r = i / c8, d = i % c8 * 8;
+      float x[8] = {};
+      if (r < w.x.rows) {
+        const int64_t t = (r0 + r) / a.G;
+        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * a.G + (int)((r0 + r) % a.G)) * c + d, x);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq[r * LD + d + e] = x[e];
+    }
+    for (int r = tid; r < ROWS; r += PA_THREADS) { sm[r] = -INFINITY; sl[r] = 0.f; }
+    float o[RT][CT][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    for (int st = w.first; st < w.first + w.count; ++st) {
+      const int64_t key0 = w.x.first_key + (int64_t)st * PA_KT;
+      __syncthreads();
+      for (int i = tid; i < PA_KT * c8; i += PA_THREADS) {     // keys and values of the tile, 0 behind the sequence's end
+        const int j = i / c8, d = i % c8 * 8;
+        const int64_t pos = key0 + j;
+        float kx[8] = {}, vx[8] = {};
+        if (pos < w.s.kv) {
+          const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
+          if (pg >= 0) {
+            const int64_t row = (pg * a.n_kv + w.h) * a.page + (pos & (a.page - 1));
+            PgStored<P>::load(a.k, row * c + d, kx);
+            PgStored<P>::load(a.v, row * c + d, vx);
+            if (PgStored<P>::ES == 1) {
+              const float fk = __ldg(a.ks + row), fv = __ldg(a.vs + row);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) { kx[e] *= fk; vx[e] *= fv; }
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { sk[j * LD + d + e] = kx[e]; sv[j * LD + d + e] = vx[e]; }
+      }
+      __syncthreads();
+      float acc[RT][4];                                        // rows ty + 16 i, keys tx + 16 j
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+      for (int d = 0; d < c; d += 4) {
+        float4 kk[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * LD + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float4 qq = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * LD + d);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            acc[i][j] = fmaf(qq.x, kk[j].x, acc[i][j]);
+            acc[i][j] = fmaf(qq.y, kk[j].y, acc[i][j]);
+            acc[i][j] = fmaf(qq.z, kk[j].z, acc[i][j]);
+            acc[i][j] = fmaf(qq.w, kk[j].w, acc[i][j]);
+          }
+        }
+      }
+      // the 16 threads of a row keep its maximum and sum together
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = ty + 16 * i;
+        const int64_t pos = w.s.t0 + (r0 + r) / a.G, from = a.window > 0 ? pos - a.window + 1 : 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t key = key0 + tx + 16 * j;
+          const bool sees = r < w.x.rows && key >= from && key <= pos && key < w.s.kv;
+          acc[i][j] = sees ? acc[i][j] * a.scale : -INFINITY;
+          top = fmaxf(top, acc[i][j]);
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float was = sm[r], now = fmaxf(was, top), shift = now == -INFINITY ? 0.f : now;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = exp2f(acc[i][j] - shift);
+          sp[r * LS + tx + 16 * j] = p;
+          sum += p;
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        __syncwarp();
+        if (tx == 0) {
+          const float keep = exp2f(was - shift);               // (0 where nothing was)
+          sa[r] = keep;
+          sl[r] = sl[r] * keep + sum;
+          sm[r] = now;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const float keep = sa[ty + 16 * i];
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][j][e] *= keep;
+      }
+      // A key that a row does not see must not reach it: 0 times an infinity or a NaN is no 0.  In a tile where every row
+      // sees every key nothing is to be skipped.
+      const int64_t low = w.s.t0 + r0 / a.G, high = w.s.t0 + (r0 + w.x.rows - 1) / a.G;
+      const bool whole = key0 + PA_KT - 1 <= low && (a.window == 0 || key0 > high - a.window) && key0 + PA_KT <= w.s.kv;
+      auto product = [&](auto masked) {
+        for (int j = 0; j < PA_KT; ++j) {
+          float p[RT];
+#pragma unroll
+          for (int i = 0; i < RT; ++i) p[i] = sp[(ty + 16 * i) * LS + j];
+#pragma unroll
+          for (int x = 0; x < CT; ++x) {
+            const float4 vv = *reinterpret_cast<const float4*>(sv + j * LD + tx * 4 + 64 * x);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              if (masked() && p[i] == 0.f) continue;
+              o[i][x][0] = fmaf(p[i], vv.x, o[i][x][0]);
+              o[i][x][1] = fmaf(p[i], vv.y, o[i][x][1]);
+              o[i][x][2] = fmaf(p[i], vv.z, o[i][x][2]);
+              o[i][x][3] = fmaf(p[i], vv.w, o[i][x][3]);
+            }
+          }
+        }
+      };
+      if (whole) product([] { return false; });
+      else product([] { return true; });
+    }
+    // ---- the item's end: its rows, or its part of them ---------------------------------------------------------------------
+    const bool direct = w.starts() && w.ends();
+    float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(ROWS, c);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty + 16 * i;
+      if (r >= w.x.rows) continue;
+      const int64_t t = (r0 + r) / a.G;
+      const int h = w.h * a.G + (int)((r0 + r) % a.G);
+      float f = 1.f;
+      if (direct) {
+        const float m = sm[r], l = sl[r];
+        float below = l;
+        if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - m);
+        f = l == 0.f ? 0.f : 1.f / below;
+      }
+      T* orow = (T*)a.out + ((w.s.row0 + t) * (int64_t)(a.n_kv * a.G) + h) * c;
+#pragma unroll
+      for (int x = 0; x < CT; ++x) {
+        const int d = tx * 4 + 64 * x;
+        if (d >= c) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (direct) stf(orow + d + e, o[i][x][e] * f);
+          else slot[(int64_t)r * c + d + e] = o[i][x][e];
+        }
+      }
+      if (!direct && tx == 0) {
+        slot[(int64_t)ROWS * c + r] = sm[r];
+        slot[(int64_t)ROWS * c + ROWS + r] = sl[r];
+      }
+    }
+    if (w.starts() && !w.ends()) {
+      rec.valid = 1; rec.b = w.b; rec.h = w.h; rec.block = w.block; rec.rows = w.x.rows; rec.row0 = w.s.row0;
+      rec.last = (int)((place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per);   // (it is the last of the range)
+    }
+  }
+  if (tid == 0) a.records[blockIdx.x] = rec;
+}
+
+// ---- joining ----------------------------------------------------------------------------------------------------------------
+// Block (i, y): the item that starts in CTA i's range and ends in another's, rows y * 8 .. ; a warp a row, its lanes over the
+// columns.  Launched to start while the kernel before it drains.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_join_kernel(PgJoinArgs a) {
+  chain_wait();
+  const PgRecord* rp = a.records + blockIdx.x;
+  if (!rp->valid) return;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, rows = rp->rows;
+  if (r >= rows) return;
+  const int first = blockIdx.x, last = rp->last;
+  const int64_t size = pg_slot_floats(a.R, a.c), row = (int64_t)rp->block * a.R + r, t = row / a.G;
+  const int h = rp->h * a.G + (int)(row % a.G);
+  auto slot = [&](int i) { return a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size; };
+  float m = -INFINITY;
+  for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(int64_t)a.R * a.c + r]);
+  m = warp_max(m);
+  const float shift = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[8] = {};
+  for (int i = first; i <= last; ++i) {
+    const float* s = slot(i);
+    const float f = exp2f(s[(int64_t)a.R * a.c + r] - shift), part = s[(int64_t)a.R * a.c + a.R + r];
+    if (f == 0.f && part == part) continue;                     // a part without keys, or one that the others outweigh; not a NaN
+    l = fmaf(f, part, l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (32 * e + lane < a.c) o[e] = fmaf(f, s[(int64_t)r * a.c + 32 * e + lane], o[e]);
+  }
+  float below = l;
+  if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
+  const float f = l == 0.f ? 0.f : 1.f / below;
+  T* out = (T*)a.out + ((rp->row0 + t) * (int64_t)a.nh + h) * a.c;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (32 * e + lane < a.c) stf(out + 32 * e + lane, o[e] * f);
+}
+
+int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
+  const dim3 grid(ctas, (a.R + 7) / 8);
+  KCH_DISPATCH_FLOAT(a.dtype, T, KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T>, grid, dim3(256), 0, s, 1, a)));
+  KCH_LAUNCH_OK();
+  return KCH_OK;
+}
+
+// ---- entry point --------------------------------------------------------------------------------------------------------------
+int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtype, const char* fn);
+PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
+
+#define PA_CTAS (2 * KCH_SMS)
+static int pa_rows(const kch_paged_attend_args* p) { return p->batch.N * (p->nh / p->cache.n_kv) <= 16 * (int64_t)p->batch.B ? 16 : 64; }
+
+extern "C" int64_t kch_paged_attend_workspace_bytes(const kch_paged_attend_args* p) {
+  if (!p || p->cache.n_kv < 1 || p->nh < 1 || p->cache.c < 1) return 0;
+  return pg_workspace_bytes(PA_CTAS, pa_rows(p), p->cache.c);
+}
+
+extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
+  KCH_REQUIRE(p != nullptr, "kch_paged_attend: null arguments");
+  const int rc = kch_paged_check(&p->cache, &p->batch, p->dtype, "kch_paged_attend");
+  if (rc != KCH_OK) return rc;
+  const int c = p->cache.c, n_kv = p->cache.n_kv;
+  KCH_REQUIRE(p->nh >= 1 && p->nh % n_kv == 0, "kch_paged_attend: nh=%d must be a multiple of n_kv=%d", p->nh, n_kv);
+  KCH_REQUIRE(p->sliding_window >= 0, "kch_paged_attend: sliding_window=%d must be >= 0 (0: every key)", p->sliding_window);
+  KCH_REQUIRE(isfinite(p->scale), "kch_paged_attend: scale must be finite");
+  KCH_REQUIRE(!p->sink || p->sink_dtype == KCH_F32 || p->sink_dtype == KCH_BF16, "kch_paged_attend: sink dtype tag %d", p->sink_dtype);
+  if (p->batch.N == 0) return KCH_OK;
+  const int es = p->dtype == KCH_BF16 ? 2 : 4;
+  KCH_REQUIRE(p->q && p->out, "kch_paged_attend: null q or out");
+  KCH_REQUIRE(p->ld_q >= (int64_t)p->nh * c && p->ld_q * es % 16 == 0 && ((uintptr_t)p->q & 15) == 0 && ((uintptr_t)p->out & 15) == 0,
+              "kch_paged_attend: q and out must be 16-byte aligned, tokens of q (ld_q=%lld elements) at least nh * c apart in multiples of 16 bytes",
+              (long long)p->ld_q);
+  const int64_t need = kch_paged_attend_workspace_bytes(p);
+  KCH_REQUIRE(p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= need,
+              "kch_paged_attend: workspace of %lld bytes (256-byte aligned) is too small: %lld needed", (long long)p->workspace_bytes, (long long)need);
+  PgAttend a = {};
+  a.bt = kch_paged_batch_of(&p->cache, &p->batch);
+  KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
+  a.q = p->q; a.k = p->cache.k; a.v = p->cache.v; a.ks = p->cache.k_scales; a.vs = p->cache.v_scales;
+  a.out = p->out; a.ld_q = p->ld_q; a.n_kv = n_kv; a.G = p->nh / n_kv; a.c = c; a.page = p->cache.page_size;
+  a.window = p->sliding_window; a.zero_rest = p->zero_rest;
+  a.scale = p->scale * PG_LOG2E;
+  a.sink = p->sink; a.sink_dtype = p->sink_dtype;
+  a.records = (PgRecord*)p->workspace;
+  a.slots = (float*)((char*)p->workspace + pg_records_bytes(PA_CTAS));
+  cudaStream_t s = kch_stream(stream);
+  const int rows = pa_rows(p), dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);
+#define PA_GO(T_, P_, R_, D_)                                                                                                 \
+  do {                                                                                                                        \
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
+    paged_attend_simt_kernel<T_, P_, R_, D_><<<PA_CTAS, PA_THREADS, smem, s>>>(a);                                            \
+  } while (0)
+#define PA_WIDTH(T_, P_, R_)                                                                                                  \
+  do {                                                                                                                        \
+    if (dmax == 64) PA_GO(T_, P_, R_, 64);                                                                                    \
+    else if (dmax == 128) PA_GO(T_, P_, R_, 128);                                                                             \
+    else PA_GO(T_, P_, R_, 256);                                                                                              \
+  } while (0)
+#define PA_ROWS(T_, P_)                                                                                                       \
+  do {                                                                                                                        \
+    if (rows == 16) PA_WIDTH(T_, P_, 16);                                                                                     \
+    else PA_WIDTH(T_, P_, 64);                                                                                                \
+  } while (0)
+  if (p->cache.kind == KCH_FP8_E4M3) { if (p->dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
+  else if (p->cache.kind == KCH_INT8) { if (p->dtype == KCH_F32) PA_ROWS(float, int8_t); else PA_ROWS(bf16, int8_t); }
+  else if (p->dtype == KCH_F32) PA_ROWS(float, float);
+  else PA_ROWS(bf16, bf16);
+  KCH_LAUNCH_OK();
+  PgJoinArgs j = {a.out, p->dtype, p->nh, a.G, c, rows, a.sink, a.sink_dtype, a.records, a.slots};
+  return kch_paged_join(j, PA_CTAS, s);
+}

@@ -90,11 +90,27 @@ class KdaLayerArgs(C.Structure):
                 ("W_gup", _vp), ("ld_wg", _i64), ("state", _vp), ("state_out", _vp)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scales", _vp), ("v_scales", _vp), ("kind", _i), ("num_pages", _i64),
+                ("page_size", _i), ("n_kv", _i), ("c", _i)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("table", _vp), ("ld_table", _i64), ("max_pages", _i), ("t0", _vp), ("cu_seqlens", _vp), ("B", _i), ("N", _i64)]
+
+
+class PagedAttendArgs(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("q", _vp), ("ld_q", _i64), ("dtype", _i), ("nh", _i), ("scale", _f),
+                ("sliding_window", _i), ("sink", _vp), ("sink_dtype", _i), ("out", _vp), ("zero_rest", _i),
+                ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
 # indices into a cache's device counters (include/kch_b200.h KCH_CTR_*)
 CTR_ACC_LEN, CTR_N_BLOCKS, CTR_RING_N, CTR_HAS_PREV, CTR_TOKENS, CTR_ARRIVALS, CTR_WORDS = 0, 1, 2, 3, 4, 5, 8
 STATUS_CACHE_CAPACITY = 64
 STATUS_SELFTEST_WAIT = 0x5E1F
 STATUS_PEER_GATHER = 0x9A7E
+STATUS_PAGED_TABLE = 0x6D06
 
 
 # name -> (restype, argtypes); must list every symbol declared in include/kch_b200.h
@@ -147,6 +163,10 @@ PROTOTYPES = {
     "kch_attend_decode_splits": (_i, [_i]),
     "kch_attend_decode_workspace_bytes": (_i64, [_i, _i, _i]),
     "kch_attend_decode": (_i, [C.POINTER(AttendDecodeArgs), _vp]),
+    "kch_paged_append": (_i, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _i64, _vp, _i64, _i, _vp]),
+    "kch_paged_read": (_i, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _i64, _vp, _i64, _i, _i, _vp]),
+    "kch_paged_attend_workspace_bytes": (_i64, [C.POINTER(PagedAttendArgs)]),
+    "kch_paged_attend": (_i, [C.POINTER(PagedAttendArgs), _vp]),
     "kch_cache_append_prompt_workspace_bytes": (_i64, [C.POINTER(CacheAppendArgs), _i64]),
     "kch_cache_append_prompt": (_i, [C.POINTER(CacheAppendArgs), _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "kch_csa_layer_workspace_bytes": (_i64, [C.POINTER(CsaLayerArgs)]),
