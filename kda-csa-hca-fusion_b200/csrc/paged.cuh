@@ -202,7 +202,7 @@ struct PgWalk {
 };
 
 // Parts of items in the workspace: one record a CTA (the item that starts in its range and ends in another's), then two slots
-// a CTA of R rows: c sums, the row's maximum (base 2) and its sum.
+// a CTA of R rows (or what rows the call has, where these are fewer): c sums a row, the rows' maxima (base 2), their sums.
 struct PgRecord { int valid, b, h, block, last, rows; int64_t row0; };       // last: the CTA that has the item's end
 __host__ __device__ __forceinline__ int64_t pg_slot_floats(int R, int c) { return (int64_t)R * (c + 2); }
 __host__ __device__ __forceinline__ int64_t pg_records_bytes(int ctas) { return ((int64_t)ctas * (int64_t)sizeof(PgRecord) + 255) / 256 * 256; }
@@ -210,7 +210,7 @@ static inline int64_t pg_workspace_bytes(int ctas, int R, int c) { return pg_rec
 
 struct PgJoinArgs {
   void* out; int dtype;                // [N, nh, c]
-  int nh, G, c, R;
+  int nh, G, c, R, slot_rows;          // R: rows of an item
   const void* sink; int sink_dtype;
   const PgRecord* records; const float* slots;
 };
@@ -221,7 +221,7 @@ struct PgAttend {                      // what both attention kernels get
   const void *q, *k, *v; const float *ks, *vs;
   void* out;
   int64_t ld_q;
-  int n_kv, G, c, page, window, zero_rest;
+  int n_kv, G, c, page, window, zero_rest, slot_rows;
   float scale;                         // times log2(e)
   const void* sink; int sink_dtype;
   PgRecord* records; float* slots;

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     }
     // ---- the item's end: its rows, or its part of them ---------------------------------------------------------------------
     const bool direct = w.starts() && w.ends();
-    float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(ROWS, c);
+    float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(a.slot_rows, c);
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int r = ty + 16 * i;
@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         }
       }
       if (!direct && tx == 0) {
-        slot[(int64_t)ROWS * c + r] = sm[r];
-        slot[(int64_t)ROWS * c + ROWS + r] = sl[r];
+        slot[(int64_t)a.slot_rows * c + r] = sm[r];
+        slot[(int64_t)a.slot_rows * c + a.slot_rows + r] = sl[r];
       }
     }
     if (w.starts() && !w.ends()) {
@@ -253,17 +253,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PgJoinArgs a) {
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, rows = rp->rows;
   if (r >= rows) return;
   const int first = blockIdx.x, last = rp->last;
-  const int64_t size = pg_slot_floats(a.R, a.c), row = (int64_t)rp->block * a.R + r, t = row / a.G;
+  const int64_t size = pg_slot_floats(a.slot_rows, a.c), row = (int64_t)rp->block * a.R + r, t = row / a.G;
   const int h = rp->h * a.G + (int)(row % a.G);
   auto slot = [&](int i) { return a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size; };
   float m = -INFINITY;
-  for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(int64_t)a.R * a.c + r]);
+  for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(int64_t)a.slot_rows * a.c + r]);
   m = warp_max(m);
   const float shift = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[8] = {};
   for (int i = first; i <= last; ++i) {
     const float* s = slot(i);
-    const float f = exp2f(s[(int64_t)a.R * a.c + r] - shift), part = s[(int64_t)a.R * a.c + a.R + r];
+    const float f = exp2f(s[(int64_t)a.slot_rows * a.c + r] - shift), part = s[(int64_t)a.slot_rows * a.c + a.slot_rows + r];
     if (f == 0.f && part == part) continue;                     // a part without keys, or one that the others outweigh; not a NaN
     l = fmaf(f, part, l);
 #pragma unroll
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PgJoinArgs a) {
 }
 
 int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
-  const dim3 grid(ctas, (a.R + 7) / 8);
+  const dim3 grid(ctas, (a.slot_rows + 7) / 8);
   KCH_DISPATCH_FLOAT(a.dtype, T, KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T>, grid, dim3(256), 0, s, 1, a)));
   KCH_LAUNCH_OK();
   return KCH_OK;
@@ -290,12 +290,25 @@ int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
 int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtype, const char* fn);
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
-#define PA_CTAS (2 * KCH_SMS)
-static int pa_rows(const kch_paged_attend_args* p) { return p->batch.N * (p->nh / p->cache.n_kv) <= 16 * (int64_t)p->batch.B ? 16 : 64; }
+bool kch_paged_attend_tc5_supported(int dtype, int c);
+int kch_paged_attend_tc5(const PgAttend& a, int kind, int ctas, cudaStream_t s);
+
+// How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.
+struct PaPlan { bool tc5; int rows, ctas, slot_rows; };
+static PaPlan pa_plan(const kch_paged_attend_args* p) {
+  PaPlan x;
+  const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
+  x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
+  x.rows = x.tc5 ? 256 : rows <= 16 * (int64_t)p->batch.B ? 16 : 64;
+  x.ctas = x.tc5 ? KCH_SMS : 2 * KCH_SMS;
+  x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
+  return x;
+}
 
 extern "C" int64_t kch_paged_attend_workspace_bytes(const kch_paged_attend_args* p) {
   if (!p || p->cache.n_kv < 1 || p->nh < 1 || p->cache.c < 1) return 0;
-  return pg_workspace_bytes(PA_CTAS, pa_rows(p), p->cache.c);
+  const PaPlan x = pa_plan(p);
+  return pg_workspace_bytes(x.ctas, x.slot_rows, p->cache.c);
 }
 
 extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
@@ -325,13 +338,20 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   a.records = (PgRecord*)p->workspace;
-  a.slots = (float*)((char*)p->workspace + pg_records_bytes(PA_CTAS));
+  const PaPlan x = pa_plan(p);
+  a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
+  a.slot_rows = x.slot_rows;
   cudaStream_t s = kch_stream(stream);
-  const int rows = pa_rows(p), dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);
+  const PgJoinArgs j = {a.out, p->dtype, p->nh, a.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
+  if (x.tc5) {
+    const int rc5 = kch_paged_attend_tc5(a, p->cache.kind, x.ctas, s);
+    return rc5 != KCH_OK ? rc5 : kch_paged_join(j, x.ctas, s);
+  }
+  const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);
 #define PA_GO(T_, P_, R_, D_)                                                                                                 \
   do {                                                                                                                        \
     KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
-    paged_attend_simt_kernel<T_, P_, R_, D_><<<PA_CTAS, PA_THREADS, smem, s>>>(a);                                            \
+    paged_attend_simt_kernel<T_, P_, R_, D_><<<x.ctas, PA_THREADS, smem, s>>>(a);                                            \
   } while (0)
 #define PA_WIDTH(T_, P_, R_)                                                                                                  \
   do {                                                                                                                        \
@@ -349,6 +369,5 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   else if (p->dtype == KCH_F32) PA_ROWS(float, float);
   else PA_ROWS(bf16, bf16);
   KCH_LAUNCH_OK();
-  PgJoinArgs j = {a.out, p->dtype, p->nh, a.G, c, rows, a.sink, a.sink_dtype, a.records, a.slots};
-  return kch_paged_join(j, PA_CTAS, s);
+  return kch_paged_join(j, x.ctas, s);
 }
