@@ -20,51 +20,55 @@ unsigned int* kch_status_device_ptr();
 struct PgBatch {
   const int32_t* table; int64_t ld_table;
   const int32_t *t0, *cu;
-  int B; int64_t N;                    // sequences; rows of the packed tensors
-  int64_t cap;                         // positions that a row of the table covers
+  int B, N;                            // sequences; rows of the packed tensors
+  int cap;                             // positions that a row of the table covers (below 2^31)
   int64_t num_pages;
   int shift;                           // log2(page_size)
   unsigned int* status;
 };
 
-struct PgSeq { int64_t row0; int len; int64_t t0, kv; };      // first packed row, new tokens, tokens before them, keys in all
+struct PgSeq { int row0, len, t0, kv; };      // first packed row, new tokens, tokens before them, keys in all
 
 // (Whatever cu_seqlens and t0 hold, rows stay inside the packed tensors and keys inside the table.)
 __device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
   PgSeq s;
-  const int64_t lo = min(max((int64_t)__ldg(a.cu + b), (int64_t)0), a.N), hi = min(max((int64_t)__ldg(a.cu + b + 1), lo), a.N);
-  s.row0 = lo;
-  s.len = (int)(hi - lo);
-  s.t0 = max((int64_t)__ldg(a.t0 + b), (int64_t)0);
-  s.kv = min(s.t0 + s.len, a.cap);
+  s.row0 = min(max(__ldg(a.cu + b), 0), a.N);
+  s.len = min(max(__ldg(a.cu + b + 1), s.row0), a.N) - s.row0;
+  s.t0 = max(__ldg(a.t0 + b), 0);
+  s.kv = (int)min((int64_t)s.t0 + s.len, (int64_t)a.cap);
   return s;
 }
 __device__ __forceinline__ void pg_bad(const PgBatch& a) { atomicCAS(a.status, 0u, (unsigned)KCH_STATUS_PAGED_TABLE); }
 // page of `index` pages into sequence b, or -1 (and the status word) where the table holds none
-__device__ __forceinline__ int64_t pg_page(const PgBatch& a, int b, int64_t index) {
-  const int64_t p = __ldg(a.table + b * a.ld_table + index);
+__device__ __forceinline__ int pg_page(const PgBatch& a, int b, int index) {
+  const int p = __ldg(a.table + b * a.ld_table + index);
   if (p >= 0 && p < a.num_pages) return p;
   pg_bad(a);
   return -1;
 }
 
 // One block of rows of a sequence: which keys its rows see together.
-struct PgSpan { int rows; int64_t first_key; int tiles, steps; };   // tiles of KT keys from first_key (a multiple of KT) on
+struct PgSpan { int rows, first_key, tiles, steps; };   // tiles of KT keys from first_key (a multiple of KT) on
 // R rows a block, KT keys a tile; HALF: a block of at most R / 2 rows takes two tiles a step
 template <int R, int KT, bool HALF>
 __device__ __forceinline__ PgSpan pg_span(const PgSeq& s, int G, int window, int block) {
   PgSpan x;
-  const int64_t r0 = (int64_t)block * R, all = (int64_t)s.len * G, r1 = min(r0 + R, all);
-  x.rows = (int)(r1 - r0);
-  const int64_t first = s.t0 + r0 / G, last = s.t0 + (r1 - 1) / G;          // positions of the first and the last query
-  const int64_t lo = window > 0 ? max(first - window + 1, (int64_t)0) : 0, hi = min(last + 1, s.kv);
+  const int r0 = block * R, r1 = min(r0 + R, s.len * G);
+  x.rows = r1 - r0;
+  const int64_t first = (int64_t)s.t0 + r0 / G, last = (int64_t)s.t0 + (r1 - 1) / G;      // positions of the first and the last query
+  const int lo = window > 0 ? (int)min(max(first - window + 1, (int64_t)0), (int64_t)s.kv) : 0, hi = (int)min(last + 1, (int64_t)s.kv);
   x.first_key = lo / KT * KT;
-  x.tiles = hi > x.first_key ? (int)((hi - x.first_key + KT - 1) / KT) : 0;
+  x.tiles = hi > x.first_key ? (hi - x.first_key + KT - 1) / KT : 0;
   x.steps = max(HALF && x.rows <= R / 2 ? (x.tiles + 1) / 2 : x.tiles, 1);  // (a row without keys is stored all the same)
   return x;
 }
 template <int R>
-__device__ __forceinline__ int pg_blocks(const PgSeq& s, int G) { return (int)(((int64_t)s.len * G + R - 1) / R); }
+__device__ __forceinline__ int pg_blocks(const PgSeq& s, int G) { return (s.len * G + R - 1) / R; }
+// the keys [x, y) that row `row` (token * G + head of the group) of a sequence sees
+__device__ __forceinline__ int2 pg_sees(const PgSeq& s, int G, int window, int row) {
+  const int64_t pos = (int64_t)s.t0 + row / G;
+  return make_int2(window > 0 ? (int)min(max(pos - window + 1, (int64_t)0), (int64_t)s.kv) : 0, (int)min(pos + 1, (int64_t)s.kv));
+}
 
 struct PgPlace {                       // where a CTA's range of steps begins
   int64_t per, left;                   // steps of a CTA; steps of this one
@@ -102,7 +106,7 @@ __device__ PgPlace pg_plan(const PgBatch& a, int G, int n_kv, int window, void* 
       if (lane == from) mine = sum;
     }
     if (b < a.B) base[b + 1] = mine * n_kv;
-    if (b < a.B && s.t0 + s.len > a.cap) pg_bad(a);
+    if (b < a.B && (int64_t)s.t0 + s.len > a.cap) pg_bad(a);
   }
   if (tid == 0) { base[0] = 0; found[0] = -1; }
   __syncthreads();
@@ -203,7 +207,7 @@ struct PgWalk {
 
 // Parts of items in the workspace: one record a CTA (the item that starts in its range and ends in another's), then two slots
 // a CTA of R rows (or what rows the call has, where these are fewer): c sums a row, the rows' maxima (base 2), their sums.
-struct PgRecord { int valid, b, h, block, last, rows; int64_t row0; };       // last: the CTA that has the item's end
+struct PgRecord { int valid, b, h, block, last, rows, row0; };       // last: the CTA that has the item's end
 __host__ __device__ __forceinline__ int64_t pg_slot_floats(int R, int c) { return (int64_t)R * (c + 2); }
 __host__ __device__ __forceinline__ int64_t pg_records_bytes(int ctas) { return ((int64_t)ctas * (int64_t)sizeof(PgRecord) + 255) / 256 * 256; }
 static inline int64_t pg_workspace_bytes(int ctas, int R, int c) { return pg_records_bytes(ctas) + 2 * ctas * pg_slot_floats(R, c) * 4; }
@@ -230,7 +234,7 @@ struct PgAttend {                      // what both attention kernels get
 // rows behind the last sequence (and before the first), where the caller wants zeros there
 __device__ __forceinline__ void pg_zero_rest(const PgAttend& a, int es, int cta, int ctas) {
   if (!a.zero_rest) return;
-  const int64_t lo = min(max((int64_t)__ldg(a.bt.cu), (int64_t)0), a.bt.N), hi = min(max((int64_t)__ldg(a.bt.cu + a.bt.B), lo), a.bt.N);
+  const int64_t lo = min(max(__ldg(a.bt.cu), 0), a.bt.N), hi = min(max(__ldg(a.bt.cu + a.bt.B), (int)lo), a.bt.N);
   const int64_t row = (int64_t)a.n_kv * a.G * a.c * es / 16, words = (lo + a.bt.N - hi) * row;      // 16-byte words of a token
   for (int64_t i = (int64_t)cta * blockDim.x + threadIdx.x; i < words; i += (int64_t)ctas * blockDim.x) {
     const int64_t t = i / row, at = (t < lo ? t : hi + t - lo) * row + i % row;

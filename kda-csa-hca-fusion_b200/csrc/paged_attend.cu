@@ -52,6 +52,7 @@ template <> struct PgStored<int8_t> {
 
 #define PA_KT 64
 #define PA_THREADS 256
+#define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
 static int pa_smem(int ROWS, int DMAX, int B) {
   const int need = (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4, plan = PG_PLAN_BYTES(B);
@@ -73,14 +74,14 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
   PgRecord rec = {};
   PgWalk<ROWS, PA_KT, false> w(a.bt, a.G, a.n_kv, a.window, place);
   for (; w.valid(); w.next()) {
-    const int64_t r0 = (int64_t)w.block * ROWS;                // first (token, head) row of the block in its sequence
+    const int r0 = w.block * ROWS;                             // first (token, head) row of the block in its sequence
     __syncthreads();
     for (int i = tid; i < ROWS * c8; i += PA_THREADS) {
       const int r = i / c8, d = i % c8 * 8;
       float x[8] = {};
       if (r < w.x.rows) {
-        const int64_t t = (r0 + r) / a.G;
-        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * a.G + (int)((r0 + r) % a.G)) * c + d, x);
+        const int t = (r0 + r) / a.G;
+        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * a.G + r0 + r - t * a.G) * c + d, x);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq[r * LD + d + e] = x[e];
@@ -92,11 +93,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #pragma unroll
       for (int j = 0; j < CT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
     for (int st = w.first; st < w.first + w.count; ++st) {
-      const int64_t key0 = w.x.first_key + (int64_t)st * PA_KT;
+      const int key0 = w.x.first_key + st * PA_KT;
       __syncthreads();
       for (int i = tid; i < PA_KT * c8; i += PA_THREADS) {     // keys and values of the tile, 0 behind the sequence's end
         const int j = i / c8, d = i % c8 * 8;
-        const int64_t pos = key0 + j;
+        const int pos = key0 + j;
         float kx[8] = {}, vx[8] = {};
         if (pos < w.s.kv) {
           const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
@@ -138,13 +139,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         const int r = ty + 16 * i;
-        const int64_t pos = w.s.t0 + (r0 + r) / a.G, from = a.window > 0 ? pos - a.window + 1 : 0;
+        const int2 keys = r < w.x.rows ? pg_sees(w.s, a.G, a.window, r0 + r) : make_int2(0, 0);
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int64_t key = key0 + tx + 16 * j;
-          const bool sees = r < w.x.rows && key >= from && key <= pos && key < w.s.kv;
-          acc[i][j] = sees ? acc[i][j] * a.scale : -INFINITY;
+          const int key = key0 + tx + 16 * j;
+          acc[i][j] = key >= keys.x && key < keys.y ? acc[i][j] * a.scale : -INFINITY;
           top = fmaxf(top, acc[i][j]);
         }
 #pragma unroll
@@ -178,8 +178,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
       }
       // A key that a row does not see must not reach it: 0 times an infinity or a NaN is no 0.  In a tile where every row
       // sees every key nothing is to be skipped.
-      const int64_t low = w.s.t0 + r0 / a.G, high = w.s.t0 + (r0 + w.x.rows - 1) / a.G;
-      const bool whole = key0 + PA_KT - 1 <= low && (a.window == 0 || key0 > high - a.window) && key0 + PA_KT <= w.s.kv;
+      const bool whole = key0 >= pg_sees(w.s, a.G, a.window, r0 + w.x.rows - 1).x && key0 + PA_KT <= pg_sees(w.s, a.G, a.window, r0).y;
       auto product = [&](auto masked) {
         for (int j = 0; j < PA_KT; ++j) {
           float p[RT];
@@ -209,8 +208,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     for (int i = 0; i < RT; ++i) {
       const int r = ty + 16 * i;
       if (r >= w.x.rows) continue;
-      const int64_t t = (r0 + r) / a.G;
-      const int h = w.h * a.G + (int)((r0 + r) % a.G);
+      const int t = (r0 + r) / a.G, h = w.h * a.G + r0 + r - t * a.G;
       float f = 1.f;
       if (direct) {
         const float m = sm[r], l = sl[r];
@@ -218,7 +216,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - m);
         f = l == 0.f ? 0.f : 1.f / below;
       }
-      T* orow = (T*)a.out + ((w.s.row0 + t) * (int64_t)(a.n_kv * a.G) + h) * c;
+      T* orow = (T*)a.out + ((int64_t)(w.s.row0 + t) * (a.n_kv * a.G) + h) * c;
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
         const int d = tx * 4 + 64 * x;
@@ -243,45 +241,133 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------
-// Block (i, y): the item that starts in CTA i's range and ends in another's, rows y * 8 .. ; a warp a row, its lanes over the
-// columns.  Launched to start while the kernel before it drains.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_join_kernel(PgJoinArgs a) {
+// The rows of all items that are in parts, one after the other over the blocks.  Where a row has few parts it is a warp's, else a
+// block's whose warps take every eighth part; either sums them in one order.  4 (8) columns a lane.  Launched to start while
+// the kernel before it drains.  (One long sequence's step gives a row 74 or 148 parts: a warp a row took 80 us for them.)
+#define PJ_BLOCKS (2 * KCH_SMS)
+#define PJ_WARPS 8
+template <typename T, int W>          // W: columns of a lane, in fours
+__global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a, int ctas) {
+  __shared__ int before[PA_CTAS + 1], many[PA_CTAS], n_many;      // many: the items whose rows are a block's
+  __shared__ alignas(16) float part_o[PJ_WARPS][W * 128];
+  __shared__ float part_l[PJ_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   chain_wait();
-  const PgRecord* rp = a.records + blockIdx.x;
-  if (!rp->valid) return;
-  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, rows = rp->rows;
-  if (r >= rows) return;
-  const int first = blockIdx.x, last = rp->last;
-  const int64_t size = pg_slot_floats(a.slot_rows, a.c), row = (int64_t)rp->block * a.R + r, t = row / a.G;
-  const int h = rp->h * a.G + (int)(row % a.G);
-  auto slot = [&](int i) { return a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size; };
-  float m = -INFINITY;
-  for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, slot(i)[(int64_t)a.slot_rows * a.c + r]);
-  m = warp_max(m);
-  const float shift = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[8] = {};
-  for (int i = first; i <= last; ++i) {
-    const float* s = slot(i);
-    const float f = exp2f(s[(int64_t)a.slot_rows * a.c + r] - shift), part = s[(int64_t)a.slot_rows * a.c + a.slot_rows + r];
-    if (f == 0.f && part == part) continue;                     // a part without keys, or one that the others outweigh; not a NaN
-    l = fmaf(f, part, l);
+  if (warp == 0) {                     // rows of the parted items before each
+    int run = 0, wides = 0;
+    for (int i0 = 0; i0 < ctas; i0 += 32) {
+      const int i = i0 + lane;
+      const bool there = i < ctas && a.records[i].valid;
+      int x = there ? a.records[i].rows : 0;
+      const bool wide = there && a.records[i].last - i >= PJ_WARPS;
+      const unsigned who = __ballot_sync(0xffffffffu, wide);
+      if (wide) many[wides + __popc(who & ((1u << lane) - 1u))] = i;
+      wides += __popc(who);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (32 * e + lane < a.c) o[e] = fmaf(f, s[(int64_t)r * a.c + 32 * e + lane], o[e]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (i < ctas) before[i + 1] = run + x;
+      run += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) { before[0] = 0; n_many = wides; }
   }
-  float below = l;
-  if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
-  const float f = l == 0.f ? 0.f : 1.f / below;
-  T* out = (T*)a.out + ((rp->row0 + t) * (int64_t)a.nh + h) * a.c;
+  __syncthreads();
+  const int rows = before[ctas];
+  const int64_t size = pg_slot_floats(a.slot_rows, a.c), mat = (int64_t)a.slot_rows * a.c;
+  // the parts `from`, from + step, .. of a row: their sums with the weights 2^(m_i - shift)
+  float o[4 * W], l;
+  auto gather = [&](int first, int last, int r, float shift, int from, int step) {
+    l = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (32 * e + lane < a.c) stf(out + 32 * e + lane, o[e] * f);
+    for (int e = 0; e < 4 * W; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = first + from; i <= last; i += step) {
+      const float* s = a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size;
+      const float f = exp2f(s[mat + r] - shift), part = s[mat + a.slot_rows + r];
+      l = fmaf(f, part, l);
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+        const int d = 128 * x + 4 * lane;
+        if (d >= a.c) continue;
+        const float4 v = *reinterpret_cast<const float4*>(s + (int64_t)r * a.c + d);
+        // (weight 0: a part without keys; what its sums hold does not matter)
+        o[4 * x] = f == 0.f ? o[4 * x] : fmaf(f, v.x, o[4 * x]);
+        o[4 * x + 1] = f == 0.f ? o[4 * x + 1] : fmaf(f, v.y, o[4 * x + 1]);
+        o[4 * x + 2] = f == 0.f ? o[4 * x + 2] : fmaf(f, v.z, o[4 * x + 2]);
+        o[4 * x + 3] = f == 0.f ? o[4 * x + 3] : fmaf(f, v.w, o[4 * x + 3]);
+      }
+    }
+  };
+  auto highest = [&](int first, int last, int r) {
+    float m = -INFINITY;
+    for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, a.slots[(2 * (int64_t)i + (i == first ? 1 : 0)) * size + mat + r]);
+    return warp_max(m);
+  };
+  auto store = [&](const PgRecord& rec, int r, float shift) {
+    const int row = rec.block * a.R + r, t = row / a.G, h = rec.h * a.G + row - t * a.G;
+    float below = l;
+    if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
+    const float f = l == 0.f ? 0.f : 1.f / below;
+    T* out = (T*)a.out + ((int64_t)(rec.row0 + t) * a.nh + h) * a.c;
+#pragma unroll
+    for (int x = 0; x < W; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 128 * x + 4 * lane + e;
+        if (d < a.c) stf(out + d, o[4 * x + e] * f);
+      }
+  };
+  auto item_of = [&](int row) {        // the last i with before[i] <= row
+    int lo = 0, hi = ctas;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  // rows of few parts: a warp each; the others are left to the blocks
+  for (int row = blockIdx.x * PJ_WARPS + warp; row < rows; row += gridDim.x * PJ_WARPS) {
+    const int i = item_of(row), r = row - before[i];
+    const PgRecord rec = a.records[i];
+    if (rec.last - i >= PJ_WARPS) continue;
+    const float m = highest(i, rec.last, r), shift = m == -INFINITY ? 0.f : m;
+    gather(i, rec.last, r, shift, 0, 1);
+    store(rec, r, shift);
+  }
+  for (int k = 0; k < n_many; ++k) {
+    const int i = many[k];
+    const PgRecord rec = a.records[i];
+    for (int row = before[i] + (int)((blockIdx.x + gridDim.x - before[i] % gridDim.x) % gridDim.x); row < before[i + 1]; row += gridDim.x) {
+      const int r = row - before[i];
+      const float m = highest(i, rec.last, r), shift = m == -INFINITY ? 0.f : m;
+      gather(i, rec.last, r, shift, warp, PJ_WARPS);
+      __syncthreads();                 // (what was there has been read)
+#pragma unroll
+      for (int x = 0; x < W; ++x) *reinterpret_cast<float4*>(&part_o[warp][128 * x + 4 * lane]) = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+      if (lane == 0) part_l[warp] = l;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < PJ_WARPS; ++w) {
+          l += part_l[w];
+#pragma unroll
+          for (int x = 0; x < W; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * x + e] += part_o[w][128 * x + 4 * lane + e];
+        }
+        store(rec, r, shift);
+      }
+    }
+  }
 }
 
 int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
-  const dim3 grid(ctas, (a.slot_rows + 7) / 8);
-  KCH_DISPATCH_FLOAT(a.dtype, T, KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T>, grid, dim3(256), 0, s, 1, a)));
+  const dim3 grid(PJ_BLOCKS), block(32 * PJ_WARPS);
+  KCH_DISPATCH_FLOAT(a.dtype, T, {
+    if (a.c <= 128) KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 1>, grid, block, 0, s, 1, a, ctas));
+    else KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 2>, grid, block, 0, s, 1, a, ctas));
+  });
   KCH_LAUNCH_OK();
   return KCH_OK;
 }
@@ -300,7 +386,7 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
   x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
   x.rows = x.tc5 ? 256 : rows <= 16 * (int64_t)p->batch.B ? 16 : 64;
-  x.ctas = x.tc5 ? KCH_SMS : 2 * KCH_SMS;
+  x.ctas = x.tc5 ? KCH_SMS : PA_CTAS;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
 }
@@ -320,6 +406,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   KCH_REQUIRE(p->sliding_window >= 0, "kch_paged_attend: sliding_window=%d must be >= 0 (0: every key)", p->sliding_window);
   KCH_REQUIRE(isfinite(p->scale), "kch_paged_attend: scale must be finite");
   KCH_REQUIRE(!p->sink || p->sink_dtype == KCH_F32 || p->sink_dtype == KCH_BF16, "kch_paged_attend: sink dtype tag %d", p->sink_dtype);
+  KCH_REQUIRE(p->batch.N * p->nh <= 0x7FFFFFFFLL, "kch_paged_attend: N * nh = %lld rows of q", (long long)(p->batch.N * p->nh));
   if (p->batch.N == 0) return KCH_OK;
   const int es = p->dtype == KCH_BF16 ? 2 : 4;
   KCH_REQUIRE(p->q && p->out, "kch_paged_attend: null q or out");

@@ -36,6 +36,9 @@ struct PtCfg {
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
   static constexpr int THREADS = Q8 ? 512 : 384;
+  // registers of the warpgroups (threads * registers at launch: 65536 and 64512)
+  static constexpr int REG_FEED = Q8 ? 104 : 80, REG_SOFT = Q8 ? 144 : 208;
+  static_assert(128 * (REG_FEED * (Q8 ? 2 : 1) + 2 * REG_SOFT) <= (Q8 ? 65536 : 64512), "register split");
 };
 
 template <int D, int KIND>
@@ -81,11 +84,6 @@ __device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) 
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t pt_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -98,27 +96,31 @@ __device__ __forceinline__ uint32_t pt_range(int lo, int hi) {
   return hi > lo ? (0xFFFFFFFFu >> (32 - (hi - lo))) << lo : 0u;
 }
 // two bf16 values from two 8-bit codes, exactly
-__device__ __forceinline__ uint32_t pt_bf16_mul(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-__device__ __forceinline__ uint32_t pt_bf16_sub(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+// (as FMAs: mul and sub of bf16 pairs become conversions to fp32 and back, and 4500 cycles for a tile of 128 x 128 instead of ~900)
+__device__ __forceinline__ uint32_t pt_bf16_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 template <int KIND>
 __device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (KIND == KCH_FP8_E4M3) {
     // sign, exponent and mantissa moved to their places are 2^-120 of the value (subnormal codes become subnormal bf16 values)
     const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
-    lo = pt_bf16_mul((a & 0x80008000u) | ((a >> 4) & 0x07F007F0u), 0x7B807B80u);
-    hi = pt_bf16_mul((b & 0x80008000u) | ((b >> 4) & 0x07F007F0u), 0x7B807B80u);
+    lo = pt_bf16_fma((a & 0x80008000u) | ((a >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
+    hi = pt_bf16_fma((b & 0x80008000u) | ((b >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
   } else {
     // 128 + the low 7 bits, less 256 or 128 by the sign
     const uint32_t a = __byte_perm(w, 0x43434343u, 0x5140), b = __byte_perm(w, 0x43434343u, 0x7362);
-    lo = pt_bf16_sub(a & 0xFF7FFF7Fu, a & 0xFF80FF80u);
-    hi = pt_bf16_sub(b & 0xFF7FFF7Fu, b & 0xFF80FF80u);
+    lo = pt_bf16_fma(a & 0xFF80FF80u, 0xBF80BF80u, a & 0xFF7FFF7Fu);
+    hi = pt_bf16_fma(b & 0xFF80FF80u, 0xBF80BF80u, b & 0xFF7FFF7Fu);
   }
 }
 
 // One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns c0 ..
 // c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).
 template <int D, int KIND>
-__device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int64_t from, int64_t to, float sc, float shift,
+__device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int from, int to, float sc, float shift,
                                          float f, bf16* out, float* dst, int c0, int c1) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
@@ -130,7 +132,7 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
     if (KIND == KCH_INT8) return (float)((const int8_t*)p)[i];
     return float(((const __nv_fp8_e4m3*)p)[i]);
   };
-  for (int64_t j = from; j < to; ++j) {
+  for (int j = from; j < to; ++j) {
     const int64_t pg = pg_page(a.bt, b, j >> a.bt.shift);
     const int64_t row = (pg * a.n_kv + h) * a.page + (j & (a.page - 1));
     float s = 0.f;
@@ -170,7 +172,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 128 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
-    for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 128); mbarrier_init(&sm.sc_empty[i], 8); }
+    for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, 64);
     mbarrier_init(&sm.q_empty, 1);
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
@@ -189,60 +191,67 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   const uint32_t tmem = sm.tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, PT_SPIN, a.bt.status); };
   typedef PgWalk<PT_R, PT_KT, true> Walk;
-  // the tiles of an item's part in the order in which they are used: f(tile, is it the values)
-  auto tiles_of = [](const Walk& w, auto f) {
-    const int s0 = w.first, s1 = w.first + w.count;
-    if (w.x.rows > PT_R / 2) {
-      if (!f(s0, false)) return false;
-      for (int s = s0; s < s1; ++s) {
-        if (!f(s, true)) return false;
-        if (s + 1 < s1 && !f(s + 1, false)) return false;
-      }
-    } else {
-      if (!f(2 * s0, false) || !f(2 * s0 + 1, false)) return false;
-      for (int s = s0; s < s1; ++s)
-        for (int x = 0; x < 2; ++x) {
-          if (!f(2 * s + x, true)) return false;
-          if (s + 1 < s1 && !f(2 * s + 2 + x, false)) return false;
-        }
-    }
-    return true;
-  };
+  // The ring holds an item's tiles in the order in which they are used.  Rows of both: K0, then V0 K1, V1 K2, ..; rows of one: K0 K1,
+  // then V0 K2 V1 K3, V2 K4 V3 K5, ..
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::Q8 ? 56 : 80));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
     if (warp == 0) {
       // ------------------------------ pages into the ring -----------------------------------------------------------------
       // A tile is 128 / rows-of-a-box copies for each panel of 64 channels (8-bit pages: whole rows), a lane each.
       const int box = min(a.page, PT_KT), boxes = PT_KT / box, panels = C::Q8 ? 1 : C::PANELS;
       const int mybox = lane / panels, mypanel = lane % panels;
       const bool mine = lane < boxes * panels;
+      constexpr int N = C::Q8 ? C::RAWS : C::STAGES;
+      uint64_t *fb = C::Q8 ? sm.raw_full : sm.full, *eb = C::Q8 ? sm.raw_empty : sm.empty;
       int g = 0;
       bool ok = true;
       for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next()) {
-        ok = tiles_of(w, [&](int tile, bool v) {
-          const int64_t key = w.x.first_key + (int64_t)tile * PT_KT + mybox * box;
-          int64_t pg = a.bt.num_pages;                   // out of range: zeros
-          if (mine && tile < w.x.tiles && key < w.s.kv) {
-            pg = pg_page(a.bt, w.b, key >> a.bt.shift);
-            if (pg < 0) pg = a.bt.num_pages;
-          }
-          constexpr int N = C::Q8 ? (C::RAWS ? C::RAWS : 1) : C::STAGES;
-          const int st = g % N;
-          uint64_t *fb = C::Q8 ? &sm.raw_full[C::Q8 ? st : 0] : &sm.full[C::Q8 ? 0 : st], *eb = C::Q8 ? &sm.raw_empty[C::Q8 ? st : 0] : &sm.empty[C::Q8 ? 0 : st];
-          bool fine = true;
-          if (g >= N) fine = wait(eb, g / N - 1);
+        const bool pair = w.x.rows > PT_R / 2;
+        const int per = pair ? 1 : 2, end = (w.first + w.count) * per;
+        const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
+        // the page of this lane's box of a tile, asked for a tile ahead; -1 behind the part's or the sequence's end
+        auto ask = [&](int tile) -> int {
+          const int key = w.x.first_key + tile * PT_KT + mybox * box;
+          return mine && tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+        };
+        auto copy = [&](int tile, bool v, int id) {
+          const int st = g % N, key = w.x.first_key + tile * PT_KT + mybox * box;
+          bool fine = g < N || wait(eb + st, g / N - 1);
           fine = __all_sync(0xffffffffu, fine);
           if (!fine) return false;
-          if (lane == 0) mbarrier_expect_tx(fb, C::Q8 ? C::RAW : C::TILE);
+          if (lane == 0) mbarrier_expect_tx(fb + st, C::Q8 ? C::RAW : C::TILE);
           __syncwarp();
           if (mine) {
+            if ((unsigned)id >= (unsigned)a.bt.num_pages) {            // out of range: zeros
+              if (tile < w.x.tiles && key < w.s.kv) pg_bad(a.bt);
+              id = (int)a.bt.num_pages;
+            }
             uint8_t* dst = C::Q8 ? sm.raw[C::Q8 ? st : 0] + mybox * box * D : sm.kv[C::Q8 ? 0 : st] + mypanel * (PT_KT * 128) + mybox * box * 128;
-            pt_tma_4d(dst, v ? &vmap : &kmap, mypanel * 64, (int)(key & (a.page - 1)), w.h, (int)pg, fb);
+            pt_tma_4d(dst, v ? &vmap : &kmap, mypanel * 64, key & (a.page - 1), w.h, id, fb + st);
           }
           ++g;
           return true;
-        });
+        };
+        int t = w.first * per;
+        int id0 = ask(t), id1 = ask(t + 1);              // of tiles t and t + 1
+        ok = copy(t, false, id0) && (pair || copy(t + 1, false, id1));
+        if (pair) {
+          for (; t < end && ok; ++t) {
+            const int id2 = ask(t + 2);
+            ok = copy(t, true, id0) && (t + 1 >= end || copy(t + 1, false, id1));
+            id0 = id1;
+            id1 = id2;
+          }
+        } else {
+          for (; t < end && ok; t += 2) {
+            const int id2 = ask(t + 2), id3 = ask(t + 3);
+            ok = copy(t, true, id0) && (t + 2 >= end || copy(t + 2, false, id2)) && copy(t + 1, true, id1) &&
+                 (t + 2 >= end || copy(t + 3, false, id3));
+            id0 = id2;
+            id1 = id3;
+          }
+        }
       }
       // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones)
       for (int i = 1, n = C::Q8 ? C::RAWS : C::STAGES; i <= n && i <= g; ++i)
@@ -302,7 +311,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     } else {
       // ------------------------------ queries ------------------------------------------------------------------------------
       const int t = tid - 64;
-      int c = 0;
+      int c = 0, kt = 0;
       bool ok = true;
       for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next(), ++c) {
         if (c) ok = wait(&sm.q_empty, c - 1);
@@ -310,96 +319,136 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const int chunks = D / 8, rows = w.x.rows;
         for (int i = t; i < rows * chunks; i += 64) {
           const int r = i / chunks, k = i % chunks;
-          const int64_t row = (int64_t)w.block * PT_R + r, tok = row / a.G;
-          const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (int64_t)(w.h * a.G + (int)(row - tok * a.G)) * D + k * 8;
+          const int row = w.block * PT_R + r, tok = row / a.G;
+          const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * a.G + row - tok * a.G) * D + k * 8;
           const uint32_t dst = smem_addr_u32(sm.q[r >> 7]) + (k >> 3) * (128 * 128) + (r & 127) * 128 + (((k & 7) ^ (r & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          if (a.scale < 0.f) {                           // (the softmax takes the scale's size: a maximum stays one)
+            uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+            u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u;
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+          } else {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         t5_fence_async_smem();
         mbarrier_arrive(&sm.q_full);
+        if constexpr (C::Q8) {
+          // the scales of the item's key tiles: two keys a thread, 0 behind the end (a scale there may be anything); the page is
+          // asked for a tile ahead, and the copies report to the barrier by themselves
+          const int per = rows > PT_R / 2 ? 1 : 2, end = (w.first + w.count) * per;
+          const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
+          auto ask = [&](int tile, int i) -> int {
+            const int key = w.x.first_key + tile * PT_KT + t + 64 * i;
+            return tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+          };
+          int id0 = ask(w.first * per, 0), id1 = ask(w.first * per, 1);
+          for (int tile = w.first * per; tile < end && ok; ++tile, ++kt) {
+            const int n0 = ask(tile + 1, 0), n1 = ask(tile + 1, 1), slot = kt % C::SCALES;
+            if (kt >= C::SCALES) ok = wait(&sm.sc_empty[slot], kt / C::SCALES - 1);
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int id = i ? id1 : id0, key = w.x.first_key + tile * PT_KT + t + 64 * i;
+              const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
+              const int64_t at = there ? ((int64_t)id * a.n_kv + w.h) * a.page + (key & (a.page - 1)) : 0;
+              const int bytes = there ? 4 : 0;           // (none: 4 bytes of zeros)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                           ::"r"(smem_addr_u32(&sm.scale[slot][0][t + 64 * i])), "l"(a.ks + at), "r"(bytes) : "memory");
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                           ::"r"(smem_addr_u32(&sm.scale[slot][1][t + 64 * i])), "l"(a.vs + at), "r"(bytes) : "memory");
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr_u32(&sm.sc_full[slot])) : "memory");
+            id0 = n0;
+            id1 = n1;
+          }
+        }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else if (warp < 12) {
     // ------------------------------ softmax and the items' ends: a row per thread -----------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::Q8 ? 184 : 208));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFT));
     const int x = (warp >> 2) - 1, r = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + 128u * x + lane_base, tO = tmem + 256u + lane_base;
-    const bool flip = a.scale < 0.f;
     const float sc = fmaxf(fabsf(a.scale), 1e-30f);      // (not 0: a masked logit is -inf)
     const float raise = 8.f / sc;
     bool ok = true;
     int n = 0, kt = 0;                                   // tiles of this warpgroup; key tiles of the CTA
-    PgRecord rec = {};
+    bool part = false;                                   // the CTA's last item goes on in the next one
     for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid(); w.next()) {
       const bool pair = w.x.rows > PT_R / 2;
       const int ri = pair ? x * 128 + r : r;             // row of the item
       const bool live = ri < w.x.rows;
-      const int64_t row = (int64_t)w.block * PT_R + ri, tok = row / a.G, pos = w.s.t0 + tok;
-      const int64_t key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos + 1, w.s.kv);      // the keys of the row
+      const int row = w.block * PT_R + ri, tok = row / a.G;
+      const int2 keys = pg_sees(w.s, a.G, a.window, row);      // those of the row
       float m = -INFINITY, l = 0.f;
       for (int s = 0; s < w.count; ++s, ++n) {
         const int tile = pair ? w.first + s : 2 * (w.first + s) + x;
-        const int64_t key0 = w.x.first_key + (int64_t)tile * PT_KT;
-        const int lo = (int)max(min(key_lo - key0, (int64_t)PT_KT), (int64_t)0), hi = (int)max(min(key_hi - key0, (int64_t)PT_KT), (int64_t)0);
-        const bool whole = __all_sync(0xffffffffu, !live || (lo == 0 && hi == PT_KT)), none = __all_sync(0xffffffffu, !live || hi <= lo);
+        const int key0 = w.x.first_key + tile * PT_KT, lo = keys.x - key0, hi = keys.y - key0;
+        const bool whole = __all_sync(0xffffffffu, !live || (lo <= 0 && hi >= PT_KT)), none = __all_sync(0xffffffffu, !live || hi <= max(lo, 0) || lo >= PT_KT);
         const int slot = (pair ? kt : kt + x) % C::SCALES, turn = (pair ? kt : kt + x) / C::SCALES;
         kt += pair ? 1 : 2;
         if (ok) ok = wait(&sm.s_full[x], n);
         if (C::Q8 && ok) ok = wait(&sm.sc_full[slot], turn);
         ok = __all_sync(0xffffffffu, ok);
         t5_fence_after();
-        uint32_t pk[64];
         if (none || !ok) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) pk[e] = 0u;
+          const uint32_t zero[32] = {};
+          t5_st32(tS, zero);
+          t5_st32(tS + 32u, zero);
         } else {
-          uint32_t sv[128];
+          // The row's scores come from tensor memory twice, in halves: for the maximum, and for P.  Kept in registers they would
+          // be 128 of them, and both passes unrolled: the code of all roles then outgrows the instruction cache, and a tile took
+          // 3000 cycles (8-bit pages: 7000) where its arithmetic is ~1200.
+          uint32_t sv[64];
+          const float4* ks = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][0]);
+          const float4* vs = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][1]);
+          auto fetch = [&](int k) {                      // 64 scores, scaled and masked
+            t5_ld32(tS + 64u * k, *reinterpret_cast<uint32_t(*)[32]>(sv));
+            t5_ld32(tS + 64u * k + 32u, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+            t5_wait_ld();
+            if (C::Q8) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) t5_ld32(tS + 32u * k, *reinterpret_cast<uint32_t(*)[32]>(sv + 32 * k));
-          t5_wait_ld();
-          if (C::Q8) {
-            const float4* ks = reinterpret_cast<const float4*>(sm.scale[slot][0]);
+              for (int e = 0; e < 16; ++e) {
+                const float4 f = ks[16 * k + e];
+                sv[4 * e] = __float_as_uint(__uint_as_float(sv[4 * e]) * f.x);
+                sv[4 * e + 1] = __float_as_uint(__uint_as_float(sv[4 * e + 1]) * f.y);
+                sv[4 * e + 2] = __float_as_uint(__uint_as_float(sv[4 * e + 2]) * f.z);
+                sv[4 * e + 3] = __float_as_uint(__uint_as_float(sv[4 * e + 3]) * f.w);
+              }
+            }
+            if (!whole) {
+              const uint32_t m0 = pt_range(lo - 64 * k, hi - 64 * k), m1 = pt_range(lo - 64 * k - 32, hi - 64 * k - 32);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float4 f = ks[k];
-              sv[4 * k] = __float_as_uint(__uint_as_float(sv[4 * k]) * f.x);
-              sv[4 * k + 1] = __float_as_uint(__uint_as_float(sv[4 * k + 1]) * f.y);
-              sv[4 * k + 2] = __float_as_uint(__uint_as_float(sv[4 * k + 2]) * f.z);
-              sv[4 * k + 3] = __float_as_uint(__uint_as_float(sv[4 * k + 3]) * f.w);
+              for (int e = 0; e < 32; ++e) {
+                sv[e] = m0 & (1u << e) ? sv[e] : 0xFF800000u;
+                sv[32 + e] = m1 & (1u << e) ? sv[32 + e] : 0xFF800000u;
+              }
+            }
+          };
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            fetch(k);
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+              t0 = fmaxf(t0, fmaxf(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])));
+              t1 = fmaxf(t1, fmaxf(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])));
             }
           }
-          if (flip) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e) sv[e] ^= 0x80000000u;
-          }
-          if (!whole) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t mk = pt_range(lo - 32 * k, hi - 32 * k);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sv[32 * k + e] = mk & (1u << e) ? sv[32 * k + e] : 0xFF800000u;
-            }
-          }
-          float t0 = __uint_as_float(sv[0]), t1 = __uint_as_float(sv[1]), t2 = __uint_as_float(sv[2]), t3 = __uint_as_float(sv[3]);
-#pragma unroll
-          for (int e = 4; e < 128; e += 4) {
-            t0 = fmaxf(t0, __uint_as_float(sv[e]));
-            t1 = fmaxf(t1, __uint_as_float(sv[e + 1]));
-            t2 = fmaxf(t2, __uint_as_float(sv[e + 2]));
-            t3 = fmaxf(t3, __uint_as_float(sv[e + 3]));
-          }
-          const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+          const float top = fmaxf(t0, t1);
           if (s == 0) m = top;
-          else if (__any_sync(0xffffffffu, top > m + raise)) {
-            const float now = fmaxf(m, top), keep = now == -INFINITY ? 1.f : ex2_fast((m - now) * sc);
+          else if (__any_sync(0xffffffffu, live && top > m + raise)) {
+            // (each row by itself: neither the other rows nor what lies in unused ones changes a result's bits)
+            const float now = top > m + raise ? top : m, keep = now == m ? 1.f : ex2_fast((m - now) * sc);
             m = now;
             l *= keep;
             if (ok) ok = wait(&sm.pv_done[x], n - 1);
             ok = __all_sync(0xffffffffu, ok);
             t5_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < D / 32; ++k) {
               uint32_t ov[32];
               t5_ld32(tO + 128u * x + 32u * k, ov);
@@ -412,26 +461,29 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           const float shift = m == -INFINITY ? 0.f : m * sc;
           const uint64_t sc2 = pt_pack(sc, sc), sh2 = pt_pack(-shift, -shift);
           uint64_t sum2 = 0;
-          const float4* vs = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][1]);
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            fetch(k);                                    // (P of the first half lies over scores that have been read)
+            uint32_t pk[32];
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            float x0, x1;
-            pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
-            float p0 = ex2_fast(x0), p1 = ex2_fast(x1);
-            sum2 = pt_add2(sum2, pt_pack(p0, p1));
-            if (C::Q8) {
-              const float4 f = vs[e >> 1];
-              p0 *= e & 1 ? f.z : f.x;
-              p1 *= e & 1 ? f.w : f.y;
+            for (int e = 0; e < 32; ++e) {
+              float x0, x1;
+              pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
+              float p0 = ex2_fast(x0), p1 = ex2_fast(x1);
+              sum2 = pt_add2(sum2, pt_pack(p0, p1));
+              if (C::Q8) {
+                const float4 f = vs[16 * k + (e >> 1)];
+                p0 *= e & 1 ? f.z : f.x;
+                p1 *= e & 1 ? f.w : f.y;
+              }
+              pk[e] = pack2_bf16(p0, p1);
             }
-            pk[e] = pack2_bf16(p0, p1);
+            t5_st32(tS + 32u * k, pk);
           }
           float la, lb;
           pt_unpack(sum2, la, lb);
           l += la + lb;
         }
-        t5_st32(tS, *reinterpret_cast<const uint32_t(*)[32]>(pk));
-        t5_st32(tS + 32u, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
         t5_wait_st();
         t5_fence_before();
         __syncwarp();
@@ -460,7 +512,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       t5_fence_after();
       const bool direct = w.starts() && w.ends();
       const float shift = mm == -INFINITY ? 0.f : mm * sc;
-      const int head = w.h * a.G + (int)(row - tok * a.G);
+      const int head = w.h * a.G + row - tok * a.G;
       float f = 1.f;
       if (direct && live) {
         float below = l;
@@ -468,10 +520,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         f = l == 0.f ? 0.f : 1.f / below;
       }
       float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(slot_rows, D);
-      bf16* orow = (bf16*)a.out + ((w.s.row0 + tok) * (int64_t)(a.n_kv * a.G) + head) * D;
+      bf16* orow = (bf16*)a.out + ((int64_t)(w.s.row0 + tok) * (a.n_kv * a.G) + head) * D;
       const int c0 = pair ? 0 : x * (D / 2), c1 = pair ? D : c0 + D / 2;
       float odd = 0.f;                                   // 0 unless a value of the row is not finite
       // (a pass before the stores: a row that is not finite is summed again instead of being stored)
+#pragma unroll 1
       for (int col = c0; col < c1; col += 32) {
         uint32_t ov[32];
         t5_ld32(tO + (pair ? 128u * x : 0u) + col, ov);
@@ -511,76 +564,67 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       unsigned redo = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
       if (redo) {
         __syncwarp();
-        const int64_t part0 = w.x.first_key + (int64_t)w.first * PT_KT * (pair ? 1 : 2), part1 = part0 + (int64_t)w.count * PT_KT * (pair ? 1 : 2);
+        const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
         while (redo) {
           const int src = __ffs(redo) - 1;
           redo &= redo - 1;
-          const int64_t rr = __shfl_sync(0xffffffffu, row, src), lo = __shfl_sync(0xffffffffu, key_lo, src), hi = __shfl_sync(0xffffffffu, key_hi, src);
+          const int rr = __shfl_sync(0xffffffffu, row, src), lo = __shfl_sync(0xffffffffu, keys.x, src), hi = __shfl_sync(0xffffffffu, keys.y, src);
           const float sh = __shfl_sync(0xffffffffu, shift, src), ff = __shfl_sync(0xffffffffu, f, src);
-          const int64_t tk = rr / a.G;
-          const int hd = w.h * a.G + (int)(rr - tk * a.G), ir = (int)(rr - (int64_t)w.block * PT_R);
-          pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (int64_t)hd * D, max(max(lo, part0), (int64_t)0), min(hi, part1),
-                               flip ? -sc : sc, sh, ff, (bf16*)a.out + ((w.s.row0 + tk) * (int64_t)(a.n_kv * a.G) + hd) * D,
+          const int tk = rr / a.G, hd = w.h * a.G + rr - tk * a.G, ir = rr - w.block * PT_R;
+          pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + hd * D, max(lo, part0), min(hi, part1),
+                               a.scale < 0.f ? -sc : sc, sh, ff, (bf16*)a.out + ((int64_t)(w.s.row0 + tk) * (a.n_kv * a.G) + hd) * D,
                                direct ? nullptr : slot + (int64_t)ir * D, c0, c1);
         }
       }
       t5_fence_before();
       if (!pair) asm volatile("bar.sync 1, 256;" ::: "memory");        // both have read O of both
       if (w.starts() && !w.ends()) {
-        rec.valid = 1; rec.b = w.b; rec.h = w.h; rec.block = w.block; rec.rows = w.x.rows; rec.row0 = w.s.row0;
-        rec.last = (int)((place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per);
+        part = true;
+        if (tid == 128)
+          a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)((place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
+                                   w.x.rows, w.s.row0};
       }
     }
-    if (tid == 128) a.records[blockIdx.x] = rec;
+    if (tid == 128 && !part) a.records[blockIdx.x].valid = 0;
   } else {
     // ------------------------------ 8-bit pages: payloads to bf16 tiles, scales ------------------------------------------------
     if constexpr (C::Q8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(80));
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
       const int t = tid - 384;
       bool ok = true;
-      int g = 0, kt = 0;
+      int g = 0;
       for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next()) {
-        ok = tiles_of(w, [&](int tile, bool v) {
-          const int64_t key = w.x.first_key + (int64_t)tile * PT_KT + t;
-          float fk = 0.f, fv = 0.f;                      // (0 behind the end: a scale there may be anything)
-          if (!v && tile < w.x.tiles && key < w.s.kv) {
-            const int64_t pg = __ldg(a.bt.table + w.b * a.bt.ld_table + (key >> a.bt.shift));
-            if (pg >= 0 && pg < a.bt.num_pages) {
-              const int64_t srow = (pg * a.n_kv + w.h) * a.page + (key & (a.page - 1));
-              fk = __ldg(a.ks + srow);
-              fv = __ldg(a.vs + srow);
-            }
-          }
-          bool fine = wait(&sm.raw_full[g % C::RAWS], g / C::RAWS);
-          if (fine && g >= C::STAGES) fine = wait(&sm.empty[g % C::STAGES], g / C::STAGES - 1);
-          if (fine && !v && kt >= C::SCALES) fine = wait(&sm.sc_empty[kt % C::SCALES], kt / C::SCALES - 1);
-          fine = __all_sync(0xffffffffu, fine);
-          if (!fine) return false;
+        const int tiles = 2 * w.count * (w.x.rows > PT_R / 2 ? 1 : 2);       // of keys and values
+        for (int i = 0; i < tiles && ok; ++i, ++g) {
+          ok = wait(&sm.raw_full[g % C::RAWS], g / C::RAWS);
+          if (ok && g >= C::STAGES) ok = wait(&sm.empty[g % C::STAGES], g / C::STAGES - 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           const uint8_t* src = sm.raw[g % C::RAWS];
           uint8_t* dst = sm.kv[g % C::STAGES];
-          constexpr int PIECES = D / 8;                  // 8 codes each: 16 bytes of a tile's row
-#pragma unroll 4
-          for (int i = t; i < PT_KT * PIECES; i += 128) {
-            const int row = i / PIECES, k = i % PIECES;
-            const uint2 u = *reinterpret_cast<const uint2*>(src + row * D + k * 8);
-            uint4 o;
-            pt_codes4<KIND>(u.x, o.x, o.y);
-            pt_codes4<KIND>(u.y, o.z, o.w);
-            *reinterpret_cast<uint4*>(dst + (k >> 3) * (PT_KT * 128) + row * 128 + (((k & 7) ^ (row & 7)) << 4)) = o;
-          }
-          if (!v) {
-            sm.scale[kt % C::SCALES][0][t] = fk;
-            sm.scale[kt % C::SCALES][1][t] = fv;
-            mbarrier_arrive(&sm.sc_full[kt % C::SCALES]);
-            ++kt;
+          constexpr int PIECES = D / 16, ROUNDS = PT_KT * PIECES / 128;       // 16 codes each: 2 words of a tile's row
+          uint4 u[ROUNDS];
+#pragma unroll
+          for (int n = 0; n < ROUNDS; ++n) u[n] = *reinterpret_cast<const uint4*>(src + (n * 128 + t) * 16);
+#pragma unroll
+          for (int n = 0; n < ROUNDS; ++n) {
+            const int row = (n * 128 + t) / PIECES, k = (n * 128 + t) % PIECES;
+            uint4 lo, hi;
+            pt_codes4<KIND>(u[n].x, lo.x, lo.y);
+            pt_codes4<KIND>(u[n].y, lo.z, lo.w);
+            pt_codes4<KIND>(u[n].z, hi.x, hi.y);
+            pt_codes4<KIND>(u[n].w, hi.z, hi.w);
+            uint8_t* line = dst + (k >> 2) * (PT_KT * 128) + row * 128;
+            const int first = (2 * (k & 3)) ^ (row & 7);                     // (the second panel's threads store in the other
+            const bool turn = k >> 2;                                        // order: no two of a row meet in a bank)
+            *reinterpret_cast<uint4*>(line + ((turn ? first ^ 1 : first) << 4)) = turn ? hi : lo;
+            *reinterpret_cast<uint4*>(line + ((turn ? first : first ^ 1) << 4)) = turn ? lo : hi;
           }
           t5_fence_async_smem();
           mbarrier_arrive(&sm.full[g % C::STAGES]);
           __syncwarp();
           if (lane == 0) mbarrier_arrive(&sm.raw_empty[g % C::RAWS]);
-          ++g;
-          return true;
-        });
+        }
       }
     }
   }

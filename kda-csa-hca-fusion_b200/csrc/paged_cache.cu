@@ -32,8 +32,9 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b) {
   PgBatch a;
   a.table = b->table; a.ld_table = b->ld_table; a.t0 = b->t0; a.cu = b->cu_seqlens;
-  a.B = b->B; a.N = b->N;
-  a.cap = (int64_t)b->max_pages * p->page_size;
+  a.B = b->B; a.N = (int)b->N;
+  const int64_t cap = (int64_t)b->max_pages * p->page_size;
+  a.cap = (int)(cap < 0x7FFFFE00LL ? cap : 0x7FFFFE00LL);      // positions, and the ends of their tiles, in 32 bits
   a.num_pages = p->num_pages;
   a.shift = 0;
   while ((1 << a.shift) < p->page_size) ++a.shift;
@@ -88,7 +89,7 @@ __device__ __forceinline__ int64_t pc_site(const PgRows& a, const int32_t* cu, i
   }
   const int64_t pos = max((int64_t)__ldg(a.bt.t0 + lo), (int64_t)0) + (t - cu[lo]);
   if (pos >= a.bt.cap) { pg_bad(a.bt); return -2; }
-  const int64_t pg = pg_page(a.bt, lo, pos >> a.bt.shift);
+  const int64_t pg = pg_page(a.bt, lo, (int)(pos >> a.bt.shift));
   return pg < 0 ? -2 : (pg * a.n_kv + h) * a.page + (pos & (a.page - 1));
 }
 
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(PgRows a) {
     __syncthreads();
     cu = scu;
   }
-  const int64_t rows = a.bt.N * a.n_kv * 2, groups = (int64_t)gridDim.x * (PC_THREADS / GROUP);
+  const int64_t rows = (int64_t)a.bt.N * a.n_kv * 2, groups = (int64_t)gridDim.x * (PC_THREADS / GROUP);
   const int g = threadIdx.x % GROUP, d = g * W;
   const int64_t first = (int64_t)blockIdx.x * (PC_THREADS / GROUP) + threadIdx.x / GROUP;
   // (all threads of a warp take the same number of rounds: the maximum is found by shuffles)
