@@ -25,7 +25,19 @@ struct PgBatch {
   int64_t num_pages;
   int shift;                           // log2(page_size)
   unsigned int* status;
+  int n_kv, G, window;                 // key heads, query heads of one, window (attention only)
+  uint32_t g_mul; int g_shift;         // n / G = n * g_mul >> 32 + g_shift for n < 2^31; g_mul 0: n >> g_shift
 };
+// With s = floor(log2 G) and M = floor(2^(32 + s) / G) + 1, M G exceeds 2^(32 + s) by at most G < 2^(s + 1): exact below 2^31.
+static inline void pg_set_group(PgBatch& a, int G) {
+  a.G = G;
+  a.g_shift = 0;
+  while ((2LL << a.g_shift) <= G) ++a.g_shift;
+  a.g_mul = (G & (G - 1)) == 0 ? 0u : (uint32_t)((1ULL << (32 + a.g_shift)) / (uint32_t)G + 1);
+}
+__device__ __forceinline__ int pg_token(const PgBatch& a, int row) {          // row / G
+  return a.g_mul ? (int)(__umulhi((uint32_t)row, a.g_mul) >> a.g_shift) : row >> a.g_shift;
+}
 
 struct PgSeq { int row0, len, t0, kv; };      // first packed row, new tokens, tokens before them, keys in all
 
@@ -49,25 +61,25 @@ __device__ __forceinline__ int pg_page(const PgBatch& a, int b, int index) {
 
 // One block of rows of a sequence: which keys its rows see together.
 struct PgSpan { int rows, first_key, tiles, steps; };   // tiles of KT keys from first_key (a multiple of KT) on
-// R rows a block, KT keys a tile; HALF: a block of at most R / 2 rows takes two tiles a step
-template <int R, int KT, bool HALF>
-__device__ __forceinline__ PgSpan pg_span(const PgSeq& s, int G, int window, int block) {
+// R rows a block, KT keys a tile.  TWO: blocks of at most TWO rows take two tiles a step.
+template <int R, int KT, int TWO>
+__device__ __forceinline__ PgSpan pg_span(const PgBatch& a, const PgSeq& s, int block) {
   PgSpan x;
-  const int r0 = block * R, r1 = min(r0 + R, s.len * G);
+  const int r0 = block * R, r1 = min(r0 + R, s.len * a.G);
   x.rows = r1 - r0;
-  const int64_t first = (int64_t)s.t0 + r0 / G, last = (int64_t)s.t0 + (r1 - 1) / G;      // positions of the first and the last query
-  const int lo = window > 0 ? (int)min(max(first - window + 1, (int64_t)0), (int64_t)s.kv) : 0, hi = (int)min(last + 1, (int64_t)s.kv);
+  const int64_t first = (int64_t)s.t0 + pg_token(a, r0), last = (int64_t)s.t0 + pg_token(a, r1 - 1);      // positions of the first and the last query
+  const int lo = a.window > 0 ? (int)min(max(first - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0, hi = (int)min(last + 1, (int64_t)s.kv);
   x.first_key = lo / KT * KT;
   x.tiles = hi > x.first_key ? (hi - x.first_key + KT - 1) / KT : 0;
-  x.steps = max(HALF && x.rows <= R / 2 ? (x.tiles + 1) / 2 : x.tiles, 1);  // (a row without keys is stored all the same)
+  x.steps = max(x.rows <= TWO ? (x.tiles + 1) / 2 : x.tiles, 1);            // (a row without keys is stored all the same)
   return x;
 }
 template <int R>
-__device__ __forceinline__ int pg_blocks(const PgSeq& s, int G) { return (s.len * G + R - 1) / R; }
+__device__ __forceinline__ int pg_blocks(const PgBatch& a, const PgSeq& s) { return (s.len * a.G + R - 1) / R; }
 // the keys [x, y) that row `row` (token * G + head of the group) of a sequence sees
-__device__ __forceinline__ int2 pg_sees(const PgSeq& s, int G, int window, int row) {
-  const int64_t pos = (int64_t)s.t0 + row / G;
-  return make_int2(window > 0 ? (int)min(max(pos - window + 1, (int64_t)0), (int64_t)s.kv) : 0, (int)min(pos + 1, (int64_t)s.kv));
+__device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int row) {
+  const int64_t pos = (int64_t)s.t0 + pg_token(a, row);
+  return make_int2(a.window > 0 ? (int)min(max(pos - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0, (int)min(pos + 1, (int64_t)s.kv));
 }
 
 struct PgPlace {                       // where a CTA's range of steps begins
@@ -75,81 +87,109 @@ struct PgPlace {                       // where a CTA's range of steps begins
   int b, h, block, step;
 };
 
+// steps of sequence b0 + lane (0 behind the last): by the lane where it is one block, as in a batch of single tokens, else by the
+// warp over its blocks
+template <int R, int KT, int TWO>
+__device__ __forceinline__ int64_t pg_steps(const PgBatch& a, int b0) {
+  const int lane = threadIdx.x & 31, b = b0 + lane;
+  PgSeq s = {0, 0, 0, 0};
+  if (b < a.B) {
+    s = pg_seq(a, b);
+    if ((int64_t)s.t0 + s.len > a.cap) pg_bad(a);
+  }
+  const int blocks = pg_blocks<R>(a, s);
+  int64_t mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps : 0;
+  for (unsigned many = __ballot_sync(0xffffffffu, blocks > 1); many; many &= many - 1) {
+    const int from = __ffs(many) - 1;
+    PgSeq t;
+    t.row0 = 0;
+    t.len = __shfl_sync(0xffffffffu, s.len, from);
+    t.t0 = __shfl_sync(0xffffffffu, s.t0, from);
+    t.kv = __shfl_sync(0xffffffffu, s.kv, from);
+    const int nb = pg_blocks<R>(a, t);
+    int64_t sum = 0;
+#pragma unroll 1
+    for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == from) mine = sum;
+  }
+  return mine * a.n_kv;
+}
+__device__ __forceinline__ int64_t pg_scan(int64_t x) {      // sums over the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((threadIdx.x & 31) >= o) x += y;
+  }
+  return x;
+}
+
 // The whole block calls it; `mem`: PG_PLAN_BYTES(B) of shared memory, free again after the next __syncthreads().
-#define PG_PLAN_BYTES(B) (16 + 8 * ((B) + 1))
-template <int R, int KT, bool HALF>
-__device__ PgPlace pg_plan(const PgBatch& a, int G, int n_kv, int window, void* mem, int cta, int ctas) {
-  int64_t* base = reinterpret_cast<int64_t*>(mem);          // [B + 1] steps before sequence b
-  int* found = reinterpret_cast<int*>(base + a.B + 1);
+#define PG_PLAN_BYTES(B) (32 + 8 * ((B) + 1))
+template <int R, int KT, int TWO>
+__device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  // steps of a sequence: a lane each where it is one block (a batch of single tokens), else a warp over its blocks
-  for (int b0 = warp * 32; b0 < a.B; b0 += warps * 32) {
-    const int b = b0 + lane;
-    PgSeq s = {0, 0, 0, 0};
-    if (b < a.B) s = pg_seq(a, b);
-    const int blocks = pg_blocks<R>(s, G);
-    int64_t mine = blocks == 1 ? pg_span<R, KT, HALF>(s, G, window, 0).steps : 0;
-    unsigned many = __ballot_sync(0xffffffffu, blocks > 1);
-    while (many) {
-      const int from = __ffs(many) - 1;
-      many &= many - 1;
-      PgSeq t;
-      t.row0 = 0;
-      t.len = __shfl_sync(0xffffffffu, s.len, from);
-      t.t0 = __shfl_sync(0xffffffffu, s.t0, from);
-      t.kv = __shfl_sync(0xffffffffu, s.kv, from);
-      const int nb = __shfl_sync(0xffffffffu, blocks, from);
-      int64_t sum = 0;
-      for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, HALF>(t, G, window, i).steps;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == from) mine = sum;
-    }
-    if (b < a.B) base[b + 1] = mine * n_kv;
-    if (b < a.B && (int64_t)s.t0 + s.len > a.cap) pg_bad(a);
-  }
-  if (tid == 0) { base[0] = 0; found[0] = -1; }
-  __syncthreads();
-  if (warp == 0) {
-    int64_t run = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int b = b0 + lane;
-      int64_t x = b < a.B ? base[b + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (b < a.B) base[b + 1] = run + x;
-      run += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
-  __syncthreads();
   PgPlace p = {};
-  const int64_t total = base[a.B];
-  p.per = max((total + ctas - 1) / ctas, (int64_t)1);
-  const int64_t start = p.per * cta;
-  p.left = max(min(p.per, total - start), (int64_t)0);
-  if (p.left > 0)
-    for (int b = tid; b < a.B; b += blockDim.x)
-      if (base[b] <= start && start < base[b + 1]) found[0] = b;
-  __syncthreads();
-  if (p.left > 0) {                    // every warp finds the block by itself
-    p.b = found[0];
+  int64_t total, before = 0, mine = 0;                      // steps: of all, before sequence p.b, of it
+  auto range = [&] {
+    p.per = max((total + ctas - 1) / ctas, (int64_t)1);
+    p.left = max(min(p.per, total - p.per * cta), (int64_t)0);
+    return p.per * cta;
+  };
+  if (a.B <= 32) {                     // every warp by itself: no memory, no barrier
+    const int64_t x = pg_steps<R, KT, TWO>(a, 0), upto = pg_scan(x);
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    const int64_t start = range();
+    const unsigned hit = __ballot_sync(0xffffffffu, upto > start);
+    if (p.left > 0) {
+      p.b = __ffs(hit) - 1;
+      mine = __shfl_sync(0xffffffffu, x, p.b);
+      before = __shfl_sync(0xffffffffu, upto, p.b) - mine;
+    }
+  } else {
+    int64_t* base = reinterpret_cast<int64_t*>(mem);        // [B + 1] steps before sequence b
+    int* found = reinterpret_cast<int*>(base + a.B + 1);
+#pragma unroll 1
+    for (int b0 = warp * 32; b0 < a.B; b0 += warps * 32) {
+      const int64_t x = pg_steps<R, KT, TWO>(a, b0);
+      if (b0 + lane < a.B) base[b0 + lane + 1] = x;
+    }
+    if (tid == 0) base[0] = 0;
+    __syncthreads();
+    if (warp == 0) {
+      int64_t run = 0;
+#pragma unroll 1
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int64_t x = run + pg_scan(b0 + lane < a.B ? base[b0 + lane + 1] : 0);
+        if (b0 + lane < a.B) base[b0 + lane + 1] = x;
+        run = __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
+    __syncthreads();
+    total = base[a.B];
+    const int64_t start = range();
+    if (p.left > 0)
+      for (int b = tid; b < a.B; b += blockDim.x)
+        if (base[b] <= start && start < base[b + 1]) found[0] = b;
+    __syncthreads();
+    if (p.left > 0) {
+      p.b = found[0];
+      before = base[p.b];
+      mine = base[p.b + 1] - before;
+    }
+  }
+  if (p.left > 0) {                    // the key head, then the block, by every warp
     const PgSeq s = pg_seq(a, p.b);
-    const int blocks = pg_blocks<R>(s, G);
-    const int64_t head = (base[p.b + 1] - base[p.b]) / n_kv;
-    p.h = (int)((start - base[p.b]) / head);
-    int64_t rest = start - base[p.b] - p.h * head;
+    const int blocks = pg_blocks<R>(a, s);
+    int64_t rest = p.per * cta - before;
+    const int64_t head = mine / a.n_kv;
+    if (a.n_kv > 1) p.h = (int)(rest / head);
+    rest -= p.h * head;
+#pragma unroll 1
     for (int i0 = 0; i0 < blocks; i0 += 32) {
       const int i = i0 + lane;
-      const int64_t n = i < blocks ? pg_span<R, KT, HALF>(s, G, window, i).steps : 0;
-      int64_t x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
+      const int64_t n = i < blocks ? pg_span<R, KT, TWO>(a, s, i).steps : 0, x = pg_scan(n);
       const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
       if (hit) {
         const int at = __ffs(hit) - 1;
@@ -164,17 +204,16 @@ __device__ PgPlace pg_plan(const PgBatch& a, int G, int n_kv, int window, void* 
 }
 
 // The items of a CTA, one after the other; every role of a kernel walks them by itself.
-template <int R, int KT, bool HALF>
+template <int R, int KT, int TWO>
 struct PgWalk {
   const PgBatch& a;
-  int G, n_kv, window;
   int b, h, block;                     // the item
   int first, count;                    // its steps that belong to this CTA
   PgSeq s;
   PgSpan x;
   int64_t left;                        // steps of the CTA behind them
-  __device__ __forceinline__ PgWalk(const PgBatch& a_, int G_, int n_kv_, int window_, const PgPlace& p)
-      : a(a_), G(G_), n_kv(n_kv_), window(window_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), left(p.left) {
+  __device__ __forceinline__ PgWalk(const PgBatch& a_, const PgPlace& p)
+      : a(a_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), left(p.left) {
     if (left > 0) {
       s = pg_seq(a, b);
       open();
@@ -187,9 +226,9 @@ struct PgWalk {
     first = 0;
     count = 0;
     if (left <= 0) return;
-    if (++block == pg_blocks<R>(s, G)) {
+    if (++block == pg_blocks<R>(a, s)) {
       block = 0;
-      if (++h == n_kv) {
+      if (++h == a.n_kv) {
         h = 0;
         do { s = pg_seq(a, ++b); } while (s.len == 0);       // (steps are left, so a sequence with rows follows)
       }
@@ -199,7 +238,7 @@ struct PgWalk {
 
  private:
   __device__ __forceinline__ void open() {
-    x = pg_span<R, KT, HALF>(s, G, window, block);
+    x = pg_span<R, KT, TWO>(a, s, block);
     count = (int)min((int64_t)(x.steps - first), left);
     left -= count;
   }
@@ -225,7 +264,7 @@ struct PgAttend {                      // what both attention kernels get
   const void *q, *k, *v; const float *ks, *vs;
   void* out;
   int64_t ld_q;
-  int n_kv, G, c, page, window, zero_rest, slot_rows;
+  int c, page, zero_rest, slot_rows;
   float scale;                         // times log2(e)
   const void* sink; int sink_dtype;
   PgRecord* records; float* slots;
@@ -235,7 +274,7 @@ struct PgAttend {                      // what both attention kernels get
 __device__ __forceinline__ void pg_zero_rest(const PgAttend& a, int es, int cta, int ctas) {
   if (!a.zero_rest) return;
   const int64_t lo = min(max(__ldg(a.bt.cu), 0), a.bt.N), hi = min(max(__ldg(a.bt.cu + a.bt.B), (int)lo), a.bt.N);
-  const int64_t row = (int64_t)a.n_kv * a.G * a.c * es / 16, words = (lo + a.bt.N - hi) * row;      // 16-byte words of a token
+  const int64_t row = (int64_t)a.bt.n_kv * a.bt.G * a.c * es / 16, words = (lo + a.bt.N - hi) * row;      // 16-byte words of a token
   for (int64_t i = (int64_t)cta * blockDim.x + threadIdx.x; i < words; i += (int64_t)ctas * blockDim.x) {
     const int64_t t = i / row, at = (t < lo ? t : hi + t - lo) * row + i % row;
     reinterpret_cast<uint4*>(a.out)[at] = make_uint4(0u, 0u, 0u, 0u);

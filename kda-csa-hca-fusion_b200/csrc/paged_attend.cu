@@ -67,12 +67,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
   float* sq = reinterpret_cast<float*>(pa_mem);
   float *sk = sq + ROWS * LD, *sv = sk + PA_KT * LD, *sp = sv + PA_KT * LD, *sm = sp + ROWS * LS, *sl = sm + ROWS, *sa = sl + ROWS;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, c = a.c, c8 = c >> 3;
-  const PgPlace place = pg_plan<ROWS, PA_KT, false>(a.bt, a.G, a.n_kv, a.window, pa_mem, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<ROWS, PA_KT, 0>(a.bt, pa_mem, blockIdx.x, gridDim.x);
   pg_zero_rest(a, sizeof(T), blockIdx.x, gridDim.x);
   __syncthreads();
   for (int i = tid; i < (ROWS + 2 * PA_KT) * LD; i += PA_THREADS) sq[i] = 0.f;      // columns c .. DMAX of all three stay 0
   PgRecord rec = {};
-  PgWalk<ROWS, PA_KT, false> w(a.bt, a.G, a.n_kv, a.window, place);
+  const int G = a.bt.G, n_kv = a.bt.n_kv;
+  PgWalk<ROWS, PA_KT, 0> w(a.bt, place);
   for (; w.valid(); w.next()) {
     const int r0 = w.block * ROWS;                             // first (token, head) row of the block in its sequence
     __syncthreads();
@@ -80,8 +81,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
       const int r = i / c8, d = i % c8 * 8;
       float x[8] = {};
       if (r < w.x.rows) {
-        const int t = (r0 + r) / a.G;
-        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * a.G + r0 + r - t * a.G) * c + d, x);
+        const int t = pg_token(a.bt, r0 + r);
+        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * G + r0 + r - t * G) * c + d, x);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq[r * LD + d + e] = x[e];
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         if (pos < w.s.kv) {
           const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
           if (pg >= 0) {
-            const int64_t row = (pg * a.n_kv + w.h) * a.page + (pos & (a.page - 1));
+            const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));
             PgStored<P>::load(a.k, row * c + d, kx);
             PgStored<P>::load(a.v, row * c + d, vx);
             if (PgStored<P>::ES == 1) {
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
         const int r = ty + 16 * i;
-        const int2 keys = r < w.x.rows ? pg_sees(w.s, a.G, a.window, r0 + r) : make_int2(0, 0);
+        const int2 keys = r < w.x.rows ? pg_sees(a.bt, w.s, r0 + r) : make_int2(0, 0);
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
       }
       // A key that a row does not see must not reach it: 0 times an infinity or a NaN is no 0.  In a tile where every row
       // sees every key nothing is to be skipped.
-      const bool whole = key0 >= pg_sees(w.s, a.G, a.window, r0 + w.x.rows - 1).x && key0 + PA_KT <= pg_sees(w.s, a.G, a.window, r0).y;
+      const bool whole = key0 >= pg_sees(a.bt, w.s, r0 + w.x.rows - 1).x && key0 + PA_KT <= pg_sees(a.bt, w.s, r0).y;
       auto product = [&](auto masked) {
         for (int j = 0; j < PA_KT; ++j) {
           float p[RT];
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     for (int i = 0; i < RT; ++i) {
       const int r = ty + 16 * i;
       if (r >= w.x.rows) continue;
-      const int t = (r0 + r) / a.G, h = w.h * a.G + r0 + r - t * a.G;
+      const int t = pg_token(a.bt, r0 + r), h = w.h * G + r0 + r - t * G;
       float f = 1.f;
       if (direct) {
         const float m = sm[r], l = sl[r];
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - m);
         f = l == 0.f ? 0.f : 1.f / below;
       }
-      T* orow = (T*)a.out + ((int64_t)(w.s.row0 + t) * (a.n_kv * a.G) + h) * c;
+      T* orow = (T*)a.out + ((int64_t)(w.s.row0 + t) * (n_kv * G) + h) * c;
 #pragma unroll
       for (int x = 0; x < CT; ++x) {
         const int d = tx * 4 + 64 * x;
@@ -377,7 +378,7 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c);
-int kch_paged_attend_tc5(const PgAttend& a, int kind, int ctas, cudaStream_t s);
+int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.
 struct PaPlan { bool tc5; int rows, ctas, slot_rows; };
@@ -385,7 +386,9 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   PaPlan x;
   const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
   x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
-  x.rows = x.tc5 ? 256 : rows <= 16 * (int64_t)p->batch.B ? 16 : 64;
+  const int64_t B = p->batch.B;
+  if (x.tc5) x.rows = rows <= 32 * B && p->batch.N <= 4 * B ? 32 : 256;
+  else x.rows = rows <= 16 * B ? 16 : 64;
   x.ctas = x.tc5 ? KCH_SMS : PA_CTAS;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
@@ -420,8 +423,9 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.bt = kch_paged_batch_of(&p->cache, &p->batch);
   KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
   a.q = p->q; a.k = p->cache.k; a.v = p->cache.v; a.ks = p->cache.k_scales; a.vs = p->cache.v_scales;
-  a.out = p->out; a.ld_q = p->ld_q; a.n_kv = n_kv; a.G = p->nh / n_kv; a.c = c; a.page = p->cache.page_size;
-  a.window = p->sliding_window; a.zero_rest = p->zero_rest;
+  a.out = p->out; a.ld_q = p->ld_q; a.c = c; a.page = p->cache.page_size; a.zero_rest = p->zero_rest;
+  a.bt.window = p->sliding_window;
+  pg_set_group(a.bt, p->nh / n_kv);
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   a.records = (PgRecord*)p->workspace;
@@ -429,9 +433,9 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;
   cudaStream_t s = kch_stream(stream);
-  const PgJoinArgs j = {a.out, p->dtype, p->nh, a.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
+  const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.tc5) {
-    const int rc5 = kch_paged_attend_tc5(a, p->cache.kind, x.ctas, s);
+    const int rc5 = kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
     return rc5 != KCH_OK ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);

@@ -1,11 +1,14 @@
 // Attention of new tokens over a paged cache on tcgen05 (bf16 activations, heads of 64 or 128; pages in bf16, e4m3 or int8).
 // Mathematics and division of the work: paged_attend.cu, paged.cuh.
 //
-// One persistent CTA an SM.  An item is up to 256 (token, head of the group) rows of a sequence against the key tiles of 128 that
-// they see; two softmax warpgroups X = 0, 1 of a row per thread work on
-//   rows 0..127 and 128..255 against the same key tile, where the item has more than 128 rows, or
-//   the same rows against the even and the odd key tiles (joined in tensor memory when the item ends), where it has not:
-//     a step of single tokens then has two tiles under way as well, and is bound by the loads of its keys.
+// One persistent CTA an SM; two softmax warpgroups X = 0, 1 of a row per thread.  An item is a block of (token, head of the group)
+// rows of a sequence against the key tiles of 128 that they see:
+//   chunks:  up to 256 rows, X = rows 0..127 and 128..255 against the same key tile; 128 rows or fewer: X = the even and the odd tiles;
+//   steps (FEW, where a sequence has few rows): up to 32 rows, X = the even and the odd tiles, and the rows lie in the 128 of the
+//     query tile four times: warp w of a warpgroup has a row per thread as well, but only keys 32 w .. 32 w + 31 of a tile (its
+//     probabilities of the others are 0), with a maximum, a sum and an O of its own.  One warp of four would have all the work
+//     otherwise, and a tile's softmax would be the longest link of the chain.
+// Parts of a row with sums of their own are joined through shared memory when the item ends.
 // Roles: warp 0 copies pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
 // issues  S_X = Q_X K^T  (M = N = 128) into 128 columns of tensor memory and  O_X += P_X V  with P_X, written by the softmax over
 // S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile; warps 2, 3 fetch the
@@ -25,12 +28,12 @@
 #include "paged.cuh"
 #include "tc5_utils.cuh"
 
-#define PT_R 256
 #define PT_KT 128
 #define PT_SPIN (1u << 22)
 
-template <int D, int KIND>
+template <int D, int KIND, bool FEW>
 struct PtCfg {
+  static constexpr int R = FEW ? 32 : 256, TWO = FEW ? 32 : 128, COPIES = FEW ? 4 : 1;
   static constexpr bool Q8 = KIND >= KCH_FP8_E4M3;
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
@@ -41,21 +44,23 @@ struct PtCfg {
   static_assert(128 * (REG_FEED * (Q8 ? 2 : 1) + 2 * REG_SOFT) <= (Q8 ? 65536 : 64512), "register split");
 };
 
-template <int D, int KIND>
+template <int D, int KIND, bool FEW>
 struct PtSmem {
-  typedef PtCfg<D, KIND> C;
+  typedef PtCfg<D, KIND, FEW> C;
   alignas(1024) uint8_t q[2][128 * D * 2];
   alignas(1024) uint8_t kv[C::STAGES][C::TILE];
   alignas(16) uint8_t raw[C::RAWS ? C::RAWS : 1][C::RAWS ? C::RAW : 16];      // (a multiple of 1024 before it)
   alignas(16) float scale[C::Q8 ? C::SCALES : 1][2][C::Q8 ? PT_KT : 4];
-  float ml[2][2][128];                                   // maximum and sum of either half of an item's keys
+  float ml[2][256];                                      // maxima and sums of the parts of an item's keys
+  float factor[128];                                     // of its rows: 1 / the denominator
+  uint32_t odd[4];                                       // rows of it that are not finite
   alignas(8) uint64_t full[C::STAGES], empty[C::STAGES];
   uint64_t raw_full[C::RAWS ? C::RAWS : 1], raw_empty[C::RAWS ? C::RAWS : 1];
   uint64_t sc_full[C::SCALES], sc_empty[C::SCALES];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2];
+  uint64_t q_full, q_empty, join_done, s_full[2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
-static_assert(sizeof(PtSmem<128, KCH_BF16>) <= 232448 && sizeof(PtSmem<128, KCH_INT8>) <= 232448, "shared memory of the paged attention");
+static_assert(sizeof(PtSmem<128, KCH_BF16, false>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, false>) <= 232448, "shared memory of the paged attention");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * 16384, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pt_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -72,6 +77,22 @@ __device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
 __device__ __forceinline__ void pt_arrive_n(uint64_t* bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr_u32(bar)), "r"(n) : "memory");
 }
+__device__ __forceinline__ void pt_st(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void pt_st(uint32_t taddr, const uint32_t (&r)[32]) { t5_st32(taddr, r); }
+__device__ __forceinline__ void pt_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pt_ld(uint32_t taddr, uint32_t (&r)[32]) { t5_ld32(taddr, r); }
 // pairs of fp32 values: one issue slot for two of them
 __device__ __forceinline__ uint64_t pt_pack(float x, float y) {
   uint64_t r;
@@ -117,11 +138,11 @@ __device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi
   }
 }
 
-// One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns c0 ..
-// c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).
+// One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift), to `dst` (fp32,
+// a part) or `out` (times f, rounded).
 template <int D, int KIND>
 __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int from, int to, float sc, float shift,
-                                         float f, bf16* out, float* dst, int c0, int c1) {
+                                         float f, bf16* out, float* dst) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
   float qv[E], o[E];
@@ -134,7 +155,7 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
   };
   for (int j = from; j < to; ++j) {
     const int64_t pg = pg_page(a.bt, b, j >> a.bt.shift);
-    const int64_t row = (pg * a.n_kv + h) * a.page + (j & (a.page - 1));
+    const int64_t row = (pg * a.bt.n_kv + h) * a.page + (j & (a.page - 1));
     float s = 0.f;
     if (pg >= 0) {
 #pragma unroll
@@ -152,37 +173,40 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane * E + e;
-    if (d < c0 || d >= c1) continue;
     if (dst) dst[d] = o[e]; else stf(out + d, o[e] * f);
   }
 }
 
-template <int D, int KIND>
-__global__ void __launch_bounds__(PtCfg<D, KIND>::THREADS, 1)
+template <int D, int KIND, bool FEW>
+__global__ void __launch_bounds__(PtCfg<D, KIND, FEW>::THREADS, 1)
 paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
-  const int slot_rows = a.slot_rows;
-  typedef PtCfg<D, KIND> C;
+  typedef PtCfg<D, KIND, FEW> C;
+  typedef PgWalk<C::R, PT_KT, C::TWO> Walk;
   extern __shared__ __align__(1024) uint8_t pt_raw[];    // (no room to align it by hand; every block begins its memory there)
-  PtSmem<D, KIND>& sm = *reinterpret_cast<PtSmem<D, KIND>*>(pt_raw);
+  PtSmem<D, KIND, FEW>& sm = *reinterpret_cast<PtSmem<D, KIND, FEW>*>(pt_raw);
   if (smem_addr_u32(pt_raw) & 1023) {
     if (threadIdx.x == 0) atomicCAS(a.bt.status, 0u, (unsigned)KCH_STATUS_PAGED_ATTEND);
     return;
   }
-  const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31;
+  const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 128 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, 64);
     mbarrier_init(&sm.q_empty, 1);
+    mbarrier_init(&sm.join_done, 8);
+    for (int i = 0; i < 4; ++i) sm.odd[i] = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr_u32(&sm.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const PgPlace place = pg_plan<PT_R, PT_KT, true>(a.bt, a.G, a.n_kv, a.window, sm.kv, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<C::R, PT_KT, C::TWO>(a.bt, sm.kv, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   t5_fence_before();
@@ -190,7 +214,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   t5_fence_after();
   const uint32_t tmem = sm.tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, PT_SPIN, a.bt.status); };
-  typedef PgWalk<PT_R, PT_KT, true> Walk;
+  // do the warpgroups have rows of their own, or the same rows and every other tile?
+  auto paired = [](const Walk& w) { return !FEW && w.x.rows > C::TWO; };
   // The ring holds an item's tiles in the order in which they are used.  Rows of both: K0, then V0 K1, V1 K2, ..; rows of one: K0 K1,
   // then V0 K2 V1 K3, V2 K4 V3 K5, ..
 
@@ -206,8 +231,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       uint64_t *fb = C::Q8 ? sm.raw_full : sm.full, *eb = C::Q8 ? sm.raw_empty : sm.empty;
       int g = 0;
       bool ok = true;
-      for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next()) {
-        const bool pair = w.x.rows > PT_R / 2;
+      for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
+        const bool pair = paired(w);
         const int per = pair ? 1 : 2, end = (w.first + w.count) * per;
         const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
         // the page of this lane's box of a tile, asked for a tile ahead; -1 behind the part's or the sequence's end
@@ -282,8 +307,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           t5_commit(&sm.pv_done[x]);                     // (behind it no arrival is under way that nobody waits for)
         };
         auto filled = [&](int i) { return wait(&sm.full[i % C::STAGES], i / C::STAGES); };
-        for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next(), ++c) {
-          const bool pair = w.x.rows > PT_R / 2;
+        for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
+          const bool pair = paired(w);
           ok = wait(&sm.q_full, c);
           for (int x = 0; x < 2 && ok; ++x) {            // the first scores
             if (!(pair && x)) ok = filled(g);
@@ -311,23 +336,36 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     } else {
       // ------------------------------ queries ------------------------------------------------------------------------------
       const int t = tid - 64;
-      int c = 0, kt = 0;
+      int c = 0, kt = 0, halves = 0, joined = 0;
       bool ok = true;
-      for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next(), ++c) {
+      for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
         if (c) ok = wait(&sm.q_empty, c - 1);
         if (!ok) break;
-        const int chunks = D / 8, rows = w.x.rows;
-        for (int i = t; i < rows * chunks; i += 64) {
-          const int r = i / chunks, k = i % chunks;
-          const int row = w.block * PT_R + r, tok = row / a.G;
-          const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * a.G + row - tok * a.G) * D + k * 8;
+        if (!FEW) {
+          // The second tile's memory joins the parts of items of few rows: all of those before have to be done with it, and the
+          // barrier is never left two phases behind.
+          const bool pair = paired(w);
+          for (; joined < (pair ? halves : halves - 1) && ok; ++joined) ok = wait(&sm.join_done, joined);
+          if (!ok) break;
+          halves += pair ? 0 : 1;
+        }
+        constexpr int CHUNKS = D / 8, STEP = 64 / CHUNKS;      // 16 bytes a thread
+        const int rows = w.x.rows, k = t % CHUNKS;
+#pragma unroll 1
+        for (int r = t / CHUNKS; r < rows; r += STEP) {
+          const int row = w.block * C::R + r, tok = pg_token(a.bt, row);
+          const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + k * 8;
           const uint32_t dst = smem_addr_u32(sm.q[r >> 7]) + (k >> 3) * (128 * 128) + (r & 127) * 128 + (((k & 7) ^ (r & 7)) << 4);
           if (a.scale < 0.f) {                           // (the softmax takes the scale's size: a maximum stays one)
             uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
             u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u;
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+#pragma unroll
+            for (int i = 0; i < C::COPIES; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (32 * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
           } else {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+#pragma unroll
+            for (int i = 0; i < C::COPIES; ++i)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (32 * 128)), "l"(src) : "memory");
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -336,7 +374,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         if constexpr (C::Q8) {
           // the scales of the item's key tiles: two keys a thread, 0 behind the end (a scale there may be anything); the page is
           // asked for a tile ahead, and the copies report to the barrier by themselves
-          const int per = rows > PT_R / 2 ? 1 : 2, end = (w.first + w.count) * per;
+          const int per = paired(w) ? 1 : 2, end = (w.first + w.count) * per;
           const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
           auto ask = [&](int tile, int i) -> int {
             const int key = w.x.first_key + tile * PT_KT + t + 64 * i;
@@ -351,7 +389,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             for (int i = 0; i < 2; ++i) {
               const int id = i ? id1 : id0, key = w.x.first_key + tile * PT_KT + t + 64 * i;
               const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
-              const int64_t at = there ? ((int64_t)id * a.n_kv + w.h) * a.page + (key & (a.page - 1)) : 0;
+              const int64_t at = there ? ((int64_t)id * n_kv + w.h) * a.page + (key & (a.page - 1)) : 0;
               const int bytes = there ? 4 : 0;           // (none: 4 bytes of zeros)
               asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
                            ::"r"(smem_addr_u32(&sm.scale[slot][0][t + 64 * i])), "l"(a.ks + at), "r"(bytes) : "memory");
@@ -377,17 +415,19 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     bool ok = true;
     int n = 0, kt = 0;                                   // tiles of this warpgroup; key tiles of the CTA
     bool part = false;                                   // the CTA's last item goes on in the next one
-    for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid(); w.next()) {
-      const bool pair = w.x.rows > PT_R / 2;
-      const int ri = pair ? x * 128 + r : r;             // row of the item
+    for (Walk w(a.bt, place); w.valid(); w.next()) {
+      const bool pair = paired(w);
+      constexpr int APART = 128 / C::COPIES;
+      const int ri = pair ? x * 128 + r : r % APART, sub = r / APART;      // row of the item, part of a tile's keys
       const bool live = ri < w.x.rows;
-      const int row = w.block * PT_R + ri, tok = row / a.G;
-      const int2 keys = pg_sees(w.s, a.G, a.window, row);      // those of the row
+      const int2 keys = pg_sees(a.bt, w.s, w.block * C::R + ri);           // those of the row
       float m = -INFINITY, l = 0.f;
       for (int s = 0; s < w.count; ++s, ++n) {
         const int tile = pair ? w.first + s : 2 * (w.first + s) + x;
         const int key0 = w.x.first_key + tile * PT_KT, lo = keys.x - key0, hi = keys.y - key0;
-        const bool whole = __all_sync(0xffffffffu, !live || (lo <= 0 && hi >= PT_KT)), none = __all_sync(0xffffffffu, !live || hi <= max(lo, 0) || lo >= PT_KT);
+        const int from = sub * APART, to = from + APART;
+        const bool whole = __all_sync(0xffffffffu, !live || (lo <= from && hi >= to));
+        const bool none = __all_sync(0xffffffffu, !live || min(hi, to) <= max(lo, from));
         const int slot = (pair ? kt : kt + x) % C::SCALES, turn = (pair ? kt : kt + x) / C::SCALES;
         kt += pair ? 1 : 2;
         if (ok) ok = wait(&sm.s_full[x], n);
@@ -396,23 +436,23 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         t5_fence_after();
         if (none || !ok) {
           const uint32_t zero[32] = {};
-          t5_st32(tS, zero);
-          t5_st32(tS + 32u, zero);
+          pt_st(tS, zero);
+          pt_st(tS + 32u, zero);
         } else {
-          // The row's scores come from tensor memory twice, in halves: for the maximum, and for P.  Kept in registers they would
-          // be 128 of them, and both passes unrolled: the code of all roles then outgrows the instruction cache, and a tile took
-          // 3000 cycles (8-bit pages: 7000) where its arithmetic is ~1200.
-          uint32_t sv[64];
+          // Chunks: the row's scores come from tensor memory twice, in halves: for the maximum, and for P.  Kept in registers they
+          // would be 128 of them, and both passes unrolled: the code of all roles then outgrows the instruction cache, and a tile
+          // took 3000 cycles (8-bit pages: 7000) where its arithmetic is ~1200.
           const float4* ks = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][0]);
           const float4* vs = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][1]);
-          auto fetch = [&](int k) {                      // 64 scores, scaled and masked
-            t5_ld32(tS + 64u * k, *reinterpret_cast<uint32_t(*)[32]>(sv));
-            t5_ld32(tS + 64u * k + 32u, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+          auto fetch = [&](auto& sv, int col) {          // 32 or 64 scores from column `col` on, scaled and masked
+            constexpr int N = sizeof(sv) / 4;
+#pragma unroll
+            for (int k = 0; k < N; k += 32) t5_ld32(tS + col + k, *reinterpret_cast<uint32_t(*)[32]>(sv + k));
             t5_wait_ld();
             if (C::Q8) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float4 f = ks[16 * k + e];
+              for (int e = 0; e < N / 4; ++e) {
+                const float4 f = ks[col / 4 + e];
                 sv[4 * e] = __float_as_uint(__uint_as_float(sv[4 * e]) * f.x);
                 sv[4 * e + 1] = __float_as_uint(__uint_as_float(sv[4 * e + 1]) * f.y);
                 sv[4 * e + 2] = __float_as_uint(__uint_as_float(sv[4 * e + 2]) * f.z);
@@ -420,22 +460,32 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               }
             }
             if (!whole) {
-              const uint32_t m0 = pt_range(lo - 64 * k, hi - 64 * k), m1 = pt_range(lo - 64 * k - 32, hi - 64 * k - 32);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                sv[e] = m0 & (1u << e) ? sv[e] : 0xFF800000u;
-                sv[32 + e] = m1 & (1u << e) ? sv[32 + e] : 0xFF800000u;
+              for (int k = 0; k < N; k += 32) {
+                const uint32_t mk = pt_range(lo - col - k, hi - col - k);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sv[k + e] = mk & (1u << e) ? sv[k + e] : 0xFF800000u;
               }
             }
           };
           float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll 1
-          for (int k = 0; k < 2; ++k) {
-            fetch(k);
+          auto highest = [&](const auto& sv) {
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
+            for (int e = 0; e < sizeof(sv) / 4; e += 4) {
               t0 = fmaxf(t0, fmaxf(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])));
               t1 = fmaxf(t1, fmaxf(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])));
+            }
+          };
+          uint32_t few[32];                              // (FEW: 32 keys a warp, which stay)
+          if constexpr (FEW) {
+            fetch(few, from);
+            highest(few);
+          } else {
+#pragma unroll 1
+            for (int col = 0; col < PT_KT; col += 64) {
+              uint32_t sv[64];
+              fetch(sv, col);
+              highest(sv);
             }
           }
           const float top = fmaxf(t0, t1);
@@ -461,24 +511,36 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           const float shift = m == -INFINITY ? 0.f : m * sc;
           const uint64_t sc2 = pt_pack(sc, sc), sh2 = pt_pack(-shift, -shift);
           uint64_t sum2 = 0;
-#pragma unroll 1
-          for (int k = 0; k < 2; ++k) {
-            fetch(k);                                    // (P of the first half lies over scores that have been read)
-            uint32_t pk[32];
+          auto weigh = [&](const auto& sv, int col) {    // P of those columns, over scores that have been read
+            constexpr int N = sizeof(sv) / 4;
+            uint32_t pk[N / 2];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < N / 2; ++e) {
               float x0, x1;
               pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
               float p0 = ex2_fast(x0), p1 = ex2_fast(x1);
               sum2 = pt_add2(sum2, pt_pack(p0, p1));
               if (C::Q8) {
-                const float4 f = vs[16 * k + (e >> 1)];
+                const float4 f = vs[col / 4 + (e >> 1)];
                 p0 *= e & 1 ? f.z : f.x;
                 p1 *= e & 1 ? f.w : f.y;
               }
               pk[e] = pack2_bf16(p0, p1);
             }
-            t5_st32(tS + 32u * k, pk);
+            pt_st(tS + col / 2, pk);
+          };
+          if constexpr (FEW) {
+            const uint32_t zero[16] = {};
+#pragma unroll
+            for (int k = 1; k < 4; ++k) pt_st(tS + 16u * ((sub + k) & 3), zero);
+            weigh(few, from);
+          } else {
+#pragma unroll 1
+            for (int col = 0; col < PT_KT; col += 64) {
+              uint32_t sv[64];
+              fetch(sv, col);
+              weigh(sv, col);
+            }
           }
           float la, lb;
           pt_unpack(sum2, la, lb);
@@ -495,89 +557,145 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // ---- the item's end: its rows, or its part of them ------------------------------------------------------------------------
       if (ok) ok = wait(&sm.pv_done[x], n - 1);
       ok = __all_sync(0xffffffffu, ok);
-      float w0 = 1.f, w1 = 0.f;                          // weights of O_0 and O_1 in this row
-      float mm = m;
-      if (!pair) {
-        sm.ml[x][0][r] = m;
-        sm.ml[x][1][r] = l;
-        asm volatile("bar.sync 1, 256;" ::: "memory");   // (O of both is complete)
-        const float m0 = sm.ml[0][0][r], m1 = sm.ml[1][0][r];
-        mm = fmaxf(m0, m1);
-        const float ref = mm == -INFINITY ? 0.f : mm;
-        w0 = ex2_fast((m0 - ref) * sc);
-        w1 = ex2_fast((m1 - ref) * sc);
-        // (a row without a key in one half has weight 0 there and a NaN of that half's sum stays)
-        l = sm.ml[0][1][r] * w0 + sm.ml[1][1][r] * w1;
-      }
       t5_fence_after();
       const bool direct = w.starts() && w.ends();
-      const float shift = mm == -INFINITY ? 0.f : mm * sc;
-      const int head = w.h * a.G + row - tok * a.G;
-      float f = 1.f;
-      if (direct && live) {
-        float below = l;
-        if (a.sink && l > 0.f) below += ex2_fast(ld_any(a.sink, head, a.sink_dtype) * PG_LOG2E - shift);
-        f = l == 0.f ? 0.f : 1.f / below;
-      }
       float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(slot_rows, D);
-      bf16* orow = (bf16*)a.out + ((int64_t)(w.s.row0 + tok) * (a.n_kv * a.G) + head) * D;
-      const int c0 = pair ? 0 : x * (D / 2), c1 = pair ? D : c0 + D / 2;
-      float odd = 0.f;                                   // 0 unless a value of the row is not finite
-      // (a pass before the stores: a row that is not finite is summed again instead of being stored)
+      auto out_row = [&](int i) {                        // of the item's row i
+        const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
+        return (bf16*)a.out + ((int64_t)(w.s.row0 + tk) * (n_kv * G) + w.h * G + rr - tk * G) * D;
+      };
+      auto factor = [&](int i, float l, float shift) {   // 1 / the row's denominator
+        if (!direct) return 1.f;
+        float below = l;
+        if (a.sink && l > 0.f) {
+          const int rr = w.block * C::R + i;
+          below += ex2_fast(ld_any(a.sink, w.h * G + rr - pg_token(a.bt, rr) * G, a.sink_dtype) * PG_LOG2E - shift);
+        }
+        return l == 0.f ? 0.f : 1.f / below;
+      };
+      auto redo = [&](int i, float shift, float f) {     // a row that is not finite, key by key, on the warp
+        const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
+        const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
+        const int2 k = pg_sees(a.bt, w.s, rr);
+        pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (w.h * G + rr - tk * G) * D, max(k.x, part0),
+                             min(k.y, part1), a.scale < 0.f ? -sc : sc, shift, f, out_row(i), direct ? nullptr : slot + (int64_t)i * D);
+      };
+      if (pair) {
+        const float shift = m == -INFINITY ? 0.f : m * sc, f = live ? factor(ri, l, shift) : 0.f;
+        bf16* orow = out_row(ri);
+        float odd = 0.f;                                 // 0 unless a value of the row is not finite
 #pragma unroll 1
-      for (int col = c0; col < c1; col += 32) {
-        uint32_t ov[32];
-        t5_ld32(tO + (pair ? 128u * x : 0u) + col, ov);
-        t5_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) odd += __uint_as_float(ov[e]) * 0.f;
-        if (!pair) {
-          uint32_t o1[32];
-          t5_ld32(tO + 128u + col, o1);
+        for (int col = 0; col < D; col += 32) {
+          uint32_t ov[32];
+          t5_ld32(tO + 128u * x + col, ov);
           t5_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            odd += __uint_as_float(o1[e]) * 0.f;
-            ov[e] = __float_as_uint(__uint_as_float(ov[e]) * w0 + __uint_as_float(o1[e]) * w1);
-          }
-        }
-        if (live && ok) {
-          if (direct) {
+          for (int e = 0; e < 32; ++e) odd += __uint_as_float(ov[e]) * 0.f;
+          if (live && ok) {
+            if (direct) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t o4[4];
+              for (int v = 0; v < 4; ++v) {
+                uint32_t o4[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o4[e] = pack2_bf16(__uint_as_float(ov[8 * v + 2 * e]) * f, __uint_as_float(ov[8 * v + 2 * e + 1]) * f);
-              *reinterpret_cast<uint4*>(orow + col + 8 * v) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+                for (int e = 0; e < 4; ++e) o4[e] = pack2_bf16(__uint_as_float(ov[8 * v + 2 * e]) * f, __uint_as_float(ov[8 * v + 2 * e + 1]) * f);
+                *reinterpret_cast<uint4*>(orow + col + 8 * v) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+              }
+            } else {
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(slot + (int64_t)ri * D + col + 4 * v) = make_uint4(ov[4 * v], ov[4 * v + 1], ov[4 * v + 2], ov[4 * v + 3]);
             }
-          } else {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(slot + (int64_t)ri * D + col + 4 * v) = make_uint4(ov[4 * v], ov[4 * v + 1], ov[4 * v + 2], ov[4 * v + 3]);
           }
         }
-      }
-      if (!direct && live && (pair || x == 0)) {
-        slot[(int64_t)slot_rows * D + ri] = mm * sc;
-        slot[(int64_t)slot_rows * D + slot_rows + ri] = l;
-      }
-      unsigned redo = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
-      if (redo) {
+        if (!direct && live) {
+          slot[(int64_t)slot_rows * D + ri] = m * sc;
+          slot[(int64_t)slot_rows * D + slot_rows + ri] = l;
+        }
+        unsigned again = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
         __syncwarp();
-        const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
-        while (redo) {
-          const int src = __ffs(redo) - 1;
-          redo &= redo - 1;
-          const int rr = __shfl_sync(0xffffffffu, row, src), lo = __shfl_sync(0xffffffffu, keys.x, src), hi = __shfl_sync(0xffffffffu, keys.y, src);
-          const float sh = __shfl_sync(0xffffffffu, shift, src), ff = __shfl_sync(0xffffffffu, f, src);
-          const int tk = rr / a.G, hd = w.h * a.G + rr - tk * a.G, ir = rr - w.block * PT_R;
-          pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + hd * D, max(lo, part0), min(hi, part1),
-                               a.scale < 0.f ? -sc : sc, sh, ff, (bf16*)a.out + ((int64_t)(w.s.row0 + tk) * (a.n_kv * a.G) + hd) * D,
-                               direct ? nullptr : slot + (int64_t)ir * D, c0, c1);
+        for (; again; again &= again - 1) {
+          const int src = __ffs(again) - 1;
+          redo(__shfl_sync(0xffffffffu, ri, src), __shfl_sync(0xffffffffu, shift, src), __shfl_sync(0xffffffffu, f, src));
+        }
+      } else {
+        // The 2 * COPIES parts of each row: 256 rows of D sums, a quarter of the columns at a time through the second query tile.
+        const int u = x * 128 + r;
+        auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        sm.ml[0][u] = m;
+        sm.ml[1][u] = l;
+        sync();
+        float mm = sm.ml[0][ri];
+#pragma unroll
+        for (int k = APART; k < 256; k += APART) mm = fmaxf(mm, sm.ml[0][ri + k]);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        const float mine = ex2_fast((m - ref) * sc);     // (0 for a part without a key: what its sums hold does not matter)
+        if (u < APART && live) {
+          float ll = 0.f;                                // (a NaN of a part's sum stays one)
+#pragma unroll
+          for (int k = 0; k < 256; k += APART) ll += sm.ml[1][ri + k] * ex2_fast((sm.ml[0][ri + k] - ref) * sc);
+          sm.factor[ri] = factor(ri, ll, ref * sc);
+          if (!direct) {
+            slot[(int64_t)slot_rows * D + ri] = mm * sc;
+            slot[(int64_t)slot_rows * D + slot_rows + ri] = ll;
+          }
+        }
+        constexpr int CW = D / 4, WORDS = CW / 4;        // columns, and 16-byte words, of a row at a time
+        float4* stage = reinterpret_cast<float4*>(sm.q[1]);
+        float odd = 0.f;
+#pragma unroll 1
+        for (int col = 0; col < D; col += CW) {
+          uint32_t ov[CW];
+          pt_ld(tO + 128u * x + col, ov);
+          t5_wait_ld();
+#pragma unroll
+          for (int v = 0; v < WORDS; ++v) {
+            float o4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float o = __uint_as_float(ov[4 * v + e]);
+              odd += o * 0.f;
+              o4[e] = mine == 0.f ? 0.f : o * mine;
+            }
+            stage[u * WORDS + (v ^ (u & (WORDS - 1)))] = make_float4(o4[0], o4[1], o4[2], o4[3]);
+          }
+          if (col == D - CW && live && ok && odd != 0.f) atomicOr(&sm.odd[ri >> 5], 1u << (ri & 31));
+          sync();
+#pragma unroll 1
+          for (int k = u; k < APART * WORDS; k += 256) {
+            const int i = k / WORDS, v = k % WORDS;
+            if (i >= w.x.rows || !ok) break;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int n2 = 0; n2 < 256; n2 += APART) {    // (APART is a multiple of WORDS: one place in the swizzle)
+              const float4 p = stage[(n2 + i) * WORDS + (v ^ (i & (WORDS - 1)))];
+              o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
+            }
+            if (direct) {
+              const float f = sm.factor[i];
+              *reinterpret_cast<uint2*>(out_row(i) + col + 4 * v) = make_uint2(pack2_bf16(o.x * f, o.y * f), pack2_bf16(o.z * f, o.w * f));
+            } else {
+              *reinterpret_cast<float4*>(slot + (int64_t)i * D + col + 4 * v) = o;
+            }
+          }
+          sync();
+        }
+        if (sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) {
+          for (int i = u >> 5; i < APART; i += 8) {
+            if (!((sm.odd[i >> 5] >> (i & 31)) & 1u)) continue;
+            float top = -INFINITY;
+            for (int k = i; k < 256; k += APART) top = fmaxf(top, sm.ml[0][k]);
+            redo(i, top == -INFINITY ? 0.f : top * sc, sm.factor[i]);
+          }
+          sync();
+          if (u < 4) sm.odd[u] = 0u;
+          sync();
+        }
+        if (!FEW) {
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(&sm.join_done);
         }
       }
       t5_fence_before();
-      if (!pair) asm volatile("bar.sync 1, 256;" ::: "memory");        // both have read O of both
       if (w.starts() && !w.ends()) {
         part = true;
         if (tid == 128)
@@ -593,32 +711,31 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const int t = tid - 384;
       bool ok = true;
       int g = 0;
-      for (Walk w(a.bt, a.G, a.n_kv, a.window, place); w.valid() && ok; w.next()) {
-        const int tiles = 2 * w.count * (w.x.rows > PT_R / 2 ? 1 : 2);       // of keys and values
+      for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
+        const int tiles = 2 * w.count * (paired(w) ? 1 : 2);       // of keys and values
         for (int i = 0; i < tiles && ok; ++i, ++g) {
           ok = wait(&sm.raw_full[g % C::RAWS], g / C::RAWS);
           if (ok && g >= C::STAGES) ok = wait(&sm.empty[g % C::STAGES], g / C::STAGES - 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const uint8_t* src = sm.raw[g % C::RAWS];
-          uint8_t* dst = sm.kv[g % C::STAGES];
-          constexpr int PIECES = D / 16, ROUNDS = PT_KT * PIECES / 128;       // 16 codes each: 2 words of a tile's row
-          uint4 u[ROUNDS];
-#pragma unroll
-          for (int n = 0; n < ROUNDS; ++n) u[n] = *reinterpret_cast<const uint4*>(src + (n * 128 + t) * 16);
-#pragma unroll
-          for (int n = 0; n < ROUNDS; ++n) {
-            const int row = (n * 128 + t) / PIECES, k = (n * 128 + t) % PIECES;
+          // 16 codes each: 2 words of a tile's row; 128 threads take whole groups of 8 rows, so that a thread's place in the
+          // swizzle is the same in every round.  The threads of the second panel store in the other order: no two of a row meet
+          // in a bank.
+          constexpr uint32_t PIECES = D / 16, ROUNDS = PT_KT * PIECES / 128;
+          const uint32_t row = (uint32_t)t / PIECES, k = (uint32_t)t % PIECES, turn = k >> 2, first = (2 * (k & 3)) ^ (row & 7);
+          const uint8_t* src = sm.raw[g % C::RAWS] + t * 16;
+          uint8_t* line = sm.kv[g % C::STAGES] + (k >> 2) * (PT_KT * 128) + row * 128;
+          uint8_t *to0 = line + ((first ^ turn) << 4), *to1 = line + ((first ^ turn ^ 1) << 4);
+#pragma unroll 4
+          for (uint32_t n = 0; n < ROUNDS; ++n) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src + n * 2048);
             uint4 lo, hi;
-            pt_codes4<KIND>(u[n].x, lo.x, lo.y);
-            pt_codes4<KIND>(u[n].y, lo.z, lo.w);
-            pt_codes4<KIND>(u[n].z, hi.x, hi.y);
-            pt_codes4<KIND>(u[n].w, hi.z, hi.w);
-            uint8_t* line = dst + (k >> 2) * (PT_KT * 128) + row * 128;
-            const int first = (2 * (k & 3)) ^ (row & 7);                     // (the second panel's threads store in the other
-            const bool turn = k >> 2;                                        // order: no two of a row meet in a bank)
-            *reinterpret_cast<uint4*>(line + ((turn ? first ^ 1 : first) << 4)) = turn ? hi : lo;
-            *reinterpret_cast<uint4*>(line + ((turn ? first : first ^ 1) << 4)) = turn ? lo : hi;
+            pt_codes4<KIND>(turn ? u.z : u.x, lo.x, lo.y);
+            pt_codes4<KIND>(turn ? u.w : u.y, lo.z, lo.w);
+            pt_codes4<KIND>(turn ? u.x : u.z, hi.x, hi.y);
+            pt_codes4<KIND>(turn ? u.y : u.w, hi.z, hi.w);
+            *reinterpret_cast<uint4*>(to0 + n * (128 / PIECES * 128)) = lo;
+            *reinterpret_cast<uint4*>(to1 + n * (128 / PIECES * 128)) = hi;
           }
           t5_fence_async_smem();
           mbarrier_arrive(&sm.full[g % C::STAGES]);
@@ -641,25 +758,24 @@ int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes
 
 bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16 && (c == 64 || c == 128); }
 
-template <int D, int KIND>
+template <int D, int KIND, bool FEW>
 static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
-  const int smem = (int)sizeof(PtSmem<D, KIND>);
-  KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_tc5_kernel<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  paged_attend_tc5_kernel<D, KIND><<<ctas, PtCfg<D, KIND>::THREADS, smem, s>>>(km, vm, a);
+  const int smem = (int)sizeof(PtSmem<D, KIND, FEW>);
+  KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_tc5_kernel<D, KIND, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  paged_attend_tc5_kernel<D, KIND, FEW><<<ctas, PtCfg<D, KIND, FEW>::THREADS, smem, s>>>(km, vm, a);
   KCH_LAUNCH_OK();
   return KCH_OK;
 }
 
-int kch_paged_attend_tc5(const PgAttend& a, int kind, int ctas, cudaStream_t s) {
+int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
   const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT;
-  int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.n_kv, a.page, a.c, box);
-  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.n_kv, a.page, a.c, box);
+  int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
+  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc != KCH_OK) return rc;
-#define PT_KIND(D_)                                                                        \
-  (kind == KCH_BF16 ? pt_launch<D_, KCH_BF16>(km, vm, a, ctas, s)               \
-   : kind == KCH_FP8_E4M3 ? pt_launch<D_, KCH_FP8_E4M3>(km, vm, a, ctas, s)     \
-                          : pt_launch<D_, KCH_INT8>(km, vm, a, ctas, s))
+#define PT_FEW(D_, K_) (few ? pt_launch<D_, K_, true>(km, vm, a, ctas, s) : pt_launch<D_, K_, false>(km, vm, a, ctas, s))
+#define PT_KIND(D_) (kind == KCH_BF16 ? PT_FEW(D_, KCH_BF16) : kind == KCH_FP8_E4M3 ? PT_FEW(D_, KCH_FP8_E4M3) : PT_FEW(D_, KCH_INT8))
   return a.c == 64 ? PT_KIND(64) : PT_KIND(128);
 #undef PT_KIND
+#undef PT_FEW
 }

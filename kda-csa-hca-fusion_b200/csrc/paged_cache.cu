@@ -30,7 +30,8 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
 }
 
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b) {
-  PgBatch a;
+  PgBatch a = {};
+  a.n_kv = p->n_kv;
   a.table = b->table; a.ld_table = b->ld_table; a.t0 = b->t0; a.cu = b->cu_seqlens;
   a.B = b->B; a.N = (int)b->N;
   const int64_t cap = (int64_t)b->max_pages * p->page_size;
