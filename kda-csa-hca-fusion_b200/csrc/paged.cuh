@@ -125,6 +125,9 @@ __device__ __forceinline__ int64_t pg_scan(int64_t x) {      // sums over the la
   return x;
 }
 
+// n / d: counts are small in earnest, and a 64-bit division takes some 500 cycles
+__device__ __forceinline__ int64_t pg_div(int64_t n, int64_t d) { return ((n | d) >> 31) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d; }
+
 // The whole block calls it; `mem`: PG_PLAN_BYTES(B) of shared memory, free again after the next __syncthreads().
 #define PG_PLAN_BYTES(B) (32 + 8 * ((B) + 1))
 template <int R, int KT, int TWO>
@@ -133,7 +136,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
   PgPlace p = {};
   int64_t total, before = 0, mine = 0;                      // steps: of all, before sequence p.b, of it
   auto range = [&] {
-    p.per = max((total + ctas - 1) / ctas, (int64_t)1);
+    p.per = max(pg_div(total + ctas - 1, ctas), (int64_t)1);
     p.left = max(min(p.per, total - p.per * cta), (int64_t)0);
     return p.per * cta;
   };
@@ -183,8 +186,8 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     const PgSeq s = pg_seq(a, p.b);
     const int blocks = pg_blocks<R>(a, s);
     int64_t rest = p.per * cta - before;
-    const int64_t head = mine / a.n_kv;
-    if (a.n_kv > 1) p.h = (int)(rest / head);
+    const int64_t head = pg_div(mine, a.n_kv);
+    if (a.n_kv > 1) p.h = (int)pg_div(rest, head);
     rest -= p.h * head;
 #pragma unroll 1
     for (int i0 = 0; i0 < blocks; i0 += 32) {

@@ -29,6 +29,9 @@
 #include "tc5_utils.cuh"
 
 #define PT_KT 128
+#ifndef PT_POLY
+#define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks)
+#endif
 #define PT_SPIN (1u << 22)
 
 template <int D, int KIND, bool FEW>
@@ -38,10 +41,12 @@ struct PtCfg {
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
-  static constexpr int THREADS = Q8 ? 512 : 384;
-  // registers of the warpgroups (threads * registers at launch: 65536 and 64512)
-  static constexpr int REG_FEED = Q8 ? 104 : 80, REG_SOFT = Q8 ? 144 : 208;
-  static_assert(128 * (REG_FEED * (Q8 ? 2 : 1) + 2 * REG_SOFT) <= (Q8 ? 65536 : 64512), "register split");
+  static constexpr int CONV = FEW ? 2 : 1;               // warpgroups that turn 8-bit pages into tiles
+  static constexpr int THREADS = 384 + (Q8 ? 128 * CONV : 0);
+  // registers of the warpgroups, and of a thread at launch
+  static constexpr int REG_FEED = Q8 && !FEW ? 104 : 80, REG_SOFT = !Q8 ? 208 : FEW ? 136 : 144, REG_CONV = FEW ? 64 : 104;
+  static constexpr int REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? CONV * REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
 
 template <int D, int KIND, bool FEW>
@@ -49,15 +54,15 @@ struct PtSmem {
   typedef PtCfg<D, KIND, FEW> C;
   alignas(1024) uint8_t q[2][128 * D * 2];
   alignas(1024) uint8_t kv[C::STAGES][C::TILE];
-  alignas(16) uint8_t raw[C::RAWS ? C::RAWS : 1][C::RAWS ? C::RAW : 16];      // (a multiple of 1024 before it)
+  alignas(C::Q8 ? 1024 : 16) uint8_t raw[C::RAWS ? C::RAWS : 1][C::RAWS ? C::RAW : 16];
   alignas(16) float scale[C::Q8 ? C::SCALES : 1][2][C::Q8 ? PT_KT : 4];
   float ml[2][256];                                      // maxima and sums of the parts of an item's keys
-  float factor[128];                                     // of its rows: 1 / the denominator
-  uint32_t odd[4];                                       // rows of it that are not finite
+  float factor[2][32];                                   // of its rows: 1 / the denominator
+  uint32_t odd[2];                                       // rows of it that are not finite, by column half
   alignas(8) uint64_t full[C::STAGES], empty[C::STAGES];
   uint64_t raw_full[C::RAWS ? C::RAWS : 1], raw_empty[C::RAWS ? C::RAWS : 1];
   uint64_t sc_full[C::SCALES], sc_empty[C::SCALES];
-  uint64_t q_full, q_empty, join_done, s_full[2], p_full[2], pv_done[2];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
 static_assert(sizeof(PtSmem<128, KCH_BF16, false>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, false>) <= 232448, "shared memory of the paged attention");
@@ -110,6 +115,21 @@ __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// 2^x of a pair by FMAs: x = n + f, |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative error is smallest (2.6e-6;
+// Remez exchange), n added to its exponent.  x below -126 counts as -126.
+__device__ __forceinline__ void pt_ex2_fma(float& x0, float& x1) {
+  const uint64_t big = pt_pack(12582912.f, 12582912.f), x = pt_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));      // 1.5 * 2^23
+  const uint64_t t = pt_add2(x, big), n = pt_add2(t, pt_pack(-12582912.f, -12582912.f)), f = pt_fma2(n, pt_pack(-1.f, -1.f), x);
+  uint64_t p = pt_fma2(f, pt_pack(0.009570102207362652f, 0.009570102207362652f), pt_pack(0.05591785907745361f, 0.05591785907745361f));
+  p = pt_fma2(p, f, pt_pack(0.240247443318367f, 0.240247443318367f));
+  p = pt_fma2(p, f, pt_pack(0.6931217908859253f, 0.6931217908859253f));
+  p = pt_fma2(p, f, pt_pack(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1, p0, p1;
+  pt_unpack(t, t0, t1);
+  pt_unpack(p, p0, p1);
+  x0 = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0));
+  x1 = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1));
+}
 // bits [lo, hi) of a 32-bit word (any lo, hi)
 __device__ __forceinline__ uint32_t pt_range(int lo, int hi) {
   lo = max(lo, 0);
@@ -138,11 +158,11 @@ __device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi
   }
 }
 
-// One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift), to `dst` (fp32,
-// a part) or `out` (times f, rounded).
+// One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns
+// c0 .. c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).
 template <int D, int KIND>
 __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int from, int to, float sc, float shift,
-                                         float f, bf16* out, float* dst) {
+                                         float f, bf16* out, float* dst, int c0, int c1) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
   float qv[E], o[E];
@@ -173,6 +193,7 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane * E + e;
+    if (d < c0 || d >= c1) continue;
     if (dst) dst[d] = o[e]; else stf(out + d, o[e] * f);
   }
 }
@@ -190,13 +211,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 128 : 1); mbarrier_init(&sm.empty[i], 1); }
-    for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
+    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 128 * C::CONV : 1); mbarrier_init(&sm.empty[i], 1); }
+    for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4 * C::CONV); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, 64);
     mbarrier_init(&sm.q_empty, 1);
-    mbarrier_init(&sm.join_done, 8);
-    for (int i = 0; i < 4; ++i) sm.odd[i] = 0u;
+    sm.odd[0] = sm.odd[1] = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
@@ -336,19 +356,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     } else {
       // ------------------------------ queries ------------------------------------------------------------------------------
       const int t = tid - 64;
-      int c = 0, kt = 0, halves = 0, joined = 0;
+      int c = 0, kt = 0;
       bool ok = true;
       for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
         if (c) ok = wait(&sm.q_empty, c - 1);
         if (!ok) break;
-        if (!FEW) {
-          // The second tile's memory joins the parts of items of few rows: all of those before have to be done with it, and the
-          // barrier is never left two phases behind.
-          const bool pair = paired(w);
-          for (; joined < (pair ? halves : halves - 1) && ok; ++joined) ok = wait(&sm.join_done, joined);
-          if (!ok) break;
-          halves += pair ? 0 : 1;
-        }
         constexpr int CHUNKS = D / 8, STEP = 64 / CHUNKS;      // 16 bytes a thread
         const int rows = w.x.rows, k = t % CHUNKS;
 #pragma unroll 1
@@ -518,7 +530,15 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             for (int e = 0; e < N / 2; ++e) {
               float x0, x1;
               pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
-              float p0 = ex2_fast(x0), p1 = ex2_fast(x1);
+              float p0, p1;
+              if (!FEW && (e & 3) >= 4 - PT_POLY) {
+                pt_ex2_fma(x0, x1);
+                p0 = x0;
+                p1 = x1;
+              } else {
+                p0 = ex2_fast(x0);
+                p1 = ex2_fast(x1);
+              }
               sum2 = pt_add2(sum2, pt_pack(p0, p1));
               if (C::Q8) {
                 const float4 f = vs[col / 4 + (e >> 1)];
@@ -573,129 +593,121 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
         return l == 0.f ? 0.f : 1.f / below;
       };
-      auto redo = [&](int i, float shift, float f) {     // a row that is not finite, key by key, on the warp
+      auto redo = [&](int i, float shift, float f, int c0, int c1) {     // a row that is not finite, key by key, on the warp
         const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
         const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
         const int2 k = pg_sees(a.bt, w.s, rr);
         pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (w.h * G + rr - tk * G) * D, max(k.x, part0),
-                             min(k.y, part1), a.scale < 0.f ? -sc : sc, shift, f, out_row(i), direct ? nullptr : slot + (int64_t)i * D);
+                             min(k.y, part1), a.scale < 0.f ? -sc : sc, shift, f, out_row(i), direct ? nullptr : slot + (int64_t)i * D, c0, c1);
       };
-      if (pair) {
-        const float shift = m == -INFINITY ? 0.f : m * sc, f = live ? factor(ri, l, shift) : 0.f;
-        bf16* orow = out_row(ri);
-        float odd = 0.f;                                 // 0 unless a value of the row is not finite
-#pragma unroll 1
-        for (int col = 0; col < D; col += 32) {
-          uint32_t ov[32];
-          t5_ld32(tO + 128u * x + col, ov);
-          t5_wait_ld();
+      // The parts of a row: its O_0 and O_1 with weights w0, w1 where the warpgroups had other tiles of the same rows (each then
+      // stores half of the columns), and with FEW those of four warps.
+      const auto sync = [](int bar, int n) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(n) : "memory"); };
+      float w0 = 1.f, w1 = 0.f, mm = m, ll = l;
+      if (!pair) {
+        sm.ml[0][x * 128 + r] = m;
+        sm.ml[1][x * 128 + r] = l;
+        sync(1, 256);
+        const float m0 = sm.ml[0][r], m1 = sm.ml[0][128 + r];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) odd += __uint_as_float(ov[e]) * 0.f;
-          if (live && ok) {
-            if (direct) {
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t o4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o4[e] = pack2_bf16(__uint_as_float(ov[8 * v + 2 * e]) * f, __uint_as_float(ov[8 * v + 2 * e + 1]) * f);
-                *reinterpret_cast<uint4*>(orow + col + 8 * v) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
-              }
-            } else {
-#pragma unroll
-              for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(slot + (int64_t)ri * D + col + 4 * v) = make_uint4(ov[4 * v], ov[4 * v + 1], ov[4 * v + 2], ov[4 * v + 3]);
-            }
-          }
-        }
-        if (!direct && live) {
-          slot[(int64_t)slot_rows * D + ri] = m * sc;
-          slot[(int64_t)slot_rows * D + slot_rows + ri] = l;
-        }
-        unsigned again = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
-        __syncwarp();
-        for (; again; again &= again - 1) {
-          const int src = __ffs(again) - 1;
-          redo(__shfl_sync(0xffffffffu, ri, src), __shfl_sync(0xffffffffu, shift, src), __shfl_sync(0xffffffffu, f, src));
-        }
-      } else {
-        // The 2 * COPIES parts of each row: 256 rows of D sums, a quarter of the columns at a time through the second query tile.
-        const int u = x * 128 + r;
-        auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-        sm.ml[0][u] = m;
-        sm.ml[1][u] = l;
-        sync();
-        float mm = sm.ml[0][ri];
-#pragma unroll
-        for (int k = APART; k < 256; k += APART) mm = fmaxf(mm, sm.ml[0][ri + k]);
+        for (int k = 0; k < 256; k += APART) mm = fmaxf(mm, sm.ml[0][ri + k]);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        const float mine = ex2_fast((m - ref) * sc);     // (0 for a part without a key: what its sums hold does not matter)
-        if (u < APART && live) {
-          float ll = 0.f;                                // (a NaN of a part's sum stays one)
+        w0 = ex2_fast((m0 - ref) * sc);                  // (0 for a part without a key: what its sums hold does not matter)
+        w1 = ex2_fast((m1 - ref) * sc);
+        if (!FEW || r < 32) {
+          ll = 0.f;                                      // (a NaN of a part's sum stays one)
 #pragma unroll
           for (int k = 0; k < 256; k += APART) ll += sm.ml[1][ri + k] * ex2_fast((sm.ml[0][ri + k] - ref) * sc);
-          sm.factor[ri] = factor(ri, ll, ref * sc);
-          if (!direct) {
-            slot[(int64_t)slot_rows * D + ri] = mm * sc;
-            slot[(int64_t)slot_rows * D + slot_rows + ri] = ll;
-          }
         }
-        constexpr int CW = D / 4, WORDS = CW / 4;        // columns, and 16-byte words, of a row at a time
-        float4* stage = reinterpret_cast<float4*>(sm.q[1]);
-        float odd = 0.f;
+      }
+      const float shift = mm == -INFINITY ? 0.f : mm * sc;
+      float f = 1.f;
+      if (live && direct && (!FEW || r < 32)) f = factor(ri, ll, shift);
+      if (live && !direct && (pair || (x == 0 && r < APART))) {
+        slot[(int64_t)slot_rows * D + ri] = mm * sc;
+        slot[(int64_t)slot_rows * D + slot_rows + ri] = ll;
+      }
+      if (FEW && r < 32) sm.factor[x][r] = f;
+      const int c0 = pair ? 0 : x * (D / 2), c1 = pair ? D : c0 + D / 2;
+      constexpr int CW = FEW ? D / 4 : 32, WORDS = CW / 4;       // columns, and 16-byte words, of a row at a time
+      float odd = 0.f;                                   // 0 unless a value of the row is not finite
+      bf16* orow = FEW ? nullptr : out_row(ri);
 #pragma unroll 1
-        for (int col = 0; col < D; col += CW) {
-          uint32_t ov[CW];
-          pt_ld(tO + 128u * x + col, ov);
+      for (int col = c0; col < c1; col += CW) {
+        uint32_t o0[CW];
+        pt_ld(tO + (pair ? 128u * x : 0u) + col, o0);
+        if (pair) {
           t5_wait_ld();
 #pragma unroll
-          for (int v = 0; v < WORDS; ++v) {
-            float o4[4];
+          for (int e = 0; e < CW; ++e) odd += __uint_as_float(o0[e]) * 0.f;
+        } else {
+          uint32_t o1[CW];
+          pt_ld(tO + 128u + col, o1);
+          t5_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float o = __uint_as_float(ov[4 * v + e]);
-              odd += o * 0.f;
-              o4[e] = mine == 0.f ? 0.f : o * mine;
-            }
-            stage[u * WORDS + (v ^ (u & (WORDS - 1)))] = make_float4(o4[0], o4[1], o4[2], o4[3]);
+          for (int e = 0; e < CW; ++e) {
+            const float a0 = __uint_as_float(o0[e]), a1 = __uint_as_float(o1[e]);
+            odd += a0 * 0.f + a1 * 0.f;
+            o0[e] = __float_as_uint((w0 == 0.f ? 0.f : a0 * w0) + (w1 == 0.f ? 0.f : a1 * w1));
           }
-          if (col == D - CW && live && ok && odd != 0.f) atomicOr(&sm.odd[ri >> 5], 1u << (ri & 31));
-          sync();
+        }
+        if constexpr (FEW) {                             // through the second query tile, 128 rows of either warpgroup
+          float4* stage = reinterpret_cast<float4*>(sm.q[1]) + x * 128 * WORDS;
+          if (live) {
+#pragma unroll
+            for (int v = 0; v < WORDS; ++v)
+              stage[r * WORDS + (v ^ (r & (WORDS - 1)))] = make_float4(__uint_as_float(o0[4 * v]), __uint_as_float(o0[4 * v + 1]),
+                                                                       __uint_as_float(o0[4 * v + 2]), __uint_as_float(o0[4 * v + 3]));
+            if (col + CW == c1 && ok && odd != 0.f) atomicOr(&sm.odd[x], 1u << ri);
+          }
+          sync(2 + x, 128);
 #pragma unroll 1
-          for (int k = u; k < APART * WORDS; k += 256) {
+          for (int k = r; k < w.x.rows * WORDS && ok; k += 128) {
             const int i = k / WORDS, v = k % WORDS;
-            if (i >= w.x.rows || !ok) break;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int n2 = 0; n2 < 256; n2 += APART) {    // (APART is a multiple of WORDS: one place in the swizzle)
+            for (int n2 = 0; n2 < 128; n2 += APART) {    // (APART is a multiple of WORDS: one place in the swizzle)
               const float4 p = stage[(n2 + i) * WORDS + (v ^ (i & (WORDS - 1)))];
               o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
             }
             if (direct) {
-              const float f = sm.factor[i];
-              *reinterpret_cast<uint2*>(out_row(i) + col + 4 * v) = make_uint2(pack2_bf16(o.x * f, o.y * f), pack2_bf16(o.z * f, o.w * f));
+              const float fi = sm.factor[x][i];
+              *reinterpret_cast<uint2*>(out_row(i) + col + 4 * v) = make_uint2(pack2_bf16(o.x * fi, o.y * fi), pack2_bf16(o.z * fi, o.w * fi));
             } else {
               *reinterpret_cast<float4*>(slot + (int64_t)i * D + col + 4 * v) = o;
             }
           }
-          sync();
-        }
-        if (sm.odd[0] | sm.odd[1] | sm.odd[2] | sm.odd[3]) {
-          for (int i = u >> 5; i < APART; i += 8) {
-            if (!((sm.odd[i >> 5] >> (i & 31)) & 1u)) continue;
-            float top = -INFINITY;
-            for (int k = i; k < 256; k += APART) top = fmaxf(top, sm.ml[0][k]);
-            redo(i, top == -INFINITY ? 0.f : top * sc, sm.factor[i]);
+          sync(2 + x, 128);
+        } else if (live && ok) {
+          if (direct) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t o4[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o4[e] = pack2_bf16(__uint_as_float(o0[8 * v + 2 * e]) * f, __uint_as_float(o0[8 * v + 2 * e + 1]) * f);
+              *reinterpret_cast<uint4*>(orow + col + 8 * v) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < WORDS; ++v)
+              *reinterpret_cast<uint4*>(slot + (int64_t)ri * D + col + 4 * v) = make_uint4(o0[4 * v], o0[4 * v + 1], o0[4 * v + 2], o0[4 * v + 3]);
           }
-          sync();
-          if (u < 4) sm.odd[u] = 0u;
-          sync();
         }
-        if (!FEW) {
-          __syncwarp();
-          if (lane == 0) mbarrier_arrive(&sm.join_done);
+      }
+      // rows that are not finite: again, over the columns stored here
+      unsigned again;
+      if constexpr (FEW) again = (warp & 3) == 0 ? sm.odd[x] : 0u;       // (row i is lane i's of the first warp)
+      else again = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
+      if (again) {
+        __syncwarp();
+        if (FEW && lane == 0) sm.odd[x] = 0u;
+        for (; again; again &= again - 1) {
+          const int src = __ffs(again) - 1;
+          redo(__shfl_sync(0xffffffffu, ri, src), __shfl_sync(0xffffffffu, shift, src), __shfl_sync(0xffffffffu, f, src), c0, c1);
         }
       }
       t5_fence_before();
+      if (!pair) sync(1, 256);                           // both have read O of both, and the maxima and sums
       if (w.starts() && !w.ends()) {
         part = true;
         if (tid == 128)
@@ -707,7 +719,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   } else {
     // ------------------------------ 8-bit pages: payloads to bf16 tiles, scales ------------------------------------------------
     if constexpr (C::Q8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_CONV));
       const int t = tid - 384;
       bool ok = true;
       int g = 0;
@@ -718,24 +730,26 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           if (ok && g >= C::STAGES) ok = wait(&sm.empty[g % C::STAGES], g / C::STAGES - 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          // 16 codes each: 2 words of a tile's row; 128 threads take whole groups of 8 rows, so that a thread's place in the
-          // swizzle is the same in every round.  The threads of the second panel store in the other order: no two of a row meet
-          // in a bank.
-          constexpr uint32_t PIECES = D / 16, ROUNDS = PT_KT * PIECES / 128;
-          const uint32_t row = (uint32_t)t / PIECES, k = (uint32_t)t % PIECES, turn = k >> 2, first = (2 * (k & 3)) ^ (row & 7);
-          const uint8_t* src = sm.raw[g % C::RAWS] + t * 16;
-          uint8_t* line = sm.kv[g % C::STAGES] + (k >> 2) * (PT_KT * 128) + row * 128;
-          uint8_t *to0 = line + ((first ^ turn) << 4), *to1 = line + ((first ^ turn ^ 1) << 4);
+          // 16 codes each: 2 words of a tile's row, 4 such pieces a row and panel.  8 threads that meet in the banks have 4 pieces of
+          // two rows: one of an even and one of an odd number (whose words lie apart in the tile), and where the codes are
+          // swizzled too, numbers that differ in bit 2 as well (5 = 101b: their pieces lie apart there).  A thread's place in
+          // both swizzles is the same in every round.
+          constexpr int ROWS = D == 128 ? 16 * C::CONV : 32 * C::CONV, ROUNDS = PT_KT / ROWS;      // rows between two rounds
+          const int k = lane & 3, wq = t >> 5;
+          const int row = D == 128 ? (wq >> 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : wq * 8 + (lane >> 2), panel = D == 128 ? wq & 1 : 0;
+          const uint8_t* src = sm.raw[g % C::RAWS] + row * D + (D == 128 ? ((panel * 4 + k) ^ (row & 7)) << 4 : k * 16);
+          uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
+          uint8_t *to0 = line + (((2 * k) ^ (row & 7)) << 4), *to1 = line + (((2 * k + 1) ^ (row & 7)) << 4);
 #pragma unroll 4
-          for (uint32_t n = 0; n < ROUNDS; ++n) {
-            const uint4 u = *reinterpret_cast<const uint4*>(src + n * 2048);
+          for (int n = 0; n < ROUNDS; ++n) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src + n * (ROWS * D));
             uint4 lo, hi;
-            pt_codes4<KIND>(turn ? u.z : u.x, lo.x, lo.y);
-            pt_codes4<KIND>(turn ? u.w : u.y, lo.z, lo.w);
-            pt_codes4<KIND>(turn ? u.x : u.z, hi.x, hi.y);
-            pt_codes4<KIND>(turn ? u.y : u.w, hi.z, hi.w);
-            *reinterpret_cast<uint4*>(to0 + n * (128 / PIECES * 128)) = lo;
-            *reinterpret_cast<uint4*>(to1 + n * (128 / PIECES * 128)) = hi;
+            pt_codes4<KIND>(u.x, lo.x, lo.y);
+            pt_codes4<KIND>(u.y, lo.z, lo.w);
+            pt_codes4<KIND>(u.z, hi.x, hi.y);
+            pt_codes4<KIND>(u.w, hi.z, hi.w);
+            *reinterpret_cast<uint4*>(to0 + n * (ROWS * 128)) = lo;
+            *reinterpret_cast<uint4*>(to1 + n * (ROWS * 128)) = hi;
           }
           t5_fence_async_smem();
           mbarrier_arrive(&sm.full[g % C::STAGES]);

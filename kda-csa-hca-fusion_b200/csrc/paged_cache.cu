@@ -5,7 +5,9 @@
 //
 // One scale a row of c values and key head: it is then a factor of a logit (keys) or of a probability (values), and the products
 // of the attention run on payloads, which bf16 holds exactly.  Bound by the bytes: 8 values a thread, a group of threads a row
-// (as many as it has such pieces, rounded up to a power of two), the row's maximum over that group by shuffles.
+// (as many as it has such pieces, rounded up to a power of two), the row's maximum over that group by shuffles.  A warp has a token
+// and looks its page up once: with the bisection, two lookups and 64-bit divisions for every row of every head, a copy ran at
+// half the memory's rate.
 #include <math.h>
 
 #include "paged.cuh"
@@ -48,6 +50,7 @@ struct PgRows {
   void *x[2]; int64_t ld[2];           // packed rows of k and v, tokens ld elements apart
   void* pages[2]; float* scales[2];
   int n_kv, c, page, kind, zero_rest;
+  int tokens;                          // of a warp at a time: 1 or 2
 };
 #define PC_THREADS 256
 #define PC_SMEM_B 2048                 // batches up to this search cu_seqlens in shared memory
@@ -79,19 +82,19 @@ __device__ __forceinline__ uint32_t pc_codes2(float x0, float x1, float s, float
   return ((uint32_t)a0 & 0xFFu) | (((uint32_t)a1 & 0xFFu) << 8);
 }
 
-// where packed row t lies: its sequence by bisection of cu_seqlens, then page and row; -1: it belongs to no sequence, -2: the
-// table has no page for it
-__device__ __forceinline__ int64_t pc_site(const PgRows& a, const int32_t* cu, int64_t t, int h) {
+// where packed row t lies: its sequence by bisection of cu_seqlens, then page and row.  Rows (page * n_kv * page_size + row) of the
+// pool, -1: it belongs to no sequence, -2: the table has no page for it.
+__device__ __forceinline__ int64_t pc_site(const PgRows& a, const int32_t* cu, int t) {
   if (t < cu[0] || t >= cu[a.bt.B]) return -1;
   int lo = 0, hi = a.bt.B;                               // cu[lo] <= t < cu[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (cu[mid] <= t) lo = mid; else hi = mid;
   }
-  const int64_t pos = max((int64_t)__ldg(a.bt.t0 + lo), (int64_t)0) + (t - cu[lo]);
+  const int64_t pos = (int64_t)max(__ldg(a.bt.t0 + lo), 0) + (t - cu[lo]);
   if (pos >= a.bt.cap) { pg_bad(a.bt); return -2; }
-  const int64_t pg = pg_page(a.bt, lo, (int)(pos >> a.bt.shift));
-  return pg < 0 ? -2 : (pg * a.n_kv + h) * a.page + (pos & (a.page - 1));
+  const int64_t pg = pg_page(a.bt, lo, (int)pos >> a.bt.shift);
+  return pg < 0 ? -2 : pg * a.n_kv * a.page + ((int)pos & (a.page - 1));
 }
 
 // 8 activations of a row, as floats
@@ -118,14 +121,21 @@ __device__ __forceinline__ void pc_store(bf16* p, const float (&x)[8]) {
   }
   *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void pc_copy(void* to, const void* from, int words) {
-  for (int i = 0; i < words; ++i) ((uint4*)to)[i] = __ldg((const uint4*)from + i);
+// What a row of c values is in 16-byte words: 8 values a thread.
+template <typename T> struct PcWords { uint4 w[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ PcWords<T> pc_words(const void* p) {
+  PcWords<T> x;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.w[i] = __ldg((const uint4*)p + i);
+  return x;
 }
 
-// GROUP threads a row (token, key head, k or v); READ: pages -> packed rows, else packed rows -> pages
-template <typename T, int GROUP, bool READ>
-__global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(PgRows a) {
-  constexpr int W = 8;
+// A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
+// looked up once a token, and four rows a thread are in flight.  READ: pages -> packed rows, else packed rows -> pages.
+#define PC_FLIGHT 4
+template <typename T, int GROUP, bool READ, bool Q8>
+__global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_constant__ PgRows a) {
   __shared__ int32_t scu[PC_SMEM_B + 1];
   const int32_t* cu = a.bt.cu;
   if (a.bt.B <= PC_SMEM_B) {
@@ -133,62 +143,97 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(PgRows a) {
     __syncthreads();
     cu = scu;
   }
-  const int64_t rows = (int64_t)a.bt.N * a.n_kv * 2, groups = (int64_t)gridDim.x * (PC_THREADS / GROUP);
-  const int g = threadIdx.x % GROUP, d = g * W;
-  const int64_t first = (int64_t)blockIdx.x * (PC_THREADS / GROUP) + threadIdx.x / GROUP;
-  // (all threads of a warp take the same number of rounds: the maximum is found by shuffles)
-  const int64_t rounds = (rows - (int64_t)blockIdx.x * (PC_THREADS / GROUP) + groups - 1) / groups;
-  for (int64_t k = 0; k < rounds; ++k) {
-    const int64_t row = first + k * groups;
-    const bool in = row < rows;
-    const int64_t th = in ? row >> 1 : 0, t = th / a.n_kv;
-    const int h = (int)(th - t * a.n_kv), kv = in ? (int)(row & 1) : 0;
-    const int64_t site = in ? pc_site(a, cu, t, h) : -1;
-    const bool mine = site >= 0 && d < a.c;
-    T* px = (T*)a.x[kv] + t * a.ld[kv] + (int64_t)h * a.c + d;
-    float x[W] = {};
-    if (READ) {
-      if (in && d < a.c && (site == -2 || (site == -1 && a.zero_rest))) pc_store(px, x);
-      if (!mine) continue;
-      if (a.kind < KCH_FP8_E4M3) {
-        pc_copy(px, (const T*)a.pages[kv] + site * a.c + d, sizeof(T) / 2);
-        continue;
-      }
-      const float s = __ldg(a.scales[kv] + site);
-      const uint8_t* p = (const uint8_t*)a.pages[kv] + site * a.c + d;
-      const uint2 u = __ldg((const uint2*)p);
-      const uint32_t w[2] = {u.x, u.y};
+  const int lane = threadIdx.x & 31, each = 32 / a.tokens, mine = lane & (each - 1);      // lanes of a token, this one among them
+  const int d = (mine & (GROUP - 1)) * 8, row0 = mine / GROUP, rows = 2 * a.n_kv, step = each / GROUP;
+  const bool in_row = d < a.c;
+  for (int64_t t0 = ((int64_t)blockIdx.x * (PC_THREADS / 32) + (threadIdx.x >> 5)) * a.tokens; t0 < a.bt.N;
+       t0 += (int64_t)gridDim.x * (PC_THREADS / 32) * a.tokens) {
+    const int64_t t = t0 + lane / each;
+    const int64_t site = t < a.bt.N ? pc_site(a, cu, (int)t) : -1;
+    if (!READ && !__any_sync(0xffffffffu, site >= 0)) continue;
+    // (k and v of a head one after the other: row 2 h + kv)
+    auto packed = [&](int row) { return (T*)a.x[row & 1] + t * a.ld[row & 1] + (int64_t)(row >> 1) * a.c + d; };
+    auto pool_row = [&](int row) { return site + (int64_t)(row >> 1) * a.page; };
+    if constexpr (!Q8) {
+      if ((READ ? t >= a.bt.N : site < 0) || !in_row) continue;
+      if (READ && site == -1 && !a.zero_rest) continue;
+      for (int r = row0; r < rows; r += step * PC_FLIGHT) {
+        PcWords<T> x[PC_FLIGHT] = {};
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const uint8_t code = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
-        __nv_fp8_e4m3 v;
-        v.__x = code;
-        x[e] = (a.kind == KCH_FP8_E4M3 ? float(v) : (float)(int8_t)code) * s;
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          if (row < rows && site >= 0) x[i] = pc_words<T>(READ ? (const void*)((const T*)a.pages[row & 1] + pool_row(row) * a.c + d) : packed(row));
+        }
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          if (row >= rows) break;
+          uint4* to = (uint4*)(READ ? packed(row) : (T*)a.pages[row & 1] + pool_row(row) * a.c + d);
+#pragma unroll
+          for (int k = 0; k < (int)sizeof(T) / 2; ++k) to[k] = x[i].w[k];
+        }
       }
-      pc_store(px, x);
+    } else if constexpr (READ) {
+      if (t >= a.bt.N || !in_row || (site == -1 && !a.zero_rest)) continue;
+      for (int r = row0; r < rows; r += step * PC_FLIGHT) {
+        uint2 u[PC_FLIGHT] = {};
+        float f[PC_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          f[i] = 0.f;
+          if (row < rows && site >= 0) {
+            u[i] = __ldg((const uint2*)((const uint8_t*)a.pages[row & 1] + pool_row(row) * a.c + d));
+            f[i] = __ldg(a.scales[row & 1] + pool_row(row));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          if (row >= rows) break;
+          const uint32_t w[2] = {u[i].x, u[i].y};
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint8_t code = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            __nv_fp8_e4m3 v;
+            v.__x = code;
+            x[e] = (a.kind == KCH_FP8_E4M3 ? float(v) : (float)(int8_t)code) * f[i];
+          }
+          pc_store(packed(row), x);
+        }
+      }
     } else {
-      if (a.kind < KCH_FP8_E4M3) {
-        if (mine) pc_copy((T*)a.pages[kv] + site * a.c + d, px, sizeof(T) / 2);
-        continue;
+      const bool here = site >= 0 && in_row;
+      // (all lanes of the warp take the same rounds: a row's maximum is found by shuffles)
+      for (int r0 = 0; r0 < rows; r0 += step * PC_FLIGHT) {
+        float x[PC_FLIGHT][8] = {};
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r0 + row0 + i * step;
+          if (here && row < rows) pc_load(packed(row), x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r0 + row0 + i * step;
+          uint32_t top = 0;                              // as bits: a NaN is above an infinity, which is above every number
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+#pragma unroll
+          for (int o = GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (!here || row >= rows) continue;
+          const bool finite = top < 0x7F800000u;
+          float s = top ? fmaxf(__uint_as_float(top) / (a.kind == KCH_FP8_E4M3 ? 448.f : 127.f), 1.17549435e-38f) : 1.f;
+          const float inv = 1.f / s;
+          uint32_t w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            w[e] = finite ? pc_codes2(x[i][4 * e], x[i][4 * e + 1], s, inv, a.kind) | pc_codes2(x[i][4 * e + 2], x[i][4 * e + 3], s, inv, a.kind) << 16 : 0u;
+          if (!finite) s = __uint_as_float(0x7FC00000u); // a row that is not finite reads as NaN, whichever the kind
+          *(uint2*)((uint8_t*)a.pages[row & 1] + pool_row(row) * a.c + d) = make_uint2(w[0], w[1]);
+          if (d == 0) a.scales[row & 1][pool_row(row)] = s;
+        }
       }
-      if (mine) pc_load(px, x);
-      uint32_t top = 0;                                  // as bits: a NaN is above an infinity, which is above every number
-#pragma unroll
-      for (int e = 0; e < W; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-#pragma unroll
-      for (int o = GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!mine) continue;
-      const bool finite = top < 0x7F800000u;
-      float s = top ? fmaxf(__uint_as_float(top) / (a.kind == KCH_FP8_E4M3 ? 448.f : 127.f), 1.17549435e-38f) : 1.f;
-      const float inv = 1.f / s;
-      uint32_t w[W / 4];
-#pragma unroll
-      for (int e = 0; e < W / 4; ++e)
-        w[e] = finite ? pc_codes2(x[4 * e], x[4 * e + 1], s, inv, a.kind) | pc_codes2(x[4 * e + 2], x[4 * e + 3], s, inv, a.kind) << 16 : 0u;
-      if (!finite) s = __uint_as_float(0x7FC00000u);     // a row that is not finite reads as NaN, whichever the kind
-      uint8_t* p = (uint8_t*)a.pages[kv] + site * a.c + d;
-      *(uint2*)p = make_uint2(w[0], w[1]);
-      if (g == 0) a.scales[kv][site] = s;
     }
   }
 }
@@ -213,23 +258,29 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   a.pages[0] = p->k; a.pages[1] = p->v; a.scales[0] = p->k_scales; a.scales[1] = p->v_scales;
   a.n_kv = p->n_kv; a.c = p->c; a.page = p->page_size; a.kind = p->kind; a.zero_rest = zero_rest;
   cudaStream_t s = kch_stream(stream);
-  const int pieces = p->c / 8;
-  const int64_t rows = b->N * p->n_kv * 2;
-#define PC_GO(T_, G_)                                                                                                    \
+  const int pieces = p->c / 8, group = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
+  a.tokens = 2 * p->n_kv * group <= 16 ? 2 : 1;
+  const int64_t blocks = ceil_div64(b->N, PC_THREADS / 32 * a.tokens);
+  const unsigned grid = (unsigned)(blocks < 8 * KCH_SMS ? blocks : 8 * KCH_SMS);
+#define PC_GO(T_, G_, Q_)                                                                                                \
   do {                                                                                                                   \
-    const int64_t blocks = ceil_div64(rows, PC_THREADS / G_);                                                            \
-    const unsigned grid = (unsigned)(blocks < 64 * KCH_SMS ? blocks : 64 * KCH_SMS);                                     \
-    if (read) paged_rows_kernel<T_, G_, true><<<grid, PC_THREADS, 0, s>>>(a);                                            \
-    else paged_rows_kernel<T_, G_, false><<<grid, PC_THREADS, 0, s>>>(a);                                                \
+    if (read) paged_rows_kernel<T_, G_, true, Q_><<<grid, PC_THREADS, 0, s>>>(a);                                        \
+    else paged_rows_kernel<T_, G_, false, Q_><<<grid, PC_THREADS, 0, s>>>(a);                                            \
   } while (0)
-#define PC_WIDTH(T_)                                                                                                     \
+#define PC_WIDTH(T_, Q_)                                                                                                 \
   do {                                                                                                                   \
-    if (pieces <= 8) PC_GO(T_, 8);                                                                                       \
-    else if (pieces <= 16) PC_GO(T_, 16);                                                                                \
-    else PC_GO(T_, 32);                                                                                                  \
+    if (group == 8) PC_GO(T_, 8, Q_);                                                                                    \
+    else if (group == 16) PC_GO(T_, 16, Q_);                                                                             \
+    else PC_GO(T_, 32, Q_);                                                                                              \
   } while (0)
-  if (dtype == KCH_BF16) PC_WIDTH(bf16);
-  else PC_WIDTH(float);
+#define PC_KIND(T_)                                                                                                      \
+  do {                                                                                                                   \
+    if (p->kind < KCH_FP8_E4M3) PC_WIDTH(T_, false);                                                                     \
+    else PC_WIDTH(T_, true);                                                                                             \
+  } while (0)
+  if (dtype == KCH_BF16) PC_KIND(bf16);
+  else PC_KIND(float);
+#undef PC_KIND
 #undef PC_WIDTH
 #undef PC_GO
   KCH_LAUNCH_OK();

@@ -22,16 +22,20 @@ def _int_at_least(name, v, least):
 
 
 def _packed(x):
-    """``(tensor, elements between tokens)`` of ``x [N, heads, c]`` whose heads are dense within a token (a column slice of a
-    fused projection, say), copied where they are not, or not on 16 bytes."""
+    """``(tensor, its address, elements between tokens)`` of ``x [N, heads, c]`` whose heads are dense within a token (a column
+    slice of a fused projection, say), copied where they are not, or not on 16 bytes."""
     N, heads, c = x.shape
-    width, es = heads * c, x.element_size()
-    if (c == 1 or x.stride(2) == 1) and (heads == 1 or x.stride(1) == c) and x.data_ptr() % 16 == 0:
-        ld = x.stride(0) if N > 1 else width
-        if ld >= width and ld * es % 16 == 0:
-            return x, ld
+    width, at = heads * c, x.data_ptr()
+    if at % 16 == 0:
+        if x.is_contiguous():
+            return x, at, width
+        token, head, inner = x.stride()
+        if (c == 1 or inner == 1) and (heads == 1 or head == c) and (N <= 1 or (token >= width and token * x.element_size() % 16 == 0)):
+            return x, at, token if N > 1 else width
     x = x.contiguous()
-    return (x if x.data_ptr() % 16 == 0 else x.clone()), width
+    if x.data_ptr() % 16:
+        x = x.clone()
+    return x, x.data_ptr(), width
 
 
 class PagedKVCache:
@@ -91,42 +95,55 @@ class PagedKVCache:
                 raise ValueError(f"PagedKVCache: {name} must start on 16 bytes")
         self.device = where
         self.k_pages, self.v_pages, self.k_scales, self.v_scales = storage
-        self._tag = _lib.dtype_tag(dtype)
+        self._tag, self._index, self._lib = _lib.dtype_tag(dtype), self.k_pages.get_device(), _lib.load()
         self._c = _lib.PagedCache(self.k_pages.data_ptr(), self.v_pages.data_ptr(), _lib.ptr(self.k_scales), _lib.ptr(self.v_scales),
                                   self._tag if kv_quant is None else _QUANT[kv_quant], num_pages, page_size, n_kv, c)
 
+    # A call of a decode step takes the host longer than the GPU: the checks compare what they can in one expression, and name
+    # the argument at fault only where it fails.
     def _batch(self, fn, table, t0, cu_seqlens, N):
-        # one comparison first; which argument it is only where it fails
-        if not (table.dim() == 2 and t0.dim() == cu_seqlens.dim() == 1 and table.dtype == t0.dtype == cu_seqlens.dtype == torch.int32
-                and table.device == t0.device == cu_seqlens.device == self.device
-                and t0.shape[0] == table.shape[0] == cu_seqlens.shape[0] - 1 and 1 <= table.shape[0] <= 4096 and table.shape[1] >= 1):
-            for name, t, rank in (("table", table, 2), ("t0", t0, 1), ("cu_seqlens", cu_seqlens, 1)):
-                if t.dim() != rank:
-                    raise ValueError(f"{fn}: {name} must have rank {rank}, got shape {tuple(t.shape)}")
-                if t.dtype != torch.int32:
-                    raise TypeError(f"{fn}: {name} must be int32, got {t.dtype}")
-                if t.device != self.device:
-                    raise ValueError(f"{fn}: {name} is on {t.device}, the cache on {self.device}")
-            B = table.shape[0]
-            if not 1 <= B <= 4096:
-                raise ValueError(f"{fn}: {B} sequences; a call takes 1 to 4096")
-            if table.shape[1] < 1:
-                raise ValueError(f"{fn}: table has no columns")
-            raise ValueError(f"{fn}: t0 {tuple(t0.shape)} and cu_seqlens {tuple(cu_seqlens.shape)} must have {B} and {B + 1} entries")
-        if table.stride(1) != 1 and table.shape[1] > 1 or table.stride(0) < table.shape[1]:
+        shape, i32, index = table.shape, torch.int32, self._index
+        if not (len(shape) == 2 and table.dtype is t0.dtype is cu_seqlens.dtype is i32 and table.get_device() == index == t0.get_device()
+                and cu_seqlens.get_device() == index and t0.shape == shape[:1] and cu_seqlens.shape == (shape[0] + 1,)
+                and 1 <= shape[0] <= 4096 and shape[1] >= 1):
+            self._batch_error(fn, table, t0, cu_seqlens)
+        B, P = shape
+        ld, inner = table.stride()
+        if (inner != 1 and P > 1) or (ld < P and B > 1):
             table = table.contiguous()
-        t0, cu_seqlens = t0.contiguous(), cu_seqlens.contiguous()
-        B, P = table.shape
-        return (_lib.PagedBatch(table.data_ptr(), table.stride(0) if B > 1 else P, P, t0.data_ptr(), cu_seqlens.data_ptr(), B, N),
+            ld = P
+        if not t0.is_contiguous():
+            t0 = t0.contiguous()
+        if not cu_seqlens.is_contiguous():
+            cu_seqlens = cu_seqlens.contiguous()
+        return (_lib.PagedBatch(table.data_ptr(), ld if B > 1 else P, P, t0.data_ptr(), cu_seqlens.data_ptr(), B, N),
                 (table, t0, cu_seqlens))
 
+    def _batch_error(self, fn, table, t0, cu_seqlens):
+        for name, t, rank in (("table", table, 2), ("t0", t0, 1), ("cu_seqlens", cu_seqlens, 1)):
+            if t.dim() != rank:
+                raise ValueError(f"{fn}: {name} must have rank {rank}, got shape {tuple(t.shape)}")
+            if t.dtype != torch.int32:
+                raise TypeError(f"{fn}: {name} must be int32, got {t.dtype}")
+            if t.device != self.device:
+                raise ValueError(f"{fn}: {name} is on {t.device}, the cache on {self.device}")
+        B = table.shape[0]
+        if not 1 <= B <= 4096:
+            raise ValueError(f"{fn}: {B} sequences; a call takes 1 to 4096")
+        if table.shape[1] < 1:
+            raise ValueError(f"{fn}: table has no columns")
+        raise ValueError(f"{fn}: t0 {tuple(t0.shape)} and cu_seqlens {tuple(cu_seqlens.shape)} must have {B} and {B + 1} entries")
+
     def _rows(self, fn, name, x, heads=None):
-        if x.dim() != 3 or x.shape[2] != self.c or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{fn}: {name} must be [N, {'nh' if heads is None else heads}, {self.c}], got {tuple(x.shape)}")
+        shape = x.shape
+        if len(shape) == 3 and shape[2] == self.c and (heads is None or shape[1] == heads) and x.dtype is self.dtype \
+                and x.get_device() == self._index:
+            return shape
+        if x.dim() != 3 or shape[2] != self.c or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{fn}: {name} must be [N, {'nh' if heads is None else heads}, {self.c}], got {tuple(shape)}")
         if x.dtype != self.dtype:
             raise ValueError(f"{fn}: {name}.dtype={x.dtype} does not match the cache's {self.dtype}")
-        if x.device != self.device:
-            raise (RuntimeError if not x.is_cuda else ValueError)(f"{fn}: {name} is on {x.device}, the CUDA cache on {self.device}")
+        raise (ValueError if x.is_cuda else RuntimeError)(f"{fn}: {name} is on {x.device}, the CUDA cache on {self.device}")
 
     def _own_out(self, fn, name, x, shape):
         self._rows(fn, name, x, shape[1])
@@ -137,16 +154,14 @@ class PagedKVCache:
         """Writes the new rows ``k_new``, ``v_new`` ``[N, n_kv, c]`` into their pages.  Rows outside of
         ``[cu_seqlens[0], cu_seqlens[B])`` are not read."""
         fn = "append_step"
-        self._rows(fn, "k_new", k_new, self.n_kv)
-        self._rows(fn, "v_new", v_new, self.n_kv)
-        N = k_new.shape[0]
-        if v_new.shape[0] != N:
+        N = self._rows(fn, "k_new", k_new, self.n_kv)[0]
+        if self._rows(fn, "v_new", v_new, self.n_kv)[0] != N:
             raise ValueError(f"{fn}: v_new has {v_new.shape[0]} rows, k_new {N}")
         batch, keep = self._batch(fn, table, t0, cu_seqlens, N)
         with _lib.device(self.device):
-            k, ld_k = _packed(k_new)
-            v, ld_v = _packed(v_new)
-            _lib.check(_lib.load().kch_paged_append(self._c, batch, k.data_ptr(), ld_k, v.data_ptr(), ld_v, self._tag, _lib.stream()))
+            k, at_k, ld_k = _packed(k_new)
+            v, at_v, ld_v = _packed(v_new)
+            _lib.check(self._lib.kch_paged_append(self._c, batch, at_k, ld_k, at_v, ld_v, self._tag, _lib.stream()))
 
     def read_step(self, table, t0, cu_seqlens, *, n_rows, out=None):
         """The rows of those positions as ``(k, v)`` ``[n_rows, n_kv, c]`` in the cache's ``dtype`` (stored value times scale).
@@ -164,7 +179,7 @@ class PagedKVCache:
                 self._own_out(fn, "out[0]", k, shape)
                 self._own_out(fn, "out[1]", v, shape)
             width = self.n_kv * self.c
-            _lib.check(_lib.load().kch_paged_read(self._c, batch, k.data_ptr(), width, v.data_ptr(), width, self._tag, int(out is None),
+            _lib.check(self._lib.kch_paged_read(self._c, batch, k.data_ptr(), width, v.data_ptr(), width, self._tag, int(out is None),
                                                   _lib.stream()))
         return k, v
 
@@ -175,33 +190,29 @@ class PagedKVCache:
         ``sink_logits [nh]`` adds ``exp(sink)`` to the denominator.  Rows of no sequence are zeros, and stay as they are in a
         tensor given as ``out``."""
         fn = "forward_step"
-        self._rows(fn, "q", q)
-        N, nh, c = q.shape
+        N, nh, c = self._rows(fn, "q", q)
         if nh < 1 or nh % self.n_kv:
             raise ValueError(f"{fn}: nh={nh} must be a multiple of n_kv={self.n_kv}")
         if not isinstance(sliding_window, int) or isinstance(sliding_window, bool) or sliding_window < 0:
             raise ValueError(f"{fn}: sliding_window={sliding_window!r} must be an int >= 0 (0: every key)")
         batch, keep = self._batch(fn, table, t0, cu_seqlens, N)
-        a = _lib.PagedAttendArgs()
-        a.cache, a.batch, a.dtype, a.nh = self._c, batch, self._tag, nh
-        a.scale = c ** -0.5 if scale is None else float(scale)
-        a.sliding_window = min(sliding_window, 0x7FFFFFFF)
         with _lib.device(self.device):
+            sink, sink_tag = None, 0
             if sink_logits is not None:
-                if tuple(sink_logits.shape) != (nh,) or sink_logits.device != self.device:
+                if tuple(sink_logits.shape) != (nh,) or sink_logits.get_device() != self._index:
                     raise ValueError(f"{fn}: sink_logits must be [{nh}] on {self.device}, got {tuple(sink_logits.shape)} on {sink_logits.device}")
                 sink_logits = sink_logits.contiguous()
-                a.sink, a.sink_dtype = sink_logits.data_ptr(), _lib.dtype_tag(sink_logits.dtype)
-            q, a.ld_q = _packed(q)
+                sink, sink_tag = sink_logits.data_ptr(), _lib.dtype_tag(sink_logits.dtype)
+            q, at_q, ld_q = _packed(q)
             if out is None:
-                o = torch.empty(N, nh, c, dtype=q.dtype, device=self.device)
+                o = torch.empty(N, nh, c, dtype=self.dtype, device=self.device)
             else:
                 o = out
                 self._own_out(fn, "out", o, (N, nh, c))
-            a.q, a.out, a.zero_rest = q.data_ptr(), o.data_ptr(), int(out is None)
-            lib = _lib.load()
-            nbytes = int(lib.kch_paged_attend_workspace_bytes(a))
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+            a = _lib.PagedAttendArgs(self._c, batch, at_q, ld_q, self._tag, nh, c ** -0.5 if scale is None else float(scale),
+                                     min(sliding_window, 0x7FFFFFFF), sink, sink_tag, o.data_ptr(), int(out is None))
+            nbytes = self._lib.kch_paged_attend_workspace_bytes(a)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-            _lib.check(lib.kch_paged_attend(a, _lib.stream()))
+            _lib.check(self._lib.kch_paged_attend(a, _lib.stream()))
         return o
