@@ -82,23 +82,20 @@ __device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int ro
   return make_int2(a.window > 0 ? (int)min(max(pos - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0, (int)min(pos + 1, (int64_t)s.kv));
 }
 
-struct PgPlace {                       // where a CTA's range of steps begins
-  int64_t per, left;                   // steps of a CTA; steps of this one
+// Where a CTA's range of steps begins.  (Steps are counted in 32 bits: the host refuses a call that could have 2^31.)
+struct PgPlace {
+  int per, left;                       // steps of a CTA; steps of this one
   int b, h, block, step;
+  PgSeq s;                             // of b
+  PgSpan x;                            // of the block
 };
 
-// steps of sequence b0 + lane (0 behind the last): by the lane where it is one block, as in a batch of single tokens, else by the
-// warp over its blocks
+// steps of sequence b (0 behind the last) for each key head: by the lane where it is one block, as in a batch of single tokens, else
+// by the warp over its blocks
 template <int R, int KT, int TWO>
-__device__ __forceinline__ int64_t pg_steps(const PgBatch& a, int b0) {
-  const int lane = threadIdx.x & 31, b = b0 + lane;
-  PgSeq s = {0, 0, 0, 0};
-  if (b < a.B) {
-    s = pg_seq(a, b);
-    if ((int64_t)s.t0 + s.len > a.cap) pg_bad(a);
-  }
-  const int blocks = pg_blocks<R>(a, s);
-  int64_t mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps : 0;
+__device__ __forceinline__ int pg_steps(const PgBatch& a, const PgSeq& s) {
+  const int lane = threadIdx.x & 31, blocks = pg_blocks<R>(a, s);
+  int mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps : 0;
   for (unsigned many = __ballot_sync(0xffffffffu, blocks > 1); many; many &= many - 1) {
     const int from = __ffs(many) - 1;
     PgSeq t;
@@ -107,7 +104,7 @@ __device__ __forceinline__ int64_t pg_steps(const PgBatch& a, int b0) {
     t.t0 = __shfl_sync(0xffffffffu, s.t0, from);
     t.kv = __shfl_sync(0xffffffffu, s.kv, from);
     const int nb = pg_blocks<R>(a, t);
-    int64_t sum = 0;
+    int sum = 0;
 #pragma unroll 1
     for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps;
 #pragma unroll
@@ -116,62 +113,73 @@ __device__ __forceinline__ int64_t pg_steps(const PgBatch& a, int b0) {
   }
   return mine * a.n_kv;
 }
-__device__ __forceinline__ int64_t pg_scan(int64_t x) {      // sums over the lanes up to this one
+__device__ __forceinline__ PgSeq pg_seq_or_none(const PgBatch& a, int b) {
+  PgSeq s = {0, 0, 0, 0};
+  if (b < a.B) {
+    s = pg_seq(a, b);
+    if (s.kv - s.t0 < s.len) pg_bad(a);                     // the table ends before the sequence does
+  }
+  return s;
+}
+__device__ __forceinline__ int pg_scan(int x) {             // sums over the lanes up to this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if ((threadIdx.x & 31) >= o) x += y;
   }
   return x;
 }
 
-// n / d: counts are small in earnest, and a 64-bit division takes some 500 cycles
-__device__ __forceinline__ int64_t pg_div(int64_t n, int64_t d) { return ((n | d) >> 31) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d; }
-
 // The whole block calls it; `mem`: PG_PLAN_BYTES(B) of shared memory, free again after the next __syncthreads().
-#define PG_PLAN_BYTES(B) (32 + 8 * ((B) + 1))
+#define PG_PLAN_BYTES(B) (32 + 4 * ((B) + 1))
 template <int R, int KT, int TWO>
 __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   PgPlace p = {};
-  int64_t total, before = 0, mine = 0;                      // steps: of all, before sequence p.b, of it
+  int total, before = 0, mine = 0;                          // steps: of all, before sequence p.b, of it
   auto range = [&] {
-    p.per = max(pg_div(total + ctas - 1, ctas), (int64_t)1);
-    p.left = max(min(p.per, total - p.per * cta), (int64_t)0);
-    return p.per * cta;
+    p.per = max((int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas), 1);
+    const int64_t start = (int64_t)p.per * cta;
+    p.left = (int)max(min((int64_t)p.per, total - start), (int64_t)0);
+    return p.left > 0 ? (int)start : 0x7FFFFFFF;
   };
+  int start;
   if (a.B <= 32) {                     // every warp by itself: no memory, no barrier
-    const int64_t x = pg_steps<R, KT, TWO>(a, 0), upto = pg_scan(x);
+    const PgSeq s = pg_seq_or_none(a, lane);
+    const int x = pg_steps<R, KT, TWO>(a, s), upto = pg_scan(x);
     total = __shfl_sync(0xffffffffu, upto, 31);
-    const int64_t start = range();
-    const unsigned hit = __ballot_sync(0xffffffffu, upto > start);
+    start = range();
     if (p.left > 0) {
-      p.b = __ffs(hit) - 1;
+      p.b = __ffs(__ballot_sync(0xffffffffu, upto > start)) - 1;
       mine = __shfl_sync(0xffffffffu, x, p.b);
       before = __shfl_sync(0xffffffffu, upto, p.b) - mine;
+      p.s.row0 = __shfl_sync(0xffffffffu, s.row0, p.b);
+      p.s.len = __shfl_sync(0xffffffffu, s.len, p.b);
+      p.s.t0 = __shfl_sync(0xffffffffu, s.t0, p.b);
+      p.s.kv = __shfl_sync(0xffffffffu, s.kv, p.b);
     }
   } else {
-    int64_t* base = reinterpret_cast<int64_t*>(mem);        // [B + 1] steps before sequence b
-    int* found = reinterpret_cast<int*>(base + a.B + 1);
+    int* base = reinterpret_cast<int*>(mem);                // [B + 1] steps before sequence b
+    int* found = base + a.B + 1;
 #pragma unroll 1
     for (int b0 = warp * 32; b0 < a.B; b0 += warps * 32) {
-      const int64_t x = pg_steps<R, KT, TWO>(a, b0);
+      const int x = pg_steps<R, KT, TWO>(a, pg_seq_or_none(a, b0 + lane));
       if (b0 + lane < a.B) base[b0 + lane + 1] = x;
     }
     if (tid == 0) base[0] = 0;
     __syncthreads();
     if (warp == 0) {
-      int64_t run = 0;
+      int run = 0;
 #pragma unroll 1
       for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int64_t x = run + pg_scan(b0 + lane < a.B ? base[b0 + lane + 1] : 0);
+        const int x = run + pg_scan(b0 + lane < a.B ? base[b0 + lane + 1] : 0);
         if (b0 + lane < a.B) base[b0 + lane + 1] = x;
         run = __shfl_sync(0xffffffffu, x, 31);
       }
     }
     __syncthreads();
     total = base[a.B];
-    const int64_t start = range();
+    start = range();
     if (p.left > 0)
       for (int b = tid; b < a.B; b += blockDim.x)
         if (base[b] <= start && start < base[b + 1]) found[0] = b;
@@ -180,28 +188,33 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
       p.b = found[0];
       before = base[p.b];
       mine = base[p.b + 1] - before;
+      p.s = pg_seq(a, p.b);
     }
   }
   if (p.left > 0) {                    // the key head, then the block, by every warp
-    const PgSeq s = pg_seq(a, p.b);
-    const int blocks = pg_blocks<R>(a, s);
-    int64_t rest = p.per * cta - before;
-    const int64_t head = pg_div(mine, a.n_kv);
-    if (a.n_kv > 1) p.h = (int)pg_div(rest, head);
-    rest -= p.h * head;
-#pragma unroll 1
-    for (int i0 = 0; i0 < blocks; i0 += 32) {
-      const int i = i0 + lane;
-      const int64_t n = i < blocks ? pg_span<R, KT, TWO>(a, s, i).steps : 0, x = pg_scan(n);
-      const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
-      if (hit) {
-        const int at = __ffs(hit) - 1;
-        p.block = i0 + at;
-        p.step = (int)(rest - __shfl_sync(0xffffffffu, x - n, at));
-        break;
-      }
-      rest -= __shfl_sync(0xffffffffu, x, 31);
+    const int blocks = pg_blocks<R>(a, p.s);
+    int rest = start - before;
+    if (a.n_kv > 1) {
+      const unsigned head = (unsigned)mine / (unsigned)a.n_kv;
+      p.h = (int)((unsigned)rest / head);
+      rest -= p.h * (int)head;
     }
+    if (blocks > 1) {
+#pragma unroll 1
+      for (int i0 = 0; i0 < blocks; i0 += 32) {
+        const int i = i0 + lane, n = i < blocks ? pg_span<R, KT, TWO>(a, p.s, i).steps : 0, x = pg_scan(n);
+        const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
+        if (hit) {
+          const int at = __ffs(hit) - 1;
+          p.block = i0 + at;
+          rest -= __shfl_sync(0xffffffffu, x - n, at);
+          break;
+        }
+        rest -= __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
+    p.step = rest;
+    p.x = pg_span<R, KT, TWO>(a, p.s, p.block);
   }
   return p;
 }
@@ -214,13 +227,10 @@ struct PgWalk {
   int first, count;                    // its steps that belong to this CTA
   PgSeq s;
   PgSpan x;
-  int64_t left;                        // steps of the CTA behind them
+  int left;                            // steps of the CTA behind them
   __device__ __forceinline__ PgWalk(const PgBatch& a_, const PgPlace& p)
-      : a(a_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), left(p.left) {
-    if (left > 0) {
-      s = pg_seq(a, b);
-      open();
-    }
+      : a(a_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), s(p.s), x(p.x), left(p.left) {
+    if (left > 0) take();
   }
   __device__ __forceinline__ bool valid() const { return count > 0; }
   __device__ __forceinline__ bool starts() const { return first == 0; }
@@ -236,13 +246,13 @@ struct PgWalk {
         do { s = pg_seq(a, ++b); } while (s.len == 0);       // (steps are left, so a sequence with rows follows)
       }
     }
-    open();
+    x = pg_span<R, KT, TWO>(a, s, block);
+    take();
   }
 
  private:
-  __device__ __forceinline__ void open() {
-    x = pg_span<R, KT, TWO>(a, s, block);
-    count = (int)min((int64_t)(x.steps - first), left);
+  __device__ __forceinline__ void take() {
+    count = min(x.steps - first, left);
     left -= count;
   }
 };
@@ -277,6 +287,7 @@ struct PgAttend {                      // what both attention kernels get
 __device__ __forceinline__ void pg_zero_rest(const PgAttend& a, int es, int cta, int ctas) {
   if (!a.zero_rest) return;
   const int64_t lo = min(max(__ldg(a.bt.cu), 0), a.bt.N), hi = min(max(__ldg(a.bt.cu + a.bt.B), (int)lo), a.bt.N);
+  if (lo == 0 && hi == a.bt.N) return;
   const int64_t row = (int64_t)a.bt.n_kv * a.bt.G * a.c * es / 16, words = (lo + a.bt.N - hi) * row;      // 16-byte words of a token
   for (int64_t i = (int64_t)cta * blockDim.x + threadIdx.x; i < words; i += (int64_t)ctas * blockDim.x) {
     const int64_t t = i / row, at = (t < lo ? t : hi + t - lo) * row + i % row;

@@ -54,6 +54,12 @@ template <> struct PgStored<int8_t> {
 #define PA_THREADS 256
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
+// steps that a call can have at most, whatever the lengths on the device
+static int64_t pa_steps(const PgBatch& a, int rows, int kt, bool two) {
+  const int64_t blocks = (int64_t)a.N * a.G / rows + a.B, tiles = a.cap / kt + 1;
+  return blocks * a.n_kv * (two ? (tiles + 1) / 2 : tiles);
+}
+
 static int pa_smem(int ROWS, int DMAX, int B) {
   const int need = (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4, plan = PG_PLAN_BYTES(B);
   return need > plan ? need : plan;
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     }
     if (w.starts() && !w.ends()) {
       rec.valid = 1; rec.b = w.b; rec.h = w.h; rec.block = w.block; rec.rows = w.x.rows; rec.row0 = w.s.row0;
-      rec.last = (int)((place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per);   // (it is the last of the range)
+      rec.last = (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per);   // (it is the last of the range)
     }
   }
   if (tid == 0) a.records[blockIdx.x] = rec;
@@ -433,10 +439,14 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;
   cudaStream_t s = kch_stream(stream);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tc5 ? 128 : PA_KT, x.rows == 32) <= 0x7FFFFFFFLL,
+              "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes", (long long)p->batch.N, p->batch.max_pages);
+  // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
+  const bool whole = x.tc5 ? a.bt.cap <= 128 * (x.rows == 32 || (int64_t)a.bt.N * a.bt.G <= 128 ? 2 : 1) : a.bt.cap <= PA_KT;
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.tc5) {
     const int rc5 = kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
-    return rc5 != KCH_OK ? rc5 : kch_paged_join(j, x.ctas, s);
+    return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);
 #define PA_GO(T_, P_, R_, D_)                                                                                                 \
@@ -460,5 +470,5 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   else if (p->dtype == KCH_F32) PA_ROWS(float, float);
   else PA_ROWS(bf16, bf16);
   KCH_LAUNCH_OK();
-  return kch_paged_join(j, x.ctas, s);
+  return whole ? KCH_OK : kch_paged_join(j, x.ctas, s);
 }

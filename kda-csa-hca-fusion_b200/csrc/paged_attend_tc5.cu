@@ -25,6 +25,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc5_utils.cuh"
 
@@ -44,7 +46,7 @@ struct PtCfg {
   static constexpr int CONV = FEW ? 2 : 1;               // warpgroups that turn 8-bit pages into tiles
   static constexpr int THREADS = 384 + (Q8 ? 128 * CONV : 0);
   // registers of the warpgroups, and of a thread at launch
-  static constexpr int REG_FEED = Q8 && !FEW ? 104 : 80, REG_SOFT = !Q8 ? 208 : FEW ? 136 : 144, REG_CONV = FEW ? 64 : 104;
+  static constexpr int REG_FEED = !Q8 ? 88 : FEW ? 80 : 104, REG_SOFT = !Q8 ? 208 : FEW ? 112 : 144, REG_CONV = FEW ? 88 : 104;
   static constexpr int REG_LAUNCH = 65536 / THREADS / 8 * 8;
   static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? CONV * REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
@@ -211,10 +213,10 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 128 * C::CONV : 1); mbarrier_init(&sm.empty[i], 1); }
+    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 * C::CONV : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4 * C::CONV); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
-    mbarrier_init(&sm.q_full, 64);
+    mbarrier_init(&sm.q_full, 2);
     mbarrier_init(&sm.q_empty, 1);
     sm.odd[0] = sm.odd[1] = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
@@ -382,7 +384,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         t5_fence_async_smem();
-        mbarrier_arrive(&sm.q_full);
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&sm.q_full);
         if constexpr (C::Q8) {
           // the scales of the item's key tiles: two keys a thread, 0 behind the end (a scale there may be anything); the page is
           // asked for a tile ahead, and the copies report to the barrier by themselves
@@ -638,8 +641,6 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         pt_ld(tO + (pair ? 128u * x : 0u) + col, o0);
         if (pair) {
           t5_wait_ld();
-#pragma unroll
-          for (int e = 0; e < CW; ++e) odd += __uint_as_float(o0[e]) * 0.f;
         } else {
           uint32_t o1[CW];
           pt_ld(tO + 128u + col, o1);
@@ -647,10 +648,13 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
           for (int e = 0; e < CW; ++e) {
             const float a0 = __uint_as_float(o0[e]), a1 = __uint_as_float(o1[e]);
-            odd += a0 * 0.f + a1 * 0.f;
             o0[e] = __float_as_uint((w0 == 0.f ? 0.f : a0 * w0) + (w1 == 0.f ? 0.f : a1 * w1));
           }
         }
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < CW; ++e) z[e & 3] = fmaf(__uint_as_float(o0[e]), 0.f, z[e & 3]);
+        odd += (z[0] + z[1]) + (z[2] + z[3]);
         if constexpr (FEW) {                             // through the second query tile, 128 rows of either warpgroup
           float4* stage = reinterpret_cast<float4*>(sm.q[1]) + x * 128 * WORDS;
           if (live) {
@@ -711,7 +715,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       if (w.starts() && !w.ends()) {
         part = true;
         if (tid == 128)
-          a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)((place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
+          a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
                                    w.x.rows, w.s.row0};
       }
     }
@@ -752,9 +756,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             *reinterpret_cast<uint4*>(to1 + n * (ROWS * 128)) = hi;
           }
           t5_fence_async_smem();
-          mbarrier_arrive(&sm.full[g % C::STAGES]);
           __syncwarp();
-          if (lane == 0) mbarrier_arrive(&sm.raw_empty[g % C::RAWS]);
+          if (lane == 0) {
+            mbarrier_arrive(&sm.full[g % C::STAGES]);
+            mbarrier_arrive(&sm.raw_empty[g % C::RAWS]);
+          }
         }
       }
     }
@@ -775,7 +781,13 @@ bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16
 template <int D, int KIND, bool FEW>
 static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
   const int smem = (int)sizeof(PtSmem<D, KIND, FEW>);
-  KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_tc5_kernel<D, KIND, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
+  int dev = 0;
+  KCH_CUDA_OK(cudaGetDevice(&dev));
+  if (dev > 63 || !((done.load(std::memory_order_relaxed) >> dev) & 1)) {
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_tc5_kernel<D, KIND, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
+  }
   paged_attend_tc5_kernel<D, KIND, FEW><<<ctas, PtCfg<D, KIND, FEW>::THREADS, smem, s>>>(km, vm, a);
   KCH_LAUNCH_OK();
   return KCH_OK;

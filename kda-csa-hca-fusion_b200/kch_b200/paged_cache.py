@@ -95,6 +95,7 @@ class PagedKVCache:
                 raise ValueError(f"PagedKVCache: {name} must start on 16 bytes")
         self.device = where
         self.k_pages, self.v_pages, self.k_scales, self.v_scales = storage
+        self._ws_bytes = {}             # of attention calls, by their sizes
         self._tag, self._index, self._lib = _lib.dtype_tag(dtype), self.k_pages.get_device(), _lib.load()
         self._c = _lib.PagedCache(self.k_pages.data_ptr(), self.v_pages.data_ptr(), _lib.ptr(self.k_scales), _lib.ptr(self.v_scales),
                                   self._tag if kv_quant is None else _QUANT[kv_quant], num_pages, page_size, n_kv, c)
@@ -205,13 +206,18 @@ class PagedKVCache:
                 sink, sink_tag = sink_logits.data_ptr(), _lib.dtype_tag(sink_logits.dtype)
             q, at_q, ld_q = _packed(q)
             if out is None:
-                o = torch.empty(N, nh, c, dtype=self.dtype, device=self.device)
+                o = torch.empty_like(q, memory_format=torch.contiguous_format)
             else:
                 o = out
                 self._own_out(fn, "out", o, (N, nh, c))
             a = _lib.PagedAttendArgs(self._c, batch, at_q, ld_q, self._tag, nh, c ** -0.5 if scale is None else float(scale),
                                      min(sliding_window, 0x7FFFFFFF), sink, sink_tag, o.data_ptr(), int(out is None))
-            nbytes = self._lib.kch_paged_attend_workspace_bytes(a)
+            sizes = (N, nh, batch.B)
+            nbytes = self._ws_bytes.get(sizes)
+            if nbytes is None:
+                if len(self._ws_bytes) > 4096:
+                    self._ws_bytes.clear()
+                nbytes = self._ws_bytes[sizes] = int(self._lib.kch_paged_attend_workspace_bytes(a))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
             _lib.check(self._lib.kch_paged_attend(a, _lib.stream()))
