@@ -773,7 +773,7 @@ int kch_make_tensor_map_qtile_bf16(CUtensorMap* map, const void* base, uint64_t 
 }
 
 // pages [pages][n_kv][page_size][c] of a paged cache: a box is `box_rows` rows of one page and key head, 64 channels of them under
-// the 128-byte swizzle (bf16) or whole rows (8-bit codes; swizzled too where they have 128 bytes); a page number out of range reads as zeros
+// the 128-byte swizzle (bf16) or whole rows of 64 or 128 bytes under the swizzle of that span (8-bit codes); a page number out of range reads as zeros
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
                               uint32_t box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode_fn();
@@ -784,7 +784,7 @@ int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes
   cuuint32_t box[4] = {elem_bytes == 2 ? 64u : c, box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(map, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), gdim, gstr,
-                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, elem_bytes == 2 || c == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, elem_bytes == 2 || c == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { kch_set_error("cuTensorMapEncodeTiled (pages) failed with code %d", (int)r); return KCH_ERR_CUDA; }
   return KCH_OK;

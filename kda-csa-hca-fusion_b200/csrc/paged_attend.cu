@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 // The rows of all items that are in parts, one after the other over the blocks.  Where a row has few parts it is a warp's, else a
 // block's whose warps take every eighth part; either sums them in one order.  4 (8) columns a lane.  Launched to start while
 // the kernel before it drains.  (One long sequence's step gives a row 74 or 148 parts: a warp a row took 80 us for them.)
-#define PJ_BLOCKS (2 * KCH_SMS)
+#define PJ_BLOCKS (8 * KCH_SMS)         // at most
 #define PJ_WARPS 8
 template <typename T, int W>          // W: columns of a lane, in fours
 __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a, int ctas) {
@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
 }
 
 int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
-  const dim3 grid(PJ_BLOCKS), block(32 * PJ_WARPS);
+  const int64_t rows = (int64_t)ctas * a.slot_rows, want = (rows + PJ_WARPS - 1) / PJ_WARPS;      // that can be in parts
+  const dim3 grid((unsigned)(want < PJ_BLOCKS ? want : PJ_BLOCKS)), block(32 * PJ_WARPS);
   KCH_DISPATCH_FLOAT(a.dtype, T, {
     if (a.c <= 128) KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 1>, grid, block, 0, s, 1, a, ctas));
     else KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 2>, grid, block, 0, s, 1, a, ctas));
@@ -385,6 +386,7 @@ PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c);
 int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s);
+int kch_paged_attend_mma(const PgAttend& a, int kind, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.
 struct PaPlan { bool tc5; int rows, ctas, slot_rows; };
@@ -393,7 +395,7 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
   x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
   const int64_t B = p->batch.B;
-  if (x.tc5) x.rows = rows <= 32 * B && p->batch.N <= 4 * B ? 32 : 256;
+  if (x.tc5) x.rows = rows > 32 * B || p->batch.N > 4 * B ? 256 : p->cache.kind == KCH_BF16 ? 32 : 16;
   else x.rows = rows <= 16 * B ? 16 : 64;
   x.ctas = x.tc5 ? KCH_SMS : PA_CTAS;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
@@ -442,10 +444,10 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tc5 ? 128 : PA_KT, x.rows == 32) <= 0x7FFFFFFFLL,
               "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes", (long long)p->batch.N, p->batch.max_pages);
   // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
-  const bool whole = x.tc5 ? a.bt.cap <= 128 * (x.rows == 32 || (int64_t)a.bt.N * a.bt.G <= 128 ? 2 : 1) : a.bt.cap <= PA_KT;
+  const bool whole = x.tc5 ? a.bt.cap <= 128 * (x.rows == 32 || (x.rows == 256 && (int64_t)a.bt.N * a.bt.G <= 128) ? 2 : 1) : a.bt.cap <= PA_KT;
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.tc5) {
-    const int rc5 = kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
+    const int rc5 = x.rows == 16 ? kch_paged_attend_mma(a, p->cache.kind, x.ctas, s) : kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);

@@ -1,0 +1,351 @@
+// Attention of few new tokens a sequence over 8-bit pages (e4m3, int8; bf16 activations, heads of 64 or 128).
+// Mathematics and division of the work: paged_attend.cu, paged.cuh.
+//
+// A step of a few tokens is bound by the pages' bytes, and on its heels follows the arithmetic that turns codes into bf16: 2 ALU
+// operations a code (at 64 lanes a clock, 2048 clocks for the 256 keys and values that an SM gets from memory in 2850).  So codes are
+// converted once, in the registers of the warp that multiplies them (mma.sync; the rows are far too few for the tensor core's rate to
+// matter): through tiles of tcgen05 the same step took twice as long, for the tiles are written, fenced and read back.
+//
+// An item is up to 16 (token, head of the group) rows of a sequence; a tile is 128 keys, its payloads and scales copied into a ring by
+// one warp (TMA, 128-byte or 64-byte swizzle; scales by bulk copies).  Warp w of eight has keys 16 w .. 16 w + 15 of every tile, with a
+// maximum, a sum and an O of its own, so that nothing but the ring is waited for; they are joined when the item ends.
+//   S = Q K^T: the order of the contraction is free, so thread (g, t) of a fragment takes 32 (16) consecutive channels of key g, four of
+//     them a product: a row is read in 16-byte words, and the queries' fragments are loaded in the same order.
+//   O += P V:  the order of the columns is free, so thread (g, t) takes 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9,
+//     one of them a product; pairs of keys meet by a byte permutation.  P comes from S in place.
+// A key's scale multiplies its logit, and its probability before that is rounded to bf16; masked keys are taken out after that, so
+// that a scale that is not finite stays where it is seen.
+#include <cuda.h>
+#include <math.h>
+
+#include <atomic>
+
+#include "paged.cuh"
+#include "tc5_utils.cuh"
+
+#define PM_R 16
+#define PM_KT 128
+#define PM_WARPS 8
+#define PM_THREADS (32 * PM_WARPS + 32)
+#define PM_SPIN (1u << 22)
+
+template <int D>
+struct PmSmem {
+  static constexpr int STAGES = D == 128 ? 5 : 8;
+  alignas(1024) uint8_t k[STAGES][PM_KT * D], v[STAGES][PM_KT * D];
+  alignas(16) float ks[STAGES][PM_KT], vs[STAGES][PM_KT];
+  alignas(16) float stage[PM_WARPS][8 * D];
+  float ml[2][PM_WARPS][PM_R];
+  alignas(8) uint64_t full[STAGES], empty[STAGES];
+};
+static_assert(sizeof(PmSmem<128>) <= 232448 && sizeof(PmSmem<64>) <= 232448, "shared memory of the paged attention over 8-bit pages");
+static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 5 * PM_KT * 64, "the plan lies in the ring of tiles");
+
+__device__ __forceinline__ void pm_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_addr_u32(dst)), "l"(map), "r"(smem_addr_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ uint32_t pm_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// e4m3: a code in the high byte of either half; sign, exponent and mantissa moved to their places are 2^-120 of the value (subnormal
+// codes become subnormal bf16 values).  int8: a code in the low byte; 128 + its low 7 bits, less 256 or 128 by the sign.  Exact.
+template <int KIND>
+__device__ __forceinline__ uint32_t pm_value2(uint32_t t) {
+  if (KIND == KCH_FP8_E4M3) return pm_fma((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
+  return pm_fma((t & 0x00800080u) | 0x43004300u, 0xBF80BF80u, (t & 0x007F007Fu) | 0x43004300u);
+}
+// byte I of x and byte J of y as a pair of values
+template <int KIND>
+__device__ __forceinline__ uint32_t pm_pair(uint32_t x, uint32_t y, int i, int j) {
+  const uint32_t sel = KIND == KCH_FP8_E4M3 ? (i << 4) | ((4 + j) << 12) : i | ((4 + j) << 8);
+  return pm_value2<KIND>(__byte_perm(x, y, sel));
+}
+__device__ __forceinline__ uint4 pm_lds(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+template <int D, int KIND>
+__global__ void __launch_bounds__(PM_THREADS, 1)
+paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
+  typedef PmSmem<D> S;
+  typedef PgWalk<PM_R, PM_KT, 0> Walk;
+  extern __shared__ __align__(1024) uint8_t pm_raw[];
+  S& sm = *reinterpret_cast<S*>(pm_raw);
+  if (smem_addr_u32(pm_raw) & 1023) {                    // (every block begins its memory there)
+    if (threadIdx.x == 0) atomicCAS(a.bt.status, 0u, (unsigned)KCH_STATUS_PAGED_ATTEND);
+    return;
+  }
+  const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
+  if (tid == 0) {
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 1); mbarrier_init(&sm.empty[i], PM_WARPS); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
+  const PgPlace place = pg_plan<PM_R, PM_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
+  pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
+  t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
+  __syncthreads();
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, PM_SPIN, a.bt.status); };
+
+  if (warp == PM_WARPS) {
+    // ------------------------------ pages into the ring: a box of a tile each lane -------------------------------------------
+    const int box = min(a.page, PM_KT), boxes = PM_KT / box;
+    const bool mine = lane < boxes;
+    int g = 0;
+    bool ok = true;
+    for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
+      const int end = w.first + w.count;
+      const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
+      // asked for a tile ahead; -1 behind the part's or the sequence's end
+      auto ask = [&](int tile) -> int {
+        const int key = w.x.first_key + tile * PM_KT + lane * box;
+        return mine && tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+      };
+      int id = ask(w.first);
+      for (int tile = w.first; tile < end && ok; ++tile, ++g) {
+        const int next = ask(tile + 1), st = g % S::STAGES, key = w.x.first_key + tile * PM_KT + lane * box;
+        ok = g < S::STAGES || wait(&sm.empty[st], g / S::STAGES - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbarrier_expect_tx(&sm.full[st], 2 * PM_KT * (D + 4));
+        __syncwarp();
+        if (mine) {
+          const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
+          if (!there && tile < w.x.tiles && key < w.s.kv) pg_bad(a.bt);
+          const int pg = there ? id : (int)a.bt.num_pages, r0 = key & (a.page - 1);      // out of range: zeros,
+          const int64_t at = ((int64_t)(there ? id : 0) * n_kv + w.h) * a.page + r0;     // with the scales of some page
+          pm_tma_4d(sm.k[st] + lane * box * D, &kmap, 0, r0, w.h, pg, &sm.full[st]);
+          bulk_copy_g2s(sm.ks[st] + lane * box, a.ks + at, box * 4, &sm.full[st]);
+          pm_tma_4d(sm.v[st] + lane * box * D, &vmap, 0, r0, w.h, pg, &sm.full[st]);
+          bulk_copy_g2s(sm.vs[st] + lane * box, a.vs + at, box * 4, &sm.full[st]);
+        }
+        id = next;
+      }
+    }
+    // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones)
+    for (int i = 1; i <= S::STAGES && i <= g; ++i) wait(&sm.full[(g - i) % S::STAGES], (g - i) / S::STAGES);
+    return;
+  }
+
+  // ------------------------------ the eight warps ---------------------------------------------------------------------------------
+  constexpr int KS = D / 16, NT = D / 8, RUN = D / 4;    // contraction steps; column tiles; channels of a key a thread has
+  const int g = lane >> 2, t = lane & 3;
+  const float sc = fmaxf(fabsf(a.scale), 1e-30f);        // (not 0: a masked logit is -inf)
+  const float raise = 8.f / sc;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;      // the sign goes to the queries: a maximum stays one
+  const auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+  // byte of the tile at which the 16-byte word `c` of row r lies (D = 128: words swizzled by the row; D = 64: by every second)
+  const auto word = [](int r, int c) { return r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); };
+  int n = 0;                                             // tiles of the ring
+  bool ok = true, part = false;
+  for (Walk w(a.bt, place); w.valid(); w.next()) {
+    // queries of rows g and g + 8: channels RUN t .. RUN t + RUN - 1
+    uint32_t q[KS][4];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int i = g + 8 * hf, row = w.block * PM_R + i, tok = pg_token(a.bt, row);
+      const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + RUN * t;
+#pragma unroll
+      for (int c = 0; c < RUN / 8; ++c) {
+        const uint4 u = i < w.x.rows ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+        q[2 * c][hf] = u.x ^ flip; q[2 * c][2 + hf] = u.y ^ flip;
+        q[2 * c + 1][hf] = u.z ^ flip; q[2 * c + 1][2 + hf] = u.w ^ flip;
+      }
+    }
+    int2 keys[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+      keys[hf] = g + 8 * hf < w.x.rows ? pg_sees(a.bt, w.s, w.block * PM_R + g + 8 * hf) : make_int2(0, 0);
+    const int2 k0 = pg_sees(a.bt, w.s, w.block * PM_R), k1 = pg_sees(a.bt, w.s, w.block * PM_R + w.x.rows - 1);      // first and last row's
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
+      const int st = n % S::STAGES, key0 = w.x.first_key + tile * PM_KT + 16 * warp;      // of the warp's 16 keys
+      if (ok) ok = wait(&sm.full[st], n / S::STAGES);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && key0 < k1.y && key0 + 16 > k0.x) {
+        const uint8_t *tk = sm.k[st], *tv = sm.v[st];
+        float s[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
+          const int r = 16 * warp + 8 * h + g;
+          uint32_t c[KS];
+#pragma unroll
+          for (int i = 0; i < RUN / 16; ++i) {
+            const uint4 u = pm_lds(tk + word(r, RUN / 16 * t + i));
+            c[4 * i] = u.x; c[4 * i + 1] = u.y; c[4 * i + 2] = u.z; c[4 * i + 3] = u.w;
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) mma_bf16_16816(s[h], q[i], pm_pair<KIND>(c[i], c[i], 0, 1), pm_pair<KIND>(c[i], c[i], 2, 3));
+        }
+        // scaled; what a row does not see is -inf
+        const bool whole = key0 >= k1.x && key0 + 16 <= k0.y && w.x.rows == PM_R;
+        bool sees[2][4];
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 f = *reinterpret_cast<const float2*>(&sm.ks[st][16 * warp + 8 * h + 2 * t]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 8 * h + 2 * t + (e & 1);
+            sees[h][e] = whole || (key >= keys[e >> 1].x && key < keys[e >> 1].y);
+            s[h][e] = sees[h][e] ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
+            top[e >> 1] = fmaxf(top[e >> 1], s[h][e]);
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
+          top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
+        }
+        // a row's maximum is raised only when it is exceeded by 2^8
+        const bool up0 = m[0] == -INFINITY ? top[0] > m[0] : top[0] > m[0] + raise, up1 = m[1] == -INFINITY ? top[1] > m[1] : top[1] > m[1] + raise;
+        if (__any_sync(0xffffffffu, up0 || up1)) {
+          const float n0 = up0 ? top[0] : m[0], n1 = up1 ? top[1] : m[1];
+          const float f0 = up0 ? ex2_fast((m[0] - n0) * sc) : 1.f, f1 = up1 ? ex2_fast((m[1] - n1) * sc) : 1.f;
+          m[0] = n0; m[1] = n1;
+          l[0] *= f0; l[1] *= f1;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+        }
+        const float sh0 = m[0] == -INFINITY ? 0.f : m[0] * sc, sh1 = m[1] == -INFINITY ? 0.f : m[1] * sc;
+        uint32_t p[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][16 * warp + 8 * h + 2 * t]);
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = ex2_fast(fmaf(s[h][e], sc, -(e >> 1 ? sh1 : sh0)));
+            l[e >> 1] += x[e];
+            x[e] = sees[h][e] ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
+          }
+          p[2 * h] = pack2_bf16(x[0], x[1]);
+          p[2 * h + 1] = pack2_bf16(x[2], x[3]);
+        }
+        // channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t c[4][NT / 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * warp + 2 * t + (i & 1) + 8 * (i >> 1);
+          if (D == 128) {
+            const uint4 u = pm_lds(tv + word(r, g));
+            c[i][0] = u.x; c[i][1] = u.y; c[i][NT / 4 - 2] = u.z; c[i][NT / 4 - 1] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(tv + word(r, g >> 1) + 8 * (g & 1));
+            c[i][0] = u.x; c[i][1] = u.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          mma_bf16_16816(o[j], p, pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3));
+      }
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&sm.empty[st]);
+    }
+    // ---- the item's end: the warps' parts of its rows ---------------------------------------------------------------------------
+    const bool direct = w.starts() && w.ends();
+    float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(a.slot_rows, D);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+      if (t == 0) {
+        sm.ml[0][warp][g + 8 * hf] = m[hf];
+        sm.ml[1][warp][g + 8 * hf] = l[hf];
+      }
+    }
+    sync();
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      if (8 * hf >= w.x.rows) break;                     // (the same for all warps)
+      const int i = g + 8 * hf;
+      float mm = sm.ml[0][0][i];
+#pragma unroll
+      for (int k = 1; k < PM_WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][i]);
+      const float own = m[hf] == -INFINITY ? 0.f : ex2_fast((m[hf] - mm) * sc);      // (0 for a part without a key)
+      float4* mine = reinterpret_cast<float4*>(sm.stage[warp]) + g * (D / 4);
+      // 16-byte words of a row, swizzled within runs of 8 so that 8 threads meet in no bank
+#pragma unroll
+      for (int c = 0; c < RUN / 4; ++c) {
+        const int j = 4 * c % NT, e = 2 * hf + 4 * c / NT;
+        mine[(RUN / 4 * t + c) ^ ((D == 128 ? t : 2 * (t & 1)) + 4 * (g & 1))] =
+            own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][e] * own, o[j + 1][e] * own, o[j + 2][e] * own, o[j + 3][e] * own);
+      }
+      sync();
+      for (int k = tid; k < 8 * (D / 4); k += 32 * PM_WARPS) {
+        const int r = k / (D / 4), c = k % (D / 4), row = 8 * hf + r, tt = c / (RUN / 4);
+        if (row >= w.x.rows || !ok) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int at = r * (D / 4) + (c ^ ((D == 128 ? tt : 2 * (tt & 1)) + 4 * (r & 1)));
+#pragma unroll
+        for (int i2 = 0; i2 < PM_WARPS; ++i2) {
+          const float4 y = reinterpret_cast<const float4*>(sm.stage[i2])[at];
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+        float top = sm.ml[0][0][row], sum = 0.f;
+#pragma unroll
+        for (int i2 = 1; i2 < PM_WARPS; ++i2) top = fmaxf(top, sm.ml[0][i2][row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i2 = 0; i2 < PM_WARPS; ++i2) sum += sm.ml[1][i2][row] * ex2_fast((sm.ml[0][i2][row] - ref) * sc);      // (a NaN stays one)
+        if (direct) {
+          const int rr = w.block * PM_R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
+          float below = sum;
+          if (a.sink && sum > 0.f) below += ex2_fast(ld_any(a.sink, head, a.sink_dtype) * PG_LOG2E - ref * sc);
+          const float f = sum == 0.f ? 0.f : 1.f / below;
+          *reinterpret_cast<uint2*>((bf16*)a.out + ((int64_t)(w.s.row0 + tok) * (n_kv * G) + head) * D + 4 * c) =
+              make_uint2(pack2_bf16(x.x * f, x.y * f), pack2_bf16(x.z * f, x.w * f));
+        } else {
+          *reinterpret_cast<float4*>(slot + (int64_t)row * D + 4 * c) = x;
+          if (c == 0) {
+            slot[(int64_t)a.slot_rows * D + row] = top * sc;
+            slot[(int64_t)a.slot_rows * D + a.slot_rows + row] = sum;
+          }
+        }
+      }
+      sync();
+    }
+    if (w.starts() && !w.ends()) {
+      part = true;
+      if (tid == 0)
+        a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
+                                 w.x.rows, w.s.row0};
+    }
+  }
+  if (tid == 0 && !part) a.records[blockIdx.x].valid = 0;
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
+                              uint32_t box_rows);
+
+template <int D, int KIND>
+static int pm_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
+  const int smem = (int)sizeof(PmSmem<D>);
+  static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
+  int dev = 0;
+  KCH_CUDA_OK(cudaGetDevice(&dev));
+  if (dev > 63 || !((done.load(std::memory_order_relaxed) >> dev) & 1)) {
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_mma_kernel<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
+  }
+  paged_attend_mma_kernel<D, KIND><<<ctas, PM_THREADS, smem, s>>>(km, vm, a);
+  KCH_LAUNCH_OK();
+  return KCH_OK;
+}
+
+int kch_paged_attend_mma(const PgAttend& a, int kind, int ctas, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const int box = a.page < PM_KT ? a.page : PM_KT;
+  int rc = kch_make_tensor_map_pages(&km, a.k, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
+  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
+  if (rc != KCH_OK) return rc;
+  if (a.c == 64) return kind == KCH_FP8_E4M3 ? pm_launch<64, KCH_FP8_E4M3>(km, vm, a, ctas, s) : pm_launch<64, KCH_INT8>(km, vm, a, ctas, s);
+  return kind == KCH_FP8_E4M3 ? pm_launch<128, KCH_FP8_E4M3>(km, vm, a, ctas, s) : pm_launch<128, KCH_INT8>(km, vm, a, ctas, s);
+}

@@ -43,12 +43,10 @@ struct PtCfg {
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
-  static constexpr int CONV = FEW ? 2 : 1;               // warpgroups that turn 8-bit pages into tiles
-  static constexpr int THREADS = 384 + (Q8 ? 128 * CONV : 0);
+  static constexpr int THREADS = Q8 ? 512 : 384;         // 8-bit pages: a warpgroup that turns them into tiles
   // registers of the warpgroups, and of a thread at launch
-  static constexpr int REG_FEED = !Q8 ? 88 : FEW ? 80 : 104, REG_SOFT = !Q8 ? 208 : FEW ? 112 : 144, REG_CONV = FEW ? 88 : 104;
-  static constexpr int REG_LAUNCH = 65536 / THREADS / 8 * 8;
-  static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? CONV * REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
+  static constexpr int REG_FEED = Q8 ? 80 : 88, REG_SOFT = Q8 ? 168 : 208, REG_CONV = 88, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
 
 template <int D, int KIND, bool FEW>
@@ -111,6 +109,17 @@ __device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) 
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
+}
+__device__ __forceinline__ uint64_t pt_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void pt_scale2(uint32_t& x0, uint32_t& x1, uint64_t f) {
+  float a, b;
+  pt_unpack(pt_mul2(pt_pack(__uint_as_float(x0), __uint_as_float(x1)), f), a, b);
+  x0 = __float_as_uint(a);
+  x1 = __float_as_uint(b);
 }
 __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
   uint64_t r;
@@ -213,8 +222,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 * C::CONV : 1); mbarrier_init(&sm.empty[i], 1); }
-    for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4 * C::CONV); }
+    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
+    for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, 2);
     mbarrier_init(&sm.q_empty, 1);
@@ -457,8 +466,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           // Chunks: the row's scores come from tensor memory twice, in halves: for the maximum, and for P.  Kept in registers they
           // would be 128 of them, and both passes unrolled: the code of all roles then outgrows the instruction cache, and a tile
           // took 3000 cycles (8-bit pages: 7000) where its arithmetic is ~1200.
-          const float4* ks = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][0]);
-          const float4* vs = reinterpret_cast<const float4*>(sm.scale[C::Q8 ? slot : 0][1]);
+          const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(sm.scale[C::Q8 ? slot : 0][0]);      // pairs of scales
+          const ulonglong2* vs = reinterpret_cast<const ulonglong2*>(sm.scale[C::Q8 ? slot : 0][1]);
           auto fetch = [&](auto& sv, int col) {          // 32 or 64 scores from column `col` on, scaled and masked
             constexpr int N = sizeof(sv) / 4;
 #pragma unroll
@@ -467,11 +476,9 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (C::Q8) {
 #pragma unroll
               for (int e = 0; e < N / 4; ++e) {
-                const float4 f = ks[col / 4 + e];
-                sv[4 * e] = __float_as_uint(__uint_as_float(sv[4 * e]) * f.x);
-                sv[4 * e + 1] = __float_as_uint(__uint_as_float(sv[4 * e + 1]) * f.y);
-                sv[4 * e + 2] = __float_as_uint(__uint_as_float(sv[4 * e + 2]) * f.z);
-                sv[4 * e + 3] = __float_as_uint(__uint_as_float(sv[4 * e + 3]) * f.w);
+                const ulonglong2 f = ks[col / 4 + e];
+                pt_scale2(sv[4 * e], sv[4 * e + 1], f.x);
+                pt_scale2(sv[4 * e + 2], sv[4 * e + 3], f.y);
               }
             }
             if (!whole) {
@@ -544,9 +551,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               }
               sum2 = pt_add2(sum2, pt_pack(p0, p1));
               if (C::Q8) {
-                const float4 f = vs[col / 4 + (e >> 1)];
-                p0 *= e & 1 ? f.z : f.x;
-                p1 *= e & 1 ? f.w : f.y;
+                const ulonglong2 f = vs[col / 4 + (e >> 1)];
+                pt_unpack(pt_mul2(pt_pack(p0, p1), e & 1 ? f.y : f.x), p0, p1);
               }
               pk[e] = pack2_bf16(p0, p1);
             }
@@ -738,10 +744,10 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           // two rows: one of an even and one of an odd number (whose words lie apart in the tile), and where the codes are
           // swizzled too, numbers that differ in bit 2 as well (5 = 101b: their pieces lie apart there).  A thread's place in
           // both swizzles is the same in every round.
-          constexpr int ROWS = D == 128 ? 16 * C::CONV : 32 * C::CONV, ROUNDS = PT_KT / ROWS;      // rows between two rounds
+          constexpr int ROWS = D == 128 ? 16 : 32, ROUNDS = PT_KT / ROWS;      // rows between two rounds
           const int k = lane & 3, wq = t >> 5;
           const int row = D == 128 ? (wq >> 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : wq * 8 + (lane >> 2), panel = D == 128 ? wq & 1 : 0;
-          const uint8_t* src = sm.raw[g % C::RAWS] + row * D + (D == 128 ? ((panel * 4 + k) ^ (row & 7)) << 4 : k * 16);
+          const uint8_t* src = sm.raw[g % C::RAWS] + row * D + ((D == 128 ? (panel * 4 + k) ^ (row & 7) : k ^ ((row >> 1) & 3)) << 4);
           uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
           uint8_t *to0 = line + (((2 * k) ^ (row & 7)) << 4), *to1 = line + (((2 * k + 1) ^ (row & 7)) << 4);
 #pragma unroll 4
@@ -799,9 +805,11 @@ int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaSt
   int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc != KCH_OK) return rc;
-#define PT_FEW(D_, K_) (few ? pt_launch<D_, K_, true>(km, vm, a, ctas, s) : pt_launch<D_, K_, false>(km, vm, a, ctas, s))
-#define PT_KIND(D_) (kind == KCH_BF16 ? PT_FEW(D_, KCH_BF16) : kind == KCH_FP8_E4M3 ? PT_FEW(D_, KCH_FP8_E4M3) : PT_FEW(D_, KCH_INT8))
+#define PT_GO(D_, K_, F_) pt_launch<D_, K_, F_>(km, vm, a, ctas, s)
+#define PT_KIND(D_)                                                                            \
+  (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, false) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, false) \
+   : few ? PT_GO(D_, KCH_BF16, true) : PT_GO(D_, KCH_BF16, false))
   return a.c == 64 ? PT_KIND(64) : PT_KIND(128);
 #undef PT_KIND
-#undef PT_FEW
+#undef PT_GO
 }

@@ -27,7 +27,8 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
               (long long)b->ld_table);
   KCH_REQUIRE(b->table && b->t0 && b->cu_seqlens, "%s: null table, t0 or cu_seqlens", fn);
   KCH_REQUIRE(p->k && p->v && (((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0, "%s: pages must be 16-byte aligned", fn);
-  KCH_REQUIRE(p->kind < KCH_FP8_E4M3 || (p->k_scales && p->v_scales), "%s: 8-bit pages need their scales", fn);
+  KCH_REQUIRE(p->kind < KCH_FP8_E4M3 || (p->k_scales && p->v_scales && (((uintptr_t)p->k_scales | (uintptr_t)p->v_scales) & 15) == 0),
+              "%s: 8-bit pages need their scales, 16-byte aligned", fn);
   return KCH_OK;
 }
 
@@ -51,6 +52,7 @@ struct PgRows {
   void* pages[2]; float* scales[2];
   int n_kv, c, page, kind, zero_rest;
   int tokens;                          // of a warp at a time: 1 or 2
+  int parts;                           // warps that share a token's rows
 };
 #define PC_THREADS 256
 #define PC_SMEM_B 2048                 // batches up to this search cu_seqlens in shared memory
@@ -132,7 +134,7 @@ __device__ __forceinline__ PcWords<T> pc_words(const void* p) {
 }
 
 // A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
-// looked up once a token, and four rows a thread are in flight.  READ: pages -> packed rows, else packed rows -> pages.
+// looked up once a token, and four rows a thread are in flight.  Where tokens are few, several warps share one's rows.  READ: pages -> packed rows, else packed rows -> pages.
 #define PC_FLIGHT 4
 template <typename T, int GROUP, bool READ, bool Q8>
 __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_constant__ PgRows a) {
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
     cu = scu;
   }
   const int lane = threadIdx.x & 31, each = 32 / a.tokens, mine = lane & (each - 1);      // lanes of a token, this one among them
-  const int d = (mine & (GROUP - 1)) * 8, row0 = mine / GROUP, rows = 2 * a.n_kv, step = each / GROUP;
+  const int d = (mine & (GROUP - 1)) * 8, rows = 2 * a.n_kv, step = each / GROUP * a.parts, row0 = mine / GROUP + each / GROUP * blockIdx.y;
   const bool in_row = d < a.c;
   for (int64_t t0 = ((int64_t)blockIdx.x * (PC_THREADS / 32) + (threadIdx.x >> 5)) * a.tokens; t0 < a.bt.N;
        t0 += (int64_t)gridDim.x * (PC_THREADS / 32) * a.tokens) {
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
     } else {
       const bool here = site >= 0 && in_row;
       // (all lanes of the warp take the same rounds: a row's maximum is found by shuffles)
-      for (int r0 = 0; r0 < rows; r0 += step * PC_FLIGHT) {
+      for (int r0 = 0; r0 < rows; r0 += step * PC_FLIGHT) {      // (row0 counts from there)
         float x[PC_FLIGHT][8] = {};
 #pragma unroll
         for (int i = 0; i < PC_FLIGHT; ++i) {
@@ -261,7 +263,11 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   const int pieces = p->c / 8, group = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
   a.tokens = 2 * p->n_kv * group <= 16 ? 2 : 1;
   const int64_t blocks = ceil_div64(b->N, PC_THREADS / 32 * a.tokens);
-  const unsigned grid = (unsigned)(blocks < 8 * KCH_SMS ? blocks : 8 * KCH_SMS);
+  // as many warps to a token as it has rounds of rows, while they are fewer than 16 to an SM
+  const int rounds = (int)ceil_div64(2 * p->n_kv * group * a.tokens, 32);
+  a.parts = (int)(blocks * (PC_THREADS / 32) >= 16 * KCH_SMS ? 1 : ceil_div64(16 * KCH_SMS, blocks * (PC_THREADS / 32)));
+  if (a.parts > rounds) a.parts = rounds;
+  const dim3 grid((unsigned)(blocks < 8 * KCH_SMS ? blocks : 8 * KCH_SMS), (unsigned)a.parts);
 #define PC_GO(T_, G_, Q_)                                                                                                \
   do {                                                                                                                   \
     if (read) paged_rows_kernel<T_, G_, true, Q_><<<grid, PC_THREADS, 0, s>>>(a);                                        \
