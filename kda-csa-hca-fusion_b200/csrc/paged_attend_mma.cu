@@ -7,8 +7,9 @@
 // matter): through tiles of tcgen05 the same step took twice as long, for the tiles are written, fenced and read back.
 //
 // An item is up to 16 (token, head of the group) rows of a sequence; a tile is 128 keys, its payloads and scales copied into a ring by
-// one warp (TMA, 128-byte or 64-byte swizzle; scales by bulk copies).  Warp w of eight has keys 16 w .. 16 w + 15 of every tile, with a
-// maximum, a sum and an O of its own, so that nothing but the ring is waited for; they are joined when the item ends.
+// one warp (TMA, 128-byte or 64-byte swizzle; scales by bulk copies).  Four warps share a tile, 32 keys each, and the other four take
+// the next one; a warp has a maximum, a sum and an O of its own, so that nothing but the ring is waited for, and they are joined when
+// the item ends.  (With 16 keys a warp and tile there were too few instructions that do not wait for one another: 2900 clocks a tile.)
 //   S = Q K^T: the order of the contraction is free, so thread (g, t) of a fragment takes 32 (16) consecutive channels of key g, four of
 //     them a product: a row is read in 16-byte words, and the queries' fragments are loaded in the same order.
 //   O += P V:  the order of the columns is free, so thread (g, t) takes 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9,
@@ -31,15 +32,16 @@
 
 template <int D>
 struct PmSmem {
-  static constexpr int STAGES = D == 128 ? 5 : 8;
+  static constexpr int STAGES = D == 128 ? 4 : 8;        // (even: a stage is always the same warps')
   alignas(1024) uint8_t k[STAGES][PM_KT * D], v[STAGES][PM_KT * D];
   alignas(16) float ks[STAGES][PM_KT], vs[STAGES][PM_KT];
   alignas(16) float stage[PM_WARPS][8 * D];
+  alignas(16) uint4 q[D / 16][32];                       // fragments of the queries: contraction step, lane
   float ml[2][PM_WARPS][PM_R];
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
 static_assert(sizeof(PmSmem<128>) <= 232448 && sizeof(PmSmem<64>) <= 232448, "shared memory of the paged attention over 8-bit pages");
-static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 5 * PM_KT * 64, "the plan lies in the ring of tiles");
+static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * PM_KT * 64, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pm_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
   asm volatile(
@@ -64,6 +66,12 @@ __device__ __forceinline__ uint32_t pm_pair(uint32_t x, uint32_t y, int i, int j
   const uint32_t sel = KIND == KCH_FP8_E4M3 ? (i << 4) | ((4 + j) << 12) : i | ((4 + j) << 8);
   return pm_value2<KIND>(__byte_perm(x, y, sel));
 }
+// (not volatile: products, conversions and the softmax of a tile may be mixed)
+__device__ __forceinline__ void pm_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint4 pm_lds(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 template <int D, int KIND>
@@ -79,7 +87,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
   if (tid == 0) {
-    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 1); mbarrier_init(&sm.empty[i], PM_WARPS); }
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 1); mbarrier_init(&sm.empty[i], PM_WARPS / 2); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -142,19 +150,19 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   int n = 0;                                             // tiles of the ring
   bool ok = true, part = false;
   for (Walk w(a.bt, place); w.valid(); w.next()) {
-    // queries of rows g and g + 8: channels RUN t .. RUN t + RUN - 1
-    uint32_t q[KS][4];
+    // queries: of step i the lane (g, t) has channels RUN t + 4 i .. + 3 of rows g and g + 8
+    for (int i = tid; i < KS * 32; i += 32 * PM_WARPS) {
+      const int gg = (i & 31) >> 2, d = RUN * (i & 3) + 4 * (i >> 5);
+      uint2 u[2] = {};
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int i = g + 8 * hf, row = w.block * PM_R + i, tok = pg_token(a.bt, row);
-      const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + RUN * t;
-#pragma unroll
-      for (int c = 0; c < RUN / 8; ++c) {
-        const uint4 u = i < w.x.rows ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
-        q[2 * c][hf] = u.x ^ flip; q[2 * c][2 + hf] = u.y ^ flip;
-        q[2 * c + 1][hf] = u.z ^ flip; q[2 * c + 1][2 + hf] = u.w ^ flip;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int row = w.block * PM_R + gg + 8 * hf, tok = pg_token(a.bt, row);
+        if (gg + 8 * hf < w.x.rows)
+          u[hf] = __ldg(reinterpret_cast<const uint2*>((const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + d));
       }
+      sm.q[i >> 5][i & 31] = make_uint4(u[0].x ^ flip, u[1].x ^ flip, u[0].y ^ flip, u[1].y ^ flip);
     }
+    sync();
     int2 keys[2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
@@ -164,37 +172,51 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
     for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
-      const int st = n % S::STAGES, key0 = w.x.first_key + tile * PM_KT + 16 * warp;      // of the warp's 16 keys
+      if ((n & 1) != (warp >> 2)) continue;
+      const int st = n % S::STAGES, base = 32 * (warp & 3), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's 32 keys
       if (ok) ok = wait(&sm.full[st], n / S::STAGES);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && key0 < k1.y && key0 + 16 > k0.x) {
+      if (ok && key0 < k1.y && key0 + 32 > k0.x) {
         const uint8_t *tk = sm.k[st], *tv = sm.v[st];
-        float s[2][4];
+        float s[4][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
-          const int r = 16 * warp + 8 * h + g;
-          uint32_t c[KS];
+        for (int h = 0; h < 4; ++h) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
 #pragma unroll
-          for (int i = 0; i < RUN / 16; ++i) {
-            const uint4 u = pm_lds(tk + word(r, RUN / 16 * t + i));
-            c[4 * i] = u.x; c[4 * i + 1] = u.y; c[4 * i + 2] = u.z; c[4 * i + 3] = u.w;
+        for (int i4 = 0; i4 < KS; i4 += 4) {             // 16 bytes of each key's run
+          uint4 kc[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) kc[h] = pm_lds(tk + word(base + 8 * h + g, RUN / 16 * t + (i4 >> 2)));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 u = sm.q[i4 + i][lane];
+            const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const uint32_t c = i == 0 ? kc[h].x : i == 1 ? kc[h].y : i == 2 ? kc[h].z : kc[h].w;
+              pm_mma(s[h], q, pm_pair<KIND>(c, c, 0, 1), pm_pair<KIND>(c, c, 2, 3));
+            }
           }
-#pragma unroll
-          for (int i = 0; i < KS; ++i) mma_bf16_16816(s[h], q[i], pm_pair<KIND>(c[i], c[i], 0, 1), pm_pair<KIND>(c[i], c[i], 2, 3));
         }
         // scaled; what a row does not see is -inf
-        const bool whole = key0 >= k1.x && key0 + 16 <= k0.y && w.x.rows == PM_R;
-        bool sees[2][4];
+        const bool whole = key0 >= k1.x && key0 + 32 <= k0.y && w.x.rows == PM_R;
+        uint32_t sees = 0xFFFFu;                         // bit 4 h + e
+        if (!whole) {
+          sees = 0u;
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + 8 * h + 2 * t + (e & 1);
+              if (key >= keys[e >> 1].x && key < keys[e >> 1].y) sees |= 1u << (4 * h + e);
+            }
+        }
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 f = *reinterpret_cast<const float2*>(&sm.ks[st][16 * warp + 8 * h + 2 * t]);
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = *reinterpret_cast<const float2*>(&sm.ks[st][base + 8 * h + 2 * t]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = key0 + 8 * h + 2 * t + (e & 1);
-            sees[h][e] = whole || (key >= keys[e >> 1].x && key < keys[e >> 1].y);
-            s[h][e] = sees[h][e] ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
+            s[h][e] = sees & (1u << (4 * h + e)) ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
             top[e >> 1] = fmaxf(top[e >> 1], s[h][e]);
           }
         }
@@ -214,36 +236,39 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           for (int j = 0; j < NT; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
         }
         const float sh0 = m[0] == -INFINITY ? 0.f : m[0] * sc, sh1 = m[1] == -INFINITY ? 0.f : m[1] * sc;
-        uint32_t p[4];
+        uint32_t p[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][16 * warp + 8 * h + 2 * t]);
+        for (int h = 0; h < 4; ++h) {
+          const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][base + 8 * h + 2 * t]);
           float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             x[e] = ex2_fast(fmaf(s[h][e], sc, -(e >> 1 ? sh1 : sh0)));
             l[e >> 1] += x[e];
-            x[e] = sees[h][e] ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
+            x[e] = sees & (1u << (4 * h + e)) ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
           }
-          p[2 * h] = pack2_bf16(x[0], x[1]);
-          p[2 * h + 1] = pack2_bf16(x[2], x[3]);
+          p[h >> 1][2 * (h & 1)] = pack2_bf16(x[0], x[1]);
+          p[h >> 1][2 * (h & 1) + 1] = pack2_bf16(x[2], x[3]);
         }
-        // channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t c[4][NT / 4];
+        // of the values channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half of the 32
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * warp + 2 * t + (i & 1) + 8 * (i >> 1);
-          if (D == 128) {
-            const uint4 u = pm_lds(tv + word(r, g));
-            c[i][0] = u.x; c[i][1] = u.y; c[i][NT / 4 - 2] = u.z; c[i][NT / 4 - 1] = u.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(tv + word(r, g >> 1) + 8 * (g & 1));
-            c[i][0] = u.x; c[i][1] = u.y;
+        for (int b = 0; b < 2; ++b) {
+          uint32_t c[4][NT / 4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = base + 16 * b + 2 * t + (i & 1) + 8 * (i >> 1);
+            if constexpr (D == 128) {
+              const uint4 u = pm_lds(tv + word(r, g));
+              c[i][0] = u.x; c[i][1] = u.y; c[i][2] = u.z; c[i][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(tv + word(r, g >> 1) + 8 * (g & 1));
+              c[i][0] = u.x; c[i][1] = u.y;
+            }
           }
-        }
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          mma_bf16_16816(o[j], p, pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3));
+          for (int j = 0; j < NT; ++j)
+            pm_mma(o[j], p[b], pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3));
+        }
       }
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sm.empty[st]);
