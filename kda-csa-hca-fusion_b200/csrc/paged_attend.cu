@@ -386,7 +386,7 @@ PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c);
 int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s);
-int kch_paged_attend_mma(const PgAttend& a, int kind, int ctas, cudaStream_t s);
+int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.
 struct PaPlan { bool tc5; int rows, ctas, slot_rows; };
@@ -395,7 +395,7 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
   x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
   const int64_t B = p->batch.B;
-  if (x.tc5) x.rows = rows > 32 * B || p->batch.N > 4 * B ? 256 : p->cache.kind == KCH_BF16 ? 32 : 16;
+  if (x.tc5) x.rows = rows > 32 * B || p->batch.N > 4 * B ? 256 : p->cache.kind == KCH_BF16 ? 32 : rows <= 8 * B ? 8 : 16;
   else x.rows = rows <= 16 * B ? 16 : 64;
   x.ctas = x.tc5 ? KCH_SMS : PA_CTAS;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
@@ -447,7 +447,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   const bool whole = x.tc5 ? a.bt.cap <= 128 * (x.rows == 32 || (x.rows == 256 && (int64_t)a.bt.N * a.bt.G <= 128) ? 2 : 1) : a.bt.cap <= PA_KT;
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.tc5) {
-    const int rc5 = x.rows == 16 ? kch_paged_attend_mma(a, p->cache.kind, x.ctas, s) : kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
+    const int rc5 = x.rows <= 16 ? kch_paged_attend_mma(a, p->cache.kind, x.rows, x.ctas, s) : kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);

@@ -24,23 +24,31 @@
 #include "paged.cuh"
 #include "tc5_utils.cuh"
 
-#define PM_R 16
 #define PM_KT 128
-#define PM_WARPS 8
-#define PM_THREADS (32 * PM_WARPS + 32)
 #define PM_SPIN (1u << 22)
 
-template <int D>
+// R rows an item: 16, or 8 where a sequence has no more (one token of up to 8 heads): the lower half of every fragment is empty then, and
+// the registers that it leaves hold twice as many warps.
+template <int R>
+struct PmCfg {
+  static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;      // that compute; the first warpgroup copies
+  static constexpr int SLICE = 2 * PM_KT / WARPS, H = SLICE / 8;                // keys of a warp in a tile; in eights
+  static constexpr int HF = R / 8;                                              // rows of a thread
+  static constexpr int REG_FEED = 64, REG_WORK = 216, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
+};
+template <int D, int R>
 struct PmSmem {
+  typedef PmCfg<R> C;
   static constexpr int STAGES = D == 128 ? 4 : 8;        // (even: a stage is always the same warps')
   alignas(1024) uint8_t k[STAGES][PM_KT * D], v[STAGES][PM_KT * D];
   alignas(16) float ks[STAGES][PM_KT], vs[STAGES][PM_KT];
-  alignas(16) float stage[PM_WARPS][8 * D];
+  alignas(16) float stage[C::WARPS][8 * D];
   alignas(16) uint4 q[D / 16][32];                       // fragments of the queries: contraction step, lane
-  float ml[2][PM_WARPS][PM_R];
+  float ml[2][C::WARPS][R];
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
-static_assert(sizeof(PmSmem<128>) <= 232448 && sizeof(PmSmem<64>) <= 232448, "shared memory of the paged attention over 8-bit pages");
+static_assert(sizeof(PmSmem<128, 16>) <= 232448 && sizeof(PmSmem<128, 8>) <= 232448, "shared memory of the paged attention over 8-bit pages");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * PM_KT * 64, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pm_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -72,13 +80,20 @@ __device__ __forceinline__ void pm_mma(float (&d)[4], const uint32_t (&a)[4], ui
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void pm_mma(float (&d)[2], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // rows 8 .. 15: zeros
+  float x, y;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%9,%10,%11,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(x), "=f"(y)
+      : "r"(a[0]), "r"(0), "r"(a[2]), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(0.f));
+}
 __device__ __forceinline__ uint4 pm_lds(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-template <int D, int KIND>
-__global__ void __launch_bounds__(PM_THREADS, 1)
+template <int D, int KIND, int R>
+__global__ void __launch_bounds__(PmCfg<R>::THREADS, 1)
 paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
-  typedef PmSmem<D> S;
-  typedef PgWalk<PM_R, PM_KT, 0> Walk;
+  typedef PmSmem<D, R> S;
+  typedef PmCfg<R> C;
+  typedef PgWalk<R, PM_KT, 0> Walk;
   extern __shared__ __align__(1024) uint8_t pm_raw[];
   S& sm = *reinterpret_cast<S*>(pm_raw);
   if (smem_addr_u32(pm_raw) & 1023) {                    // (every block begins its memory there)
@@ -87,21 +102,23 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
   if (tid == 0) {
-    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 1); mbarrier_init(&sm.empty[i], PM_WARPS / 2); }
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::WARPS / 2); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
-  const PgPlace place = pg_plan<PM_R, PM_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<R, PM_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   __syncthreads();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, PM_SPIN, a.bt.status); };
 
-  if (warp == PM_WARPS) {
-    // ------------------------------ pages into the ring: a box of a tile each lane -------------------------------------------
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
+    // ------------------------------ pages into the ring: keys, values and the scales of either a warp, a box each lane ------------
+    // (one warp that issued all four took 180 us for 64 sequences in pages of 16 whose bytes are 45 us)
     const int box = min(a.page, PM_KT), boxes = PM_KT / box;
-    const bool mine = lane < boxes;
+    const bool mine = lane < boxes, scales = warp >= 2, values = warp & 1;
     int g = 0;
     bool ok = true;
     for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
@@ -118,17 +135,17 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         ok = g < S::STAGES || wait(&sm.empty[st], g / S::STAGES - 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbarrier_expect_tx(&sm.full[st], 2 * PM_KT * (D + 4));
+        if (lane == 0) mbarrier_expect_tx(&sm.full[st], PM_KT * (scales ? 4 : D));
         __syncwarp();
         if (mine) {
           const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
           if (!there && tile < w.x.tiles && key < w.s.kv) pg_bad(a.bt);
-          const int pg = there ? id : (int)a.bt.num_pages, r0 = key & (a.page - 1);      // out of range: zeros,
-          const int64_t at = ((int64_t)(there ? id : 0) * n_kv + w.h) * a.page + r0;     // with the scales of some page
-          pm_tma_4d(sm.k[st] + lane * box * D, &kmap, 0, r0, w.h, pg, &sm.full[st]);
-          bulk_copy_g2s(sm.ks[st] + lane * box, a.ks + at, box * 4, &sm.full[st]);
-          pm_tma_4d(sm.v[st] + lane * box * D, &vmap, 0, r0, w.h, pg, &sm.full[st]);
-          bulk_copy_g2s(sm.vs[st] + lane * box, a.vs + at, box * 4, &sm.full[st]);
+          const int r0 = key & (a.page - 1);             // out of range: zeros, with the scales of some page
+          if (scales)
+            bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (values ? a.vs : a.ks) + ((int64_t)(there ? id : 0) * n_kv + w.h) * a.page + r0,
+                          box * 4, &sm.full[st]);
+          else
+            pm_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * D, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
         }
         id = next;
       }
@@ -138,121 +155,132 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     return;
   }
 
-  // ------------------------------ the eight warps ---------------------------------------------------------------------------------
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_WORK));
+  // ------------------------------ the warps that compute ---------------------------------------------------------------------------------
   constexpr int KS = D / 16, NT = D / 8, RUN = D / 4;    // contraction steps; column tiles; channels of a key a thread has
-  const int g = lane >> 2, t = lane & 3;
+  const int g = lane >> 2, t = lane & 3, cw = warp - 4, ct = tid - 128;      // (counted from the first of them)
   const float sc = fmaxf(fabsf(a.scale), 1e-30f);        // (not 0: a masked logit is -inf)
   const float raise = 8.f / sc;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;      // the sign goes to the queries: a maximum stays one
-  const auto sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+  const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::WARPS) : "memory"); };
   // byte of the tile at which the 16-byte word `c` of row r lies (D = 128: words swizzled by the row; D = 64: by every second)
   const auto word = [](int r, int c) { return r * D + ((D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); };
   int n = 0;                                             // tiles of the ring
   bool ok = true, part = false;
   for (Walk w(a.bt, place); w.valid(); w.next()) {
     // queries: of step i the lane (g, t) has channels RUN t + 4 i .. + 3 of rows g and g + 8
-    for (int i = tid; i < KS * 32; i += 32 * PM_WARPS) {
+    for (int i = ct; i < KS * 32; i += 32 * C::WARPS) {
       const int gg = (i & 31) >> 2, d = RUN * (i & 3) + 4 * (i >> 5);
       uint2 u[2] = {};
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int row = w.block * PM_R + gg + 8 * hf, tok = pg_token(a.bt, row);
+      for (int hf = 0; hf < C::HF; ++hf) {
+        const int row = w.block * R + gg + 8 * hf, tok = pg_token(a.bt, row);
         if (gg + 8 * hf < w.x.rows)
           u[hf] = __ldg(reinterpret_cast<const uint2*>((const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + d));
       }
       sm.q[i >> 5][i & 31] = make_uint4(u[0].x ^ flip, u[1].x ^ flip, u[0].y ^ flip, u[1].y ^ flip);
     }
     sync();
-    int2 keys[2];
+    constexpr int HF = C::HF, E = 2 * HF;                // values of a thread in a tile of 8 keys (columns): two a row
+    int2 keys[HF];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
-      keys[hf] = g + 8 * hf < w.x.rows ? pg_sees(a.bt, w.s, w.block * PM_R + g + 8 * hf) : make_int2(0, 0);
-    const int2 k0 = pg_sees(a.bt, w.s, w.block * PM_R), k1 = pg_sees(a.bt, w.s, w.block * PM_R + w.x.rows - 1);      // first and last row's
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[NT][4];
+    for (int hf = 0; hf < HF; ++hf)
+      keys[hf] = g + 8 * hf < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + g + 8 * hf) : make_int2(0, 0);
+    const int2 k0 = pg_sees(a.bt, w.s, w.block * R), k1 = pg_sees(a.bt, w.s, w.block * R + w.x.rows - 1);      // first and last row's
+    float m[HF], l[HF], o[NT][E];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int hf = 0; hf < HF; ++hf) { m[hf] = -INFINITY; l[hf] = 0.f; }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[j][e] = 0.f;
     for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
-      if ((n & 1) != (warp >> 2)) continue;
-      const int st = n % S::STAGES, base = 32 * (warp & 3), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's 32 keys
+      if ((n & 1) != cw / (C::WARPS / 2)) continue;
+      const int st = n % S::STAGES, base = C::SLICE * (cw % (C::WARPS / 2)), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's keys
       if (ok) ok = wait(&sm.full[st], n / S::STAGES);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && key0 < k1.y && key0 + 32 > k0.x) {
+      if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
         const uint8_t *tk = sm.k[st], *tv = sm.v[st];
-        float s[4][4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
+        float s[C::H][E] = {};
 #pragma unroll
         for (int i4 = 0; i4 < KS; i4 += 4) {             // 16 bytes of each key's run
-          uint4 kc[4];
+          uint4 kc[C::H];
 #pragma unroll
-          for (int h = 0; h < 4; ++h) kc[h] = pm_lds(tk + word(base + 8 * h + g, RUN / 16 * t + (i4 >> 2)));
+          for (int h = 0; h < C::H; ++h) kc[h] = pm_lds(tk + word(base + 8 * h + g, RUN / 16 * t + (i4 >> 2)));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 u = sm.q[i4 + i][lane];
             const uint32_t q[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
+            for (int h = 0; h < C::H; ++h) {
               const uint32_t c = i == 0 ? kc[h].x : i == 1 ? kc[h].y : i == 2 ? kc[h].z : kc[h].w;
               pm_mma(s[h], q, pm_pair<KIND>(c, c, 0, 1), pm_pair<KIND>(c, c, 2, 3));
             }
           }
         }
         // scaled; what a row does not see is -inf
-        const bool whole = key0 >= k1.x && key0 + 32 <= k0.y && w.x.rows == PM_R;
-        uint32_t sees = 0xFFFFu;                         // bit 4 h + e
+        const bool whole = key0 >= k1.x && key0 + C::SLICE <= k0.y && w.x.rows == R;
+        uint32_t sees = 0xFFFFu;                         // bit E h + e
         if (!whole) {
           sees = 0u;
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
+          for (int h = 0; h < C::H; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < E; ++e) {
               const int key = key0 + 8 * h + 2 * t + (e & 1);
-              if (key >= keys[e >> 1].x && key < keys[e >> 1].y) sees |= 1u << (4 * h + e);
+              if (key >= keys[e >> 1].x && key < keys[e >> 1].y) sees |= 1u << (E * h + e);
             }
         }
-        float top[2] = {-INFINITY, -INFINITY};
+        float top[HF];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
+        for (int hf = 0; hf < HF; ++hf) top[hf] = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < C::H; ++h) {
           const float2 f = *reinterpret_cast<const float2*>(&sm.ks[st][base + 8 * h + 2 * t]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[h][e] = sees & (1u << (4 * h + e)) ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
+          for (int e = 0; e < E; ++e) {
+            s[h][e] = sees & (1u << (E * h + e)) ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
             top[e >> 1] = fmaxf(top[e >> 1], s[h][e]);
           }
         }
+        bool up[HF], any = false;                        // a row's maximum is raised only when it is exceeded by 2^8
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < HF; ++hf) {
           top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
           top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
+          up[hf] = m[hf] == -INFINITY ? top[hf] > m[hf] : top[hf] > m[hf] + raise;
+          any = any || up[hf];
         }
-        // a row's maximum is raised only when it is exceeded by 2^8
-        const bool up0 = m[0] == -INFINITY ? top[0] > m[0] : top[0] > m[0] + raise, up1 = m[1] == -INFINITY ? top[1] > m[1] : top[1] > m[1] + raise;
-        if (__any_sync(0xffffffffu, up0 || up1)) {
-          const float n0 = up0 ? top[0] : m[0], n1 = up1 ? top[1] : m[1];
-          const float f0 = up0 ? ex2_fast((m[0] - n0) * sc) : 1.f, f1 = up1 ? ex2_fast((m[1] - n1) * sc) : 1.f;
-          m[0] = n0; m[1] = n1;
-          l[0] *= f0; l[1] *= f1;
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-        }
-        const float sh0 = m[0] == -INFINITY ? 0.f : m[0] * sc, sh1 = m[1] == -INFINITY ? 0.f : m[1] * sc;
-        uint32_t p[2][4];
+          for (int hf = 0; hf < HF; ++hf) {
+            const float f = up[hf] ? ex2_fast((m[hf] - top[hf]) * sc) : 1.f;
+            if (up[hf]) m[hf] = top[hf];
+            l[hf] *= f;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][base + 8 * h + 2 * t]);
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = ex2_fast(fmaf(s[h][e], sc, -(e >> 1 ? sh1 : sh0)));
-            l[e >> 1] += x[e];
-            x[e] = sees & (1u << (4 * h + e)) ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
+            for (int j = 0; j < NT; ++j) { o[j][2 * hf] *= f; o[j][2 * hf + 1] *= f; }
           }
-          p[h >> 1][2 * (h & 1)] = pack2_bf16(x[0], x[1]);
-          p[h >> 1][2 * (h & 1) + 1] = pack2_bf16(x[2], x[3]);
+        }
+        float shift[HF];
+#pragma unroll
+        for (int hf = 0; hf < HF; ++hf) shift[hf] = m[hf] == -INFINITY ? 0.f : m[hf] * sc;
+        uint32_t p[C::H / 2][4] = {};
+#pragma unroll
+        for (int h = 0; h < C::H; ++h) {
+          const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][base + 8 * h + 2 * t]);
+          float x[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            x[e] = ex2_fast(fmaf(s[h][e], sc, -shift[e >> 1]));
+            l[e >> 1] += x[e];
+            x[e] = sees & (1u << (E * h + e)) ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
+          }
+#pragma unroll
+          for (int hf = 0; hf < HF; ++hf) p[h >> 1][2 * (h & 1) + hf] = pack2_bf16(x[2 * hf], x[2 * hf + 1]);
         }
         // of the values channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half of the 32
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < C::H / 2; ++b) {
           uint32_t c[4][NT / 4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -277,24 +305,24 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const bool direct = w.starts() && w.ends();
     float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(a.slot_rows, D);
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < HF; ++hf) {
       l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
       l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
       if (t == 0) {
-        sm.ml[0][warp][g + 8 * hf] = m[hf];
-        sm.ml[1][warp][g + 8 * hf] = l[hf];
+        sm.ml[0][cw][g + 8 * hf] = m[hf];
+        sm.ml[1][cw][g + 8 * hf] = l[hf];
       }
     }
     sync();
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < HF; ++hf) {
       if (8 * hf >= w.x.rows) break;                     // (the same for all warps)
       const int i = g + 8 * hf;
       float mm = sm.ml[0][0][i];
 #pragma unroll
-      for (int k = 1; k < PM_WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][i]);
+      for (int k = 1; k < C::WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][i]);
       const float own = m[hf] == -INFINITY ? 0.f : ex2_fast((m[hf] - mm) * sc);      // (0 for a part without a key)
-      float4* mine = reinterpret_cast<float4*>(sm.stage[warp]) + g * (D / 4);
+      float4* mine = reinterpret_cast<float4*>(sm.stage[cw]) + g * (D / 4);
       // 16-byte words of a row, swizzled within runs of 8 so that 8 threads meet in no bank
 #pragma unroll
       for (int c = 0; c < RUN / 4; ++c) {
@@ -303,24 +331,24 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][e] * own, o[j + 1][e] * own, o[j + 2][e] * own, o[j + 3][e] * own);
       }
       sync();
-      for (int k = tid; k < 8 * (D / 4); k += 32 * PM_WARPS) {
+      for (int k = ct; k < 8 * (D / 4); k += 32 * C::WARPS) {
         const int r = k / (D / 4), c = k % (D / 4), row = 8 * hf + r, tt = c / (RUN / 4);
         if (row >= w.x.rows || !ok) continue;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         const int at = r * (D / 4) + (c ^ ((D == 128 ? tt : 2 * (tt & 1)) + 4 * (r & 1)));
 #pragma unroll
-        for (int i2 = 0; i2 < PM_WARPS; ++i2) {
+        for (int i2 = 0; i2 < C::WARPS; ++i2) {
           const float4 y = reinterpret_cast<const float4*>(sm.stage[i2])[at];
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         float top = sm.ml[0][0][row], sum = 0.f;
 #pragma unroll
-        for (int i2 = 1; i2 < PM_WARPS; ++i2) top = fmaxf(top, sm.ml[0][i2][row]);
+        for (int i2 = 1; i2 < C::WARPS; ++i2) top = fmaxf(top, sm.ml[0][i2][row]);
         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int i2 = 0; i2 < PM_WARPS; ++i2) sum += sm.ml[1][i2][row] * ex2_fast((sm.ml[0][i2][row] - ref) * sc);      // (a NaN stays one)
+        for (int i2 = 0; i2 < C::WARPS; ++i2) sum += sm.ml[1][i2][row] * ex2_fast((sm.ml[0][i2][row] - ref) * sc);      // (a NaN stays one)
         if (direct) {
-          const int rr = w.block * PM_R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
+          const int rr = w.block * R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
           float below = sum;
           if (a.sink && sum > 0.f) below += ex2_fast(ld_any(a.sink, head, a.sink_dtype) * PG_LOG2E - ref * sc);
           const float f = sum == 0.f ? 0.f : 1.f / below;
@@ -338,39 +366,42 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
     if (w.starts() && !w.ends()) {
       part = true;
-      if (tid == 0)
+      if (ct == 0)
         a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
                                  w.x.rows, w.s.row0};
     }
   }
-  if (tid == 0 && !part) a.records[blockIdx.x].valid = 0;
+  if (ct == 0 && !part) a.records[blockIdx.x].valid = 0;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
                               uint32_t box_rows);
 
-template <int D, int KIND>
+template <int D, int KIND, int R>
 static int pm_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
-  const int smem = (int)sizeof(PmSmem<D>);
+  const int smem = (int)sizeof(PmSmem<D, R>);
   static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
   int dev = 0;
   KCH_CUDA_OK(cudaGetDevice(&dev));
   if (dev > 63 || !((done.load(std::memory_order_relaxed) >> dev) & 1)) {
-    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_mma_kernel<D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_mma_kernel<D, KIND, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
   }
-  paged_attend_mma_kernel<D, KIND><<<ctas, PM_THREADS, smem, s>>>(km, vm, a);
+  paged_attend_mma_kernel<D, KIND, R><<<ctas, PmCfg<R>::THREADS, smem, s>>>(km, vm, a);
   KCH_LAUNCH_OK();
   return KCH_OK;
 }
 
-int kch_paged_attend_mma(const PgAttend& a, int kind, int ctas, cudaStream_t s) {
+int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
   const int box = a.page < PM_KT ? a.page : PM_KT;
   int rc = kch_make_tensor_map_pages(&km, a.k, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc != KCH_OK) return rc;
-  if (a.c == 64) return kind == KCH_FP8_E4M3 ? pm_launch<64, KCH_FP8_E4M3>(km, vm, a, ctas, s) : pm_launch<64, KCH_INT8>(km, vm, a, ctas, s);
-  return kind == KCH_FP8_E4M3 ? pm_launch<128, KCH_FP8_E4M3>(km, vm, a, ctas, s) : pm_launch<128, KCH_INT8>(km, vm, a, ctas, s);
+#define PM_ROWS(D_, K_) (rows == 8 ? pm_launch<D_, K_, 8>(km, vm, a, ctas, s) : pm_launch<D_, K_, 16>(km, vm, a, ctas, s))
+#define PM_KIND(D_) (kind == KCH_FP8_E4M3 ? PM_ROWS(D_, KCH_FP8_E4M3) : PM_ROWS(D_, KCH_INT8))
+  return a.c == 64 ? PM_KIND(64) : PM_KIND(128);
+#undef PM_KIND
+#undef PM_ROWS
 }
