@@ -443,7 +443,7 @@ typedef struct kch_paged_batch {
 
 /* Writes the packed rows k, v [N, n_kv, c] (tokens ld_k / ld_v elements apart) into their pages.  8-bit kinds: s = max |x| / 448
  * (e4m3) or / 127 (int8) over the row of a key head, 1 for a row of zeros; stored round(x / s), ties to even.  A row that is not
- * finite reads back as NaN.  A position that occurs twice in a batch holds either row. */
+ * finite reads back as NaN.  What a position that occurs twice in a batch holds is undefined. */
 int kch_paged_append(const kch_paged_cache* cache, const kch_paged_batch* batch, const void* k, int64_t ld_k, const void* v,
                      int64_t ld_v, int dtype, void* stream);
 /* Reads the rows of those positions back as packed rows in `dtype`: stored value times scale, rounded once.  Rows of no sequence:
@@ -454,7 +454,9 @@ int kch_paged_read(const kch_paged_cache* cache, const kch_paged_batch* batch, v
 /* Attention of the new tokens over the pages, which hold them already: query i of sequence b stands at position t0[b] + i and
  * sees the keys up to it, the last `sliding_window` of them where that is not 0; query head h reads key head h / (nh / n_kv).
  * The sink logit of a head (optional) adds to the denominator.  q [N, nh, c] (tokens ld_q elements apart) and out [N, nh, c] in
- * `dtype`, which is that of the cache's activations.  Rows of no sequence: zeros with `zero_rest`, else left as they are. */
+ * `dtype`, which is that of the cache's activations.  Rows of no sequence: zeros with `zero_rest`, else left as they are.  A row
+ * without keys is 0.  What a row does not see (other pages, rows behind a sequence's end, later or older keys) does not reach it,
+ * numbers or not; an infinity or a NaN among the values that other rows of a tile see costs time, though. */
 typedef struct kch_paged_attend_args {
   kch_paged_cache cache;
   kch_paged_batch batch;

@@ -25,7 +25,7 @@
 #include "tc5_utils.cuh"
 
 #define PM_KT 128
-#define PM_SPIN (1u << 22)
+#define PM_SPIN (1u << 26)
 
 // R rows an item: 16, or 8 where a sequence has no more (one token of up to 8 heads): the lower half of every fragment is empty then, and
 // the registers that it leaves hold twice as many warps.

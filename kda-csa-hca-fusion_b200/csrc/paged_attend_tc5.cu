@@ -19,9 +19,10 @@
 // The running maximum of a row is raised, and O_X rescaled, only when a tile exceeds it by 2^8: probabilities up to 256 lose
 // nothing in bf16 or in the fp32 sums, and the accumulator makes its way through registers only a few times a row.
 //
-// Keys behind a sequence's end read as zeros where a whole page is missing (an out-of-range coordinate of the copy) or are what the
-// page holds; p = 0 there, which is no mask for an infinity or a NaN.  O shows it, and such a row is then summed again key by key,
-// reading only what it sees (pt_slow_row).  Every wait is bounded (status word, see kch_device_status).
+// Keys behind a sequence's end read as zeros where a whole page is missing (an out-of-range coordinate of the copy); in its last page
+// the softmax clears the value rows behind it, whatever earlier tokens left there.  A key that only some rows of a tile see has
+// p = 0 in the others, which is no mask for an infinity or a NaN: O shows it, and such a row is summed again key by key, reading only
+// what it sees (pt_slow_row).  Every wait is bounded (status word, see kch_device_status).
 #include <cuda.h>
 #include <math.h>
 
@@ -34,7 +35,7 @@
 #ifndef PT_POLY
 #define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks)
 #endif
-#define PT_SPIN (1u << 22)
+#define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
 
 template <int D, int KIND, bool FEW>
 struct PtCfg {
@@ -184,21 +185,29 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
     if (KIND == KCH_INT8) return (float)((const int8_t*)p)[i];
     return float(((const __nv_fp8_e4m3*)p)[i]);
   };
-  for (int j = from; j < to; ++j) {
-    const int64_t pg = pg_page(a.bt, b, j >> a.bt.shift);
-    const int64_t row = (pg * a.bt.n_kv + h) * a.page + (j & (a.page - 1));
-    float s = 0.f;
-    if (pg >= 0) {
+  constexpr int U = 8;                                   // keys in flight
+  for (int j0 = from; j0 < to; j0 += U) {
+    float s[U], v[U][E], vs[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(qv[e], value(a.k, row * D + lane * E + e), s);
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u, to - 1);
+      const int64_t pg = pg_page(a.bt, b, j >> a.bt.shift), row = (max(pg, (int64_t)0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1));
+      s[u] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s[u] = fmaf(qv[e], pg < 0 ? 0.f : value(a.k, row * D + lane * E + e), s[u]);
+        v[u][e] = pg < 0 ? 0.f : value(a.v, row * D + lane * E + e);
+      }
+      vs[u] = 1.f;
+      if (KIND != KCH_BF16) { s[u] *= a.ks[row]; vs[u] = a.vs[row]; }
     }
-    s = warp_sum(s);
-    float vs = 1.f;
-    if (KIND != KCH_BF16 && pg >= 0) { s *= a.ks[row]; vs = a.vs[row]; }
-    const float p = round_to<bf16>(ex2_fast(fmaf(s, sc, -shift)) * vs);
-    if (pg >= 0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(p, value(a.v, row * D + lane * E + e), o[e]);
+    for (int u = 0; u < U; ++u) {
+      const float p = round_to<bf16>(ex2_fast(fmaf(warp_sum(s[u]), sc, -shift)) * vs[u]);
+      if (j0 + u < to) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[u][e], o[e]);
+      }
     }
   }
 #pragma unroll
@@ -437,7 +446,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const float sc = fmaxf(fabsf(a.scale), 1e-30f);      // (not 0: a masked logit is -inf)
     const float raise = 8.f / sc;
     bool ok = true;
-    int n = 0, kt = 0;                                   // tiles of this warpgroup; key tiles of the CTA
+    int n = 0, kt = 0, ring = 0;                         // tiles of this warpgroup; key tiles of the CTA; tiles of the ring before the item
     bool part = false;                                   // the CTA's last item goes on in the next one
     for (Walk w(a.bt, place); w.valid(); w.next()) {
       const bool pair = paired(w);
@@ -574,6 +583,18 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           float la, lb;
           pt_unpack(sum2, la, lb);
           l += la + lb;
+        }
+        if (!C::Q8 && w.s.kv > key0 && w.s.kv < key0 + PT_KT) {
+          // (payloads of 8 bits are numbers, and the scales there are 0)
+          const int at = pair ? ring + 1 + 2 * s : ring + 2 + 4 * s + (s + 1 < w.count ? 2 : 1) * x;      // of the tile's values in the ring
+          if (ok) ok = wait(&sm.full[at % C::STAGES], at / C::STAGES);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && key0 + r >= w.s.kv) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<uint4*>(sm.kv[at % C::STAGES] + (i >> 3) * (PT_KT * 128) + r * 128 + ((i & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          t5_fence_async_smem();
         }
         t5_wait_st();
         t5_fence_before();
@@ -718,6 +739,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       t5_fence_before();
       if (!pair) sync(1, 256);                           // both have read O of both, and the maxima and sums
+      ring += (pair ? 2 : 4) * w.count;
       if (w.starts() && !w.ends()) {
         part = true;
         if (tid == 128)

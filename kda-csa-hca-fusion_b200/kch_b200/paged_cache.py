@@ -96,6 +96,8 @@ class PagedKVCache:
         self.device = where
         self.k_pages, self.v_pages, self.k_scales, self.v_scales = storage
         self._ws_bytes = {}             # of attention calls, by their sizes
+        self._row = torch.empty(0, dtype=dtype, device=self.device)        # (what new tensors are made from)
+        self._byte = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._tag, self._index, self._lib = _lib.dtype_tag(dtype), self.k_pages.get_device(), _lib.load()
         self._c = _lib.PagedCache(self.k_pages.data_ptr(), self.v_pages.data_ptr(), _lib.ptr(self.k_scales), _lib.ptr(self.v_scales),
                                   self._tag if kv_quant is None else _QUANT[kv_quant], num_pages, page_size, n_kv, c)
@@ -174,7 +176,7 @@ class PagedKVCache:
         batch, keep = self._batch(fn, table, t0, cu_seqlens, n_rows)
         with _lib.device(self.device):
             if out is None:
-                k, v = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
+                k, v = self._row.new_empty(shape), self._row.new_empty(shape)
             else:
                 k, v = out
                 self._own_out(fn, "out[0]", k, shape)
@@ -206,7 +208,7 @@ class PagedKVCache:
                 sink, sink_tag = sink_logits.data_ptr(), _lib.dtype_tag(sink_logits.dtype)
             q, at_q, ld_q = _packed(q)
             if out is None:
-                o = torch.empty_like(q, memory_format=torch.contiguous_format)
+                o = self._row.new_empty((N, nh, c))
             else:
                 o = out
                 self._own_out(fn, "out", o, (N, nh, c))
@@ -218,7 +220,7 @@ class PagedKVCache:
                 if len(self._ws_bytes) > 4096:
                     self._ws_bytes.clear()
                 nbytes = self._ws_bytes[sizes] = int(self._lib.kch_paged_attend_workspace_bytes(a))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            ws = self._byte.new_empty(nbytes)
             a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
             _lib.check(self._lib.kch_paged_attend(a, _lib.stream()))
         return o

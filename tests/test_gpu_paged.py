@@ -472,3 +472,36 @@ def test_large_batches_and_long_sequences(kch):
         close(m.cache.forward_step(q, *m.args), want, tol)
         want, tol = reference(m, q, window=5000)
         close(m.cache.forward_step(q, *m.args, sliding_window=5000), want, tol)
+
+
+@pytest.mark.parametrize("kind", [None, "fp8", "int8"])
+@pytest.mark.parametrize("c,nh,n_kv", [(128, 8, 2), (64, 4, 1), (128, 16, 1), (64, 2, 2), (128, 14, 2)])
+def test_batches_of_few_rows_with_one_long_chunk_among_them(kch, kind, c, nh, n_kv):
+    """What a batch is on average decides on the form of the attention; every form takes every batch."""
+    new, past = [1] * 20 + [60] + [2] * 19, [31 * i % 700 for i in range(40)]
+    m = Batch(kch, new, past, kind=kind, c=c, n_kv=n_kv, page=16)
+    q = m.randn(m.N, nh, c)
+    want, tol = reference(m, q, window=300)
+    close(m.cache.forward_step(q, *m.args, sliding_window=300), want, tol)
+    # rows that do not depend on their company: the same bits in a batch of their own kind
+    one = m.cache.forward_step(q[:20], m.table[:20], m.t0[:20], m.cu[:21])
+    want, tol = reference(m, q)
+    close(one, want[:20], tol[:20])
+
+
+@pytest.mark.parametrize("page", [8, 16, 256])
+def test_values_of_earlier_tokens_behind_a_sequence_are_cleared_not_summed_around(kch, page):
+    """NaN in the last page of every sequence, in the rows behind its end."""
+    m = Batch(kch, [1, 40, 1, 300], [6, 129, 1000, 500], page=page, n_kv=2, c=128)
+    for b, (n, p) in enumerate(zip(m.new, m.past)):
+        left = (n + p) % page
+        if left:
+            m.cache.v_pages[int(m.table[b, (n + p) // page]), :, left:] = torch.nan
+    q = m.randn(m.N, 8, 128)
+    want, tol = reference(m, q)
+    close(m.cache.forward_step(q, *m.args), want, tol)
+    # single tokens of the same sequences
+    last = torch.tensor([n + p - 1 for n, p in zip(m.new, m.past)], dtype=torch.int32, device=DEV)
+    ends = torch.tensor([sum(m.new[:i + 1]) - 1 for i in range(4)], device=DEV)
+    got = m.cache.forward_step(q[ends], m.table, last, torch.arange(5, dtype=torch.int32, device=DEV))
+    close(got, want[ends], tol[ends])
