@@ -8,45 +8,49 @@
 // scale), the softmax keeps a running maximum and sum a row, and the sums stay in registers, a row's columns over 16 threads.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
-template <typename P> struct PgStored;            // 8 stored values as floats
-template <> struct PgStored<float> {
-  static constexpr int ES = 4;
-  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>((const float*)p + i)), b = __ldg(reinterpret_cast<const float4*>((const float*)p + i) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  }
-};
-template <> struct PgStored<bf16> {
-  static constexpr int ES = 2;
-  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>((const bf16*)p + i));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 stored values: the words that hold them, and their values as floats
+template <typename P>
+struct PgStored {
+  static constexpr int ES = sizeof(P), W = 2 * ES;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    const P* p = (const P*)base + i;
+    if constexpr (W == 2) {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = a.x; w[1] = a.y;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u); }
-  }
-};
-template <> struct PgStored<__nv_fp8_e4m3> {
-  static constexpr int ES = 1;
-  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
-    const uint2 a = __ldg(reinterpret_cast<const uint2*>((const uint8_t*)p + i));
-    const uint32_t w[2] = {a.x, a.y};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      __nv_fp8_e4m3 v;
-      v.__x = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
-      x[e] = float(v);
+      for (int k = 0; k < W / 4; ++k) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + k);
+        w[4 * k] = a.x; w[4 * k + 1] = a.y; w[4 * k + 2] = a.z; w[4 * k + 3] = a.w;
+      }
     }
   }
-};
-template <> struct PgStored<int8_t> {
-  static constexpr int ES = 1;
-  __device__ static void load(const void* p, int64_t i, float (&x)[8]) {
-    const uint2 a = __ldg(reinterpret_cast<const uint2*>((const uint8_t*)p + i));
-    const uint32_t w[2] = {a.x, a.y};
+  __device__ __forceinline__ void none() {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(w[e >> 2] >> (8 * (e & 3)));
+    for (int k = 0; k < W; ++k) w[k] = 0u;
+  }
+  __device__ __forceinline__ float value(int e) const {
+    if constexpr (ES == 4) return __uint_as_float(w[e]);
+    else if constexpr (ES == 2) return __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+    else {
+      const uint8_t code = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+      if constexpr (std::is_same<P, int8_t>::value) return (float)(int8_t)code;
+      else {
+        __nv_fp8_e4m3 v;
+        v.__x = code;
+        return float(v);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* to, float f) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      reinterpret_cast<float4*>(to)[k] = make_float4(value(4 * k) * f, value(4 * k + 1) * f, value(4 * k + 2) * f, value(4 * k + 3) * f);
   }
 };
 
@@ -85,13 +89,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     __syncthreads();
     for (int i = tid; i < ROWS * c8; i += PA_THREADS) {
       const int r = i / c8, d = i % c8 * 8;
-      float x[8] = {};
+      PgStored<T> x;
+      x.none();
       if (r < w.x.rows) {
         const int t = pg_token(a.bt, r0 + r);
-        PgStored<T>::load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * G + r0 + r - t * G) * c + d, x);
+        x.load(a.q, (w.s.row0 + t) * a.ld_q + (int64_t)(w.h * G + r0 + r - t * G) * c + d);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sq[r * LD + d + e] = x[e];
+      x.put(sq + r * LD + d, 1.f);
     }
     for (int r = tid; r < ROWS; r += PA_THREADS) { sm[r] = -INFINITY; sl[r] = 0.f; }
     float o[RT][CT][4];
@@ -99,30 +103,42 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int j = 0; j < CT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-    for (int st = w.first; st < w.first + w.count; ++st) {
-      const int key0 = w.x.first_key + st * PA_KT;
-      __syncthreads();
-      for (int i = tid; i < PA_KT * c8; i += PA_THREADS) {     // keys and values of the tile, 0 behind the sequence's end
-        const int j = i / c8, d = i % c8 * 8;
-        const int pos = key0 + j;
-        float kx[8] = {}, vx[8] = {};
-        if (pos < w.s.kv) {
+    // A tile's words are asked for while the one before it is multiplied (wide rows would take too many registers: not ahead).
+    constexpr int CHUNKS = PA_KT * DMAX / 8 / PA_THREADS;
+    PgStored<P> kw[CHUNKS], vw[CHUNKS];
+    float fk[CHUNKS], fv[CHUNKS];
+    auto ask = [&](int st) {
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k) {
+        const int i = tid + k * PA_THREADS, j = i / c8, d = i % c8 * 8, pos = w.x.first_key + st * PA_KT + j;
+        kw[k].none();                                          // (0 behind the sequence's end)
+        vw[k].none();
+        fk[k] = fv[k] = 1.f;
+        if (j < PA_KT && pos < w.s.kv) {
           const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
           if (pg >= 0) {
             const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));
-            PgStored<P>::load(a.k, row * c + d, kx);
-            PgStored<P>::load(a.v, row * c + d, vx);
-            if (PgStored<P>::ES == 1) {
-              const float fk = __ldg(a.ks + row), fv = __ldg(a.vs + row);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) { kx[e] *= fk; vx[e] *= fv; }
-            }
+            kw[k].load(a.k, row * c + d);
+            vw[k].load(a.v, row * c + d);
+            if (sizeof(P) == 1) { fk[k] = __ldg(a.ks + row); fv[k] = __ldg(a.vs + row); }
           }
         }
+      }
+    };
+    if (DMAX <= 128) ask(w.first);
+    for (int st = w.first; st < w.first + w.count; ++st) {
+      const int key0 = w.x.first_key + st * PA_KT;
+      if (DMAX > 128) ask(st);
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { sk[j * LD + d + e] = kx[e]; sv[j * LD + d + e] = vx[e]; }
+      for (int k = 0; k < CHUNKS; ++k) {
+        const int i = tid + k * PA_THREADS, j = i / c8, d = i % c8 * 8;
+        if (j >= PA_KT) break;
+        kw[k].put(sk + j * LD + d, fk[k]);
+        vw[k].put(sv + j * LD + d, fv[k]);
       }
       __syncthreads();
+      if (DMAX <= 128 && st + 1 < w.first + w.count) ask(st + 1);
       float acc[RT][4];                                        // rows ty + 16 i, keys tx + 16 j
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -187,22 +203,26 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
       // sees every key nothing is to be skipped.
       const bool whole = key0 >= pg_sees(a.bt, w.s, r0 + w.x.rows - 1).x && key0 + PA_KT <= pg_sees(a.bt, w.s, r0).y;
       auto product = [&](auto masked) {
-        for (int j = 0; j < PA_KT; ++j) {
-          float p[RT];
+#pragma unroll 1
+        for (int j = 0; j < PA_KT; j += 4) {                   // four keys at a time: their probabilities in one load a row
+          float4 p[RT];
 #pragma unroll
-          for (int i = 0; i < RT; ++i) p[i] = sp[(ty + 16 * i) * LS + j];
+          for (int i = 0; i < RT; ++i) p[i] = *reinterpret_cast<const float4*>(sp + (ty + 16 * i) * LS + j);
 #pragma unroll
-          for (int x = 0; x < CT; ++x) {
-            const float4 vv = *reinterpret_cast<const float4*>(sv + j * LD + tx * 4 + 64 * x);
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              if (masked() && p[i] == 0.f) continue;
-              o[i][x][0] = fmaf(p[i], vv.x, o[i][x][0]);
-              o[i][x][1] = fmaf(p[i], vv.y, o[i][x][1]);
-              o[i][x][2] = fmaf(p[i], vv.z, o[i][x][2]);
-              o[i][x][3] = fmaf(p[i], vv.w, o[i][x][3]);
+            for (int x = 0; x < CT; ++x) {
+              const float4 vv = *reinterpret_cast<const float4*>(sv + (j + k) * LD + tx * 4 + 64 * x);
+#pragma unroll
+              for (int i = 0; i < RT; ++i) {
+                const float f = k == 0 ? p[i].x : k == 1 ? p[i].y : k == 2 ? p[i].z : p[i].w;
+                if (masked() && f == 0.f) continue;
+                o[i][x][0] = fmaf(f, vv.x, o[i][x][0]);
+                o[i][x][1] = fmaf(f, vv.y, o[i][x][1]);
+                o[i][x][2] = fmaf(f, vv.z, o[i][x][2]);
+                o[i][x][3] = fmaf(f, vv.w, o[i][x][3]);
+              }
             }
-          }
         }
       };
       if (whole) product([] { return false; });
