@@ -10,6 +10,7 @@
 
 #include <type_traits>
 
+#include "mma_utils.cuh"
 #include "paged.cuh"
 
 // 8 stored values: the words that hold them, and their values as floats
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = exp2f(acc[i][j] - shift);
+          const float p = ex2_fast(acc[i][j] - shift);
           sp[r * LS + tx + 16 * j] = p;
           sum += p;
         }
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         __syncwarp();
         if (tx == 0) {
-          const float keep = exp2f(was - shift);               // (0 where nothing was)
+          const float keep = ex2_fast(was - shift);               // (0 where nothing was)
           sa[r] = keep;
           sl[r] = sl[r] * keep + sum;
           sm[r] = now;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
       if (direct) {
         const float m = sm[r], l = sl[r];
         float below = l;
-        if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - m);
+        if (a.sink && l > 0.f) below += ex2_fast(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - m);
         f = l == 0.f ? 0.f : 1.f / below;
       }
       T* orow = (T*)a.out + ((int64_t)(w.s.row0 + t) * (n_kv * G) + h) * c;
@@ -275,28 +276,28 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #define PJ_WARPS 8
 template <typename T, int W>          // W: columns of a lane, in fours
 __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a, int ctas) {
-  __shared__ int before[PA_CTAS + 1], many[PA_CTAS], n_many;      // many: the items whose rows are a block's
+  __shared__ int before[PA_CTAS + 1], wide[PA_CTAS], many[PA_CTAS], n_many;      // many: the items whose rows are a block's
   __shared__ alignas(16) float part_o[PJ_WARPS][W * 128];
   __shared__ float part_l[PJ_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   chain_wait();
+  for (int i = threadIdx.x; i < ctas; i += 32 * PJ_WARPS) {
+    const PgRecord rec = a.records[i];
+    before[i + 1] = rec.valid ? rec.rows : 0;
+    wide[i] = rec.valid && rec.last - i >= PJ_WARPS;
+  }
+  __syncthreads();
   if (warp == 0) {                     // rows of the parted items before each
     int run = 0, wides = 0;
     for (int i0 = 0; i0 < ctas; i0 += 32) {
-      const int i = i0 + lane;
-      const bool there = i < ctas && a.records[i].valid;
-      int x = there ? a.records[i].rows : 0;
-      const bool wide = there && a.records[i].last - i >= PJ_WARPS;
-      const unsigned who = __ballot_sync(0xffffffffu, wide);
-      if (wide) many[wides + __popc(who & ((1u << lane) - 1u))] = i;
-      wides += __popc(who);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+      const int i = i0 + lane, x = run + pg_scan(i < ctas ? before[i + 1] : 0);
+      const unsigned who = __ballot_sync(0xffffffffu, i < ctas && wide[i]);
+      if (i < ctas) {
+        before[i + 1] = x;
+        if (wide[i]) many[wides + __popc(who & ((1u << lane) - 1u))] = i;
       }
-      if (i < ctas) before[i + 1] = run + x;
-      run += __shfl_sync(0xffffffffu, x, 31);
+      wides += __popc(who);
+      run = __shfl_sync(0xffffffffu, x, 31);
     }
     if (lane == 0) { before[0] = 0; n_many = wides; }
   }
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
 #pragma unroll 4
     for (int i = first + from; i <= last; i += step) {
       const float* s = a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size;
-      const float f = exp2f(s[mat + r] - shift), part = s[mat + a.slot_rows + r];
+      const float f = ex2_fast(s[mat + r] - shift), part = s[mat + a.slot_rows + r];
       l = fmaf(f, part, l);
 #pragma unroll
       for (int x = 0; x < W; ++x) {
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
   auto store = [&](const PgRecord& rec, int r, float shift) {
     const int row = rec.block * a.R + r, t = row / a.G, h = rec.h * a.G + row - t * a.G;
     float below = l;
-    if (a.sink && l > 0.f) below += exp2f(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
+    if (a.sink && l > 0.f) below += ex2_fast(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
     const float f = l == 0.f ? 0.f : 1.f / below;
     T* out = (T*)a.out + ((int64_t)(rec.row0 + t) * a.nh + h) * a.c;
 #pragma unroll
