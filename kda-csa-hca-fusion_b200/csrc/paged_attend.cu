@@ -60,10 +60,7 @@ struct PgStored {
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
 // steps that a call can have at most, whatever the lengths on the device
-static int64_t pa_steps(const PgBatch& a, int rows, int kt, bool two) {
-  const int64_t blocks = (int64_t)a.N * a.G / rows + a.B, tiles = a.cap / kt + 1;
-  return blocks * a.n_kv * (two ? (tiles + 1) / 2 : tiles);
-}
+static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1); }
 
 static int pa_smem(int ROWS, int DMAX, int B) {
   const int need = (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4, plan = PG_PLAN_BYTES(B);
@@ -409,16 +406,19 @@ bool kch_paged_attend_tc5_supported(int dtype, int c);
 int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s);
 int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 
-// How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.
-struct PaPlan { bool tc5; int rows, ctas, slot_rows; };
+// How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.  The host knows the rows of a call and its
+// sequences, not who has them: what a sequence has on average decides, every form takes every batch, and a batch counts as one of few
+// rows only up to 4 tokens a sequence, so that a long chunk among single tokens cannot be most of its work (measured figures at the
+// kernels).
+enum PaForm { PA_TC5, PA_TC5_FEW, PA_MMA, PA_SIMT };
+struct PaPlan { PaForm form; int rows, tile, ctas, slot_rows; bool two; };      // two: items of at most half the rows (FEW: all) take two tiles a step
 static PaPlan pa_plan(const kch_paged_attend_args* p) {
   PaPlan x;
-  const int64_t rows = p->batch.N * (p->nh / p->cache.n_kv);          // of a key head
-  x.tc5 = kch_paged_attend_tc5_supported(p->dtype, p->cache.c);
-  const int64_t B = p->batch.B;
-  if (x.tc5) x.rows = rows > 32 * B || p->batch.N > 4 * B ? 256 : p->cache.kind == KCH_BF16 ? 32 : rows <= 8 * B ? 8 : 16;
-  else x.rows = rows <= 16 * B ? 16 : 64;
-  x.ctas = x.tc5 ? KCH_SMS : PA_CTAS;
+  const int64_t B = p->batch.B, rows = p->batch.N * (p->nh / p->cache.n_kv);      // of a key head
+  if (!kch_paged_attend_tc5_supported(p->dtype, p->cache.c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
+  else if (rows > 32 * B || p->batch.N > 4 * B) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
+  else if (p->cache.kind == KCH_BF16) x = {PA_TC5_FEW, 32, 128, KCH_SMS, 0, true};
+  else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
 }
@@ -462,13 +462,14 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;
   cudaStream_t s = kch_stream(stream);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tc5 ? 128 : PA_KT, x.rows == 32) <= 0x7FFFFFFFLL,
-              "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes", (long long)p->batch.N, p->batch.max_pages);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) <= 0x7FFFFFFFLL, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
+              (long long)p->batch.N, p->batch.max_pages);
   // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
-  const bool whole = x.tc5 ? a.bt.cap <= 128 * (x.rows == 32 || (x.rows == 256 && (int64_t)a.bt.N * a.bt.G <= 128) ? 2 : 1) : a.bt.cap <= PA_KT;
+  const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
-  if (x.tc5) {
-    const int rc5 = x.rows <= 16 ? kch_paged_attend_mma(a, p->cache.kind, x.rows, x.ctas, s) : kch_paged_attend_tc5(a, p->cache.kind, x.rows == 32, x.ctas, s);
+  if (x.form != PA_SIMT) {
+    const int rc5 = x.form == PA_MMA ? kch_paged_attend_mma(a, p->cache.kind, x.rows, x.ctas, s)
+                                     : kch_paged_attend_tc5(a, p->cache.kind, x.form == PA_TC5_FEW, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);

@@ -6,9 +6,9 @@
 // converted once, in the registers of the warp that multiplies them (mma.sync; the rows are far too few for the tensor core's rate to
 // matter): through tiles of tcgen05 the same step took twice as long, for the tiles are written, fenced and read back.
 //
-// An item is up to 16 (token, head of the group) rows of a sequence; a tile is 128 keys, its payloads and scales copied into a ring by
+// An item is up to 32 (token, head of the group) rows of a sequence; a tile is 128 keys, its payloads and scales copied into a ring by
 // one warp (TMA, 128-byte or 64-byte swizzle; scales by bulk copies).  Four warps share a tile, 32 keys each, and the other four take
-// the next one; a warp has a maximum, a sum and an O of its own, so that nothing but the ring is waited for, and they are joined when
+// the next one (32 rows: eight share it); a warp has a maximum, a sum and an O of its own, so that nothing but the ring is waited for, and they are joined when
 // the item ends.  (With 16 keys a warp and tile there were too few instructions that do not wait for one another: 2900 clocks a tile.)
 //   S = Q K^T: the order of the contraction is free, so thread (g, t) of a fragment takes 32 (16) consecutive channels of key g, four of
 //     them a product: a row is read in 16-byte words, and the queries' fragments are loaded in the same order.
@@ -27,14 +27,14 @@
 #define PM_KT 128
 #define PM_SPIN (1u << 26)
 
-// R rows an item: 16, or 8 where a sequence has no more (one token of up to 8 heads): the lower half of every fragment is empty then, and
-// the registers that it leaves hold twice as many warps.
+// R rows an item: 8, 16 or 32, by what a sequence has.  8 (one token of up to 8 heads): the lower half of every fragment is empty, and
+// so are its registers.  32: two fragments a warp, which then takes 16 keys of every tile, for the registers' sake.
 template <int R>
 struct PmCfg {
-  static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;      // that compute; the first warpgroup copies
-  static constexpr int SLICE = 2 * PM_KT / WARPS, H = SLICE / 8;                // keys of a warp in a tile; in eights
-  static constexpr int HF = R / 8;                                              // rows of a thread
-  static constexpr int REG_FEED = 64, REG_WORK = 216, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;                   // that compute; the first warpgroup copies
+  static constexpr int SHARE = R == 32 ? 8 : 4, SLICE = PM_KT / SHARE, H = SLICE / 8;      // warps of a tile; a warp's keys; in eights
+  static constexpr int MT = R == 32 ? 2 : 1, F = R == 8 ? 2 : 4, HF = R / 8;    // fragments; values of one a thread has; rows of a thread
+  static constexpr int REG_FEED = R == 32 ? 56 : 64, REG_WORK = R == 32 ? 224 : 216, REG_LAUNCH = 65536 / THREADS / 8 * 8;
   static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
 };
 template <int D, int R>
@@ -44,11 +44,11 @@ struct PmSmem {
   alignas(1024) uint8_t k[STAGES][PM_KT * D], v[STAGES][PM_KT * D];
   alignas(16) float ks[STAGES][PM_KT], vs[STAGES][PM_KT];
   alignas(16) float stage[C::WARPS][8 * D];
-  alignas(16) uint4 q[D / 16][32];                       // fragments of the queries: contraction step, lane
+  alignas(16) uint4 q[D / 16][C::MT][32];                // fragments of the queries: contraction step, fragment, lane
   float ml[2][C::WARPS][R];
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
-static_assert(sizeof(PmSmem<128, 16>) <= 232448 && sizeof(PmSmem<128, 8>) <= 232448, "shared memory of the paged attention over 8-bit pages");
+static_assert(sizeof(PmSmem<128, 16>) <= 232448 && sizeof(PmSmem<128, 32>) <= 232448, "shared memory of the paged attention over 8-bit pages");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * PM_KT * 64, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pm_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -102,7 +102,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
   if (tid == 0) {
-    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::WARPS / 2); }
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::SHARE); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -168,40 +168,40 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   int n = 0;                                             // tiles of the ring
   bool ok = true, part = false;
   for (Walk w(a.bt, place); w.valid(); w.next()) {
-    // queries: of step i the lane (g, t) has channels RUN t + 4 i .. + 3 of rows g and g + 8
-    for (int i = ct; i < KS * 32; i += 32 * C::WARPS) {
-      const int gg = (i & 31) >> 2, d = RUN * (i & 3) + 4 * (i >> 5);
+    // queries: of step i the lane (g, t) has channels RUN t + 4 i .. + 3 of rows g and g + 8 of each fragment
+    for (int i = ct; i < KS * C::MT * 32; i += 32 * C::WARPS) {
+      const int ln = i & 31, mt = (i >> 5) % C::MT, step = (i >> 5) / C::MT, d = RUN * (ln & 3) + 4 * step;
       uint2 u[2] = {};
 #pragma unroll
-      for (int hf = 0; hf < C::HF; ++hf) {
-        const int row = w.block * R + gg + 8 * hf, tok = pg_token(a.bt, row);
-        if (gg + 8 * hf < w.x.rows)
+      for (int hf = 0; hf < C::F / 2; ++hf) {
+        const int r = 16 * mt + (ln >> 2) + 8 * hf, row = w.block * R + r, tok = pg_token(a.bt, row);
+        if (r < w.x.rows)
           u[hf] = __ldg(reinterpret_cast<const uint2*>((const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + d));
       }
-      sm.q[i >> 5][i & 31] = make_uint4(u[0].x ^ flip, u[1].x ^ flip, u[0].y ^ flip, u[1].y ^ flip);
+      sm.q[step][mt][ln] = make_uint4(u[0].x ^ flip, u[1].x ^ flip, u[0].y ^ flip, u[1].y ^ flip);
     }
     sync();
-    constexpr int HF = C::HF, E = 2 * HF;                // values of a thread in a tile of 8 keys (columns): two a row
+    constexpr int HF = C::HF, MT = C::MT, F = C::F;      // (value e of fragment mt: row 16 mt + 8 (e / 2) + g, one of two columns)
     int2 keys[HF];
 #pragma unroll
     for (int hf = 0; hf < HF; ++hf)
       keys[hf] = g + 8 * hf < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + g + 8 * hf) : make_int2(0, 0);
     const int2 k0 = pg_sees(a.bt, w.s, w.block * R), k1 = pg_sees(a.bt, w.s, w.block * R + w.x.rows - 1);      // first and last row's
-    float m[HF], l[HF], o[NT][E];
+    float m[HF], l[HF], o[NT][MT][F];
 #pragma unroll
     for (int hf = 0; hf < HF; ++hf) { m[hf] = -INFINITY; l[hf] = 0.f; }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[j][e] = 0.f;
+      for (int e = 0; e < MT * F; ++e) o[j][e / F][e % F] = 0.f;
     for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
-      if ((n & 1) != cw / (C::WARPS / 2)) continue;
-      const int st = n % S::STAGES, base = C::SLICE * (cw % (C::WARPS / 2)), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's keys
+      if (n % (C::WARPS / C::SHARE) != cw / C::SHARE) continue;
+      const int st = n % S::STAGES, base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's keys
       if (ok) ok = wait(&sm.full[st], n / S::STAGES);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
         const uint8_t *tk = sm.k[st], *tv = sm.v[st];
-        float s[C::H][E] = {};
+        float s[C::H][MT][F] = {};
 #pragma unroll
         for (int i4 = 0; i4 < KS; i4 += 4) {             // 16 bytes of each key's run
           uint4 kc[C::H];
@@ -209,18 +209,26 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           for (int h = 0; h < C::H; ++h) kc[h] = pm_lds(tk + word(base + 8 * h + g, RUN / 16 * t + (i4 >> 2)));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 u = sm.q[i4 + i][lane];
-            const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+            uint32_t q[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const uint4 u = sm.q[i4 + i][mt][lane];
+              q[mt][0] = u.x; q[mt][1] = u.y; q[mt][2] = u.z; q[mt][3] = u.w;
+            }
 #pragma unroll
             for (int h = 0; h < C::H; ++h) {
               const uint32_t c = i == 0 ? kc[h].x : i == 1 ? kc[h].y : i == 2 ? kc[h].z : kc[h].w;
-              pm_mma(s[h], q, pm_pair<KIND>(c, c, 0, 1), pm_pair<KIND>(c, c, 2, 3));
+              const uint32_t b0 = pm_pair<KIND>(c, c, 0, 1), b1 = pm_pair<KIND>(c, c, 2, 3);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) pm_mma(s[h][mt], q[mt], b0, b1);
             }
           }
         }
         // scaled; what a row does not see is -inf
         const bool whole = key0 >= k1.x && key0 + C::SLICE <= k0.y && w.x.rows == R;
-        uint32_t sees = 0xFFFFu;                         // bit E h + e
+        constexpr int E = MT * F;                        // values of a thread in 8 keys; bit E h + e of `sees`
+        uint32_t sees = 0xFFFFFFFFu;
+        static_assert(C::H * E <= 32, "a bit each");
         if (!whole) {
           sees = 0u;
 #pragma unroll
@@ -239,8 +247,9 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           const float2 f = *reinterpret_cast<const float2*>(&sm.ks[st][base + 8 * h + 2 * t]);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            s[h][e] = sees & (1u << (E * h + e)) ? s[h][e] * (e & 1 ? f.y : f.x) : -INFINITY;
-            top[e >> 1] = fmaxf(top[e >> 1], s[h][e]);
+            float& x = s[h][e / F][e % F];
+            x = sees & (1u << (E * h + e)) ? x * (e & 1 ? f.y : f.x) : -INFINITY;
+            top[e >> 1] = fmaxf(top[e >> 1], x);
           }
         }
         bool up[HF], any = false;                        // a row's maximum is raised only when it is exceeded by 2^8
@@ -258,25 +267,25 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (up[hf]) m[hf] = top[hf];
             l[hf] *= f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) { o[j][2 * hf] *= f; o[j][2 * hf + 1] *= f; }
+            for (int j = 0; j < NT; ++j) { o[j][2 * hf / F][2 * hf % F] *= f; o[j][2 * hf / F][2 * hf % F + 1] *= f; }
           }
         }
         float shift[HF];
 #pragma unroll
         for (int hf = 0; hf < HF; ++hf) shift[hf] = m[hf] == -INFINITY ? 0.f : m[hf] * sc;
-        uint32_t p[C::H / 2][4] = {};
+        uint32_t p[C::H / 2][MT][4] = {};
 #pragma unroll
         for (int h = 0; h < C::H; ++h) {
           const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][base + 8 * h + 2 * t]);
           float x[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            x[e] = ex2_fast(fmaf(s[h][e], sc, -shift[e >> 1]));
+            x[e] = ex2_fast(fmaf(s[h][e / F][e % F], sc, -shift[e >> 1]));
             l[e >> 1] += x[e];
             x[e] = sees & (1u << (E * h + e)) ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
           }
 #pragma unroll
-          for (int hf = 0; hf < HF; ++hf) p[h >> 1][2 * (h & 1) + hf] = pack2_bf16(x[2 * hf], x[2 * hf + 1]);
+          for (int hf = 0; hf < HF; ++hf) p[h >> 1][2 * hf / F][2 * (h & 1) + hf % 2] = pack2_bf16(x[2 * hf], x[2 * hf + 1]);
         }
         // of the values channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half of the 32
 #pragma unroll
@@ -294,8 +303,11 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             }
           }
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-            pm_mma(o[j], p[b], pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3));
+          for (int j = 0; j < NT; ++j) {
+            const uint32_t b0 = pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), b1 = pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) pm_mma(o[j][mt], p[b][mt], b0, b1);
+          }
         }
       }
       __syncwarp();
@@ -326,9 +338,9 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // 16-byte words of a row, swizzled within runs of 8 so that 8 threads meet in no bank
 #pragma unroll
       for (int c = 0; c < RUN / 4; ++c) {
-        const int j = 4 * c % NT, e = 2 * hf + 4 * c / NT;
+        const int j = 4 * c % NT, mt = 2 * hf / F, e = 2 * hf % F + 4 * c / NT;
         mine[(RUN / 4 * t + c) ^ ((D == 128 ? t : 2 * (t & 1)) + 4 * (g & 1))] =
-            own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][e] * own, o[j + 1][e] * own, o[j + 2][e] * own, o[j + 3][e] * own);
+            own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][mt][e] * own, o[j + 1][mt][e] * own, o[j + 2][mt][e] * own, o[j + 3][mt][e] * own);
       }
       sync();
       for (int k = ct; k < 8 * (D / 4); k += 32 * C::WARPS) {
@@ -399,7 +411,9 @@ int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaSt
   int rc = kch_make_tensor_map_pages(&km, a.k, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc != KCH_OK) return rc;
-#define PM_ROWS(D_, K_) (rows == 8 ? pm_launch<D_, K_, 8>(km, vm, a, ctas, s) : pm_launch<D_, K_, 16>(km, vm, a, ctas, s))
+#define PM_ROWS(D_, K_)                                                                                      \
+  (rows == 8 ? pm_launch<D_, K_, 8>(km, vm, a, ctas, s) : rows == 16 ? pm_launch<D_, K_, 16>(km, vm, a, ctas, s) \
+             : pm_launch<D_, K_, 32>(km, vm, a, ctas, s))
 #define PM_KIND(D_) (kind == KCH_FP8_E4M3 ? PM_ROWS(D_, KCH_FP8_E4M3) : PM_ROWS(D_, KCH_INT8))
   return a.c == 64 ? PM_KIND(64) : PM_KIND(128);
 #undef PM_KIND

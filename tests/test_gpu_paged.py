@@ -505,3 +505,16 @@ def test_values_of_earlier_tokens_behind_a_sequence_are_cleared_not_summed_aroun
     ends = torch.tensor([sum(m.new[:i + 1]) - 1 for i in range(4)], device=DEV)
     got = m.cache.forward_step(q[ends], m.table, last, torch.arange(5, dtype=torch.int32, device=DEV))
     close(got, want[ends], tol[ends])
+
+
+@pytest.mark.parametrize("kind", [None, "fp8", "int8"])
+@pytest.mark.parametrize("nh,n_kv", [(2, 2), (8, 1), (14, 1), (16, 2), (32, 1), (48, 2), (9, 3)])
+@pytest.mark.parametrize("c", [64, 128])
+def test_steps_of_one_to_four_tokens(kch, kind, nh, n_kv, c):
+    """From one row of a key head to a hundred: each form of the attention over few rows, and the one behind them."""
+    for new, past in (([1, 1, 1], [400, 0, 129]), ([4, 3, 1, 4], [1000, 5, 64, 333]), ([4], [2000])):
+        m = Batch(kch, new, past, kind=kind, c=c, n_kv=n_kv, page=32)
+        q = m.randn(m.N, nh, c)
+        sink = torch.randn(nh, generator=m.g, device=DEV)
+        want, tol = reference(m, q, sink=sink, window=700)
+        close(m.cache.forward_step(q, *m.args, sink_logits=sink, sliding_window=700), want, tol)
