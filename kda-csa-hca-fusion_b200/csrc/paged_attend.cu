@@ -62,10 +62,8 @@ struct PgStored {
 // steps that a call can have at most, whatever the lengths on the device
 static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1); }
 
-static int pa_smem(int ROWS, int DMAX, int B) {
-  const int need = (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4, plan = PG_PLAN_BYTES(B);
-  return need > plan ? need : plan;
-}
+static constexpr int pa_smem(int ROWS, int DMAX) { return (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4; }
+static_assert(pa_smem(64, 256) <= 232448 && PG_PLAN_BYTES(PG_MAX_B) <= pa_smem(16, 64), "shared memory; the plan lies in the tiles' memory");
 
 // T: activations; P: stored values; DMAX: widths up to this (columns behind the width are 0)
 template <typename T, typename P, int ROWS, int DMAX>
@@ -450,7 +448,6 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
               "kch_paged_attend: workspace of %lld bytes (256-byte aligned) is too small: %lld needed", (long long)p->workspace_bytes, (long long)need);
   PgAttend a = {};
   a.bt = kch_paged_batch_of(&p->cache, &p->batch);
-  KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
   a.q = p->q; a.k = p->cache.k; a.v = p->cache.v; a.ks = p->cache.k_scales; a.vs = p->cache.v_scales;
   a.out = p->out; a.ld_q = p->ld_q; a.c = c; a.page = p->cache.page_size; a.zero_rest = p->zero_rest;
   a.bt.window = p->sliding_window;
@@ -459,11 +456,12 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   a.records = (PgRecord*)p->workspace;
   const PaPlan x = pa_plan(p);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) <= 0x7FFFFFFFLL, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
+              (long long)p->batch.N, p->batch.max_pages);
+  KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
   a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;
   cudaStream_t s = kch_stream(stream);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) <= 0x7FFFFFFFLL, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
-              (long long)p->batch.N, p->batch.max_pages);
   // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
   const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
@@ -472,7 +470,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
                                      : kch_paged_attend_tc5(a, p->cache.kind, x.form == PA_TC5_FEW, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
-  const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax, a.bt.B);
+  const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);
 #define PA_GO(T_, P_, R_, D_)                                                                                                 \
   do {                                                                                                                        \
     KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \

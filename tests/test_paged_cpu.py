@@ -49,7 +49,9 @@ def _args(lib_mod, **over):
     (dict(cu=None), "null table"), (dict(k=None), "pages"), (dict(v=4104), "16-byte"), (dict(kind=2, ks=None), "scales"),
     (dict(nh=3), "nh=3"), (dict(nh=0), "nh=0"), (dict(window=-1), "sliding_window"), (dict(scale=float("nan")), "scale"),
     (dict(sink=4096, sink_dtype=3), "sink"), (dict(q=None), "null q"), (dict(ld_q=255), "ld_q=255"), (dict(ld_q=260), "ld_q=260"),
-    (dict(out=4100), "16-byte"), (dict(), "workspace"), (dict(ws=None, ws_bytes=1 << 40), "workspace"), (dict(ws=4112, ws_bytes=1 << 40), "workspace")])
+    (dict(out=4100), "16-byte"), (dict(), "workspace"), (dict(ws=None, ws_bytes=1 << 40), "workspace"), (dict(ws=4112, ws_bytes=1 << 40), "workspace"),
+    (dict(N=1 << 24, nh=32, ld_q=32 * 64, max_pages=1 << 26, ld_table=1 << 26, ws_bytes=1 << 40), "more than a call takes"),
+    (dict(N=1 << 30, nh=4, ws_bytes=1 << 40), "N \\* nh")])
 def test_attend_arguments_are_refused_by_name(over, what):
     from kch_b200 import _lib
     lib = _lib.load()
