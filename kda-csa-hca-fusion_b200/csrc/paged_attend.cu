@@ -401,7 +401,7 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c);
-int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s);
+int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.  The host knows the rows of a call and its
@@ -415,7 +415,7 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   const int64_t B = p->batch.B, rows = p->batch.N * (p->nh / p->cache.n_kv);      // of a key head
   if (!kch_paged_attend_tc5_supported(p->dtype, p->cache.c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
   else if (rows > 32 * B || p->batch.N > 4 * B) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
-  else if (p->cache.kind == KCH_BF16) x = {PA_TC5_FEW, 32, 128, KCH_SMS, 0, true};
+  else if (p->cache.kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
@@ -467,7 +467,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.form != PA_SIMT) {
     const int rc5 = x.form == PA_MMA ? kch_paged_attend_mma(a, p->cache.kind, x.rows, x.ctas, s)
-                                     : kch_paged_attend_tc5(a, p->cache.kind, x.form == PA_TC5_FEW, x.ctas, s);
+                                     : kch_paged_attend_tc5(a, p->cache.kind, x.rows, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);

@@ -27,13 +27,13 @@
 #define PM_KT 128
 #define PM_SPIN (1u << 26)
 
-// R rows an item: 8, 16 or 32, by what a sequence has.  8 (one token of up to 8 heads): the lower half of every fragment is empty, and
-// so are its registers.  32: two fragments a warp, which then takes 16 keys of every tile, for the registers' sake.
+// R rows an item: 8, 16 or 32, by what a sequence has.  8 (one token of up to 8 heads): the lower half of the scores' fragments is
+// empty, and that of P has what its rounding left (paged_attend_tc5.cu has the reason; 16 rows: in products of their own, 7 %; 32: none).  32: two fragments a warp, which then takes 16 keys of every tile, for the registers' sake.
 template <int R>
 struct PmCfg {
   static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;                   // that compute; the first warpgroup copies
   static constexpr int SHARE = R == 32 ? 8 : 4, SLICE = PM_KT / SHARE, H = SLICE / 8;      // warps of a tile; a warp's keys; in eights
-  static constexpr int MT = R == 32 ? 2 : 1, F = R == 8 ? 2 : 4, HF = R / 8;    // fragments; values of one a thread has; rows of a thread
+  static constexpr int MT = R == 32 ? 2 : 1, F = R == 8 ? 2 : 4, HF = R / 8;    // fragments; scores of one a thread has; rows of a thread
   static constexpr int REG_FEED = R == 32 ? 56 : 64, REG_WORK = R == 32 ? 224 : 216, REG_LAUNCH = 65536 / THREADS / 8 * 8;
   static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
 };
@@ -187,13 +187,13 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (int hf = 0; hf < HF; ++hf)
       keys[hf] = g + 8 * hf < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + g + 8 * hf) : make_int2(0, 0);
     const int2 k0 = pg_sees(a.bt, w.s, w.block * R), k1 = pg_sees(a.bt, w.s, w.block * R + w.x.rows - 1);      // first and last row's
-    float m[HF], l[HF], o[NT][MT][F];
+    float m[HF], l[HF], o[NT][MT][4];
 #pragma unroll
     for (int hf = 0; hf < HF; ++hf) { m[hf] = -INFINITY; l[hf] = 0.f; }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < MT * F; ++e) o[j][e / F][e % F] = 0.f;
+      for (int e = 0; e < MT * 4; ++e) o[j][e / 4][e % 4] = 0.f;
     for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
       if (n % (C::WARPS / C::SHARE) != cw / C::SHARE) continue;
       const int st = n % S::STAGES, base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + tile * PM_KT + base;      // the warp's keys
@@ -267,13 +267,16 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (up[hf]) m[hf] = top[hf];
             l[hf] *= f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) { o[j][2 * hf / F][2 * hf % F] *= f; o[j][2 * hf / F][2 * hf % F + 1] *= f; }
+            for (int j = 0; j < NT; ++j) {
+              o[j][hf / 2][2 * (hf % 2)] *= f; o[j][hf / 2][2 * (hf % 2) + 1] *= f;
+              if (R == 8) { o[j][0][2] *= f; o[j][0][3] *= f; }
+            }
           }
         }
         float shift[HF];
 #pragma unroll
         for (int hf = 0; hf < HF; ++hf) shift[hf] = m[hf] == -INFINITY ? 0.f : m[hf] * sc;
-        uint32_t p[C::H / 2][MT][4] = {};
+        uint32_t p[C::H / 2][MT][4] = {}, rest[R == 16 ? C::H / 2 : 1][4] = {};      // P, and what its rounding leaves
 #pragma unroll
         for (int h = 0; h < C::H; ++h) {
           const float2 f = *reinterpret_cast<const float2*>(&sm.vs[st][base + 8 * h + 2 * t]);
@@ -285,7 +288,13 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             x[e] = sees & (1u << (E * h + e)) ? x[e] * (e & 1 ? f.y : f.x) : 0.f;
           }
 #pragma unroll
-          for (int hf = 0; hf < HF; ++hf) p[h >> 1][2 * hf / F][2 * (h & 1) + hf % 2] = pack2_bf16(x[2 * hf], x[2 * hf + 1]);
+          for (int hf = 0; hf < HF; ++hf) {
+            const uint32_t u = pack2_bf16(x[2 * hf], x[2 * hf + 1]);
+            const uint32_t left = pack2_bf16(x[2 * hf] - __uint_as_float(u << 16), x[2 * hf + 1] - __uint_as_float(u & 0xFFFF0000u));
+            p[h >> 1][hf / 2][2 * (h & 1) + hf % 2] = u;
+            if (R == 8) p[h >> 1][0][2 * (h & 1) + 1] = left;
+            if (R == 16) rest[h >> 1][2 * (h & 1) + hf] = left;
+          }
         }
         // of the values channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half of the 32
 #pragma unroll
@@ -306,12 +315,19 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           for (int j = 0; j < NT; ++j) {
             const uint32_t b0 = pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), b1 = pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) pm_mma(o[j][mt], p[b][mt], b0, b1);
+            for (int mt = 0; mt < MT; ++mt) {
+              pm_mma(o[j][mt], p[b][mt], b0, b1);
+              if constexpr (R == 16) pm_mma(o[j][mt], rest[b], b0, b1);
+            }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sm.empty[st]);
+    }
+    if (R == 8) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) { o[j][0][0] += o[j][0][2]; o[j][0][1] += o[j][0][3]; }
     }
     // ---- the item's end: the warps' parts of its rows ---------------------------------------------------------------------------
     const bool direct = w.starts() && w.ends();
@@ -338,7 +354,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // 16-byte words of a row, swizzled within runs of 8 so that 8 threads meet in no bank
 #pragma unroll
       for (int c = 0; c < RUN / 4; ++c) {
-        const int j = 4 * c % NT, mt = 2 * hf / F, e = 2 * hf % F + 4 * c / NT;
+        const int j = 4 * c % NT, mt = hf / 2, e = 2 * (hf % 2) + 4 * c / NT;
         mine[(RUN / 4 * t + c) ^ ((D == 128 ? t : 2 * (t & 1)) + 4 * (g & 1))] =
             own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][mt][e] * own, o[j + 1][mt][e] * own, o[j + 2][mt][e] * own, o[j + 3][mt][e] * own);
       }

@@ -5,10 +5,13 @@
 // rows of a sequence against the key tiles of 128 that they see:
 //   chunks:  up to 256 rows, X = rows 0..127 and 128..255 against the same key tile; 128 rows or fewer: X = the even and the odd tiles;
 //   steps (FEW, where a sequence has few rows): up to 32 rows, X = the even and the odd tiles, and the rows lie in the 128 of the
-//     query tile four times: warp w of a warpgroup has a row per thread as well, but only keys 32 w .. 32 w + 31 of a tile (its
+//     query tile four times (or eight, see below): warp w of a warpgroup has a row per thread as well, but only keys 32 w .. 32 w + 31 of a tile (its
 //     probabilities of the others are 0), with a maximum, a sum and an O of its own.  One warp of four would have all the work
 //     otherwise, and a tile's softmax would be the longest link of the chain.
 // Parts of a row with sums of their own are joined through shared memory when the item ends.
+// P is rounded to bf16, which adds to a result about as much as its own rounding does.  Steps of up to 16 rows leave 16 lanes of each
+// warp idle; there the rows lie in the tile eight times, and the other copy multiplies what the rounding of the first one left: the
+// output's rounding alone remains, at no cost.
 // Roles: warp 0 copies pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
 // issues  S_X = Q_X K^T  (M = N = 128) into 128 columns of tensor memory and  O_X += P_X V  with P_X, written by the softmax over
 // S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile; warps 2, 3 fetch the
@@ -37,9 +40,9 @@
 #endif
 #define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
 
-template <int D, int KIND, bool FEW>
+template <int D, int KIND, int FEW>
 struct PtCfg {
-  static constexpr int R = FEW ? 32 : 256, TWO = FEW ? 32 : 128, COPIES = FEW ? 4 : 1;
+  static constexpr int R = FEW ? FEW : 256, TWO = FEW ? FEW : 128, COPIES = FEW ? 128 / FEW : 1;
   static constexpr bool Q8 = KIND >= KCH_FP8_E4M3;
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
@@ -50,7 +53,7 @@ struct PtCfg {
   static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
 
-template <int D, int KIND, bool FEW>
+template <int D, int KIND, int FEW>
 struct PtSmem {
   typedef PtCfg<D, KIND, FEW> C;
   alignas(1024) uint8_t q[2][128 * D * 2];
@@ -66,7 +69,7 @@ struct PtSmem {
   uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
-static_assert(sizeof(PtSmem<128, KCH_BF16, false>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, false>) <= 232448, "shared memory of the paged attention");
+static_assert(sizeof(PtSmem<128, KCH_BF16, 0>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, 0>) <= 232448, "shared memory of the paged attention");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * 16384, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pt_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -218,7 +221,7 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
   }
 }
 
-template <int D, int KIND, bool FEW>
+template <int D, int KIND, int FEW>
 __global__ void __launch_bounds__(PtCfg<D, KIND, FEW>::THREADS, 1)
 paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
   typedef PtCfg<D, KIND, FEW> C;
@@ -393,11 +396,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u;
 #pragma unroll
             for (int i = 0; i < C::COPIES; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (32 * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (C::R * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
           } else {
 #pragma unroll
             for (int i = 0; i < C::COPIES; ++i)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (32 * 128)), "l"(src) : "memory");
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (C::R * 128)), "l"(src) : "memory");
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -451,14 +454,14 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (Walk w(a.bt, place); w.valid(); w.next()) {
       const bool pair = paired(w);
       constexpr int APART = 128 / C::COPIES;
-      const int ri = pair ? x * 128 + r : r % APART, sub = r / APART;      // row of the item, part of a tile's keys
+      const int ri = pair ? x * 128 + r : r % APART, sub = FEW ? r >> 5 : 0;      // row of the item, part of a tile's keys
       const bool live = ri < w.x.rows;
       const int2 keys = pg_sees(a.bt, w.s, w.block * C::R + ri);           // those of the row
       float m = -INFINITY, l = 0.f;
       for (int s = 0; s < w.count; ++s, ++n) {
         const int tile = pair ? w.first + s : 2 * (w.first + s) + x;
         const int key0 = w.x.first_key + tile * PT_KT, lo = keys.x - key0, hi = keys.y - key0;
-        const int from = sub * APART, to = from + APART;
+        const int from = 32 * sub, to = FEW ? from + 32 : PT_KT;
         const bool whole = __all_sync(0xffffffffu, !live || (lo <= from && hi >= to));
         const bool none = __all_sync(0xffffffffu, !live || min(hi, to) <= max(lo, from));
         const int slot = (pair ? kt : kt + x) % C::SCALES, turn = (pair ? kt : kt + x) / C::SCALES;
@@ -508,7 +511,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             }
           };
           uint32_t few[32];                              // (FEW: 32 keys a warp, which stay)
-          if constexpr (FEW) {
+          if constexpr (FEW != 0) {
             fetch(few, from);
             highest(few);
           } else {
@@ -564,10 +567,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                 pt_unpack(pt_mul2(pt_pack(p0, p1), e & 1 ? f.y : f.x), p0, p1);
               }
               pk[e] = pack2_bf16(p0, p1);
+              if (FEW == 16 && (r & 16)) pk[e] = pack2_bf16(p0 - __uint_as_float(pk[e] << 16), p1 - __uint_as_float(pk[e] & 0xFFFF0000u));
             }
             pt_st(tS + col / 2, pk);
           };
-          if constexpr (FEW) {
+          if constexpr (FEW != 0) {
             const uint32_t zero[16] = {};
 #pragma unroll
             for (int k = 1; k < 4; ++k) pt_st(tS + 16u * ((sub + k) & 3), zero);
@@ -644,20 +648,20 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const float ref = mm == -INFINITY ? 0.f : mm;
         w0 = ex2_fast((m0 - ref) * sc);                  // (0 for a part without a key: what its sums hold does not matter)
         w1 = ex2_fast((m1 - ref) * sc);
-        if (!FEW || r < 32) {
+        if (!FEW || r < APART) {
           ll = 0.f;                                      // (a NaN of a part's sum stays one)
 #pragma unroll
-          for (int k = 0; k < 256; k += APART) ll += sm.ml[1][ri + k] * ex2_fast((sm.ml[0][ri + k] - ref) * sc);
+          for (int k = 0; k < 256; k += FEW ? 32 : APART) ll += sm.ml[1][ri + k] * ex2_fast((sm.ml[0][ri + k] - ref) * sc);
         }
       }
       const float shift = mm == -INFINITY ? 0.f : mm * sc;
       float f = 1.f;
-      if (live && direct && (!FEW || r < 32)) f = factor(ri, ll, shift);
+      if (live && direct && (!FEW || r < APART)) f = factor(ri, ll, shift);
       if (live && !direct && (pair || (x == 0 && r < APART))) {
         slot[(int64_t)slot_rows * D + ri] = mm * sc;
         slot[(int64_t)slot_rows * D + slot_rows + ri] = ll;
       }
-      if (FEW && r < 32) sm.factor[x][r] = f;
+      if (FEW && r < APART) sm.factor[x][r] = f;
       const int c0 = pair ? 0 : x * (D / 2), c1 = pair ? D : c0 + D / 2;
       constexpr int CW = FEW ? D / 4 : 32, WORDS = CW / 4;       // columns, and 16-byte words, of a row at a time
       float odd = 0.f;                                   // 0 unless a value of the row is not finite
@@ -682,7 +686,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
         for (int e = 0; e < CW; ++e) z[e & 3] = fmaf(__uint_as_float(o0[e]), 0.f, z[e & 3]);
         odd += (z[0] + z[1]) + (z[2] + z[3]);
-        if constexpr (FEW) {                             // through the second query tile, 128 rows of either warpgroup
+        if constexpr (FEW != 0) {                             // through the second query tile, 128 rows of either warpgroup
           float4* stage = reinterpret_cast<float4*>(sm.q[1]) + x * 128 * WORDS;
           if (live) {
 #pragma unroll
@@ -727,7 +731,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       // rows that are not finite: again, over the columns stored here
       unsigned again;
-      if constexpr (FEW) again = (warp & 3) == 0 ? sm.odd[x] : 0u;       // (row i is lane i's of the first warp)
+      if constexpr (FEW != 0) again = (warp & 3) == 0 ? sm.odd[x] : 0u;       // (row i is lane i's of the first warp)
       else again = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
       if (again) {
         __syncwarp();
@@ -806,7 +810,7 @@ int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes
 
 bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16 && (c == 64 || c == 128); }
 
-template <int D, int KIND, bool FEW>
+template <int D, int KIND, int FEW>
 static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
   const int smem = (int)sizeof(PtSmem<D, KIND, FEW>);
   static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
@@ -821,7 +825,7 @@ static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAtten
   return KCH_OK;
 }
 
-int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaStream_t s) {
+int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
   const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT;
   int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
@@ -829,8 +833,8 @@ int kch_paged_attend_tc5(const PgAttend& a, int kind, bool few, int ctas, cudaSt
   if (rc != KCH_OK) return rc;
 #define PT_GO(D_, K_, F_) pt_launch<D_, K_, F_>(km, vm, a, ctas, s)
 #define PT_KIND(D_)                                                                            \
-  (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, false) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, false) \
-   : few ? PT_GO(D_, KCH_BF16, true) : PT_GO(D_, KCH_BF16, false))
+  (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, 0) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, 0)  \
+   : rows == 16 ? PT_GO(D_, KCH_BF16, 16) : rows == 32 ? PT_GO(D_, KCH_BF16, 32) : PT_GO(D_, KCH_BF16, 0))
   return a.c == 64 ? PT_KIND(64) : PT_KIND(128);
 #undef PT_KIND
 #undef PT_GO
