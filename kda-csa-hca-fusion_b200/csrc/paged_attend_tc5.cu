@@ -12,10 +12,10 @@
 // P is rounded to bf16, which adds to a result about as much as its own rounding does.  Steps of up to 16 rows leave 16 lanes of each
 // warp idle; there the rows lie in the tile eight times, and the other copy multiplies what the rounding of the first one left: the
 // output's rounding alone remains, at no cost.
-// Roles: warp 0 copies pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
+// Roles: warp 0 copies the keys' pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
 // issues  S_X = Q_X K^T  (M = N = 128) into 128 columns of tensor memory and  O_X += P_X V  with P_X, written by the softmax over
-// S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile; warps 2, 3 fetch the
-// next item's queries.  tcgen05.mma of one CTA complete in the order of issue, so S_X of the next tile may follow P_X V.
+// S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile; warp 3 fetches the
+// next item's queries, and warp 2 copies the values' pages, or with 8-bit pages shares warp 3's work, scales among it.  tcgen05.mma of one CTA complete in the order of issue, so S_X of the next tile may follow P_X V.
 // 8-bit pages: four more warps turn the copied payloads into bf16 tiles (exactly: a payload has at most 7 bits of mantissa);
 // a row's scale multiplies its logit, or its probability before that is rounded to bf16.
 //
@@ -26,6 +26,14 @@
 // the softmax clears the value rows behind it, whatever earlier tokens left there.  A key that only some rows of a tile see has
 // p = 0 in the others, which is no mask for an infinity or a NaN: O shows it, and such a row is summed again key by key, reading only
 // what it sees (pt_slow_row).  Every wait is bounded (status word, see kch_device_status).
+//
+// Measured, 16 heads of 128 on 4.  Steps of 64 sequences over 8192 tokens, pages of 64: 166 us, 6.5 TB/s, the memory's rate; 500 to
+// 16000 tokens, pages of 32 and more 174 us, of 16 196, of 8 322 (a tile is 16 or 32 copies then; with each page asked for where it
+// was needed and not a tile ahead pages of 16 took 263).  A chunk of 4096 tokens behind 28672: 850 us, 1210 TFLOP/s, in a burst, and
+// 1000 us in a long run, where the power limit holds the clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores
+// 512, maximum 350, powers 1500, value product 512, hand-overs 500, and two warpgroups that take turns.  None of these shortened it:
+// more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the
+// maximum and P in one pass (996, registers).  fp8 pages: 1310 us, the conversion's ALU operations and the scales' products.
 #include <cuda.h>
 #include <math.h>
 
@@ -237,7 +245,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
-    mbarrier_init(&sm.q_full, 2);
+    mbarrier_init(&sm.q_full, C::Q8 ? 2 : 1);
     mbarrier_init(&sm.q_empty, 1);
     sm.odd[0] = sm.odd[1] = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
@@ -264,9 +272,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
-    if (warp == 0) {
+    if (warp == 0 || (!C::Q8 && warp == 2)) {
       // ------------------------------ pages into the ring -----------------------------------------------------------------
-      // A tile is 128 / rows-of-a-box copies for each panel of 64 channels (8-bit pages: whole rows), a lane each.
+      // A tile is 128 / rows-of-a-box copies for each panel of 64 channels (8-bit pages: whole rows), a lane each.  Keys and values
+      // are a warp's each (8-bit pages: all are one's): small pages are many copies, and a warp issues them one after the other.
+      // A warp that comes to fill a place of the ring has filled one at most three places back, so everything N before that has
+      // been used, and a barrier's parity cannot be that of two uses ago.
       const int box = min(a.page, PT_KT), boxes = PT_KT / box, panels = C::Q8 ? 1 : C::PANELS;
       const int mybox = lane / panels, mypanel = lane % panels;
       const bool mine = lane < boxes * panels;
@@ -285,6 +296,10 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         };
         auto copy = [&](int tile, bool v, int id) {
           const int st = g % N, key = w.x.first_key + tile * PT_KT + mybox * box;
+          if (!C::Q8 && v != (warp == 2)) {
+            ++g;
+            return true;
+          }
           bool fine = g < N || wait(eb + st, g / N - 1);
           fine = __all_sync(0xffffffffu, fine);
           if (!fine) return false;
@@ -378,13 +393,14 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
     } else {
       // ------------------------------ queries ------------------------------------------------------------------------------
-      const int t = tid - 64;
+      constexpr int FETCH = C::Q8 ? 64 : 32;             // threads
+      const int t = tid - (128 - FETCH);
       int c = 0, kt = 0;
       bool ok = true;
       for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
         if (c) ok = wait(&sm.q_empty, c - 1);
         if (!ok) break;
-        constexpr int CHUNKS = D / 8, STEP = 64 / CHUNKS;      // 16 bytes a thread
+        constexpr int CHUNKS = D / 8, STEP = FETCH / CHUNKS;       // 16 bytes a thread
         const int rows = w.x.rows, k = t % CHUNKS;
 #pragma unroll 1
         for (int r = t / CHUNKS; r < rows; r += STEP) {

@@ -7,7 +7,8 @@
 // of the attention run on payloads, which bf16 holds exactly.  Bound by the bytes: 8 values a thread, a group of threads a row
 // (as many as it has such pieces, rounded up to a power of two), the row's maximum over that group by shuffles.  A warp has a token
 // and looks its page up once: with the bisection, two lookups and 64-bit divisions for every row of every head, a copy ran at
-// half the memory's rate.
+// half the memory's rate.  Measured: 28708 tokens of 8 key heads of 128 written as bf16 41 us, 5.7 TB/s; 32768 read from e4m3 42 us, 4.8
+// TB/s; one token each of 64 sequences, 4 key heads, written as e4m3 and read back 7.6 us for the two launches.
 #include <math.h>
 
 #include "paged.cuh"
