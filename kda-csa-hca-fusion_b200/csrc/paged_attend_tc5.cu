@@ -5,17 +5,18 @@
 // rows of a sequence against the key tiles of 128 that they see:
 //   chunks:  up to 256 rows, X = rows 0..127 and 128..255 against the same key tile; 128 rows or fewer: X = the even and the odd tiles;
 //   steps (FEW, where a sequence has few rows): up to 32 rows, X = the even and the odd tiles, and the rows lie in the 128 of the
-//     query tile four times (or eight, see below): warp w of a warpgroup has a row per thread as well, but only keys 32 w .. 32 w + 31 of a tile (its
-//     probabilities of the others are 0), with a maximum, a sum and an O of its own.  One warp of four would have all the work
-//     otherwise, and a tile's softmax would be the longest link of the chain.
+//     query tile four times (or eight, see below): warp w of a warpgroup has a row per thread as well, but only keys 32 w ..
+//     32 w + 31 of a tile (its probabilities of the others are 0), with a maximum, a sum and an O of its own.  One warp of four
+//     would have all the work otherwise, and a tile's softmax would be the longest link of the chain.
 // Parts of a row with sums of their own are joined through shared memory when the item ends.
 // P is rounded to bf16, which adds to a result about as much as its own rounding does.  Steps of up to 16 rows leave 16 lanes of each
 // warp idle; there the rows lie in the tile eight times, and the other copy multiplies what the rounding of the first one left: the
 // output's rounding alone remains, at no cost.
-// Roles: warp 0 copies the keys' pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
+// Roles: warp 0 copies pages by TMA (128-byte swizzle) into a ring of K and V tiles, in the order in which they are used; warp 1
 // issues  S_X = Q_X K^T  (M = N = 128) into 128 columns of tensor memory and  O_X += P_X V  with P_X, written by the softmax over
-// S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile; warp 3 fetches the
-// next item's queries, and warp 2 copies the values' pages, or with 8-bit pages shares warp 3's work, scales among it.  tcgen05.mma of one CTA complete in the order of issue, so S_X of the next tile may follow P_X V.
+// S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile (tcgen05.mma of one CTA
+// complete in the order of issue, so S_X of the next tile may follow P_X V); warps 2 and 3 fetch the next item's queries, with 8-bit
+// pages its scales too, but in steps over bf16 pages warp 2 copies the values' pages and warp 0 the keys'.
 // 8-bit pages: four more warps turn the copied payloads into bf16 tiles (exactly: a payload has at most 7 bits of mantissa);
 // a row's scale multiplies its logit, or its probability before that is rounded to bf16.
 //
@@ -28,8 +29,8 @@
 // what it sees (pt_slow_row).  Every wait is bounded (status word, see kch_device_status).
 //
 // Measured, 16 heads of 128 on 4.  Steps of 64 sequences over 8192 tokens, pages of 64: 166 us, 6.5 TB/s, the memory's rate; 500 to
-// 16000 tokens, pages of 32 and more 174 us, of 16 196, of 8 322 (a tile is 16 or 32 copies then; with each page asked for where it
-// was needed and not a tile ahead pages of 16 took 263).  A chunk of 4096 tokens behind 28672: 850 us, 1210 TFLOP/s, in a burst, and
+// 16000 tokens, pages of 16 and more 177 us, of 8 206 (a tile is 16 or 32 copies then: with one warp copying keys and values pages of
+// 16 and 8 took 196 and 322, and with each page asked for where it was needed and not a tile ahead pages of 16 took 263).  A chunk of 4096 tokens behind 28672: 850 us, 1210 TFLOP/s, in a burst, and
 // 1000 us in a long run, where the power limit holds the clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores
 // 512, maximum 350, powers 1500, value product 512, hand-overs 500, and two warpgroups that take turns.  None of these shortened it:
 // more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the
@@ -52,6 +53,7 @@ template <int D, int KIND, int FEW>
 struct PtCfg {
   static constexpr int R = FEW ? FEW : 256, TWO = FEW ? FEW : 128, COPIES = FEW ? 128 / FEW : 1;
   static constexpr bool Q8 = KIND >= KCH_FP8_E4M3;
+  static constexpr bool APART = FEW && !Q8;              // keys' and values' pages are copied by a warp each
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
@@ -245,7 +247,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
-    mbarrier_init(&sm.q_full, C::Q8 ? 2 : 1);
+    mbarrier_init(&sm.q_full, C::APART ? 1 : 2);
     mbarrier_init(&sm.q_empty, 1);
     sm.odd[0] = sm.odd[1] = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
@@ -272,10 +274,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
-    if (warp == 0 || (!C::Q8 && warp == 2)) {
+    if (warp == 0 || (C::APART && warp == 2)) {
       // ------------------------------ pages into the ring -----------------------------------------------------------------
-      // A tile is 128 / rows-of-a-box copies for each panel of 64 channels (8-bit pages: whole rows), a lane each.  Keys and values
-      // are a warp's each (8-bit pages: all are one's): small pages are many copies, and a warp issues them one after the other.
+      // A tile is 128 / rows-of-a-box copies for each panel of 64 channels (8-bit pages: whole rows), a lane each.  In steps
+      // over bf16 pages keys and values are a warp's each: small pages are many copies, and a warp issues them one after the other.
+      // Otherwise all are one's, which is soon enough, and the other fetches queries (one warp for both: 256 rows of them took so long
+      // that a prompt of 8192 tokens was 6 % slower).
       // A warp that comes to fill a place of the ring has filled one at most three places back, so everything N before that has
       // been used, and a barrier's parity cannot be that of two uses ago.
       const int box = min(a.page, PT_KT), boxes = PT_KT / box, panels = C::Q8 ? 1 : C::PANELS;
@@ -296,7 +300,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         };
         auto copy = [&](int tile, bool v, int id) {
           const int st = g % N, key = w.x.first_key + tile * PT_KT + mybox * box;
-          if (!C::Q8 && v != (warp == 2)) {
+          if (C::APART && v != (warp == 2)) {
             ++g;
             return true;
           }
@@ -393,7 +397,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
     } else {
       // ------------------------------ queries ------------------------------------------------------------------------------
-      constexpr int FETCH = C::Q8 ? 64 : 32;             // threads
+      constexpr int FETCH = C::APART ? 32 : 64;          // threads
       const int t = tid - (128 - FETCH);
       int c = 0, kt = 0;
       bool ok = true;
@@ -402,14 +406,18 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         if (!ok) break;
         constexpr int CHUNKS = D / 8, STEP = FETCH / CHUNKS;       // 16 bytes a thread
         const int rows = w.x.rows, k = t % CHUNKS;
-#pragma unroll 1
+        const bf16* base = (const bf16*)a.q + w.s.row0 * a.ld_q + w.h * G * D + k * 8;
+        const uint32_t to = smem_addr_u32(sm.q[0]) + (k >> 3) * (128 * 128);
+        constexpr uint32_t SECOND = 128 * D * 2 - 128 * 128;       // rows 128 .. of the second tile
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;    // (the softmax takes the scale's size: a maximum stays one)
+#pragma unroll 4
         for (int r = t / CHUNKS; r < rows; r += STEP) {
           const int row = w.block * C::R + r, tok = pg_token(a.bt, row);
-          const bf16* src = (const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + k * 8;
-          const uint32_t dst = smem_addr_u32(sm.q[r >> 7]) + (k >> 3) * (128 * 128) + (r & 127) * 128 + (((k & 7) ^ (r & 7)) << 4);
-          if (a.scale < 0.f) {                           // (the softmax takes the scale's size: a maximum stays one)
+          const bf16* src = base + tok * a.ld_q + (row - tok * G) * D;
+          const uint32_t dst = to + r * 128 + (r >> 7) * SECOND + (((k & 7) ^ (r & 7)) << 4);
+          if (flip) {
             uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
-            u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u;
+            u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
 #pragma unroll
             for (int i = 0; i < C::COPIES; ++i)
               asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (C::R * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
