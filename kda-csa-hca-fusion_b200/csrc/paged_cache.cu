@@ -241,6 +241,19 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
   }
 }
 
+// One wave: a block's warps walk tokens, so blocks behind the ones that an SM holds (6 of 40 registers) would only wait for their end
+// (8 to an SM whichever form: 41 us where this takes PLACEHOLDER, 28708 tokens of 8 heads of 128 written as bf16).
+template <typename T, int GROUP, bool READ, bool Q8>
+static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
+  static const int resident = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, Q8>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
+  }();
+  const int64_t wave = (int64_t)resident * KCH_SMS / a.parts;
+  const dim3 grid((unsigned)(blocks < wave ? blocks : wave), (unsigned)a.parts);
+  paged_rows_kernel<T, GROUP, READ, Q8><<<grid, PC_THREADS, 0, s>>>(a);
+}
+
 static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k, int64_t ld_k, void* v, int64_t ld_v, int dtype,
                      bool read, int zero_rest, void* stream) {
   const char* fn = read ? "kch_paged_read" : "kch_paged_append";
@@ -268,11 +281,10 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   const int rounds = (int)ceil_div64(2 * p->n_kv * group * a.tokens, 32);
   a.parts = (int)(blocks * (PC_THREADS / 32) >= 16 * KCH_SMS ? 1 : ceil_div64(16 * KCH_SMS, blocks * (PC_THREADS / 32)));
   if (a.parts > rounds) a.parts = rounds;
-  const dim3 grid((unsigned)(blocks < 8 * KCH_SMS ? blocks : 8 * KCH_SMS), (unsigned)a.parts);
 #define PC_GO(T_, G_, Q_)                                                                                                \
   do {                                                                                                                   \
-    if (read) paged_rows_kernel<T_, G_, true, Q_><<<grid, PC_THREADS, 0, s>>>(a);                                        \
-    else paged_rows_kernel<T_, G_, false, Q_><<<grid, PC_THREADS, 0, s>>>(a);                                            \
+    if (read) pc_launch<T_, G_, true, Q_>(a, blocks, s);                                                                 \
+    else pc_launch<T_, G_, false, Q_>(a, blocks, s);                                                                     \
   } while (0)
 #define PC_WIDTH(T_, Q_)                                                                                                 \
   do {                                                                                                                   \
