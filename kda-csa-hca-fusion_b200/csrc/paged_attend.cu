@@ -267,12 +267,21 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------
-// The rows of all items that are in parts, one after the other over the blocks.  Where a row has few parts it is a warp's, else a
-// block's whose warps take every eighth part; either sums them in one order.  4 (8) columns a lane.  Launched to start while
-// the kernel before it drains.  (One long sequence's step gives a row 74 or 148 parts: a warp a row took 80 us for them.)
-#define PJ_BLOCKS (8 * KCH_SMS)         // at most
+// The rows of all items that are in parts, one after the other over the blocks, in groups of ROWS of an item:
+// 4, or 1 where that gives every row a warp (steps of 64 sequences: 6 us, with 4 they take 7 to 8.5).  Where a row has up
+// to 8 parts a group is a warp's: lane 8 j + i weighs part i of its row j, so that maxima, sums and sink of the group are a load
+// each, and then the group's values of a part come at once.  (A row at a time, each after a search and three dependent loads,
+// the rows of a chunk's items took 20 to 26 us where this takes 12 to 14.)  Else a row is a block's whose warps take every eighth part.
+// Either sums the parts in one order.  4 (8) columns a lane.  Launched to start while the kernel before it drains.  (One long
+// sequence's step gives a row 74 or 148 parts: a warp a row took 80 us for them.)
+#define PJ_BLOCKS (4 * KCH_SMS)         // at most: those that the SMs hold
 #define PJ_WARPS 8
-template <typename T, int W>          // W: columns of a lane, in fours
+__device__ __forceinline__ void pj_store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+__device__ __forceinline__ void pj_store4(bf16* p, float a, float b, float c, float d) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+template <typename T, int W, int ROWS>      // W: columns of a lane, in fours; ROWS: of a group
 __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a, int ctas) {
   __shared__ int before[PA_CTAS + 1], wide[PA_CTAS], many[PA_CTAS], n_many;      // many: the items whose rows are a block's
   __shared__ alignas(16) float part_o[PJ_WARPS][W * 128];
@@ -281,11 +290,11 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
   chain_wait();
   for (int i = threadIdx.x; i < ctas; i += 32 * PJ_WARPS) {
     const PgRecord rec = a.records[i];
-    before[i + 1] = rec.valid ? rec.rows : 0;
     wide[i] = rec.valid && rec.last - i >= PJ_WARPS;
+    before[i + 1] = rec.valid && !wide[i] ? (rec.rows + ROWS - 1) / ROWS : 0;
   }
   __syncthreads();
-  if (warp == 0) {                     // rows of the parted items before each
+  if (warp == 0) {                     // groups of the parted items before each
     int run = 0, wides = 0;
     for (int i0 = 0; i0 < ctas; i0 += 32) {
       const int i = i0 + lane, x = run + pg_scan(i < ctas ? before[i + 1] : 0);
@@ -300,75 +309,106 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
     if (lane == 0) { before[0] = 0; n_many = wides; }
   }
   __syncthreads();
-  const int rows = before[ctas];
+  const int groups = before[ctas];
   const int64_t size = pg_slot_floats(a.slot_rows, a.c), mat = (int64_t)a.slot_rows * a.c;
-  // the parts `from`, from + step, .. of a row: their sums with the weights 2^(m_i - shift)
-  float o[4 * W], l;
-  auto gather = [&](int first, int last, int r, float shift, int from, int step) {
-    l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4 * W; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = first + from; i <= last; i += step) {
-      const float* s = a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size;
-      const float f = ex2_fast(s[mat + r] - shift), part = s[mat + a.slot_rows + r];
-      l = fmaf(f, part, l);
-#pragma unroll
-      for (int x = 0; x < W; ++x) {
-        const int d = 128 * x + 4 * lane;
-        if (d >= a.c) continue;
-        const float4 v = *reinterpret_cast<const float4*>(s + (int64_t)r * a.c + d);
-        // (weight 0: a part without keys; what its sums hold does not matter)
-        o[4 * x] = f == 0.f ? o[4 * x] : fmaf(f, v.x, o[4 * x]);
-        o[4 * x + 1] = f == 0.f ? o[4 * x + 1] : fmaf(f, v.y, o[4 * x + 1]);
-        o[4 * x + 2] = f == 0.f ? o[4 * x + 2] : fmaf(f, v.z, o[4 * x + 2]);
-        o[4 * x + 3] = f == 0.f ? o[4 * x + 3] : fmaf(f, v.w, o[4 * x + 3]);
-      }
-    }
+  auto slot_of = [&](int i, int first) { return a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size; };
+  // (weight 0: a part without keys; what its sums hold does not matter)
+  auto add = [](float (&o)[4 * W], int x, const float4& v, float f) {
+    o[4 * x] = f == 0.f ? o[4 * x] : fmaf(f, v.x, o[4 * x]);
+    o[4 * x + 1] = f == 0.f ? o[4 * x + 1] : fmaf(f, v.y, o[4 * x + 1]);
+    o[4 * x + 2] = f == 0.f ? o[4 * x + 2] : fmaf(f, v.z, o[4 * x + 2]);
+    o[4 * x + 3] = f == 0.f ? o[4 * x + 3] : fmaf(f, v.w, o[4 * x + 3]);
   };
-  auto highest = [&](int first, int last, int r) {
-    float m = -INFINITY;
-    for (int i = first + lane; i <= last; i += 32) m = fmaxf(m, a.slots[(2 * (int64_t)i + (i == first ? 1 : 0)) * size + mat + r]);
-    return warp_max(m);
+  auto place = [&](const PgRecord& rec, int r, int& h) {      // of the item's row r in the output; its head
+    const int row = rec.block * a.R + r, t = row / a.G;
+    h = rec.h * a.G + row - t * a.G;
+    return (T*)a.out + ((int64_t)(rec.row0 + t) * a.nh + h) * a.c;
   };
-  auto store = [&](const PgRecord& rec, int r, float shift) {
-    const int row = rec.block * a.R + r, t = row / a.G, h = rec.h * a.G + row - t * a.G;
+  auto factor = [&](float l, int h, float shift) {            // 1 / the row's denominator
     float below = l;
     if (a.sink && l > 0.f) below += ex2_fast(ld_any(a.sink, h, a.sink_dtype) * PG_LOG2E - shift);
-    const float f = l == 0.f ? 0.f : 1.f / below;
-    T* out = (T*)a.out + ((int64_t)(rec.row0 + t) * a.nh + h) * a.c;
-#pragma unroll
-    for (int x = 0; x < W; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 128 * x + 4 * lane + e;
-        if (d < a.c) stf(out + d, o[4 * x + e] * f);
-      }
+    return l == 0.f ? 0.f : 1.f / below;
   };
-  auto item_of = [&](int row) {        // the last i with before[i] <= row
-    int lo = 0, hi = ctas;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before[mid] <= row) lo = mid; else hi = mid;
+  auto store = [&](T* out, const float (&o)[4 * W], float f) {
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      const int d = 128 * x + 4 * lane;
+      if (d < a.c) pj_store4(out + d, o[4 * x] * f, o[4 * x + 1] * f, o[4 * x + 2] * f, o[4 * x + 3] * f);
     }
-    return lo;
   };
-  // rows of few parts: a warp each; the others are left to the blocks
-  for (int row = blockIdx.x * PJ_WARPS + warp; row < rows; row += gridDim.x * PJ_WARPS) {
-    const int i = item_of(row), r = row - before[i];
+  for (int g = blockIdx.x * PJ_WARPS + warp; g < groups; g += gridDim.x * PJ_WARPS) {
+    int i = 0, hi = ctas;              // the last i with before[i] <= g
+    while (hi - i > 1) {
+      const int mid = (i + hi) >> 1;
+      if (before[mid] <= g) i = mid; else hi = mid;
+    }
     const PgRecord rec = a.records[i];
-    if (rec.last - i >= PJ_WARPS) continue;
-    const float m = highest(i, rec.last, r), shift = m == -INFINITY ? 0.f : m;
-    gather(i, rec.last, r, shift, 0, 1);
-    store(rec, r, shift);
+    const int r0 = (g - before[i]) * ROWS, n = rec.last - i + 1, rows = min(rec.rows - r0, ROWS);
+    const int r = r0 + (lane >> 3), part = lane & 7;
+    float m = -INFINITY, l = 0.f;
+    if (part < n && lane >> 3 < rows) {
+      const float* s = slot_of(i + part, i) + mat + r;
+      m = s[0];
+      l = s[a.slot_rows];
+    }
+    float shift = m;
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) shift = fmaxf(shift, __shfl_xor_sync(0xffffffffu, shift, k));
+    if (shift == -INFINITY) shift = 0.f;
+    const float weight = ex2_fast(m - shift);
+    l *= weight;
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    int h = 0;
+    if (lane >> 3 < rows) place(rec, r, h);
+    const float f = factor(l, h, shift);
+    float o[ROWS][4 * W] = {};
+#pragma unroll 2
+    for (int k = 0; k < n; ++k) {
+      const float* s = slot_of(i + k, i) + (int64_t)r0 * a.c;
+      float4 v[ROWS][W];
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+          const int d = 128 * x + 4 * lane;
+          v[j][x] = j < rows && d < a.c ? *reinterpret_cast<const float4*>(s + j * a.c + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) {
+        const float w = __shfl_sync(0xffffffffu, weight, 8 * j + k);
+#pragma unroll
+        for (int x = 0; x < W; ++x) add(o[j], x, v[j][x], w);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const float fj = __shfl_sync(0xffffffffu, f, 8 * j);
+      if (j < rows) store(place(rec, r0 + j, h), o[j], fj);
+    }
   }
   for (int k = 0; k < n_many; ++k) {
     const int i = many[k];
     const PgRecord rec = a.records[i];
-    for (int row = before[i] + (int)((blockIdx.x + gridDim.x - before[i] % gridDim.x) % gridDim.x); row < before[i + 1]; row += gridDim.x) {
-      const int r = row - before[i];
-      const float m = highest(i, rec.last, r), shift = m == -INFINITY ? 0.f : m;
-      gather(i, rec.last, r, shift, warp, PJ_WARPS);
+    // (items of few rows: each begins with other blocks)
+    for (int r = (int)((blockIdx.x + gridDim.x - (unsigned)(k * a.slot_rows) % gridDim.x) % gridDim.x); r < rec.rows; r += gridDim.x) {
+      float m = -INFINITY;
+      for (int p = i + lane; p <= rec.last; p += 32) m = fmaxf(m, slot_of(p, i)[mat + r]);
+      m = warp_max(m);
+      const float shift = m == -INFINITY ? 0.f : m;
+      // the parts of this warp, with the weights 2^(m_p - shift)
+      float o[4 * W] = {}, l = 0.f;
+#pragma unroll 4
+      for (int p = i + warp; p <= rec.last; p += PJ_WARPS) {
+        const float* s = slot_of(p, i);
+        const float f = ex2_fast(s[mat + r] - shift);
+        l = fmaf(f, s[mat + a.slot_rows + r], l);
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+          const int d = 128 * x + 4 * lane;
+          if (d < a.c) add(o, x, *reinterpret_cast<const float4*>(s + (int64_t)r * a.c + d), f);
+        }
+      }
       __syncthreads();                 // (what was there has been read)
 #pragma unroll
       for (int x = 0; x < W; ++x) *reinterpret_cast<float4*>(&part_o[warp][128 * x + 4 * lane]) = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
@@ -382,18 +422,21 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[4 * x + e] += part_o[w][128 * x + 4 * lane + e];
         }
-        store(rec, r, shift);
+        int h;
+        T* out = place(rec, r, h);
+        store(out, o, factor(l, h, shift));
       }
     }
   }
 }
 
 int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s) {
-  const int64_t rows = (int64_t)ctas * a.slot_rows, want = (rows + PJ_WARPS - 1) / PJ_WARPS;      // that can be in parts
+  const int64_t rows = (int64_t)ctas * a.slot_rows, want = (rows + PJ_WARPS - 1) / PJ_WARPS;      // that can be in parts (a block each, where the parts are many)
   const dim3 grid((unsigned)(want < PJ_BLOCKS ? want : PJ_BLOCKS)), block(32 * PJ_WARPS);
   KCH_DISPATCH_FLOAT(a.dtype, T, {
-    if (a.c <= 128) KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 1>, grid, block, 0, s, 1, a, ctas));
-    else KCH_CUDA_OK(kch_launch_chained(paged_join_kernel<T, 2>, grid, block, 0, s, 1, a, ctas));
+    const bool each = rows <= PJ_BLOCKS * PJ_WARPS;
+    if (a.c <= 128) KCH_CUDA_OK(kch_launch_chained(each ? paged_join_kernel<T, 1, 1> : paged_join_kernel<T, 1, 4>, grid, block, 0, s, 1, a, ctas));
+    else KCH_CUDA_OK(kch_launch_chained(each ? paged_join_kernel<T, 2, 1> : paged_join_kernel<T, 2, 4>, grid, block, 0, s, 1, a, ctas));
   });
   KCH_LAUNCH_OK();
   return KCH_OK;
