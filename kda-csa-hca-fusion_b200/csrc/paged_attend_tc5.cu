@@ -405,26 +405,39 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         if (c) ok = wait(&sm.q_empty, c - 1);
         if (!ok) break;
         constexpr int CHUNKS = D / 8, STEP = FETCH / CHUNKS;       // 16 bytes a thread
+        static_assert(128 % (4 * STEP) == 0 && 4 * STEP % 8 == 0, "rows of a round");
         const int rows = w.x.rows, k = t % CHUNKS;
-        const bf16* base = (const bf16*)a.q + w.s.row0 * a.ld_q + w.h * G * D + k * 8;
-        const uint32_t to = smem_addr_u32(sm.q[0]) + (k >> 3) * (128 * 128);
-        constexpr uint32_t SECOND = 128 * D * 2 - 128 * 128;       // rows 128 .. of the second tile
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;    // (the softmax takes the scale's size: a maximum stays one)
-#pragma unroll 4
-        for (int r = t / CHUNKS; r < rows; r += STEP) {
-          const int row = w.block * C::R + r, tok = pg_token(a.bt, row);
-          const bf16* src = base + tok * a.ld_q + (row - tok * G) * D;
-          const uint32_t dst = to + r * 128 + (r >> 7) * SECOND + (((k & 7) ^ (r & 7)) << 4);
-          if (flip) {
-            uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
-            u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
+        // Every STEP'th row is a thread's.  Head, source and place in the swizzle are counted on from row to row: computed
+        // anew for each they made 256 rows 13000 cycles, more than what is left of an item once its last scores are there.
+        const int r0 = t / CHUNKS, skip = pg_token(a.bt, STEP), turn = STEP - skip * G;
+        const int row0 = w.block * C::R + r0, tok0 = pg_token(a.bt, row0);
+        int g = row0 - tok0 * G;
+        const bf16* src = (const bf16*)a.q + (w.s.row0 + tok0) * a.ld_q + (w.h * G + g) * D + k * 8;
+        const int64_t ahead = skip * a.ld_q + turn * D, over = a.ld_q - (int64_t)G * D;
+        uint32_t to = smem_addr_u32(sm.q[0]) + (k >> 3) * (128 * 128) + r0 * 128;
+        const uint32_t at = ((k & 7) ^ (r0 & 7)) << 4;
+#pragma unroll 1
+        for (int r = r0; r < rows; r += 4 * STEP, to += 4 * STEP * 128) {
+          if (!FEW && r == 128 + r0) to += 128 * D * 2 - 128 * 128;      // the second tile
 #pragma unroll
-            for (int i = 0; i < C::COPIES; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (C::R * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
-          } else {
+          for (int j = 0; j < 4; ++j) {
+            if (r + j * STEP >= rows) break;
+            const uint32_t dst = to + j * (STEP * 128) + (at ^ ((j * STEP & 7) << 4));
+            if (flip) {
+              uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
+              u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
 #pragma unroll
-            for (int i = 0; i < C::COPIES; ++i)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (C::R * 128)), "l"(src) : "memory");
+              for (int i = 0; i < C::COPIES; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + i * (C::R * 128)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+            } else {
+#pragma unroll
+              for (int i = 0; i < C::COPIES; ++i)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * (C::R * 128)), "l"(src) : "memory");
+            }
+            g += turn;
+            src += ahead;
+            if (g >= G) { g -= G; src += over; }
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
