@@ -63,6 +63,17 @@ struct PtCfg {
   static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
 
+// 32 bytes of a row.  (The lanes' rows are as many lines, one a cycle: half of 16 bytes' stores.)
+__device__ __forceinline__ void pt_store8(void* p, const uint32_t* v, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7]) : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+    *(reinterpret_cast<uint4*>(p) + 1) = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
 template <int D, int KIND, int FEW>
 struct PtSmem {
   typedef PtCfg<D, KIND, FEW> C;
@@ -703,6 +714,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       constexpr int CW = FEW ? D / 4 : 32, WORDS = CW / 4;       // columns, and 16-byte words, of a row at a time
       float odd = 0.f;                                   // 0 unless a value of the row is not finite
       bf16* orow = FEW ? nullptr : out_row(ri);
+      const bool wide = ((uintptr_t)a.out & 31) == 0;
 #pragma unroll 1
       for (int col = c0; col < c1; col += CW) {
         uint32_t o0[CW];
@@ -753,16 +765,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         } else if (live && ok) {
           if (direct) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t o4[4];
+            for (int e = 0; e < CW / 2; ++e) o0[e] = pack2_bf16(__uint_as_float(o0[2 * e]) * f, __uint_as_float(o0[2 * e + 1]) * f);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o4[e] = pack2_bf16(__uint_as_float(o0[8 * v + 2 * e]) * f, __uint_as_float(o0[8 * v + 2 * e + 1]) * f);
-              *reinterpret_cast<uint4*>(orow + col + 8 * v) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
-            }
+            for (int v = 0; v < CW / 2; v += 8) pt_store8(orow + col + 2 * v, o0 + v, wide);
           } else {
 #pragma unroll
-            for (int v = 0; v < WORDS; ++v)
-              *reinterpret_cast<uint4*>(slot + (int64_t)ri * D + col + 4 * v) = make_uint4(o0[4 * v], o0[4 * v + 1], o0[4 * v + 2], o0[4 * v + 3]);
+            for (int v = 0; v < CW; v += 8) pt_store8(slot + (int64_t)ri * D + col + v, o0 + v, true);
           }
         }
       }
