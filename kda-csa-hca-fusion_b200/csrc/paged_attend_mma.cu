@@ -8,8 +8,8 @@
 //
 // An item is up to 32 (token, head of the group) rows of a sequence; a tile is 128 keys, its payloads and scales copied into a ring by
 // one warp (TMA, 128-byte or 64-byte swizzle; scales by bulk copies).  Four warps share a tile, 32 keys each, and the other four take
-// the next one (32 rows: eight share it); a warp has a maximum, a sum and an O of its own, so that nothing but the ring is waited for, and they are joined when
-// the item ends.  (With 16 keys a warp and tile there were too few instructions that do not wait for one another: 2900 clocks a tile.)
+// the next one (32 rows: eight share it); a warp has a maximum, a sum and an O of its own, so that nothing but the ring is waited for,
+// and they are joined when the item ends.  (With 16 keys a warp and tile there were too few instructions that do not wait for one another: 2900 clocks a tile.)
 //   S = Q K^T: the order of the contraction is free, so thread (g, t) of a fragment takes 32 (16) consecutive channels of key g, four of
 //     them a product: a row is read in 16-byte words, and the queries' fragments are loaded in the same order.
 //   O += P V:  the order of the columns is free, so thread (g, t) takes 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9,
@@ -32,7 +32,8 @@
 #define PM_SPIN (1u << 26)
 
 // R rows an item: 8, 16 or 32, by what a sequence has.  8 (one token of up to 8 heads): the lower half of the scores' fragments is
-// empty, and that of P has what its rounding left (paged_attend_tc5.cu has the reason; 16 rows: in products of their own, 7 %; 32: none).  32: two fragments a warp, which then takes 16 keys of every tile, for the registers' sake.
+// empty, and that of P has what its rounding left (paged_attend_tc5.cu has the reason; 16 rows: in products of their own, 7 %; 32:
+// none).  32: two fragments a warp, which then takes 16 keys of every tile, for the registers' sake.
 template <int R>
 struct PmCfg {
   static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;                   // that compute; the first warpgroup copies

@@ -28,13 +28,17 @@
 // p = 0 in the others, which is no mask for an infinity or a NaN: O shows it, and such a row is summed again key by key, reading only
 // what it sees (pt_slow_row).  Every wait is bounded (status word, see kch_device_status).
 //
-// Measured, 16 heads of 128 on 4.  Steps of 64 sequences over 8192 tokens, pages of 64: 166 us, 6.5 TB/s, the memory's rate; 500 to
-// 16000 tokens, pages of 16 and more 177 us, of 8 206 (a tile is 16 or 32 copies then: with one warp copying keys and values pages of
-// 16 and 8 took 196 and 322, and with each page asked for where it was needed and not a tile ahead pages of 16 took 263).  A chunk of 4096 tokens behind 28672: 850 us, 1210 TFLOP/s, in a burst, and
-// 1000 us in a long run, where the power limit holds the clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores
-// 512, maximum 350, powers 1500, value product 512, hand-overs 500, and two warpgroups that take turns.  None of these shortened it:
-// more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the
-// maximum and P in one pass (996, registers).  fp8 pages: 1310 us, the conversion's ALU operations and the scales' products.
+// Measured, 16 heads of 128 on 4.  Steps of 64 sequences over 8192 tokens, pages of 64: 169 us, 6.4 TB/s, the memory's rate; 500 to
+// 16000 tokens, pages of 16 and more 176 us, of 8 198 (a tile is 16 or 32 copies then: with one warp copying keys and values pages of
+// 16 and 8 took 196 and 322, and with each page asked for where it was needed and not a tile ahead pages of 16 took 263).
+// A chunk of 4096 tokens behind 28672: 835 us, 1240 TFLOP/s, in a burst, and 1000 us in a long run, where the power limit holds the
+// clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores 512, maximum 350, powers 1500, value product 512,
+// hand-overs 500, and two warpgroups that take turns.  None of these shortened it: more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us
+// in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the maximum and P in one pass (996, registers).  fp8 pages:
+// 1300 us, the conversion's ALU operations and the scales' products (6000 clocks a step).  Short items cost their ends: 37 x 16 items of
+// 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks until a CTA's first scores, as many for the
+// first end (its code comes from memory), then 6000 an end and 3000 until the next item's scores (its queries: 12000 clocks for two
+// warps' copies, most of them behind the last softmax).
 #include <cuda.h>
 #include <math.h>
 
@@ -44,9 +48,7 @@
 #include "tc5_utils.cuh"
 
 #define PT_KT 128
-#ifndef PT_POLY
 #define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks)
-#endif
 #define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
 
 template <int D, int KIND, int FEW>

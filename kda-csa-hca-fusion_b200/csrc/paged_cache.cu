@@ -7,7 +7,7 @@
 // of the attention run on payloads, which bf16 holds exactly.  Bound by the bytes: 8 values a thread, a group of threads a row
 // (as many as it has such pieces, rounded up to a power of two), the row's maximum over that group by shuffles.  A warp has a token
 // and looks its page up once: with the bisection, two lookups and 64-bit divisions for every row of every head, a copy ran at
-// half the memory's rate.  Measured: 28708 tokens of 8 key heads of 128 written as bf16 41 us, 5.7 TB/s; 32768 read from e4m3 42 us, 4.8
+// half the memory's rate.  Measured: 28708 tokens of 8 key heads of 128 written as bf16 41 us, 5.7 TB/s; 32768 read from e4m3 38 us, 5.4
 // TB/s; one token each of 64 sequences, 4 key heads, written as e4m3 and read back 7.6 us for the two launches.
 #include <math.h>
 
@@ -135,7 +135,8 @@ __device__ __forceinline__ PcWords<T> pc_words(const void* p) {
 }
 
 // A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
-// looked up once a token, and four rows a thread are in flight.  Where tokens are few, several warps share one's rows.  READ: pages -> packed rows, else packed rows -> pages.
+// looked up once a token, and four rows a thread are in flight.  Where tokens are few, several warps share one's rows.  READ: pages
+// -> packed rows, else packed rows -> pages.
 #define PC_FLIGHT 4
 template <typename T, int GROUP, bool READ, bool Q8>
 __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_constant__ PgRows a) {
@@ -241,12 +242,14 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
   }
 }
 
-// One wave: a block's warps walk tokens, so blocks behind the ones that an SM holds (6 of 40 registers) would only wait for their end
-// (8 to an SM whichever form: 41 us where this takes PLACEHOLDER, 28708 tokens of 8 heads of 128 written as bf16).
+// 8-bit pages: one wave of blocks, whose warps walk the tokens; more of them would only wait for the others' end (32768 tokens of 8 heads
+// of 128 read from e4m3: 38 us, 42 with 8 to an SM).  Rows that are copied: 8 to an SM, of which it holds 6 (28708 such tokens written
+// as bf16: 41 us, 44 in one wave, where an SM that is behind stays so).
 template <typename T, int GROUP, bool READ, bool Q8>
 static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
   static const int resident = [] {
     int n = 0;
+    if (!Q8) return 8;
     return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, Q8>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
   }();
   const int64_t wave = (int64_t)resident * KCH_SMS / a.parts;

@@ -155,7 +155,8 @@ class PagedKVCache:
 
     def append_step(self, k_new, v_new, table, t0, cu_seqlens):
         """Writes the new rows ``k_new``, ``v_new`` ``[N, n_kv, c]`` into their pages.  Rows outside of
-        ``[cu_seqlens[0], cu_seqlens[B])`` are not read."""
+        ``[cu_seqlens[0], cu_seqlens[B])`` are not read.  No two rows of a call go to one place of the pool (pages that sequences
+        share hold tokens before the call's)."""
         fn = "append_step"
         N = self._rows(fn, "k_new", k_new, self.n_kv)[0]
         if self._rows(fn, "v_new", v_new, self.n_kv)[0] != N:

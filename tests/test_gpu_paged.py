@@ -382,6 +382,20 @@ def test_strided_operands_and_tables(kch):
     assert torch.equal(m.cache.forward_step(q, m.table, pairs[:, 0], m.cu), want)
 
 
+@pytest.mark.parametrize("new,past", [([1, 1], [33, 700]), ([40, 300], [100, 900])])
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, "fp8", 64), (torch.bfloat16, "int8", 128), (torch.float32, None, 64)])
+def test_an_output_that_begins_on_16_bytes_and_no_more(kch, dtype, kind, c, new, past):
+    m = Batch(kch, new, past, dtype=dtype, kind=kind, c=c)
+    q = m.randn(m.N, 6, c)
+    want = m.cache.forward_step(q, *m.args)
+    ahead = 16 // want.element_size()
+    room = torch.full((ahead + want.numel() + ahead,), 7.0, dtype=dtype, device=DEV)
+    out = room[ahead:ahead + want.numel()].view(want.shape)
+    assert out.data_ptr() % 32 == 16
+    m.cache.forward_step(q, *m.args, out=out)
+    assert torch.equal(out, want) and torch.equal(room[:ahead], room[-ahead:]) and (room[:ahead] == 7).all()
+
+
 def test_offsets_that_pass_32_bits(kch):
     """A pool whose rows lie beyond 2^32 elements."""
     pages, page, c = 2 ** 32 // (64 * 128) + 40, 64, 128
