@@ -482,7 +482,8 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   KCH_REQUIRE(p->sliding_window >= 0, "kch_paged_attend: sliding_window=%d must be >= 0 (0: every key)", p->sliding_window);
   KCH_REQUIRE(isfinite(p->scale), "kch_paged_attend: scale must be finite");
   KCH_REQUIRE(!p->sink || p->sink_dtype == KCH_F32 || p->sink_dtype == KCH_BF16, "kch_paged_attend: sink dtype tag %d", p->sink_dtype);
-  KCH_REQUIRE(p->batch.N * p->nh <= 0x7FFFFFFFLL, "kch_paged_attend: N * nh = %lld rows of q", (long long)(p->batch.N * p->nh));
+  KCH_REQUIRE(p->batch.N * p->nh <= 0x7FFFFE00LL && (int64_t)p->nh * c <= 0x7FFFFFFFLL,       // (rows, a block's end among them, and columns in 32 bits)
+              "kch_paged_attend: N * nh = %lld rows of q, nh * c = %lld columns", (long long)(p->batch.N * p->nh), (long long)p->nh * c);
   if (p->batch.N == 0) return KCH_OK;
   const int es = p->dtype == KCH_BF16 ? 2 : 4;
   KCH_REQUIRE(p->q && p->out, "kch_paged_attend: null q or out");
@@ -504,6 +505,9 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   const PaPlan x = pa_plan(p);
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) <= 0x7FFFFFFFLL, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
+  // (an item's queries may be read again while its rows are stored)
+  const uintptr_t q0 = (uintptr_t)p->q, q1 = q0 + ((p->batch.N - 1) * p->ld_q + (int64_t)p->nh * c) * es, o0 = (uintptr_t)p->out;
+  KCH_REQUIRE(o0 >= q1 || o0 + p->batch.N * p->nh * c * es <= q0, "kch_paged_attend: out overlaps q");
   KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
   a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;

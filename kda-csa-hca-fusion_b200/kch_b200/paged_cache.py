@@ -94,13 +94,19 @@ class PagedKVCache:
             if t is not None and t.data_ptr() % 16:
                 raise ValueError(f"PagedKVCache: {name} must start on 16 bytes")
         self.device = where
-        self.k_pages, self.v_pages, self.k_scales, self.v_scales = storage
+        self._storage = tuple(storage)
         self._ws_bytes = {}             # of attention calls, by their sizes
         self._row = torch.empty(0, dtype=dtype, device=self.device)        # (what new tensors are made from)
         self._byte = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._tag, self._index, self._lib = _lib.dtype_tag(dtype), self.k_pages.get_device(), _lib.load()
         self._c = _lib.PagedCache(self.k_pages.data_ptr(), self.v_pages.data_ptr(), _lib.ptr(self.k_scales), _lib.ptr(self.v_scales),
                                   self._tag if kv_quant is None else _QUANT[kv_quant], num_pages, page_size, n_kv, c)
+
+    # (not to be set: the kernels have their addresses)
+    k_pages = property(lambda self: self._storage[0])
+    v_pages = property(lambda self: self._storage[1])
+    k_scales = property(lambda self: self._storage[2])
+    v_scales = property(lambda self: self._storage[3])
 
     # A call of a decode step takes the host longer than the GPU: the checks compare what they can in one expression, and name
     # the argument at fault only where it fails.
@@ -192,7 +198,7 @@ class PagedKVCache:
         multiple of ``n_kv``; query head h reads key head ``h // (nh // n_kv)``) -> ``[N, nh, c]`` in ``q.dtype``.  The query at
         position p sees the keys ``0 .. p``, or the last ``sliding_window`` of them.  ``scale``: ``c ** -0.5`` unless given;
         ``sink_logits [nh]`` adds ``exp(sink)`` to the denominator.  Rows of no sequence are zeros, and stay as they are in a
-        tensor given as ``out``."""
+        tensor given as ``out``, which does not overlap ``q``."""
         fn = "forward_step"
         N, nh, c = self._rows(fn, "q", q)
         if nh < 1 or nh % self.n_kv:

@@ -86,3 +86,27 @@ def test_workspace_grows_with_the_width_and_asks_for_nothing_where_the_arguments
     assert lib.kch_paged_attend_workspace_bytes(None) == 0
     assert lib.kch_paged_attend_workspace_bytes(_args(_lib, n_kv=0)) == 0
     assert ctypes.sizeof(_lib.PagedAttendArgs) == ctypes.sizeof(_lib.PagedCache) + ctypes.sizeof(_lib.PagedBatch) + 80
+
+
+@pytest.mark.parametrize("over", [dict(), dict(out=4096 + 2 * 256 * 2 + 2 * 248), dict(q=4096 + 2 * 256 * 3 - 16), dict(N=1, ld_q=1 << 20, out=4096 + 2 * 240)])
+def test_an_output_over_the_queries_is_refused(over):
+    from kch_b200 import _lib
+    lib = _lib.load()
+    with pytest.raises(ValueError, match="overlaps"):
+        _lib.check(lib.kch_paged_attend(_args(_lib, ws_bytes=1 << 40, **over), None))
+
+
+def test_more_rows_and_columns_than_32_bits_count_are_refused():
+    from kch_b200 import _lib
+    lib = _lib.load()
+    for over in (dict(N=0x7FFFFE00 // 4 + 1), dict(nh=1 << 26, ld_q=1 << 32, N=1)):
+        with pytest.raises(ValueError, match="N \\* nh"):
+            _lib.check(lib.kch_paged_attend(_args(_lib, ws_bytes=1 << 40, **over), None))
+
+
+def test_the_storage_of_a_cache_cannot_be_exchanged():
+    import kch_b200
+    cache = object.__new__(kch_b200.PagedKVCache)
+    for name in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(1))
