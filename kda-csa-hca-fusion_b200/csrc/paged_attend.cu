@@ -267,13 +267,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------------------
-// The rows of all items that are in parts, one after the other over the blocks, in groups of ROWS of an item:
-// 4, or 1 where that gives every row a warp (steps of 64 sequences: 6 us, with 4 they take 7 to 8.5).  Where a row has up
-// to 8 parts a group is a warp's: lane 8 j + i weighs part i of its row j, so that maxima, sums and sink of the group are a load
-// each, and then the group's values of a part come at once.  (A row at a time, each after a search and three dependent loads,
-// the rows of a chunk's items took 20 to 26 us where this takes 12 to 14.)  Else a row is a block's whose warps take every eighth part.
-// Either sums the parts in one order.  4 (8) columns a lane.  Launched to start while the kernel before it drains.  (One long
-// sequence's step gives a row 74 or 148 parts: a warp a row took 80 us for them.)
+// The rows of all items that are in parts, one after the other over the blocks, in groups of ROWS of an item: 4, or 1 where that
+// gives every row a warp (steps of 64 sequences: 6 us, with 4 they take 7 to 8.5).  Where a row has up to 8 parts a group is a warp's:
+// lane 8 j + i weighs part i of its row j, so that maxima, sums and sink of the group are a load each, and then the group's values of
+// a part come at once.  (A row at a time, each after a search and three dependent loads, the rows of a chunk's items took 20 to 26 us
+// where this takes 12 to 14.)  Else a row is a block's: a thread weighs a part, a warp sums every eighth.  (One long sequence's step gives
+// a row 74 or 148 parts: a warp a row took 80 us for them; weighed by the warp that sums them 64 rows of 74 took 10, now 8.)  Either sums
+// the parts in one order.  4 (8) columns a lane.  Launched to start while the kernel before it drains.
 #define PJ_BLOCKS (4 * KCH_SMS)         // at most: those that the SMs hold
 #define PJ_WARPS 8
 __device__ __forceinline__ void pj_store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
@@ -285,7 +285,8 @@ template <typename T, int W, int ROWS>      // W: columns of a lane, in fours; R
 __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a, int ctas) {
   __shared__ int before[PA_CTAS + 1], wide[PA_CTAS], many[PA_CTAS], n_many;      // many: the items whose rows are a block's
   __shared__ alignas(16) float part_o[PJ_WARPS][W * 128];
-  __shared__ float part_l[PJ_WARPS];
+  __shared__ float part_m[PJ_WARPS], part_l[PJ_WARPS], weight[PA_CTAS];
+  constexpr int PER = (PA_CTAS + 32 * PJ_WARPS - 1) / (32 * PJ_WARPS);       // parts of a row that a thread weighs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   chain_wait();
   for (int i = threadIdx.x; i < ctas; i += 32 * PJ_WARPS) {
@@ -392,39 +393,58 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
     const PgRecord rec = a.records[i];
     // (items of few rows: each begins with other blocks)
     for (int r = (int)((blockIdx.x + gridDim.x - (unsigned)(k * a.slot_rows) % gridDim.x) % gridDim.x); r < rec.rows; r += gridDim.x) {
-      float m = -INFINITY;
-      for (int p = i + lane; p <= rec.last; p += 32) m = fmaxf(m, slot_of(p, i)[mat + r]);
-      m = warp_max(m);
-      const float shift = m == -INFINITY ? 0.f : m;
-      // the parts of this warp, with the weights 2^(m_p - shift)
-      float o[4 * W] = {}, l = 0.f;
-#pragma unroll 4
-      for (int p = i + warp; p <= rec.last; p += PJ_WARPS) {
-        const float* s = slot_of(p, i);
-        const float f = ex2_fast(s[mat + r] - shift);
-        l = fmaf(f, s[mat + a.slot_rows + r], l);
+      // a thread weighs one part, or two: weights 2^(m_p - shift)
+      const int n = rec.last - i + 1;
+      float m[PER], l[PER], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const int p = threadIdx.x + q * 32 * PJ_WARPS;
+        const float* s = slot_of(i + (p < n ? p : 0), i) + mat + r;
+        m[q] = p < n ? s[0] : -INFINITY;
+        l[q] = p < n ? s[a.slot_rows] : 0.f;
+        top = fmaxf(top, m[q]);
+      }
+      top = warp_max(top);
+      __syncthreads();                 // (what the row before left has been read)
+      if (lane == 0) part_m[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < PJ_WARPS; ++w) top = fmaxf(top, part_m[w]);
+      const float shift = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const int p = threadIdx.x + q * 32 * PJ_WARPS;
+        const float f = ex2_fast(m[q] - shift);
+        if (p < n) weight[p] = f;
+        sum = fmaf(f, l[q], sum);
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) part_l[warp] = sum;
+      __syncthreads();
+      float o[4 * W] = {};
+#pragma unroll 8
+      for (int p = warp; p < n; p += PJ_WARPS) {
+        const float* s = slot_of(i + p, i) + (int64_t)r * a.c;
 #pragma unroll
         for (int x = 0; x < W; ++x) {
           const int d = 128 * x + 4 * lane;
-          if (d < a.c) add(o, x, *reinterpret_cast<const float4*>(s + (int64_t)r * a.c + d), f);
+          if (d < a.c) add(o, x, *reinterpret_cast<const float4*>(s + d), weight[p]);
         }
       }
-      __syncthreads();                 // (what was there has been read)
 #pragma unroll
       for (int x = 0; x < W; ++x) *reinterpret_cast<float4*>(&part_o[warp][128 * x + 4 * lane]) = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-      if (lane == 0) part_l[warp] = l;
       __syncthreads();
-      if (warp == 0) {
-        for (int w = 1; w < PJ_WARPS; ++w) {
-          l += part_l[w];
+      const int d = threadIdx.x;       // (at most 256 columns, one a thread)
+      if (d < a.c) {
+        float all = 0.f, below = 0.f;
 #pragma unroll
-          for (int x = 0; x < W; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * x + e] += part_o[w][128 * x + 4 * lane + e];
+        for (int w = 0; w < PJ_WARPS; ++w) {
+          all += part_o[w][d];
+          below += part_l[w];
         }
         int h;
         T* out = place(rec, r, h);
-        store(out, o, factor(l, h, shift));
+        stf(out + d, all * factor(below, h, shift));
       }
     }
   }
