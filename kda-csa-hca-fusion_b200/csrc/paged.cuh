@@ -82,7 +82,7 @@ __device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int ro
   return make_int2(a.window > 0 ? (int)min(max(pos - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0, (int)min(pos + 1, (int64_t)s.kv));
 }
 
-// Where a CTA's range of steps begins.  (Steps are counted in 32 bits: the host refuses a call that could have 2^31.)
+// Where a CTA's range of steps begins.  (Steps are counted in 32 bits: the host refuses a call that could have 2^31 - 1.)
 struct PgPlace {
   int per, left;                       // steps of a CTA; steps of this one
   int b, h, block, step;
@@ -121,11 +121,13 @@ __device__ __forceinline__ PgSeq pg_seq_or_none(const PgBatch& a, int b) {
   }
   return s;
 }
+#define PG_MOST 0x7FFFFFFF
+__device__ __forceinline__ int pg_sum(int x, int y) { return (int)min((unsigned)x + (unsigned)y, (unsigned)PG_MOST); }      // (of what is not negative)
 __device__ __forceinline__ int pg_scan(int x) {             // sums over the lanes up to this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if ((threadIdx.x & 31) >= o) x += y;
+    if ((threadIdx.x & 31) >= o) x = pg_sum(x, y);
   }
   return x;
 }
@@ -138,6 +140,12 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
   PgPlace p = {};
   int total, before = 0, mine = 0;                          // steps: of all, before sequence p.b, of it
   auto range = [&] {
+    // The host has counted a row once.  Where cu_seqlens falls and rises again a row is of several sequences, and there may be more
+    // steps than are counted: such a call does nothing.
+    if (total == PG_MOST) {
+      pg_bad(a);
+      total = 0;
+    }
     p.per = max((int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas), 1);
     const int64_t start = (int64_t)p.per * cta;
     p.left = (int)max(min((int64_t)p.per, total - start), (int64_t)0);
@@ -172,7 +180,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
       int run = 0;
 #pragma unroll 1
       for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int x = run + pg_scan(b0 + lane < a.B ? base[b0 + lane + 1] : 0);
+        const int x = pg_sum(run, pg_scan(b0 + lane < a.B ? base[b0 + lane + 1] : 0));
         if (b0 + lane < a.B) base[b0 + lane + 1] = x;
         run = __shfl_sync(0xffffffffu, x, 31);
       }

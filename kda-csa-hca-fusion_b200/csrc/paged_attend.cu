@@ -62,7 +62,7 @@ struct PgStored {
 #define PA_THREADS 256
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
-// steps that a call can have at most, whatever the lengths on the device
+// steps that a call can have at most, whatever the lengths on the device (of which no two share a row)
 static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1); }
 
 static constexpr int pa_smem(int ROWS, int DMAX) { return (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4; }
@@ -523,7 +523,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   a.records = (PgRecord*)p->workspace;
   const PaPlan x = pa_plan(p);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) <= 0x7FFFFFFFLL, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
   // (an item's queries may be read again while its rows are stored)
   const uintptr_t q0 = (uintptr_t)p->q, q1 = q0 + ((p->batch.N - 1) * p->ld_q + (int64_t)p->nh * c) * es, o0 = (uintptr_t)p->out;

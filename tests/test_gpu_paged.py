@@ -445,6 +445,24 @@ def test_tables_that_name_no_page_raise_the_status_and_touch_nothing(kch):
             assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
 
 
+@pytest.mark.parametrize("dtype,kind,B,N,n_kv", [(torch.bfloat16, None, 4096, 4096, 16), (torch.bfloat16, "fp8", 4096, 4096, 16),
+                                                 (torch.float32, None, 4096, 4096, 16), (torch.bfloat16, None, 4096, 16400, 16),
+                                                 (torch.bfloat16, None, 32, 65536, 128)])
+def test_lengths_that_fall_and_rise_again_beyond_what_is_counted_do_nothing(kch, dtype, kind, B, N, n_kv):
+    """Every other sequence has all rows: more steps in all than 32 bits hold, which the host, who sees N alone, cannot know."""
+    from kch_b200 import _lib
+    assert _lib.device_status() == 0
+    cache = kch.PagedKVCache(1, 256, n_kv, 64, DEV, dtype, kv_quant=kind)
+    table = torch.zeros(B, 4096, dtype=torch.int32, device=DEV)
+    t0 = torch.full((B,), 4096 * 256 - N, dtype=torch.int32, device=DEV)
+    cu = (torch.arange(B + 1, device=DEV) % 2 * N).int()
+    q, out = torch.zeros(N, n_kv, 64, dtype=dtype, device=DEV), torch.full((N, n_kv, 64), 7.0, dtype=dtype, device=DEV)
+    cache.forward_step(q, table, t0, cu, out=out)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+    assert (out == 7).all()
+
+
 def test_what_python_refuses(kch):
     m = Batch(kch, [2, 3], [5, 6])
     q, k = m.randn(5, 4, 128), m.randn(5, 2, 128)
