@@ -35,7 +35,8 @@
 // clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores 512, maximum 350, powers 1500, value product 512,
 // hand-overs 500, and two warpgroups that take turns.  None of these shortened it: more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us
 // in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the maximum and P in one pass (996, registers).  fp8 pages:
-// 1300 us, the conversion's ALU operations and the scales' products (6000 clocks a step).  Short items cost their ends: 37 x 16 items of
+// 1270 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
+// the FMAs have the scales: 1281 as with bf16 pages, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).  Short items cost their ends: 37 x 16 items of
 // 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks until a CTA's first scores, as many for the
 // first end (its code comes from memory), then 6000 an end and 3000 until the next item's scores (its queries: 12000 clocks for two
 // warps' copies, most of them behind the last softmax).
@@ -48,7 +49,7 @@
 #include "tc5_utils.cuh"
 
 #define PT_KT 128
-#define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks)
+#define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks over bf16 pages)
 #define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
 
 template <int D, int KIND, int FEW>
@@ -603,7 +604,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               float x0, x1;
               pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
               float p0, p1;
-              if (!FEW && (e & 3) >= 4 - PT_POLY) {
+              if (!FEW && !C::Q8 && (e & 3) >= 4 - PT_POLY) {
                 pt_ex2_fma(x0, x1);
                 p0 = x0;
                 p1 = x1;
