@@ -36,10 +36,10 @@
 // hand-overs 500, and two warpgroups that take turns.  None of these shortened it: more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us
 // in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the maximum and P in one pass (996, registers).  fp8 pages:
 // 1270 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
-// the FMAs have the scales: 1281 as with bf16 pages, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).  Short items cost their ends: 37 x 16 items of
-// 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks until a CTA's first scores, as many for the
-// first end (its code comes from memory), then 6000 an end and 3000 until the next item's scores (its queries: 12000 clocks for two
-// warps' copies, most of them behind the last softmax).
+// the FMAs have the scales: 1281 as with bf16 pages, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).
+// Short items cost their ends: 37 x 16 items of 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks
+// until a CTA's first scores, as many for the first end (its code comes from memory), then 6000 an end and 3000 until the next item's
+// scores (its queries: 12000 clocks for two warps' copies, most of them behind the last softmax).
 #include <cuda.h>
 #include <math.h>
 
