@@ -31,12 +31,13 @@
 // Measured, 16 heads of 128 on 4.  Steps of 64 sequences over 8192 tokens, pages of 64: 169 us, 6.4 TB/s, the memory's rate; 500 to
 // 16000 tokens, pages of 16 and more 176 us, of 8 198 (a tile is 16 or 32 copies then: with one warp copying keys and values pages of
 // 16 and 8 took 196 and 322, and with each page asked for where it was needed and not a tile ahead pages of 16 took 263).
-// A chunk of 4096 tokens behind 28672: 835 us, 1240 TFLOP/s, in a burst, and 1000 us in a long run, where the power limit holds the
+// A chunk of 4096 tokens behind 28672: 827 us, 1247 TFLOP/s, in a burst, and 1000 us in a long run, where the power limit holds the
 // clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores 512, maximum 350, powers 1500, value product 512,
-// hand-overs 500, and two warpgroups that take turns.  None of these shortened it: more powers by FMAs (PT_POLY 0, 1, 2: 878, 883, 932 us
-// in one run, heads of 64 1559, 1506, 1623), P handed over in halves (883), the maximum and P in one pass (996, registers).  fp8 pages:
-// 1270 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
-// the FMAs have the scales: 1281 as with bf16 pages, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).
+// hand-overs 500, and two warpgroups that take turns.  Powers by FMAs (POLY) help heads of 64 alone, whose products are half as long: 32 of
+// them 1486 us with one pair of four, 1579 with none, 1623 with two; heads of 128 827 with none, 825 with one, 932 against 878 with two.
+// Neither did P handed over in halves (883 where the rest took 878) shorten it, nor the maximum and P in one pass (996, registers).  fp8
+// pages: 1270 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
+// the FMAs have the scales: 1281 with one pair of four, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).
 // Short items cost their ends: 37 x 16 items of 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks
 // until a CTA's first scores, as many for the first end (its code comes from memory), then 6000 an end and 3000 until the next item's
 // scores (its queries: 12000 clocks for two warps' copies, most of them behind the last softmax).
@@ -49,7 +50,6 @@
 #include "tc5_utils.cuh"
 
 #define PT_KT 128
-#define PT_POLY 1       // of 4 pairs: how many powers are FMAs' and not the special-function unit's (chunks over bf16 pages)
 #define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
 
 template <int D, int KIND, int FEW>
@@ -59,6 +59,8 @@ struct PtCfg {
   static constexpr bool APART = FEW && !Q8;              // keys' and values' pages are copied by a warp each
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
+  // of 4 pairs: how many powers are FMAs' and not the special-function unit's
+  static constexpr int POLY = D == 64 && !FEW && !Q8 ? 1 : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
   static constexpr int THREADS = Q8 ? 512 : 384;         // 8-bit pages: a warpgroup that turns them into tiles
   // registers of the warpgroups, and of a thread at launch
@@ -155,19 +157,23 @@ __device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
   return r;
 }
 // 2^x of a pair by FMAs: x = n + f, |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative error is smallest (2.6e-6;
-// Remez exchange), n added to its exponent.  x below -126 counts as -126.
+// Remez exchange), times 2^n.  A NaN stays one through the clamp and the product (added to the exponent, n would make a number of it),
+// and 2^-127, for everything below -126.5 and -inf too, is an exponent of 0: a key that is masked or weighs nothing gets 0.
+__device__ __forceinline__ float pt_clamp(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(r) : "f"(x));      // -127
+  return r;
+}
 __device__ __forceinline__ void pt_ex2_fma(float& x0, float& x1) {
-  const uint64_t big = pt_pack(12582912.f, 12582912.f), x = pt_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));      // 1.5 * 2^23
-  const uint64_t t = pt_add2(x, big), n = pt_add2(t, pt_pack(-12582912.f, -12582912.f)), f = pt_fma2(n, pt_pack(-1.f, -1.f), x);
+  const uint64_t big = pt_pack(12583039.f, 12583039.f), x = pt_pack(pt_clamp(x0), pt_clamp(x1));      // 1.5 * 2^23 + 127
+  const uint64_t t = pt_add2(x, big), n = pt_add2(t, pt_pack(-12583039.f, -12583039.f)), f = pt_fma2(n, pt_pack(-1.f, -1.f), x);
   uint64_t p = pt_fma2(f, pt_pack(0.009570102207362652f, 0.009570102207362652f), pt_pack(0.05591785907745361f, 0.05591785907745361f));
   p = pt_fma2(p, f, pt_pack(0.240247443318367f, 0.240247443318367f));
   p = pt_fma2(p, f, pt_pack(0.6931217908859253f, 0.6931217908859253f));
   p = pt_fma2(p, f, pt_pack(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1, p0, p1;
+  float t0, t1;
   pt_unpack(t, t0, t1);
-  pt_unpack(p, p0, p1);
-  x0 = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0));
-  x1 = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1));
+  pt_unpack(pt_mul2(p, pt_pack(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23))), x0, x1);
 }
 // bits [lo, hi) of a 32-bit word (any lo, hi)
 __device__ __forceinline__ uint32_t pt_range(int lo, int hi) {
@@ -603,8 +609,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             for (int e = 0; e < N / 2; ++e) {
               float x0, x1;
               pt_unpack(pt_fma2(pt_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, sh2), x0, x1);
-              float p0, p1;
-              if (!FEW && !C::Q8 && (e & 3) >= 4 - PT_POLY) {
+              float p0, p1;                              // (of -inf 0, of a NaN a NaN)
+              if ((e & 3) >= 4 - C::POLY) {
                 pt_ex2_fma(x0, x1);
                 p0 = x0;
                 p1 = x1;

@@ -1,0 +1,109 @@
+"""The paged cache where numbers, masks, tables and lengths run out: what a query sees reaches it whatever it is, what it does not see
+does not, and a batch with an entry at fault leaves the others alone.
+
+The reference takes a row's visible keys alone, in 64 bits, and takes nothing out of them.  Tolerances as in test_gpu_paged.py.
+"""
+import pytest
+import torch
+
+from test_gpu_paged import Batch, DEV, close
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kch():
+    import kch_b200
+    from kch_b200 import _lib
+    _lib.load()
+    yield kch_b200
+    assert _lib.device_status() == 0, "a device-side status was raised"
+
+
+def by_rows(m, q, *, window=0, missing=()):
+    """(outputs, tolerances) in 64 bits, a row at a time over the keys that it sees.  missing: (sequence, page index) pairs whose table entry
+    names no page: zeros."""
+    G, scale = q.shape[1] // m.n_kv, m.c ** -0.5
+    out = torch.zeros(q.shape, dtype=torch.double, device=DEV)
+    tol = torch.zeros_like(out)
+    for b, (n, p) in enumerate(zip(m.new, m.past)):
+        r0 = m.first + sum(m.new[:b])
+        if n == 0:
+            continue
+        whole = m.table.clone()
+        m.table = m.table.clamp(0, m.cache.num_pages - 1)
+        k, v = (m.values(x, b, p + n).clone() for x in "kv")
+        m.table = whole
+        for s, page in missing:
+            if s == b:
+                k[:, page * m.page:(page + 1) * m.page] = 0.
+                v[:, page * m.page:(page + 1) * m.page] = 0.
+        for i in range(n):
+            lo, hi = max(0, p + i + 1 - window) if window else 0, p + i + 1
+            kk, vv = (x[:, lo:hi].repeat_interleave(G, 0) for x in (k, v))              # [nh, keys, c]
+            qq = q[r0 + i].double()[:, None]
+            l = scale * (qq * kk).sum(-1)
+            w = (l - l.amax(-1, keepdim=True)).exp()
+            w = w / w.sum(-1, keepdim=True)
+            out[r0 + i] = (w[..., None] * vv).sum(1)
+            size = scale * (qq.abs() * kk.abs()).sum(-1).nan_to_num(0., 0., 0.).amax(-1)
+            rel = 2 * (m.c + 4) * 2.0 ** -24 * size + (hi - lo + 64) * 2.0 ** -24
+            if m.dtype == torch.bfloat16:
+                rel = rel + 2.0 ** -8
+            tol[r0 + i] = rel[:, None] * (w[..., None] * vv.abs()).nan_to_num(0., 0., 0.).sum(1)
+            if m.dtype == torch.bfloat16:
+                tol[r0 + i] += 2.0 ** -8 * out[r0 + i].nan_to_num(0., 0., 0.).abs()
+    return out, tol
+
+
+def at(m, b, pos):
+    return int(m.table[b, pos // m.page]), pos % m.page
+
+
+# ---- numbers ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("col", range(8))
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_a_visible_key_that_is_not_finite(kch, dtype, c, bad, col):
+    """A logit that is NaN or +inf makes the rows that see it NaN, one that is -inf takes its key out, at every place of a tile's words."""
+    m = Batch(kch, [140], [60], dtype=dtype, c=c, n_kv=1, page=16)
+    q = m.randn(m.N, 2, c)
+    q[..., 3] = 1.
+    pg, row = at(m, 0, 96 + col)
+    m.cache.k_pages[pg, 0, row, 3] = bad
+    m.cache.v_pages[pg, 0, row, 5] = 1e36          # (large and finite: nothing of it where its weight is 0)
+    want, tol = by_rows(m, q)
+    assert want[:36 + col].isfinite().all()
+    assert want[36 + col:].isfinite().all() if bad == float("-inf") else want[36 + col:].isnan().all()
+    close(m.cache.forward_step(q, *m.args), want, tol)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_a_large_finite_value_that_is_hidden_adds_nothing(kch, dtype, c, window):
+    m = Batch(kch, [150], [50], dtype=dtype, c=c, n_kv=1, page=16)
+    q = m.randn(m.N, 2, c)
+    want, tol = by_rows(m, q, window=window)
+    for key in (118, 119, 126, 127):               # one after the other: what a row that sees them gets is not compared
+        pg, row = at(m, 0, key)
+        m.cache.v_pages[pg, 0, row] = 3e38
+    got = m.cache.forward_step(q, *m.args, sliding_window=window)
+    rows = torch.arange(50, 200, device=DEV)
+    hidden = rows < 118
+    if window:
+        hidden |= rows - 127 >= window
+    close(got[hidden], want[hidden], tol[hidden])
+
+
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_rows_behind_a_table_that_ends_too_early_and_whose_window_ends_there_too_are_zero(kch, dtype, c):
+    """They see no key, in tiles of which other rows see some."""
+    from kch_b200 import _lib
+    m = Batch(kch, [150], [20], dtype=dtype, c=c, n_kv=1, page=16)
+    q = m.randn(m.N, 2, c)
+    want, tol = by_rows(m, q, window=30)
+    got = m.cache.forward_step(q, m.table[:, :5], m.t0, m.cu, sliding_window=30)        # 80 positions
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+    close(got[:60], want[:60], tol[:60])
+    assert (got[109 - 20:] == 0).all()
