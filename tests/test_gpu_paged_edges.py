@@ -107,3 +107,20 @@ def test_rows_behind_a_table_that_ends_too_early_and_whose_window_ends_there_too
     assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
     close(got[:60], want[:60], tol[:60])
     assert (got[109 - 20:] == 0).all()
+
+
+# ---- batches ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, "fp8", 128), (torch.float32, "int8", 64)])
+@pytest.mark.parametrize("first,last", [(-1, 30), (-2 ** 31, 30), (0, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1)])
+def test_rows_in_front_of_the_packed_tensors_and_behind_them_count_as_their_ends(kch, dtype, kind, c, first, last):
+    a, b = (Batch(kch, [13, 17], [40, 3], dtype=dtype, kind=kind, c=c, seed=3) for _ in range(2))
+    k, v, q = a.randn(30, 2, c), a.randn(30, 2, c), a.randn(30, 4, c)
+    cu = torch.tensor([first, 13, last], dtype=torch.int32, device=DEV)
+    a.cache.append_step(k, v, *a.args)
+    b.cache.append_step(k, v, b.table, b.t0, cu)
+    for x in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        one, other = getattr(a.cache, x), getattr(b.cache, x)
+        assert one is None or torch.equal(one.view(torch.uint8), other.view(torch.uint8))
+    for one, other in zip(a.cache.read_step(*a.args, n_rows=30), b.cache.read_step(b.table, b.t0, cu, n_rows=30)):
+        assert torch.equal(one, other)
+    assert torch.equal(a.cache.forward_step(q, *a.args), b.cache.forward_step(q, b.table, b.t0, cu))
