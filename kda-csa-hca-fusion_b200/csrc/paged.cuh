@@ -117,7 +117,7 @@ __device__ __forceinline__ PgSeq pg_seq_or_none(const PgBatch& a, int b) {
   PgSeq s = {0, 0, 0, 0};
   if (b < a.B) {
     s = pg_seq(a, b);
-    if (s.kv - s.t0 < s.len) pg_bad(a);                     // the table ends before the sequence does
+    if (s.len > 0 && s.kv - s.t0 < s.len) pg_bad(a);        // the table ends before the sequence does (one without new tokens needs no page)
   }
   return s;
 }

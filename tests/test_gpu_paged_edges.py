@@ -124,3 +124,20 @@ def test_rows_in_front_of_the_packed_tensors_and_behind_them_count_as_their_ends
     for one, other in zip(a.cache.read_step(*a.args, n_rows=30), b.cache.read_step(b.table, b.t0, cu, n_rows=30)):
         assert torch.equal(one, other)
     assert torch.equal(a.cache.forward_step(q, *a.args), b.cache.forward_step(q, b.table, b.t0, cu))
+
+
+@pytest.mark.parametrize("B", [4, 40])
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, "fp8", 128), (torch.float32, None, 64)])
+def test_sequences_without_new_tokens_need_no_page(kch, dtype, kind, c, B):
+    """Idle places of a captured batch: lengths of long ago, far behind the table."""
+    from kch_b200 import _lib
+    m = Batch(kch, [1 + b % 3 if b % 2 else 0 for b in range(B)], [40 + b if b % 2 else 0 for b in range(B)], dtype=dtype, kind=kind, c=c, page=16)
+    q, k = m.randn(m.N, 4, c), m.randn(m.N, 2, c)
+    for far in (200, 10 ** 6, 2 ** 31 - 1):
+        m.t0[::2] = far
+        m.cache.append_step(k, k, *m.args)
+        got = m.cache.forward_step(q, *m.args)
+        torch.cuda.synchronize()
+        assert _lib.device_status(reset=True) == 0
+        want, tol = by_rows(m, q)
+        close(got, want, tol)
