@@ -453,7 +453,8 @@ int kch_paged_read(const kch_paged_cache* cache, const kch_paged_batch* batch, v
                    int zero_rest, void* stream);
 
 /* Attention of the new tokens over the pages, which hold them already: query i of sequence b stands at position t0[b] + i and
- * sees the keys up to it, the last `sliding_window` of them where that is not 0; query head h reads key head h / (nh / n_kv).
+ * sees the keys up to it, the last `sliding_window` of them where that is not 0 (pages that no query of a sequence reaches any more
+ * need not be in the table: their entries are not used); query head h reads key head h / (nh / n_kv).
  * The sink logit of a head (optional) adds to the denominator.  q [N, nh, c] (tokens ld_q elements apart) and out [N, nh, c] in
  * `dtype`, which is that of the cache's activations; they do not overlap.  Rows of no sequence: zeros with `zero_rest`, else left as they are.  A row
  * without keys is 0.  What a row does not see (other pages, rows behind a sequence's end, later or older keys) does not reach it,

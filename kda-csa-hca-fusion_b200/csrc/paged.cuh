@@ -60,7 +60,8 @@ __device__ __forceinline__ int pg_page(const PgBatch& a, int b, int index) {
 }
 
 // One block of rows of a sequence: which keys its rows see together.
-struct PgSpan { int rows, first_key, tiles, steps; };   // tiles of KT keys from first_key (a multiple of KT) on
+// tiles of KT keys from first_key (a multiple of KT) on; the keys before `lo` no row sees: their pages need not be there any more
+struct PgSpan { int rows, lo, first_key, tiles, steps; };
 // R rows a block, KT keys a tile.  TWO: blocks of at most TWO rows take two tiles a step.
 template <int R, int KT, int TWO>
 __device__ __forceinline__ PgSpan pg_span(const PgBatch& a, const PgSeq& s, int block) {
@@ -68,8 +69,9 @@ __device__ __forceinline__ PgSpan pg_span(const PgBatch& a, const PgSeq& s, int 
   const int r0 = block * R, r1 = min(r0 + R, s.len * a.G);
   x.rows = r1 - r0;
   const int64_t first = (int64_t)s.t0 + pg_token(a, r0), last = (int64_t)s.t0 + pg_token(a, r1 - 1);      // positions of the first and the last query
-  const int lo = a.window > 0 ? (int)min(max(first - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0, hi = (int)min(last + 1, (int64_t)s.kv);
-  x.first_key = lo / KT * KT;
+  const int hi = (int)min(last + 1, (int64_t)s.kv);
+  x.lo = a.window > 0 ? (int)min(max(first - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0;
+  x.first_key = x.lo / KT * KT;
   x.tiles = hi > x.first_key ? (hi - x.first_key + KT - 1) / KT : 0;
   x.steps = max(x.rows <= TWO ? (x.tiles + 1) / 2 : x.tiles, 1);            // (a row without keys is stored all the same)
   return x;

@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #pragma unroll
       for (int k = 0; k < CHUNKS; ++k) {
         const int i = tid + k * PA_THREADS, j = i / c8, d = i % c8 * 8, pos = w.x.first_key + st * PA_KT + j;
-        kw[k].none();                                          // (0 behind the sequence's end)
+        kw[k].none();                                          // (0 before the window and behind the sequence's end)
         vw[k].none();
         fk[k] = fv[k] = 1.f;
-        if (j < PA_KT && pos < w.s.kv) {
+        if (j < PA_KT && pos >= w.x.lo && pos < w.s.kv) {
           const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
           if (pg >= 0) {
             const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));

@@ -129,10 +129,12 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
       const int end = w.first + w.count;
       const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
-      // asked for a tile ahead; -1 behind the part's or the sequence's end
+      // a box of which some row may see a key: not before the first window, not behind the sequence's end
+      auto needed = [&](int tile, int key) { return mine && tile < w.x.tiles && key + box > w.x.lo && key < w.s.kv; };
+      // asked for a tile ahead; -1 where it is not needed
       auto ask = [&](int tile) -> int {
         const int key = w.x.first_key + tile * PM_KT + lane * box;
-        return mine && tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+        return tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
       };
       int id = ask(w.first);
       for (int tile = w.first; tile < end && ok; ++tile, ++g) {
@@ -144,7 +146,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         __syncwarp();
         if (mine) {
           const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
-          if (!there && tile < w.x.tiles && key < w.s.kv) pg_bad(a.bt);
+          if (!there && needed(tile, key)) pg_bad(a.bt);
           const int r0 = key & (a.page - 1);             // out of range: zeros, with the scales of some page
           if (scales)
             bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (values ? a.vs : a.ks) + ((int64_t)(there ? id : 0) * n_kv + w.h) * a.page + r0,

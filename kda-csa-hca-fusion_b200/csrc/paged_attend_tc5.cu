@@ -313,10 +313,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const bool pair = paired(w);
         const int per = pair ? 1 : 2, end = (w.first + w.count) * per;
         const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
-        // the page of this lane's box of a tile, asked for a tile ahead; -1 behind the part's or the sequence's end
+        // a box of which some row may see a key: not before the first window, not behind the sequence's end
+        auto needed = [&](int tile, int key) { return mine && tile < w.x.tiles && key + box > w.x.lo && key < w.s.kv; };
+        // the page of this lane's box of a tile, asked for a tile ahead; -1 where it is not needed
         auto ask = [&](int tile) -> int {
           const int key = w.x.first_key + tile * PT_KT + mybox * box;
-          return mine && tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+          return tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
         };
         auto copy = [&](int tile, bool v, int id) {
           const int st = g % N, key = w.x.first_key + tile * PT_KT + mybox * box;
@@ -331,7 +333,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           __syncwarp();
           if (mine) {
             if ((unsigned)id >= (unsigned)a.bt.num_pages) {            // out of range: zeros
-              if (tile < w.x.tiles && key < w.s.kv) pg_bad(a.bt);
+              if (needed(tile, key)) pg_bad(a.bt);
               id = (int)a.bt.num_pages;
             }
             uint8_t* dst = C::Q8 ? sm.raw[C::Q8 ? st : 0] + mybox * box * D : sm.kv[C::Q8 ? 0 : st] + mypanel * (PT_KT * 128) + mybox * box * 128;
@@ -465,13 +467,13 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         __syncwarp();
         if (lane == 0) mbarrier_arrive(&sm.q_full);
         if constexpr (C::Q8) {
-          // the scales of the item's key tiles: two keys a thread, 0 behind the end (a scale there may be anything); the page is
+          // the scales of the item's key tiles: two keys a thread, 0 before the window and behind the end (a scale there may be anything); the page is
           // asked for a tile ahead, and the copies report to the barrier by themselves
           const int per = paired(w) ? 1 : 2, end = (w.first + w.count) * per;
           const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
           auto ask = [&](int tile, int i) -> int {
             const int key = w.x.first_key + tile * PT_KT + t + 64 * i;
-            return tile < min(end, w.x.tiles) && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
+            return tile < min(end, w.x.tiles) && key >= w.x.lo && key < w.s.kv ? __ldg(pages + (key >> a.bt.shift)) : -1;
           };
           int id0 = ask(w.first * per, 0), id1 = ask(w.first * per, 1);
           for (int tile = w.first * per; tile < end && ok; ++tile, ++kt) {

@@ -196,7 +196,8 @@ class PagedKVCache:
     def forward_step(self, q, table, t0, cu_seqlens, *, scale=None, sink_logits=None, sliding_window=0, out=None):
         """Attention of the batch's new tokens, whose own rows :meth:`append_step` has written: ``q [N, nh, c]`` (``nh`` a
         multiple of ``n_kv``; query head h reads key head ``h // (nh // n_kv)``) -> ``[N, nh, c]`` in ``q.dtype``.  The query at
-        position p sees the keys ``0 .. p``, or the last ``sliding_window`` of them.  ``scale``: ``c ** -0.5`` unless given;
+        position p sees the keys ``0 .. p``, or the last ``sliding_window`` of them (entries of pages that no query of a sequence
+        reaches any more are not used).  ``scale``: ``c ** -0.5`` unless given;
         ``sink_logits [nh]`` adds ``exp(sink)`` to the denominator.  Rows of no sequence are zeros, and stay as they are in a
         tensor given as ``out``, which does not overlap ``q``."""
         fn = "forward_step"

@@ -141,3 +141,24 @@ def test_sequences_without_new_tokens_need_no_page(kch, dtype, kind, c, B):
         assert _lib.device_status(reset=True) == 0
         want, tol = by_rows(m, q)
         close(got, want, tol)
+
+
+@pytest.mark.parametrize("new,past", [([1, 3, 1], [1000, 700, 90]), ([1, 150], [3, 1000]), ([300], [777])])
+@pytest.mark.parametrize("dtype,kind,c,page", [(torch.bfloat16, None, 128, 16), (torch.bfloat16, None, 64, 8), (torch.bfloat16, "fp8", 128, 16),
+                                               (torch.bfloat16, "int8", 64, 32), (torch.float32, None, 64, 16), (torch.float32, "fp8", 128, 8),
+                                               (torch.bfloat16, None, 128, 256)])
+def test_pages_that_every_window_has_left_behind_may_be_gone(kch, dtype, kind, c, page, new, past):
+    """The caller gives them to other sequences and takes them out of the table."""
+    from kch_b200 import _lib
+    m = Batch(kch, new, past, dtype=dtype, kind=kind, c=c, page=page)
+    q, window = m.randn(m.N, 4, c), 100
+    want, tol = by_rows(m, q, window=window)
+    for b, p in enumerate(past):
+        gone = max(p - window + 1, 0) // page
+        for x in ("k_pages", "v_pages") if kind is None else ("k_scales", "v_scales"):
+            getattr(m.cache, x)[m.table[b, :gone].long()] = torch.nan
+        m.table[b, :gone] = -1
+    got = m.cache.forward_step(q, *m.args, sliding_window=window)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == 0
+    close(got, want, tol)
