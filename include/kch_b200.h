@@ -54,7 +54,8 @@ long long kch_launch_count(int reset);      /* kernels launched by this library 
 #define KCH_STATUS_KDA_STEP 0x6D03       /* status word: the state copy of the one-token KDA step did not arrive */
 #define KCH_STATUS_KDA_CHUNK 0x6D04      /* status word: a chunk record of the fp32 KDA scan did not arrive */
 #define KCH_STATUS_ATTEND_TILES 0x6D05   /* status word: a wait of the attention over key tiles (operands / accumulator) expired */
-#define KCH_STATUS_PAGED_TABLE 0x6D06    /* status word: a block table named no page of the pool, or ended before its sequence did */
+#define KCH_STATUS_PAGED_TABLE 0x6D06    /* status word: a block table named no page of the pool, or ended before its sequence did.  The caller's
+                                          * mistake and no expired wait: it cuts no wait short, and an expired wait is reported before it */
 #define KCH_STATUS_PAGED_ATTEND 0x6D07   /* status word: a wait of the attention over pages (operands / accumulator) expired */
 #define KCH_STATUS_INDEXER_DECODE 0x6D02 /* status word: a wait of the one-token indexer (key tiles / accumulator) expired */
 int kch_selftest_bounded_wait(unsigned int limit_polls, unsigned int* polls_out, void* stream);

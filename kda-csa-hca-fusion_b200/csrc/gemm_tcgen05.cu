@@ -37,7 +37,11 @@
 #define TG_EPI_LD 80
 #define TG_SPIN_LIMIT (1u << 24)
 
-__device__ unsigned int g_kch_status = 0;  // nonzero: a bounded wait expired (see kch_device_status)
+// Two words that kch_device_status reads as one: [0] a bounded wait expired, or a cache's storage was full; all bounded waits give up while
+// it is set.  [1] a block table was at fault (KCH_STATUS_PAGED_TABLE): the caller's mistake, after which every wait still ends by
+// itself, so that it costs nobody else anything.
+__device__ unsigned int g_kch_words[2] = {0, 0};
+#define g_kch_status g_kch_words[0]
 
 // ---- PTX wrappers ------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -1241,7 +1245,7 @@ unsigned int* kch_status_device_ptr() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (!cached[dev]) {
     unsigned int* p = nullptr;
-    if (cudaGetSymbolAddress((void**)&p, g_kch_status) != cudaSuccess) return nullptr;
+    if (cudaGetSymbolAddress((void**)&p, g_kch_words) != cudaSuccess) return nullptr;
     cached[dev] = p;
   }
   return cached[dev];
@@ -1269,11 +1273,11 @@ extern "C" int kch_selftest_bounded_wait(unsigned int limit_polls, unsigned int*
 }
 
 extern "C" unsigned int kch_device_status(int reset) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_kch_status, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
-  if (reset && v) {
-    unsigned int z = 0;
-    cudaMemcpyToSymbol(g_kch_status, &z, sizeof(z));
+  unsigned int v[2] = {0, 0};
+  if (cudaMemcpyFromSymbol(v, g_kch_words, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
+  if (reset && (v[0] || v[1])) {
+    const unsigned int z[2] = {0, 0};
+    cudaMemcpyToSymbol(g_kch_words, z, sizeof(z));
   }
-  return v;
+  return v[0] ? v[0] : v[1];
 }

@@ -24,7 +24,7 @@ struct PgBatch {
   int cap;                             // positions that a row of the table covers (below 2^31)
   int64_t num_pages;
   int shift;                           // log2(page_size)
-  unsigned int* status;
+  unsigned int* status;                // [0]: of expired waits, which ends the others; [1]: of tables, which ends none
   int n_kv, G, window;                 // key heads, query heads of one, window (attention only)
   uint32_t g_mul; int g_shift;         // n / G = n * g_mul >> 32 + g_shift for n < 2^31; g_mul 0: n >> g_shift
 };
@@ -50,7 +50,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
   s.kv = (int)min((int64_t)s.t0 + s.len, (int64_t)a.cap);
   return s;
 }
-__device__ __forceinline__ void pg_bad(const PgBatch& a) { atomicCAS(a.status, 0u, (unsigned)KCH_STATUS_PAGED_TABLE); }
+__device__ __forceinline__ void pg_bad(const PgBatch& a) { atomicCAS(a.status + 1, 0u, (unsigned)KCH_STATUS_PAGED_TABLE); }
 // page of `index` pages into sequence b, or -1 (and the status word) where the table holds none
 __device__ __forceinline__ int pg_page(const PgBatch& a, int b, int index) {
   const int p = __ldg(a.table + b * a.ld_table + index);

@@ -254,15 +254,19 @@ def device_status(reset=False) -> int:
 
 
 def raise_on_device_status(where: str) -> None:
-    """Synchronise the current device and raise if a bounded device-side wait has expired since the last check.
+    """Synchronise the current device and raise if a bounded device-side wait has expired since the last check, or a block table
+    of a paged cache was at fault.
 
     The status word is sticky on purpose: after one wait gives up, every later wait returns at its first poll, so
-    kernels drain instead of spinning, but they also leave their outputs unwritten.  Callers that keep a process
+    kernels drain instead of spinning, but they also leave their outputs unwritten (a table at fault has no such effect).  Callers that keep a process
     alive across requests should call this (or `device_status(reset=True)`) at their own synchronisation points;
     the package does so in `HostPipeline.run` and `HybridDecoding.export_state`."""
     import torch
     torch.cuda.synchronize()
     st = device_status(reset=True)
+    if st == STATUS_PAGED_TABLE:
+        raise RuntimeError(f"kch_b200 ({where}): a block table named no page of the pool, or ended before its sequence did; such positions "
+                           f"were not stored and read as zeros (status 0x{st:x}).  The status word has been cleared.")
     if st:
         raise RuntimeError(f"kch_b200 ({where}): a device-side bounded wait expired (status 0x{st:x}); results since "
                            f"the previous check are not valid.  The status word has been cleared.")

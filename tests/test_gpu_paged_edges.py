@@ -162,3 +162,36 @@ def test_pages_that_every_window_has_left_behind_may_be_gone(kch, dtype, kind, c
     torch.cuda.synchronize()
     assert _lib.device_status(reset=True) == 0
     close(got, want, tol)
+
+
+def test_a_table_at_fault_cuts_no_wait_short(kch):
+    """The status it raises is the caller's to read; kernels that wait for their copies do not give up because of it."""
+    from kch_b200 import _lib
+    m = Batch(kch, [3], [70])
+    m.table[0, 1] = -1
+    m.cache.forward_step(m.randn(3, 4, 128), *m.args)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == _lib.STATUS_PAGED_TABLE
+    _lib.check(_lib.load().kch_selftest_bounded_wait(4096, None, _lib.stream()))       # a wait that nothing ends: to its own limit
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == _lib.STATUS_SELFTEST_WAIT                 # (and it is reported first)
+    assert _lib.device_status() == 0
+    m.cache.forward_step(m.randn(3, 4, 128), *m.args)
+    with pytest.raises(RuntimeError, match="block table"):
+        _lib.raise_on_device_status("test")
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [200, 130, 5]])
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, "fp8", 128), (torch.bfloat16, "int8", 64), (torch.float32, None, 64)])
+def test_a_table_at_fault_leaves_the_other_sequences_alone(kch, dtype, kind, c, new):
+    from kch_b200 import _lib
+    m = Batch(kch, new, [1500, 700, 3], dtype=dtype, kind=kind, c=c)
+    q = m.randn(m.N, 4, c)
+    m.table[1, 20] = 1 << 30
+    want, tol = by_rows(m, q, missing=[(1, 20)])           # (what it does not name reads as zeros)
+    for _ in range(3):
+        got = m.cache.forward_step(q, *m.args)
+        torch.cuda.synchronize()
+        assert _lib.device_status() == _lib.STATUS_PAGED_TABLE
+        close(got, want, tol)
+    assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
