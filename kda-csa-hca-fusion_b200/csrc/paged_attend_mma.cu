@@ -142,17 +142,26 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         ok = g < S::STAGES || wait(&sm.empty[st], g / S::STAGES - 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbarrier_expect_tx(&sm.full[st], PM_KT * (scales ? 4 : D));
+        const bool there = mine && (unsigned)id < (unsigned)a.bt.num_pages;
+        const unsigned some = __ballot_sync(0xffffffffu, there);
+        if (mine && !there) {                            // zeros: codes by a coordinate out of range, scales by hand
+          if (needed(tile, key)) pg_bad(a.bt);
+          if (scales) {
+            float4* to = reinterpret_cast<float4*>((values ? sm.vs[st] : sm.ks[st]) + lane * box);
+            for (int i = 0; i < box / 4; ++i) to[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            t5_fence_async_smem();                       // (a copy writes there next)
+          }
+        }
         __syncwarp();
-        if (mine) {
-          const bool there = (unsigned)id < (unsigned)a.bt.num_pages;
-          if (!there && needed(tile, key)) pg_bad(a.bt);
-          const int r0 = key & (a.page - 1);             // out of range: zeros, with the scales of some page
-          if (scales)
-            bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (values ? a.vs : a.ks) + ((int64_t)(there ? id : 0) * n_kv + w.h) * a.page + r0,
-                          box * 4, &sm.full[st]);
-          else
-            pm_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * D, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
+        if (lane == 0) mbarrier_expect_tx(&sm.full[st], scales ? __popc(some) * box * 4 : PM_KT * D);
+        __syncwarp();
+        const int r0 = key & (a.page - 1);
+        if (scales) {
+          if (there)
+            bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (values ? a.vs : a.ks) + ((int64_t)id * n_kv + w.h) * a.page + r0, box * 4,
+                          &sm.full[st]);
+        } else if (mine) {
+          pm_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * D, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
         }
         id = next;
       }

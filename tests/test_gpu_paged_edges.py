@@ -195,3 +195,24 @@ def test_a_table_at_fault_leaves_the_other_sequences_alone(kch, dtype, kind, c, 
         assert _lib.device_status() == _lib.STATUS_PAGED_TABLE
         close(got, want, tol)
     assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [8, 8, 8], [200, 130, 5]])
+@pytest.mark.parametrize("kind,c", [("fp8", 128), ("int8", 64), ("fp8", 72)])
+def test_pages_that_are_missing_have_scales_of_zero_not_those_of_another_page(kch, kind, c, new):
+    from kch_b200 import _lib
+    for page in (16, 128):
+        m = Batch(kch, new, [1500, 700, 3], kind=kind, c=c, page=page)
+        held = set(m.table[m.table >= 0].tolist())
+        if 0 in held:                                      # page 0 is nobody's
+            spare = next(i for i in range(m.cache.num_pages) if i not in held)
+            m.table[m.table == 0] = spare
+        for scales in (m.cache.k_scales, m.cache.v_scales):
+            scales[0] = torch.nan
+        q = m.randn(m.N, 4, c)
+        m.table[1, 4] = -1
+        want, tol = by_rows(m, q, missing=[(1, 4)])
+        got = m.cache.forward_step(q, *m.args)
+        torch.cuda.synchronize()
+        assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+        close(got, want, tol)
