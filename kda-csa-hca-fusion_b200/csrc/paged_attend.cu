@@ -58,6 +58,9 @@ struct PgStored {
   }
 };
 
+// a weight of -0: nothing is seen there (a weight that is merely too small is 0, and 0 times a NaN is one)
+__device__ __forceinline__ bool pa_none(float weight) { return __float_as_uint(weight) == 0x80000000u; }
+
 #define PA_KT 64
 #define PA_THREADS 256
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
@@ -175,8 +178,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          const int key = key0 + tx + 16 * j;
           const float p = ex2_fast(acc[i][j] - shift);
-          sp[r * LS + tx + 16 * j] = p;
+          sp[r * LS + tx + 16 * j] = key >= keys.x && key < keys.y ? p : -0.f;       // (-0: not seen; 0: seen, but too little for 32 bits)
           sum += p;
         }
 #pragma unroll
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
 #pragma unroll
               for (int i = 0; i < RT; ++i) {
                 const float f = k == 0 ? p[i].x : k == 1 ? p[i].y : k == 2 ? p[i].z : p[i].w;
-                if (masked() && f == 0.f) continue;
+                if (masked() && pa_none(f)) continue;
                 o[i][x][0] = fmaf(f, vv.x, o[i][x][0]);
                 o[i][x][1] = fmaf(f, vv.y, o[i][x][1]);
                 o[i][x][2] = fmaf(f, vv.z, o[i][x][2]);
@@ -313,12 +317,14 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
   const int groups = before[ctas];
   const int64_t size = pg_slot_floats(a.slot_rows, a.c), mat = (int64_t)a.slot_rows * a.c;
   auto slot_of = [&](int i, int first) { return a.slots + (2 * (int64_t)i + (i == first ? 1 : 0)) * size; };
-  // (weight 0: a part without keys; what its sums hold does not matter)
+  // (a part without keys: what its sums hold does not matter)
+  auto weigh = [](float m, float shift) { return m == -INFINITY ? -0.f : ex2_fast(m - shift); };
   auto add = [](float (&o)[4 * W], int x, const float4& v, float f) {
-    o[4 * x] = f == 0.f ? o[4 * x] : fmaf(f, v.x, o[4 * x]);
-    o[4 * x + 1] = f == 0.f ? o[4 * x + 1] : fmaf(f, v.y, o[4 * x + 1]);
-    o[4 * x + 2] = f == 0.f ? o[4 * x + 2] : fmaf(f, v.z, o[4 * x + 2]);
-    o[4 * x + 3] = f == 0.f ? o[4 * x + 3] : fmaf(f, v.w, o[4 * x + 3]);
+    const bool none = pa_none(f);
+    o[4 * x] = none ? o[4 * x] : fmaf(f, v.x, o[4 * x]);
+    o[4 * x + 1] = none ? o[4 * x + 1] : fmaf(f, v.y, o[4 * x + 1]);
+    o[4 * x + 2] = none ? o[4 * x + 2] : fmaf(f, v.z, o[4 * x + 2]);
+    o[4 * x + 3] = none ? o[4 * x + 3] : fmaf(f, v.w, o[4 * x + 3]);
   };
   auto place = [&](const PgRecord& rec, int r, int& h) {      // of the item's row r in the output; its head
     const int row = rec.block * a.R + r, t = row / a.G;
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
 #pragma unroll
     for (int k = 4; k > 0; k >>= 1) shift = fmaxf(shift, __shfl_xor_sync(0xffffffffu, shift, k));
     if (shift == -INFINITY) shift = 0.f;
-    const float weight = ex2_fast(m - shift);
+    const float weight = weigh(m, shift);
     l *= weight;
 #pragma unroll
     for (int k = 4; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
@@ -414,7 +420,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(PgJoinArgs a,
 #pragma unroll
       for (int q = 0; q < PER; ++q) {
         const int p = threadIdx.x + q * 32 * PJ_WARPS;
-        const float f = ex2_fast(m[q] - shift);
+        const float f = weigh(m[q], shift);
         if (p < n) weight[p] = f;
         sum = fmaf(f, l[q], sum);
       }

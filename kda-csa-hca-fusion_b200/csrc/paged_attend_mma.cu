@@ -365,14 +365,15 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       float mm = sm.ml[0][0][i];
 #pragma unroll
       for (int k = 1; k < C::WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][i]);
-      const float own = m[hf] == -INFINITY ? 0.f : ex2_fast((m[hf] - mm) * sc);      // (0 for a part without a key)
+      const bool none = m[hf] == -INFINITY;              // (a part without a key)
+      const float own = none ? 0.f : ex2_fast((m[hf] - mm) * sc);
       float4* mine = reinterpret_cast<float4*>(sm.stage[cw]) + g * (D / 4);
       // 16-byte words of a row, swizzled within runs of 8 so that 8 threads meet in no bank
 #pragma unroll
       for (int c = 0; c < RUN / 4; ++c) {
         const int j = 4 * c % NT, mt = hf / 2, e = 2 * (hf % 2) + 4 * c / NT;
         mine[(RUN / 4 * t + c) ^ ((D == 128 ? t : 2 * (t & 1)) + 4 * (g & 1))] =
-            own == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][mt][e] * own, o[j + 1][mt][e] * own, o[j + 2][mt][e] * own, o[j + 3][mt][e] * own);
+            none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[j][mt][e] * own, o[j + 1][mt][e] * own, o[j + 2][mt][e] * own, o[j + 3][mt][e] * own);
       }
       sync();
       for (int k = ct; k < 8 * (D / 4); k += 32 * C::WARPS) {

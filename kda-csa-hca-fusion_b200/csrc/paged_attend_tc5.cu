@@ -697,6 +697,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // stores half of the columns), and with FEW those of four warps.
       const auto sync = [](int bar, int n) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(n) : "memory"); };
       float w0 = 1.f, w1 = 0.f, mm = m, ll = l;
+      bool none0 = false, none1 = true;                  // a part without a key: what its sums hold does not matter
       if (!pair) {
         sm.ml[0][x * 128 + r] = m;
         sm.ml[1][x * 128 + r] = l;
@@ -705,8 +706,10 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
         for (int k = 0; k < 256; k += APART) mm = fmaxf(mm, sm.ml[0][ri + k]);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        w0 = ex2_fast((m0 - ref) * sc);                  // (0 for a part without a key: what its sums hold does not matter)
+        w0 = ex2_fast((m0 - ref) * sc);
         w1 = ex2_fast((m1 - ref) * sc);
+        none0 = m0 == -INFINITY;
+        none1 = m1 == -INFINITY;
         if (!FEW || r < APART) {
           ll = 0.f;                                      // (a NaN of a part's sum stays one)
 #pragma unroll
@@ -739,7 +742,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
           for (int e = 0; e < CW; ++e) {
             const float a0 = __uint_as_float(o0[e]), a1 = __uint_as_float(o1[e]);
-            o0[e] = __float_as_uint((w0 == 0.f ? 0.f : a0 * w0) + (w1 == 0.f ? 0.f : a1 * w1));
+            o0[e] = __float_as_uint((none0 ? 0.f : a0 * w0) + (none1 ? 0.f : a1 * w1));
           }
         }
         float z[4] = {0.f, 0.f, 0.f, 0.f};

@@ -216,3 +216,30 @@ def test_pages_that_are_missing_have_scales_of_zero_not_those_of_another_page(kc
         torch.cuda.synchronize()
         assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
         close(got, want, tol)
+
+
+@pytest.mark.parametrize("low", [0., 0.6])
+@pytest.mark.parametrize("new,past", [([1], [400]), ([1], [30000]), ([4, 1], [700, 250]), ([40], [9000]), ([150, 90], [300, 1000])])
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, None, 64), (torch.bfloat16, "fp8", 128), (torch.bfloat16, "int8", 64),
+                                          (torch.float32, None, 64), (torch.float32, "int8", 72)])
+def test_a_value_that_is_not_a_number_reaches_the_rows_that_see_it_however_little_it_weighs(kch, dtype, kind, c, new, past, low):
+    """NaN values of keys far below the others (less than 2^-1000 of the weight), among others or, with `low`, among their like: 0 times a NaN is
+    one, whatever tile, warp or part of a row has it."""
+    m = Batch(kch, new, past, dtype=dtype, kind=kind, c=c, n_kv=1, page=16)
+    q = m.randn(m.N, 2, c)
+    q[..., 0] = 1000.
+    for b, (n, p) in enumerate(zip(new, past)):
+        pos = torch.arange(p + n, device=DEV)
+        bad = torch.tensor([1, p // 2, p - 1] if b == 0 and not low else [p // 3], device=DEV)
+        down = (pos < low * p) | torch.isin(pos, bad)
+        pages, rows = m.table[b].long()[pos // 16], pos % 16
+        if kind is None:
+            m.cache.k_pages[pages, 0, rows, 0] = torch.where(down, -60., 0.).to(dtype)
+            m.cache.v_pages[pages[bad], 0, rows[bad], 5] = torch.nan
+        else:
+            m.cache.k_pages.view(torch.uint8)[pages, 0, rows, 0] = torch.where(down, 0x81 if kind == "int8" else 0xF6, 0).byte()
+            m.cache.k_scales[pages[down], 0, rows[down]] = 0.3
+            m.cache.v_scales[pages[bad], 0, rows[bad]] = torch.nan
+    want, tol = by_rows(m, q)
+    assert want[..., 5].isnan().any()
+    close(m.cache.forward_step(q, *m.args), want, tol)
