@@ -429,9 +429,9 @@ typedef struct kch_paged_cache {
 /* A ragged batch: rows cu_seqlens[b] .. cu_seqlens[b + 1] of the packed tensors [N, ..] are the positions t0[b], t0[b] + 1, .. of
  * sequence b, and position p of it lies in page table[b, p / page_size] of the pool, row p % page_size.  All lengths are read on
  * the device: a captured call replays with other ones.  Entries of the table behind a sequence's last page are not read, nor is any
- * of a sequence that has no rows in the call, whatever its t0.  An
- * entry that is needed and names no page of the pool, or a position behind the table, raises KCH_STATUS_PAGED_TABLE; nothing is
- * stored for it, and it reads as zeros.  cu_seqlens does not decrease and stays within 0 .. N; rows outside
+ * of a sequence that has no rows in the call, whatever its t0.  An entry that is needed and names no page of the pool, a position
+ * behind the table, or a negative t0 raises KCH_STATUS_PAGED_TABLE; nothing is stored for it, and it reads as zeros (queries of a
+ * negative t0 see no keys).  cu_seqlens does not decrease and stays within 0 .. N; rows outside
  * [cu_seqlens[0], cu_seqlens[B]) belong to no sequence.  Up to 4096 sequences. */
 typedef struct kch_paged_batch {
   const int32_t* table;      /* [B, max_pages] rows ld_table apart */

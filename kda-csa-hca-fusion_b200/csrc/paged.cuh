@@ -46,8 +46,9 @@ __device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
   PgSeq s;
   s.row0 = min(max(__ldg(a.cu + b), 0), a.N);
   s.len = min(max(__ldg(a.cu + b + 1), s.row0), a.N) - s.row0;
-  s.t0 = max(__ldg(a.t0 + b), 0);
-  s.kv = (int)min((int64_t)s.t0 + s.len, (int64_t)a.cap);
+  const int t0 = __ldg(a.t0 + b);
+  s.t0 = max(t0, 0);
+  s.kv = t0 < 0 ? 0 : (int)min((int64_t)t0 + s.len, (int64_t)a.cap);       // (positions before 0: no keys)
   return s;
 }
 __device__ __forceinline__ void pg_bad(const PgBatch& a) { atomicCAS(a.status + 1, 0u, (unsigned)KCH_STATUS_PAGED_TABLE); }
@@ -119,7 +120,7 @@ __device__ __forceinline__ PgSeq pg_seq_or_none(const PgBatch& a, int b) {
   PgSeq s = {0, 0, 0, 0};
   if (b < a.B) {
     s = pg_seq(a, b);
-    if (s.len > 0 && s.kv - s.t0 < s.len) pg_bad(a);        // the table ends before the sequence does (one without new tokens needs no page)
+    if (s.len > 0 && s.kv - s.t0 < s.len) pg_bad(a);        // it begins before position 0, or the table ends before it does (without new tokens it needs no page)
   }
   return s;
 }

@@ -94,8 +94,9 @@ __device__ __forceinline__ int64_t pc_site(const PgRows& a, const int32_t* cu, i
     const int mid = (lo + hi) >> 1;
     if (cu[mid] <= t) lo = mid; else hi = mid;
   }
-  const int64_t pos = (int64_t)max(__ldg(a.bt.t0 + lo), 0) + (t - max(cu[lo], 0));      // (a first row in front of the tensor counts as row 0, as in pg_seq)
-  if (pos >= a.bt.cap) { pg_bad(a.bt); return -2; }
+  const int before = __ldg(a.bt.t0 + lo);
+  const int64_t pos = (int64_t)before + (t - max(cu[lo], 0));      // (a first row in front of the tensor counts as row 0, as in pg_seq)
+  if (before < 0 || pos >= a.bt.cap) { pg_bad(a.bt); return -2; }
   const int64_t pg = pg_page(a.bt, lo, (int)pos >> a.bt.shift);
   return pg < 0 ? -2 : pg * a.n_kv * a.page + ((int)pos & (a.page - 1));
 }

@@ -49,7 +49,7 @@ class PagedKVCache:
     (tokens of a sequence before this call's) and ``cu_seqlens`` int32 ``[B + 1]``: rows ``cu_seqlens[b] .. cu_seqlens[b+1]`` of
     the packed tensors are the positions ``t0[b], t0[b] + 1, ..`` of sequence b, and position p lies in row ``p % page_size``
     of page ``table[b, p // page_size]``.  A table that names no page of the pool where one is needed, or ends before its
-    sequence does, raises the device status ``KCH_STATUS_PAGED_TABLE``.
+    sequence does, and a negative ``t0`` raise the device status ``KCH_STATUS_PAGED_TABLE``.
     """
 
     def __init__(self, num_pages, page_size, n_kv, c, device, dtype, *, kv_quant=None, storage=None):

@@ -243,3 +243,27 @@ def test_a_value_that_is_not_a_number_reaches_the_rows_that_see_it_however_littl
     want, tol = by_rows(m, q)
     assert want[..., 5].isnan().any()
     close(m.cache.forward_step(q, *m.args), want, tol)
+
+
+@pytest.mark.parametrize("new", [[2, 3, 1], [90, 140, 20]])
+@pytest.mark.parametrize("dtype,kind,c", [(torch.bfloat16, None, 128), (torch.bfloat16, "fp8", 128), (torch.bfloat16, "int8", 64), (torch.float32, None, 64)])
+@pytest.mark.parametrize("t0", [-1, -100, -2 ** 31])
+def test_a_negative_count_of_earlier_tokens_is_the_callers_mistake_and_touches_nothing(kch, dtype, kind, c, new, t0):
+    from kch_b200 import _lib
+    m = Batch(kch, new, [70, 0, 33], dtype=dtype, kind=kind, c=c)
+    k, q = m.randn(m.N, 2, c), m.randn(m.N, 4, c)
+    before = m.cache.k_pages.clone().view(torch.uint8)
+    m.t0[1] = t0
+    mine = slice(new[0], new[0] + new[1])
+    for call in (lambda: m.cache.append_step(k, k, *m.args), lambda: m.cache.read_step(*m.args, n_rows=m.N), lambda: m.cache.forward_step(q, *m.args)):
+        got = call()
+        torch.cuda.synchronize()
+        assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+        if isinstance(got, tuple):
+            assert not got[0][mine].any() and got[0][:new[0]].any()
+    held = m.table[1][m.table[1] >= 0].long()
+    assert torch.equal(m.cache.k_pages.view(torch.uint8)[held], before[held])
+    assert (got[mine] == 0).all()
+    want, tol = by_rows(m, q)
+    rows = torch.cat([torch.arange(0, new[0]), torch.arange(new[0] + new[1], m.N)]).to(DEV)
+    close(got[rows], want[rows], tol[rows])
