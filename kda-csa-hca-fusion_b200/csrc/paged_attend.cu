@@ -506,7 +506,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   const int c = p->cache.c, n_kv = p->cache.n_kv;
   KCH_REQUIRE(p->nh >= 1 && p->nh % n_kv == 0, "kch_paged_attend: nh=%d must be a multiple of n_kv=%d", p->nh, n_kv);
   KCH_REQUIRE(p->sliding_window >= 0, "kch_paged_attend: sliding_window=%d must be >= 0 (0: every key)", p->sliding_window);
-  KCH_REQUIRE(isfinite(p->scale), "kch_paged_attend: scale must be finite");
+  KCH_REQUIRE(isfinite(p->scale * PG_LOG2E), "kch_paged_attend: scale=%g must be finite, times log2(e) too", (double)p->scale);
   KCH_REQUIRE(!p->sink || p->sink_dtype == KCH_F32 || p->sink_dtype == KCH_BF16, "kch_paged_attend: sink dtype tag %d", p->sink_dtype);
   KCH_REQUIRE(p->batch.N * p->nh <= 0x7FFFFE00LL && (int64_t)p->nh * c <= 0x7FFFFFFFLL,       // (rows, a block's end among them, and columns in 32 bits)
               "kch_paged_attend: N * nh = %lld rows of q, nh * c = %lld columns", (long long)(p->batch.N * p->nh), (long long)p->nh * c);
