@@ -445,7 +445,7 @@ typedef struct kch_paged_batch {
 
 /* Writes the packed rows k, v [N, n_kv, c] (tokens ld_k / ld_v elements apart) into their pages.  8-bit kinds: s = max |x| / 448
  * (e4m3) or / 127 (int8) over the row of a key head, 1 for a row of zeros; stored round(x / s), ties to even.  A row that is not
- * finite reads back as NaN.  What a position that occurs twice in a batch holds is undefined. */
+ * finite gets the scale NaN and reads back as NaN; codes of NaN are never written (but read as what they are).  What a position that occurs twice in a batch holds is undefined. */
 int kch_paged_append(const kch_paged_cache* cache, const kch_paged_batch* batch, const void* k, int64_t ld_k, const void* v,
                      int64_t ld_v, int dtype, void* stream);
 /* Reads the rows of those positions back as packed rows in `dtype`: stored value times scale, rounded once.  Rows of no sequence:
@@ -459,7 +459,8 @@ int kch_paged_read(const kch_paged_cache* cache, const kch_paged_batch* batch, v
  * The sink logit of a head (optional) adds to the denominator.  q [N, nh, c] (tokens ld_q elements apart) and out [N, nh, c] in
  * `dtype`, which is that of the cache's activations; they do not overlap.  Rows of no sequence: zeros with `zero_rest`, else left as they are.  A row
  * without keys is 0.  What a row does not see (other pages, rows behind a sequence's end, later or older keys) does not reach it,
- * numbers or not; an infinity or a NaN among the values that other rows of a tile see costs time, though. */
+ * numbers or not; an infinity or a NaN among the values that other rows of a tile see costs time, though, and so does a code of NaN
+ * (0x7F, 0xFF) anywhere in an e4m3 tile. */
 typedef struct kch_paged_attend_args {
   kch_paged_cache cache;
   kch_paged_batch batch;

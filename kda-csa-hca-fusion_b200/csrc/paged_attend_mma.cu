@@ -15,10 +15,12 @@
 //   O += P V:  the order of the columns is free, so thread (g, t) takes 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9,
 //     one of them a product; pairs of keys meet by a byte permutation.  P comes from S in place.
 // A key's scale multiplies its logit, and its probability before that is rounded to bf16; masked keys are taken out after that, so
-// that a scale that is not finite stays where it is seen.
+// that a scale that is not finite stays where it is seen.  e4m3's codes of NaN (an append writes none, but a pool that existed before may
+// hold some) convert to 480; the largest code of a tile is kept, an instruction more for four codes, and where it is one of them the
+// item's keys are looked through when it ends and what sees one is made NaN (5 % of a step; a test of each word for such bytes took 7 to 10).
 //
-// Measured, 64 sequences, 16 heads of 128 on 4, pages of 64: 8192 tokens, e4m3, 136 us (4.1 TB/s of pages); 500 to 16000 tokens, e4m3 150,
-// int8 163, and on one key head 56 and 59.  Bound by what two warps of a scheduler have in flight (half of the issue slots are used).
+// Measured, 64 sequences, 16 heads of 128 on 4, pages of 64: 8192 tokens, e4m3, 143 us (3.9 TB/s of pages); 500 to 16000 tokens, e4m3 158,
+// int8 163, and on one key head 58 and 59.  Bound by what two warps of a scheduler have in flight (half of the issue slots are used).
 // Through tcgen05 tiles 8192 tokens took 179 us and one key head 65; with sixteen warps of 104 registers (they spill) 166.
 #include <cuda.h>
 #include <math.h>
@@ -51,6 +53,7 @@ struct PmSmem {
   alignas(16) float stage[C::WARPS][8 * D];
   alignas(16) uint4 q[D / 16][C::MT][32];                // fragments of the queries: contraction step, fragment, lane
   float ml[2][C::WARPS][R];
+  uint32_t nan_code, nan[R][D / 32];                     // e4m3: a code of NaN among the item's tiles; the channels that it makes NaN, by row
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
 static_assert(sizeof(PmSmem<128, 16>) <= 232448 && sizeof(PmSmem<128, 32>) <= 232448, "shared memory of the paged attention over 8-bit pages");
@@ -67,18 +70,28 @@ __device__ __forceinline__ uint32_t pm_fma(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 // e4m3: a code in the high byte of either half; sign, exponent and mantissa moved to their places are 2^-120 of the value (subnormal
-// codes become subnormal bf16 values).  int8: a code in the low byte; 128 + its low 7 bits, less 256 or 128 by the sign.  Exact.
+// codes become subnormal bf16 values).  int8: a code in the low byte; 128 + its low 7 bits, less 256 or 128 by the sign.  Exact, but that
+// e4m3's codes of NaN come out as 480.
 template <int KIND>
-__device__ __forceinline__ uint32_t pm_value2(uint32_t t) {
-  if (KIND == KCH_FP8_E4M3) return pm_fma((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
+__device__ __forceinline__ uint32_t pm_value2(uint32_t t, uint32_t& size) {      // size: e4m3, of the codes without their signs
+  if (KIND == KCH_FP8_E4M3) {
+    size = (t >> 4) & 0x07F007F0u;
+    return pm_fma((t & 0x80008000u) | size, 0x7B807B80u, 0x80008000u);
+  }
   return pm_fma((t & 0x00800080u) | 0x43004300u, 0xBF80BF80u, (t & 0x007F007Fu) | 0x43004300u);
 }
 // byte I of x and byte J of y as a pair of values
 template <int KIND>
-__device__ __forceinline__ uint32_t pm_pair(uint32_t x, uint32_t y, int i, int j) {
+__device__ __forceinline__ uint32_t pm_pair(uint32_t x, uint32_t y, int i, int j, uint32_t& size) {
   const uint32_t sel = KIND == KCH_FP8_E4M3 ? (i << 4) | ((4 + j) << 12) : i | ((4 + j) << 8);
-  return pm_value2<KIND>(__byte_perm(x, y, sel));
+  return pm_value2<KIND>(__byte_perm(x, y, sel), size);
 }
+// the largest size of two pairs and `most`; a NaN's is the largest of all, 0x7F0
+template <int KIND>
+__device__ __forceinline__ void pm_most(uint32_t& most, uint32_t s0, uint32_t s1) {
+  if (KIND == KCH_FP8_E4M3) most = __vimax3_u16x2(most, s0, s1);
+}
+__device__ __forceinline__ bool pm_has_nan(uint32_t most) { return most >= 0x07F00000u || (most & 0xFFFFu) >= 0x07F0u; }
 // (not volatile: products, conversions and the softmax of a tile may be mixed)
 __device__ __forceinline__ void pm_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -91,7 +104,33 @@ __device__ __forceinline__ void pm_mma(float (&d)[2], const uint32_t (&a)[4], ui
       : "=f"(d[0]), "=f"(d[1]), "=f"(x), "=f"(y)
       : "r"(a[0]), "r"(0), "r"(a[2]), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(0.f));
 }
+// which bytes of w are e4m3 codes of NaN (0x7F, 0xFF): their top bits
+__device__ __forceinline__ uint32_t pm_nan(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint4 pm_lds(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// The codes of NaN among the keys [from, to) of a sequence: which channels of which of the item's rows see one (all of them, where it is a
+// key's).  Of 256 threads.
+template <int D>
+__device__ __noinline__ void pm_find_nan(const PgAttend& a, int b, int h, int row0, int rows, PgSeq s, int from, int to, uint32_t (*nan)[D / 32], int tid) {
+  constexpr int PIECES = 2 * D / 16;                     // of a key: its own and its value's
+  for (int64_t i = tid; i < (int64_t)(to - from) * PIECES; i += 256) {
+    const int key = from + (int)(i / PIECES), piece = (int)(i % (D / 16)), page = __ldg(a.bt.table + b * a.bt.ld_table + (key >> a.bt.shift));
+    const bool value = i % PIECES >= D / 16;
+    if ((unsigned)page >= (unsigned)a.bt.num_pages) continue;
+    const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (key & (a.page - 1));
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>((const uint8_t*)(value ? a.v : a.k) + row * D) + piece);
+    const uint32_t w[4] = {pm_nan(u.x), pm_nan(u.y), pm_nan(u.z), pm_nan(u.w)};
+    uint32_t bits = 0u;
+    for (int e = 0; e < 16; ++e) bits |= (w[e >> 2] >> (8 * (e & 3) + 7) & 1u) << e;
+    if (!bits) continue;
+    for (int r = 0; r < rows; ++r) {
+      const int2 keys = pg_sees(a.bt, s, row0 + r);
+      if (key < keys.x || key >= keys.y) continue;
+      if (value) atomicOr(&nan[r][piece / 2], bits << (16 * (piece & 1)));
+      else for (int k = 0; k < D / 32; ++k) atomicOr(&nan[r][k], 0xFFFFFFFFu);
+    }
+  }
+}
 
 template <int D, int KIND, int R>
 __global__ void __launch_bounds__(PmCfg<R>::THREADS, 1)
@@ -108,6 +147,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
   if (tid == 0) {
     for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::SHARE); }
+    sm.nan_code = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -218,6 +258,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
         const uint8_t *tk = sm.k[st], *tv = sm.v[st];
         float s[C::H][MT][F] = {};
+        uint32_t most = 0u;                              // e4m3: the largest code
 #pragma unroll
         for (int i4 = 0; i4 < KS; i4 += 4) {             // 16 bytes of each key's run
           uint4 kc[C::H];
@@ -234,12 +275,15 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 #pragma unroll
             for (int h = 0; h < C::H; ++h) {
               const uint32_t c = i == 0 ? kc[h].x : i == 1 ? kc[h].y : i == 2 ? kc[h].z : kc[h].w;
-              const uint32_t b0 = pm_pair<KIND>(c, c, 0, 1), b1 = pm_pair<KIND>(c, c, 2, 3);
+              uint32_t s0, s1;
+              const uint32_t b0 = pm_pair<KIND>(c, c, 0, 1, s0), b1 = pm_pair<KIND>(c, c, 2, 3, s1);
+              pm_most<KIND>(most, s0, s1);
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) pm_mma(s[h][mt], q[mt], b0, b1);
             }
           }
         }
+        if (KIND == KCH_FP8_E4M3 && pm_has_nan(most)) *(volatile uint32_t*)&sm.nan_code = 1u;      // (checked behind either product: one word held to the tile's end takes 2 % more)
         // scaled; what a row does not see is -inf
         const bool whole = key0 >= k1.x && key0 + C::SLICE <= k0.y && w.x.rows == R;
         constexpr int E = MT * F;                        // values of a thread in 8 keys; bit E h + e of `sees`
@@ -313,6 +357,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           }
         }
         // of the values channels NT g .. NT g + NT - 1 of keys 2t, 2t + 1, 2t + 8, 2t + 9 of either half of the 32
+        most = 0u;
 #pragma unroll
         for (int b = 0; b < C::H / 2; ++b) {
           uint32_t c[4][NT / 4];
@@ -329,7 +374,9 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const uint32_t b0 = pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3), b1 = pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3);
+            uint32_t s0, s1;
+            const uint32_t b0 = pm_pair<KIND>(c[0][j >> 2], c[1][j >> 2], j & 3, j & 3, s0), b1 = pm_pair<KIND>(c[2][j >> 2], c[3][j >> 2], j & 3, j & 3, s1);
+            pm_most<KIND>(most, s0, s1);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               pm_mma(o[j][mt], p[b][mt], b0, b1);
@@ -337,6 +384,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             }
           }
         }
+        if (KIND == KCH_FP8_E4M3 && pm_has_nan(most)) *(volatile uint32_t*)&sm.nan_code = 1u;
       }
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sm.empty[st]);
@@ -408,6 +456,23 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
       }
       sync();
+    }
+    // Codes of NaN (an append writes none) have counted as 480 so far, which reaches no sum but those that they make NaN: all of a row that
+    // sees one among the keys, and its channel in a row that sees one among the values.  They are looked for only where there is one.
+    if (KIND == KCH_FP8_E4M3 && *(volatile uint32_t*)&sm.nan_code != 0u) {
+      sync();                                            // (all have read the word)
+      if (ct == 0) *(volatile uint32_t*)&sm.nan_code = 0u;
+      for (int i = ct; i < R * (D / 32); i += 32 * C::WARPS) sm.nan[i / (D / 32)][i % (D / 32)] = 0u;
+      sync();
+      const int part0 = w.x.first_key + w.first * PM_KT;
+      pm_find_nan<D>(a, w.b, w.h, w.block * R, w.x.rows, w.s, max(part0, w.x.lo), min(part0 + w.count * PM_KT, w.s.kv), sm.nan, ct);
+      sync();
+      for (int i = ct; i < w.x.rows * D && ok; i += 32 * C::WARPS) {
+        const int row = i / D, d = i % D, rr = w.block * R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
+        if (!(sm.nan[row][d / 32] >> (d & 31) & 1u)) continue;
+        if (direct) ((uint16_t*)a.out)[((int64_t)(w.s.row0 + tok) * (n_kv * G) + head) * D + d] = 0x7FC0u;
+        else slot[(int64_t)row * D + d] = __uint_as_float(0x7FC00000u);
+      }
     }
     if (w.starts() && !w.ends()) {
       part = true;

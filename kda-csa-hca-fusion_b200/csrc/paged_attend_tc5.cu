@@ -17,7 +17,8 @@
 // S_X's columns, as the operand from tensor memory and V as an MN-major operand from the same kind of tile (tcgen05.mma of one CTA
 // complete in the order of issue, so S_X of the next tile may follow P_X V); warps 2 and 3 fetch the next item's queries, with 8-bit
 // pages its scales too, but in steps over bf16 pages warp 2 copies the values' pages and warp 0 the keys'.
-// 8-bit pages: four more warps turn the copied payloads into bf16 tiles (exactly: a payload has at most 7 bits of mantissa);
+// 8-bit pages: four more warps turn the copied payloads into bf16 tiles (exactly: a payload has at most 7 bits of mantissa;
+// only e4m3's codes of NaN become 480, and where a tile has one the rows that may see it are summed again);
 // a row's scale multiplies its logit, or its probability before that is rounded to bf16.
 //
 // The running maximum of a row is raised, and O_X rescaled, only when a tile exceeds it by 2^8: probabilities up to 256 lose
@@ -89,6 +90,7 @@ struct PtSmem {
   float ml[2][256];                                      // maxima and sums of the parts of an item's keys
   float factor[2][32];                                   // of its rows: 1 / the denominator
   uint32_t odd[2];                                       // rows of it that are not finite, by column half
+  uint32_t nan_code;                                     // e4m3: a code of NaN among the tiles so far
   alignas(8) uint64_t full[C::STAGES], empty[C::STAGES];
   uint64_t raw_full[C::RAWS ? C::RAWS : 1], raw_empty[C::RAWS ? C::RAWS : 1];
   uint64_t sc_full[C::SCALES], sc_empty[C::SCALES];
@@ -181,26 +183,48 @@ __device__ __forceinline__ uint32_t pt_range(int lo, int hi) {
   hi = min(hi, 32);
   return hi > lo ? (0xFFFFFFFFu >> (32 - (hi - lo))) << lo : 0u;
 }
-// two bf16 values from two 8-bit codes, exactly
+// two bf16 values from two 8-bit codes, exactly (but see `most`)
 // (as FMAs: mul and sub of bf16 pairs become conversions to fp32 and back, and 4500 cycles for a tile of 128 x 128 instead of ~900)
 __device__ __forceinline__ uint32_t pt_bf16_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
+// most: e4m3, the largest of the codes without their signs; a NaN's (which comes out as 480) is the largest of all, 0x7F0
 template <int KIND>
-__device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+__device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi, uint32_t& most) {
   if (KIND == KCH_FP8_E4M3) {
     // sign, exponent and mantissa moved to their places are 2^-120 of the value (subnormal codes become subnormal bf16 values)
-    const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
-    lo = pt_bf16_fma((a & 0x80008000u) | ((a >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
-    hi = pt_bf16_fma((b & 0x80008000u) | ((b >> 4) & 0x07F007F0u), 0x7B807B80u, 0x80008000u);
+    const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424), sa = (a >> 4) & 0x07F007F0u, sb = (b >> 4) & 0x07F007F0u;
+    lo = pt_bf16_fma((a & 0x80008000u) | sa, 0x7B807B80u, 0x80008000u);
+    hi = pt_bf16_fma((b & 0x80008000u) | sb, 0x7B807B80u, 0x80008000u);
+    most = __vimax3_u16x2(most, sa, sb);
   } else {
     // 128 + the low 7 bits, less 256 or 128 by the sign
     const uint32_t a = __byte_perm(w, 0x43434343u, 0x5140), b = __byte_perm(w, 0x43434343u, 0x7362);
     lo = pt_bf16_fma(a & 0xFF80FF80u, 0xBF80BF80u, a & 0xFF7FFF7Fu);
     hi = pt_bf16_fma(b & 0xFF80FF80u, 0xBF80BF80u, b & 0xFF7FFF7Fu);
   }
+}
+
+// Is there a code of NaN (0x7F, 0xFF) among the keys [from, to) of a sequence, or their values?  A warp's.
+template <int D>
+__device__ __noinline__ bool pt_nan_among(const PgAttend& a, int b, int h, int from, int to) {
+  constexpr int PIECES = D / 16;
+  const int lane = threadIdx.x & 31;
+  uint32_t x = 0u;
+#pragma unroll 4
+  for (int j = from + lane / PIECES; j < to; j += 32 / PIECES) {
+    const int page = __ldg(a.bt.table + b * a.bt.ld_table + (j >> a.bt.shift));
+    if ((unsigned)page >= (unsigned)a.bt.num_pages) continue;
+    const int64_t at = (((int64_t)page * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * PIECES + lane % PIECES;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(kv ? a.v : a.k) + at);
+      x |= ((u.x & 0x7F7F7F7Fu) + 0x01010101u) | ((u.y & 0x7F7F7F7Fu) + 0x01010101u) | ((u.z & 0x7F7F7F7Fu) + 0x01010101u) | ((u.w & 0x7F7F7F7Fu) + 0x01010101u);
+    }
+  }
+  return __any_sync(0xffffffffu, (x & 0x80808080u) != 0u);
 }
 
 // One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns
@@ -269,7 +293,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, C::APART ? 1 : 2);
     mbarrier_init(&sm.q_empty, 1);
-    sm.odd[0] = sm.odd[1] = 0u;
+    sm.odd[0] = sm.odd[1] = sm.nan_code = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
@@ -648,7 +672,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           l += la + lb;
         }
         if (!C::Q8 && w.s.kv > key0 && w.s.kv < key0 + PT_KT) {
-          // (payloads of 8 bits are numbers, and the scales there are 0)
+          // (payloads of 8 bits are numbers by now, and the scales there are 0)
           const int at = pair ? ring + 1 + 2 * s : ring + 2 + 4 * s + (s + 1 < w.count ? 2 : 1) * x;      // of the tile's values in the ring
           if (ok) ok = wait(&sm.full[at % C::STAGES], at / C::STAGES);
           ok = __all_sync(0xffffffffu, ok);
@@ -788,10 +812,17 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           }
         }
       }
+      // e4m3: codes of NaN have counted as 480 so far, which reaches no sum but those that they make NaN.  Where there is one, the rows are
+      // summed again as well.
+      bool nan = false;
+      if (KIND == KCH_FP8_E4M3 && *(volatile uint32_t*)&sm.nan_code != 0u) {
+        const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span;
+        nan = pt_nan_among<D>(a, w.b, w.h, max(part0, w.x.lo), min(part0 + w.count * span, w.s.kv));
+      }
       // rows that are not finite: again, over the columns stored here
       unsigned again;
       if constexpr (FEW != 0) again = (warp & 3) == 0 ? sm.odd[x] : 0u;       // (row i is lane i's of the first warp)
-      else again = __ballot_sync(0xffffffffu, live && ok && odd != 0.f);
+      else again = __ballot_sync(0xffffffffu, live && ok && (odd != 0.f || nan));
       if (again) {
         __syncwarp();
         if (FEW && lane == 0) sm.odd[x] = 0u;
@@ -834,18 +865,22 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           const int row = D == 128 ? (wq >> 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : wq * 8 + (lane >> 2), panel = D == 128 ? wq & 1 : 0;
           const uint8_t* src = sm.raw[g % C::RAWS] + row * D + ((D == 128 ? (panel * 4 + k) ^ (row & 7) : k ^ ((row >> 1) & 3)) << 4);
           uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
+          uint32_t most = 0u;
           uint8_t *to0 = line + (((2 * k) ^ (row & 7)) << 4), *to1 = line + (((2 * k + 1) ^ (row & 7)) << 4);
 #pragma unroll 4
           for (int n = 0; n < ROUNDS; ++n) {
             const uint4 u = *reinterpret_cast<const uint4*>(src + n * (ROWS * D));
             uint4 lo, hi;
-            pt_codes4<KIND>(u.x, lo.x, lo.y);
-            pt_codes4<KIND>(u.y, lo.z, lo.w);
-            pt_codes4<KIND>(u.z, hi.x, hi.y);
-            pt_codes4<KIND>(u.w, hi.z, hi.w);
+            pt_codes4<KIND>(u.x, lo.x, lo.y, most);
+            pt_codes4<KIND>(u.y, lo.z, lo.w, most);
+            pt_codes4<KIND>(u.z, hi.x, hi.y, most);
+            pt_codes4<KIND>(u.w, hi.z, hi.w, most);
             *reinterpret_cast<uint4*>(to0 + n * (ROWS * 128)) = lo;
             *reinterpret_cast<uint4*>(to1 + n * (ROWS * 128)) = hi;
           }
+          // a code of NaN (an append writes none): at the ends of items from here on it is looked for among what the sequences have
+          if (KIND == KCH_FP8_E4M3 && (most >= 0x07F00000u || (most & 0xFFFFu) >= 0x07F0u))
+            *(volatile uint32_t*)&sm.nan_code = 1u;
           t5_fence_async_smem();
           __syncwarp();
           if (lane == 0) {

@@ -267,3 +267,42 @@ def test_a_negative_count_of_earlier_tokens_is_the_callers_mistake_and_touches_n
     want, tol = by_rows(m, q)
     rows = torch.cat([torch.arange(0, new[0]), torch.arange(new[0] + new[1], m.N)]).to(DEV)
     close(got[rows], want[rows], tol[rows])
+
+
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("where", ["nowhere", "key", "value", "both"])
+@pytest.mark.parametrize("new,past", [([1, 1], [300, 4000]), ([4, 2], [700, 31]), ([140, 3], [60, 500]), ([70], [2000])])
+@pytest.mark.parametrize("dtype,c,nh,n_kv", [(torch.bfloat16, 128, 4, 2), (torch.bfloat16, 64, 16, 1), (torch.bfloat16, 128, 24, 1), (torch.float32, 64, 4, 2)])
+def test_a_pool_that_holds_codes_of_nan(kch, dtype, c, nh, n_kv, new, past, where, window):
+    """e4m3 has two codes of NaN.  Rows written here have none, but a pool that existed already may: what sees one is what read_step's values give,
+    and what does not see it is as ever."""
+    m = Batch(kch, new, past, dtype=dtype, kind="fp8", c=c, n_kv=n_kv, page=16)
+    m.cache = kch.PagedKVCache(m.cache.num_pages, 16, n_kv, c, DEV, dtype, kv_quant="fp8",
+                               storage=(m.cache.k_pages, m.cache.v_pages, m.cache.k_scales, m.cache.v_scales))
+    owned = torch.zeros(m.cache.num_pages, 16, dtype=torch.bool, device=DEV)
+    for b, (n, p) in enumerate(zip(new, past)):
+        lo = max(p + 1 - window, 0) if window else 0
+        pos = torch.arange(lo, n + p, device=DEV)
+        owned[m.table[b].long()[pos // 16], pos % 16] = True
+    raw = [x.view(torch.uint8) for x in (m.cache.k_pages, m.cache.v_pages)]
+    for x in raw:                                          # behind the ends, before the windows and in pages of nobody: anything
+        x.masked_fill_((~owned)[:, None, :, None].expand_as(x), 0x7F)
+        x[:, :, ::3].masked_fill_((~owned)[:, None, ::3, None].expand_as(x[:, :, ::3]), 0xFF)
+    pg, row = at(m, 0, past[0] - 3)
+    if where in ("key", "both"):
+        raw[0][pg, n_kv - 1, row, c - 1] = 0xFF
+    if where in ("value", "both"):
+        raw[1][pg, 0, row, 9], raw[1][pg, 0, row, c - 2] = 0x7F, 0xFF
+        pg, row = at(m, 0, past[0] + new[0] - 1)           # the newest token's: its own query alone sees it
+        raw[1][pg, n_kv - 1, row, 40] = 0x7F
+    if where != "nowhere":
+        first = torch.tensor([past[0] - 3], dtype=torch.int32, device=DEV)
+        k, v = m.cache.read_step(m.table[:1], first, torch.tensor([0, new[0] + 3], dtype=torch.int32, device=DEV), n_rows=new[0] + 3)
+        want_k, want_v = (m.values(x, 0, past[0] + new[0])[:, past[0] - 3:].transpose(0, 1).to(dtype) for x in "kv")
+        for got, want in ((k, want_k), (v, want_v)):
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    q = m.randn(m.N, nh, c)
+    want, tol = by_rows(m, q, window=window)
+    assert bool(want.isnan().any()) == (where != "nowhere")
+    for _ in range(2):
+        close(m.cache.forward_step(q, *m.args, sliding_window=window), want, tol)
