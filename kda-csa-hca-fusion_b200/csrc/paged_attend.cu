@@ -477,9 +477,16 @@ int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaSt
 int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.  The host knows the rows of a call and its
-// sequences, not who has them: what a sequence has on average decides, every form takes every batch, and a batch counts as one of few
-// rows only up to 4 tokens a sequence, so that a long chunk among single tokens cannot be most of its work (measured figures at the
-// kernels).
+// sequences, not who has them: what a sequence has on average decides, and every form takes every batch.  Either side, us, few rows /
+// chunks, of 64 sequences over 4000 tokens, 16 heads of 128, pages of 64:
+//   rows (tokens x heads of a key head) of a sequence: up to 32, an item of the forms for few rows; behind that they read the keys twice.
+//     bf16  8 heads: 1 token 55 / 58, 4 (32 rows) 57 / 60, 5 (40 rows) 100 / 61;  16 heads: 2 tokens 37 / 41, 3 (48 rows) 52 / 42
+//     e4m3  8 heads: 1 token 46 / 80, 4 68 / 81, 5 126 / 81;  16 heads: 2 tokens 42 / 47, 3 72 / 48;  int8: 47 / 74, 68 / 74, 125 / 75; 41 / 45, 72 / 46
+//   tokens of a sequence: up to 4, so that a long chunk among single tokens cannot be most of a batch's work.  With 190 tokens in one sequence
+//     and one in each other (4 on average) 4 heads take 118 / 96 (bf16), 145 / 147 (e4m3), 146 / 141 (int8), 2 heads 191 / 174, 245 / 267, 254 / 254; with
+//     448 (8 on average) 127 / 100, 223 / 165, 222 / 156, and 246 / 182, 300 / 277, 302 / 265.  Alike ones would go on to 32 rows: 8 tokens of 4 heads
+//     96 / 99, 120 / 141, 119 / 133.
+//   CUDA cores, 2000 tokens: items of 16 rows / of 64, 4 fp32 heads of 64 on 2: 16 rows 100 / 161, 24 rows 193 / 162;  256 wide, bf16: 375 / 573, 737 / 575.
 enum PaForm { PA_TC5, PA_TC5_FEW, PA_MMA, PA_SIMT };
 struct PaPlan { PaForm form; int rows, tile, ctas, slot_rows; bool two; };      // two: items of at most half the rows (FEW: all) take two tiles a step
 static PaPlan pa_plan(const kch_paged_attend_args* p) {
