@@ -46,12 +46,15 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tc5_utils.cuh"
 
 #define PT_KT 128
-#define PT_SPIN (1u << 26)               // (a row that is summed again key by key makes the others wait)
+// Polls of a wait, eight seconds: a warp that sums its 32 rows again makes the others wait 5 us a key, so that the limit is 1.6 million keys
+// in the part that a CTA has of them.
+#define PT_SPIN (1u << 28)
 
 template <int D, int KIND, int FEW>
 struct PtCfg {
@@ -228,44 +231,77 @@ __device__ __noinline__ bool pt_nan_among(const PgAttend& a, int b, int h, int f
 }
 
 // One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns
-// c0 .. c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).
+// c0 .. c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).  16 keys at a time, a lane with D / 32 channels of each; their pages
+// are asked for 16 keys ahead, and the sums of the lanes are halved over and over until lane l has that of key l mod 16: 0.15 us a key on
+// all warps.  (With each key's page asked for where it is needed, and a sum of its own, 0.5 us.)
 template <int D, int KIND>
 __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int from, int to, float sc, float shift,
                                          float f, bf16* out, float* dst, int c0, int c1) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
+  constexpr int E = D / 32, ES = KIND == KCH_BF16 ? 2 : 1, BYTES = E * ES, U = 16;       // channels and bytes of a lane, keys in flight
+  typedef typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type Raw;
+  const int lane = threadIdx.x & 31, own = lane & (U - 1);
   float qv[E], o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { qv[e] = ldf(q + lane * E + e); o[e] = 0.f; }
-  auto value = [&](const void* p, int64_t i) -> float {
-    if (KIND == KCH_BF16) return ldf((const bf16*)p + i);
-    if (KIND == KCH_INT8) return (float)((const int8_t*)p)[i];
-    return float(((const __nv_fp8_e4m3*)p)[i]);
+  auto value = [](const Raw& x, int e) -> float {
+    uint32_t w;
+    if constexpr (BYTES == 8) w = e < 2 ? x.x : x.y;
+    else w = x;
+    if constexpr (KIND == KCH_BF16) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+    const uint8_t code = (uint8_t)(w >> (8 * e));
+    if constexpr (KIND == KCH_INT8) return (float)(int8_t)code;
+    __nv_fp8_e4m3 v;
+    v.__x = code;
+    return float(v);
   };
-  constexpr int U = 8;                                   // keys in flight
+  auto ask = [&](int j0) { return j0 < to ? pg_page(a.bt, b, min(j0 + own, to - 1) >> a.bt.shift) : -1; };
+  int page = ask(from);
+#pragma unroll 1
   for (int j0 = from; j0 < to; j0 += U) {
-    float s[U], v[U][E], vs[U];
+    const int next = ask(j0 + U);
+    Raw k[U], v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = min(j0 + u, to - 1);
-      const int64_t pg = pg_page(a.bt, b, j >> a.bt.shift), row = (max(pg, (int64_t)0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1));
+      const int pg = __shfl_sync(0xffffffffu, page, u), j = min(j0 + u, to - 1);
+      const int64_t at = ((((int64_t)max(pg, 0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * 32 + lane) * BYTES;
+      k[u] = v[u] = Raw{};                               // (a page that is missing: zeros)
+      if (pg >= 0) {
+        k[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.k + at));
+        v[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.v + at));
+      }
+    }
+    float ks = 1.f, vs = 1.f;
+    if (KIND != KCH_BF16 && page >= 0) {
+      const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (min(j0 + own, to - 1) & (a.page - 1));
+      ks = __ldg(a.ks + row);
+      vs = __ldg(a.vs + row);
+    }
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       s[u] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        s[u] = fmaf(qv[e], pg < 0 ? 0.f : value(a.k, row * D + lane * E + e), s[u]);
-        v[u][e] = pg < 0 ? 0.f : value(a.v, row * D + lane * E + e);
-      }
-      vs[u] = 1.f;
-      if (KIND != KCH_BF16) { s[u] *= a.ks[row]; vs[u] = a.vs[row]; }
+      for (int e = 0; e < E; ++e) s[u] = fmaf(qv[e], value(k[u], e), s[u]);
     }
+#pragma unroll
+    for (int n = U / 2; n > 0; n >>= 1) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float keep = lane & n ? s[i + n] : s[i], give = lane & n ? s[i] : s[i + n];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+      }
+    }
+    s[0] += __shfl_xor_sync(0xffffffffu, s[0], 16);
+    const float p = round_to<bf16>(ex2_fast(fmaf(s[0] * ks, sc, -shift)) * vs);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float p = round_to<bf16>(ex2_fast(fmaf(warp_sum(s[u]), sc, -shift)) * vs[u]);
+      const float pu = __shfl_sync(0xffffffffu, p, u);
       if (j0 + u < to) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p, v[u][e], o[e]);
+        for (int e = 0; e < E; ++e) o[e] = fmaf(pu, value(v[u], e), o[e]);
       }
     }
+    page = next;
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {

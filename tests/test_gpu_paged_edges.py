@@ -306,3 +306,34 @@ def test_a_pool_that_holds_codes_of_nan(kch, dtype, c, nh, n_kv, new, past, wher
     assert bool(want.isnan().any()) == (where != "nowhere")
     for _ in range(2):
         close(m.cache.forward_step(q, *m.args, sliding_window=window), want, tol)
+
+
+@pytest.mark.parametrize("kind", [None, "fp8"])
+def test_rows_that_are_summed_again_over_a_long_sequence_do_not_run_the_others_waits_out(kch, kind):
+    """A NaN at the start of 131072 keys: every row of a chunk of 4096 tokens has one, and all of them are summed key by key."""
+    from kch_b200 import _lib
+    new, past = 4096, 131072 - 4096
+    n = 131072 // 64
+    cache = kch.PagedKVCache(n, 64, 4, 128, DEV, torch.bfloat16, kv_quant=kind)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    for x in (cache.k_pages, cache.v_pages):
+        x.normal_(generator=g) if kind is None else x.view(torch.uint8).random_(0, 0x60, generator=g)
+    if kind is None:
+        cache.v_pages[0, :, 3, 5] = torch.nan
+    else:
+        cache.v_pages.view(torch.uint8)[0, :, 3, 5] = 0x7F
+    table = torch.arange(n, dtype=torch.int32, device=DEV)[None]
+    t0, cu = torch.tensor([past], dtype=torch.int32, device=DEV), torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    q = torch.randn(new, 16, 128, generator=g, device=DEV).bfloat16()
+    got = cache.forward_step(q, table, t0, cu)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == 0
+    assert got[..., 5].isnan().all() and got.isnan().sum() == new * 16
+    # the same without the NaN, the other channels: P (2^-8 of the weighed sizes of the values) and the output are rounded in either call
+    pages = cache.v_pages.view(torch.uint8) if kind else cache.v_pages
+    pages[0, :, 3, 5] = 0
+    want = cache.forward_step(q, table, t0, cu).float()
+    pages.copy_(pages & 0x7F if kind else pages.abs())
+    size = cache.forward_step(q, table, t0, cu).float()
+    rest = torch.arange(128, device=DEV) != 5
+    assert ((got.float() - want).abs() <= 2.0 ** -7 * (1 + 2.0 ** -7) * (size + want.abs()) + 2.0 ** -14 * size)[..., rest].all()
