@@ -6,9 +6,9 @@
 // fp32 (whose products the tensor cores would round) and head widths that the tcgen05 kernel does not have.  An item's ROWS x KT
 // scores are a register tile of 4 (1) x 4 a thread over rows and keys staged in shared memory in fp32 (stored values times their
 // scale), the softmax keeps a running maximum and sum a row, and the sums stay in registers, a row's columns over 16 threads.
-// Measured: chunks of 391 to 700 tokens of three sequences, 4 heads of 64 on 2, fp32: 102 us; a step of the two CTAs of an SM takes
-// 12500 clocks, of which the products are 8200 at the FMA rate, the softmax 2600 and the tile's stores 1200.  16 rows (few tokens): the
-// rows are padded, 64 sequences of 500 to 4000 tokens take 470 us for 608 MB.
+// Measured: chunks of 391 to 700 tokens of three sequences, 4 heads of 64 on 2, fp32: 102 us, of which the join is 11: 8 steps
+// a CTA, 19500 clocks each where two CTAs share an SM (13000 where one has it), 8200 of which are the products of both at the FMA rate; the
+// plan 5500 clocks and the first loads 3000.  16 rows (few tokens): the rows are padded, 64 sequences of 500 to 4000 tokens take 470 us for 608 MB.
 #include <math.h>
 
 #include <type_traits>

@@ -33,11 +33,11 @@
 // 16000 tokens, pages of 16 and more 176 us, of 8 198 (a tile is 16 or 32 copies then: with one warp copying keys and values pages of
 // 16 and 8 took 196 and 322, and with each page asked for where it was needed and not a tile ahead pages of 16 took 263).
 // A chunk of 4096 tokens behind 28672: 827 us, 1247 TFLOP/s, in a burst, and 1000 us in a long run, where the power limit holds the
-// clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores 512, maximum 350, powers 1500, value product 512,
+// clock at 1.6 GHz.  A step of it is 3500 clocks, 2048 of them products: scores 512, maximum 350, powers 1500 (a pair of four by FMAs then), value product 512,
 // hand-overs 500, and two warpgroups that take turns.  Powers by FMAs (POLY) help heads of 64 alone, whose products are half as long: 32 of
 // them 1486 us with one pair of four, 1579 with none, 1623 with two; heads of 128 827 with none, 825 with one, 932 against 878 with two.
 // Neither did P handed over in halves (883 where the rest took 878) shorten it, nor the maximum and P in one pass (996, registers).  fp8
-// pages: 1270 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
+// pages: 1210 us, the conversion's ALU operations and the scales' products (6000 clocks a step; all powers are the special-function unit's, for
 // the FMAs have the scales: 1281 with one pair of four, and 124 against 119 for a ragged batch of 24 sequences with a window of 1000).
 // Short items cost their ends: 37 x 16 items of 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks
 // until a CTA's first scores, as many for the first end (its code comes from memory), then 6000 an end and 3000 until the next item's
