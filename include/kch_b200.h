@@ -480,6 +480,52 @@ typedef struct kch_paged_attend_args {
 int64_t kch_paged_attend_workspace_bytes(const kch_paged_attend_args* args);
 int kch_paged_attend(const kch_paged_attend_args* args, void* stream);
 
+/* The same attention of whole prompts whose keys and values are packed rows like the queries: k, v [N, n_kv, c] (tokens ld_k, ld_v elements
+ * apart), key j of sequence b in row cu_seqlens[b] + j, no earlier tokens.  All else as in kch_paged_attend_args: q, k, v and out 16-byte aligned,
+ * out apart from all three.  A call takes as many rows as it can have steps, were all of them one sequence: (N nh / n_kv / 256 + B) n_kv (N / 128 + 1) below
+ * 2^31 (bf16 heads of 64 and 128; else 64 for both). */
+typedef struct kch_prompt_attend_args {
+  const void *q, *k, *v;
+  int64_t ld_q, ld_k, ld_v;
+  const int32_t* cu_seqlens; /* [B + 1] */
+  int B;
+  int64_t N;
+  int dtype, nh, n_kv, c;
+  float scale;
+  int sliding_window;
+  const void* sink;          /* [nh] or NULL */
+  int sink_dtype;
+  void* out;
+  int zero_rest;
+  void* workspace;           /* 256-byte aligned */
+  int64_t workspace_bytes;
+} kch_prompt_attend_args;
+int64_t kch_prompt_attend_workspace_bytes(const kch_prompt_attend_args* args);
+int kch_prompt_attend(const kch_prompt_attend_args* args, void* stream);
+
+/* ---- rotary positions -------------------------------------------------------------------------------- */
+
+/* No counterpart in the reference, whose layers carry no positions.  Pairs of channels (a, b) of queries q [N, nh, c] and keys k
+ * [N, n_kv, c] (n_kv = 0: none) are turned by t = positions[token][axis] * f_i, where turns[i] = f_i / (2 pi) on the device:
+ * y_a = x_a cos t - x_b sin t, y_b = x_b cos t + x_a sin t, and by -t with `inverse` (which is the gradient).  Pair i of
+ * rotary_dim / 2 is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `neighbours`; channels behind rotary_dim stay.  sections: pairs of
+ * each axis, the first axis' first.  Heads are dense within a token, tokens ld elements apart; everything 16-byte aligned.  An output may be its
+ * own input (same address and ld) and shares no element with anything else.  c: a multiple of 8 up to 256. */
+typedef struct kch_rotary_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t ld_q, ld_k, ld_q_out, ld_k_out;
+  int64_t N;
+  int nh, n_kv, c, dtype;
+  const int32_t* positions;  /* [N, axes] rows ld_positions apart */
+  int64_t ld_positions;
+  int axes;                  /* 1 to 4 */
+  int sections[4];
+  const double* turns;       /* [rotary_dim / 2] */
+  int rotary_dim, neighbours, inverse;
+} kch_rotary_args;
+int kch_rotary(const kch_rotary_args* args, void* stream);
+
 /* ---- whole layers ------------------------------------------------------------------------------------------- */
 
 /* The launches of one layer over several tokens from one call; every step is one of the entry points above with the

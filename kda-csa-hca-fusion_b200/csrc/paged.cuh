@@ -14,12 +14,13 @@
 
 #define PG_MAX_B 4096                  // sequences of a call: their table of steps is kept in shared memory
 #define PG_LOG2E 1.4426950408889634f
+#define PG_ROWS 16                     // kind of keys and values that are packed rows like the queries, and not in pages (beside the KCH_ types)
 
 unsigned int* kch_status_device_ptr();
 
 struct PgBatch {
-  const int32_t* table; int64_t ld_table;
-  const int32_t *t0, *cu;
+  const int32_t* table; int64_t ld_table;      // NULL: keys and values are packed rows
+  const int32_t *t0, *cu;              // t0 NULL: no sequence has earlier tokens
   int B, N;                            // sequences; rows of the packed tensors
   int cap;                             // positions that a row of the table covers (below 2^31)
   int64_t num_pages;
@@ -46,7 +47,7 @@ __device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
   PgSeq s;
   s.row0 = min(max(__ldg(a.cu + b), 0), a.N);
   s.len = min(max(__ldg(a.cu + b + 1), s.row0), a.N) - s.row0;
-  const int t0 = __ldg(a.t0 + b);
+  const int t0 = a.t0 ? __ldg(a.t0 + b) : 0;
   s.t0 = max(t0, 0);
   s.kv = t0 < 0 ? 0 : (int)min((int64_t)t0 + s.len, (int64_t)a.cap);       // (positions before 0: no keys)
   return s;
@@ -287,7 +288,7 @@ struct PgAttend {                      // what both attention kernels get
   PgBatch bt;
   const void *q, *k, *v; const float *ks, *vs;
   void* out;
-  int64_t ld_q;
+  int64_t ld_q, ld_k, ld_v;             // (ld_k, ld_v: of packed rows)
   int c, page, zero_rest, slot_rows;
   float scale;                         // times log2(e)
   const void* sink; int sink_dtype;

@@ -117,6 +117,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         vw[k].none();
         fk[k] = fv[k] = 1.f;
         if (j < PA_KT && pos >= w.x.lo && pos < w.s.kv) {
+          if (!a.bt.table) {                                   // packed rows
+            kw[k].load(a.k, (w.s.row0 + pos) * a.ld_k + (int64_t)w.h * c + d);
+            vw[k].load(a.v, (w.s.row0 + pos) * a.ld_v + (int64_t)w.h * c + d);
+            continue;
+          }
           const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
           if (pg >= 0) {
             const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));
@@ -487,17 +492,60 @@ int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaSt
 //     448 (8 on average) 127 / 100, 223 / 165, 222 / 156, and 246 / 182, 300 / 277, 302 / 265.  Alike ones would go on to 32 rows: 8 tokens of 4 heads
 //     96 / 99, 120 / 141, 119 / 133.
 //   CUDA cores, 2000 tokens: items of 16 rows / of 64, 4 fp32 heads of 64 on 2: 16 rows 100 / 161, 24 rows 193 / 162;  256 wide, bf16: 375 / 573, 737 / 575.
+//   Packed rows (prompts) are chunks, whatever their lengths.
 enum PaForm { PA_TC5, PA_TC5_FEW, PA_MMA, PA_SIMT };
 struct PaPlan { PaForm form; int rows, tile, ctas, slot_rows; bool two; };      // two: items of at most half the rows (FEW: all) take two tiles a step
-static PaPlan pa_plan(const kch_paged_attend_args* p) {
+static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   PaPlan x;
-  const int64_t B = p->batch.B, rows = p->batch.N * (p->nh / p->cache.n_kv);      // of a key head
-  if (!kch_paged_attend_tc5_supported(p->dtype, p->cache.c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
-  else if (rows > 32 * B || p->batch.N > 4 * B) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
-  else if (p->cache.kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
+  const int64_t rows = N * G;                            // of a key head
+  if (!kch_paged_attend_tc5_supported(dtype, c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
+  else if (rows > 32 * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
+  else if (kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
+}
+static PaPlan pa_plan(const kch_paged_attend_args* p) {
+  return pa_plan(p->batch.B, p->batch.N, p->nh / p->cache.n_kv, p->cache.kind, p->dtype, p->cache.c);
+}
+static PaPlan pa_plan(const kch_prompt_attend_args* p) { return pa_plan(p->B, p->N, p->nh / p->n_kv, PG_ROWS, p->dtype, p->c); }
+
+// The launches of a call whose arguments are in order: the attention, and the joining of the items that are in parts.
+static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, void* workspace, cudaStream_t s) {
+  const int c = a.c;
+  a.records = (PgRecord*)workspace;
+  a.slots = (float*)((char*)workspace + pg_records_bytes(x.ctas));
+  a.slot_rows = x.slot_rows;
+  // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
+  const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
+  const PgJoinArgs j = {a.out, dtype, nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
+  if (x.form != PA_SIMT) {
+    const int rc5 = x.form == PA_MMA ? kch_paged_attend_mma(a, kind, x.rows, x.ctas, s) : kch_paged_attend_tc5(a, kind, x.rows, x.ctas, s);
+    return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
+  }
+  const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);
+#define PA_GO(T_, P_, R_, D_)                                                                                                 \
+  do {                                                                                                                        \
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
+    paged_attend_simt_kernel<T_, P_, R_, D_><<<x.ctas, PA_THREADS, smem, s>>>(a);                                            \
+  } while (0)
+#define PA_WIDTH(T_, P_, R_)                                                                                                  \
+  do {                                                                                                                        \
+    if (dmax == 64) PA_GO(T_, P_, R_, 64);                                                                                    \
+    else if (dmax == 128) PA_GO(T_, P_, R_, 128);                                                                             \
+    else PA_GO(T_, P_, R_, 256);                                                                                              \
+  } while (0)
+#define PA_ROWS(T_, P_)                                                                                                       \
+  do {                                                                                                                        \
+    if (rows == 16) PA_WIDTH(T_, P_, 16);                                                                                     \
+    else PA_WIDTH(T_, P_, 64);                                                                                                \
+  } while (0)
+  if (kind == KCH_FP8_E4M3) { if (dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
+  else if (kind == KCH_INT8) { if (dtype == KCH_F32) PA_ROWS(float, int8_t); else PA_ROWS(bf16, int8_t); }
+  else if (dtype == KCH_F32) PA_ROWS(float, float);
+  else PA_ROWS(bf16, bf16);
+  KCH_LAUNCH_OK();
+  return whole ? KCH_OK : kch_paged_join(j, x.ctas, s);
 }
 
 extern "C" int64_t kch_paged_attend_workspace_bytes(const kch_paged_attend_args* p) {
@@ -534,7 +582,6 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   pg_set_group(a.bt, p->nh / n_kv);
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
-  a.records = (PgRecord*)p->workspace;
   const PaPlan x = pa_plan(p);
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
@@ -542,38 +589,59 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   const uintptr_t q0 = (uintptr_t)p->q, q1 = q0 + ((p->batch.N - 1) * p->ld_q + (int64_t)p->nh * c) * es, o0 = (uintptr_t)p->out;
   KCH_REQUIRE(o0 >= q1 || o0 + p->batch.N * p->nh * c * es <= q0, "kch_paged_attend: out overlaps q");
   KCH_REQUIRE(a.bt.status != nullptr, "kch_paged_attend: cannot resolve the device status word");
-  a.slots = (float*)((char*)p->workspace + pg_records_bytes(x.ctas));
-  a.slot_rows = x.slot_rows;
-  cudaStream_t s = kch_stream(stream);
-  // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
-  const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
-  const PgJoinArgs j = {a.out, p->dtype, p->nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
-  if (x.form != PA_SIMT) {
-    const int rc5 = x.form == PA_MMA ? kch_paged_attend_mma(a, p->cache.kind, x.rows, x.ctas, s)
-                                     : kch_paged_attend_tc5(a, p->cache.kind, x.rows, x.ctas, s);
-    return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
+  return pa_launch(a, x, p->cache.kind, p->dtype, p->nh, p->workspace, kch_stream(stream));
+}
+
+extern "C" int64_t kch_prompt_attend_workspace_bytes(const kch_prompt_attend_args* p) {
+  if (!p || p->n_kv < 1 || p->nh < 1 || p->c < 1) return 0;
+  const PaPlan x = pa_plan(p);
+  return pg_workspace_bytes(x.ctas, x.slot_rows, p->c);
+}
+
+// Packed rows are pages of their own kind to the kernels: row cu_seqlens[b] + j of k and v is key j of sequence b, and no sequence has
+// earlier tokens.
+extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) {
+  const char* fn = "kch_prompt_attend";
+  KCH_REQUIRE(p != nullptr, "%s: null arguments", fn);
+  KCH_REQUIRE(p->dtype == KCH_F32 || p->dtype == KCH_BF16, "%s: unsupported dtype tag %d", fn, p->dtype);
+  KCH_REQUIRE(p->c >= 8 && p->c <= 256 && p->c % 8 == 0, "%s: c=%d must be a multiple of 8 from 8 to 256", fn, p->c);
+  KCH_REQUIRE(p->n_kv >= 1, "%s: n_kv=%d must be >= 1", fn, p->n_kv);
+  KCH_REQUIRE(p->nh >= 1 && p->nh % p->n_kv == 0, "%s: nh=%d must be a multiple of n_kv=%d", fn, p->nh, p->n_kv);
+  KCH_REQUIRE(p->B >= 1 && p->B <= PG_MAX_B, "%s: B=%d sequences must be from 1 to %d", fn, p->B, PG_MAX_B);
+  KCH_REQUIRE(p->N >= 0 && p->N <= 0x7FFFFFFFLL, "%s: N=%lld rows out of range", fn, (long long)p->N);
+  KCH_REQUIRE(p->cu_seqlens != nullptr, "%s: null cu_seqlens", fn);
+  KCH_REQUIRE(p->sliding_window >= 0, "%s: sliding_window=%d must be >= 0 (0: every key)", fn, p->sliding_window);
+  KCH_REQUIRE(isfinite(p->scale * PG_LOG2E), "%s: scale=%g must be finite, times log2(e) too", fn, (double)p->scale);
+  KCH_REQUIRE(!p->sink || p->sink_dtype == KCH_F32 || p->sink_dtype == KCH_BF16, "%s: sink dtype tag %d", fn, p->sink_dtype);
+  KCH_REQUIRE(p->N * p->nh <= 0x7FFFFE00LL && (int64_t)p->nh * p->c <= 0x7FFFFFFFLL, "%s: N * nh = %lld rows of q, nh * c = %lld columns", fn,
+              (long long)(p->N * p->nh), (long long)p->nh * p->c);
+  if (p->N == 0) return KCH_OK;
+  const int es = p->dtype == KCH_BF16 ? 2 : 4;
+  const int64_t wq = (int64_t)p->nh * p->c, wk = (int64_t)p->n_kv * p->c;
+  KCH_REQUIRE(p->q && p->k && p->v && p->out, "%s: null q, k, v or out", fn);
+  const struct { const void* x; int64_t ld, width; const char* name; } in[3] = {{p->q, p->ld_q, wq, "q"}, {p->k, p->ld_k, wk, "k"}, {p->v, p->ld_v, wk, "v"}};
+  const uintptr_t o0 = (uintptr_t)p->out, o1 = o0 + p->N * wq * es;
+  for (const auto& t : in) {
+    KCH_REQUIRE(t.ld >= t.width && t.ld * es % 16 == 0 && ((uintptr_t)t.x & 15) == 0,
+                "%s: %s must be 16-byte aligned, its tokens (%lld elements) at least heads * c apart in multiples of 16 bytes", fn, t.name, (long long)t.ld);
+    KCH_REQUIRE((uintptr_t)t.x >= o1 || (uintptr_t)t.x + ((p->N - 1) * t.ld + t.width) * es <= o0, "%s: out overlaps %s", fn, t.name);
   }
-  const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);
-#define PA_GO(T_, P_, R_, D_)                                                                                                 \
-  do {                                                                                                                        \
-    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
-    paged_attend_simt_kernel<T_, P_, R_, D_><<<x.ctas, PA_THREADS, smem, s>>>(a);                                            \
-  } while (0)
-#define PA_WIDTH(T_, P_, R_)                                                                                                  \
-  do {                                                                                                                        \
-    if (dmax == 64) PA_GO(T_, P_, R_, 64);                                                                                    \
-    else if (dmax == 128) PA_GO(T_, P_, R_, 128);                                                                             \
-    else PA_GO(T_, P_, R_, 256);                                                                                              \
-  } while (0)
-#define PA_ROWS(T_, P_)                                                                                                       \
-  do {                                                                                                                        \
-    if (rows == 16) PA_WIDTH(T_, P_, 16);                                                                                     \
-    else PA_WIDTH(T_, P_, 64);                                                                                                \
-  } while (0)
-  if (p->cache.kind == KCH_FP8_E4M3) { if (p->dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
-  else if (p->cache.kind == KCH_INT8) { if (p->dtype == KCH_F32) PA_ROWS(float, int8_t); else PA_ROWS(bf16, int8_t); }
-  else if (p->dtype == KCH_F32) PA_ROWS(float, float);
-  else PA_ROWS(bf16, bf16);
-  KCH_LAUNCH_OK();
-  return whole ? KCH_OK : kch_paged_join(j, x.ctas, s);
+  KCH_REQUIRE((o0 & 15) == 0, "%s: out must be 16-byte aligned", fn);
+  const int64_t need = kch_prompt_attend_workspace_bytes(p);
+  KCH_REQUIRE(p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= need,
+              "%s: workspace of %lld bytes (256-byte aligned) is too small: %lld needed", fn, (long long)p->workspace_bytes, (long long)need);
+  PgAttend a = {};
+  a.bt.cu = p->cu_seqlens;
+  a.bt.B = p->B; a.bt.N = (int)p->N; a.bt.cap = (int)p->N;
+  a.bt.status = kch_status_device_ptr();
+  a.bt.n_kv = p->n_kv; a.bt.window = p->sliding_window;
+  pg_set_group(a.bt, p->nh / p->n_kv);
+  a.q = p->q; a.k = p->k; a.v = p->v; a.ld_q = p->ld_q; a.ld_k = p->ld_k; a.ld_v = p->ld_v;
+  a.out = p->out; a.c = p->c; a.page = 128; a.zero_rest = p->zero_rest;      // (page: rows of a box)
+  a.scale = p->scale * PG_LOG2E;
+  a.sink = p->sink; a.sink_dtype = p->sink_dtype;
+  const PaPlan x = pa_plan(p);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
+  KCH_REQUIRE(a.bt.status != nullptr, "%s: cannot resolve the device status word", fn);
+  return pa_launch(a, x, PG_ROWS, p->dtype, p->nh, p->workspace, kch_stream(stream));
 }

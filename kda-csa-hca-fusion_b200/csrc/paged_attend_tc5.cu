@@ -59,7 +59,7 @@
 template <int D, int KIND, int FEW>
 struct PtCfg {
   static constexpr int R = FEW ? FEW : 256, TWO = FEW ? FEW : 128, COPIES = FEW ? 128 / FEW : 1;
-  static constexpr bool Q8 = KIND >= KCH_FP8_E4M3;
+  static constexpr bool Q8 = KIND == KCH_FP8_E4M3 || KIND == KCH_INT8, ROWS = KIND == PG_ROWS;
   static constexpr bool APART = FEW && !Q8;              // keys' and values' pages are copied by a warp each
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
   static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
@@ -107,6 +107,11 @@ __device__ __forceinline__ void pt_tma_4d(void* dst, const void* map, int c0, in
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(smem_addr_u32(dst)), "l"(map), "r"(smem_addr_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ void pt_tma_3d(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_addr_u32(dst)), "l"(map), "r"(smem_addr_u32(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 __device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -235,9 +240,10 @@ __device__ __noinline__ bool pt_nan_among(const PgAttend& a, int b, int h, int f
 // are asked for 16 keys ahead, and the sums of the lanes are halved over and over until lane l has that of key l mod 16: 0.15 us a key on
 // all warps.  (With each key's page asked for where it is needed, and a sum of its own, 0.5 us.)
 template <int D, int KIND>
-__device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const bf16* q, int from, int to, float sc, float shift,
+__device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int h, const bf16* q, int from, int to, float sc, float shift,
                                          float f, bf16* out, float* dst, int c0, int c1) {
-  constexpr int E = D / 32, ES = KIND == KCH_BF16 ? 2 : 1, BYTES = E * ES, U = 16;       // channels and bytes of a lane, keys in flight
+  constexpr bool Q8 = PtCfg<D, KIND, 0>::Q8, ROWS = PtCfg<D, KIND, 0>::ROWS;
+  constexpr int E = D / 32, ES = Q8 ? 1 : 2, BYTES = E * ES, U = 16;       // channels and bytes of a lane, keys in flight
   typedef typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type Raw;
   const int lane = threadIdx.x & 31, own = lane & (U - 1);
   float qv[E], o[E];
@@ -247,14 +253,14 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
     uint32_t w;
     if constexpr (BYTES == 8) w = e < 2 ? x.x : x.y;
     else w = x;
-    if constexpr (KIND == KCH_BF16) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+    if constexpr (!Q8) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
     const uint8_t code = (uint8_t)(w >> (8 * e));
     if constexpr (KIND == KCH_INT8) return (float)(int8_t)code;
     __nv_fp8_e4m3 v;
     v.__x = code;
     return float(v);
   };
-  auto ask = [&](int j0) { return j0 < to ? pg_page(a.bt, b, min(j0 + own, to - 1) >> a.bt.shift) : -1; };
+  auto ask = [&](int j0) { return ROWS ? 0 : j0 < to ? pg_page(a.bt, b, min(j0 + own, to - 1) >> a.bt.shift) : -1; };
   int page = ask(from);
 #pragma unroll 1
   for (int j0 = from; j0 < to; j0 += U) {
@@ -263,15 +269,21 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int h, const 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int pg = __shfl_sync(0xffffffffu, page, u), j = min(j0 + u, to - 1);
-      const int64_t at = ((((int64_t)max(pg, 0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * 32 + lane) * BYTES;
+      int64_t at_k, at_v;
+      if constexpr (ROWS) {
+        at_k = ((row0 + j) * a.ld_k + h * D) * 2 + lane * BYTES;
+        at_v = ((row0 + j) * a.ld_v + h * D) * 2 + lane * BYTES;
+      } else {
+        at_k = at_v = ((((int64_t)max(pg, 0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * 32 + lane) * BYTES;
+      }
       k[u] = v[u] = Raw{};                               // (a page that is missing: zeros)
       if (pg >= 0) {
-        k[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.k + at));
-        v[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.v + at));
+        k[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.k + at_k));
+        v[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.v + at_v));
       }
     }
     float ks = 1.f, vs = 1.f;
-    if (KIND != KCH_BF16 && page >= 0) {
+    if (Q8 && page >= 0) {
       const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (min(j0 + own, to - 1) & (a.page - 1));
       ks = __ldg(a.ks + row);
       vs = __ldg(a.vs + row);
@@ -378,7 +390,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         // the page of this lane's box of a tile, asked for a tile ahead; -1 where it is not needed
         auto ask = [&](int tile) -> int {
           const int key = w.x.first_key + tile * PT_KT + mybox * box;
-          return tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
+          return !C::ROWS && tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
         };
         auto copy = [&](int tile, bool v, int id) {
           const int st = g % N, key = w.x.first_key + tile * PT_KT + mybox * box;
@@ -391,7 +403,10 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           if (!fine) return false;
           if (lane == 0) mbarrier_expect_tx(fb + st, C::Q8 ? C::RAW : C::TILE);
           __syncwarp();
-          if (mine) {
+          if (C::ROWS && mine) {
+            // (a tile of which no row sees a key: zeros.  The rows behind a sequence's end are the next one's: masked, their values cleared below.)
+            pt_tma_3d(sm.kv[st] + mypanel * (PT_KT * 128), v ? &vmap : &kmap, mypanel * 64, w.h, needed(tile, key) ? w.s.row0 + key : a.bt.N, fb + st);
+          } else if (mine) {
             if ((unsigned)id >= (unsigned)a.bt.num_pages) {            // out of range: zeros
               if (needed(tile, key)) pg_bad(a.bt);
               id = (int)a.bt.num_pages;
@@ -750,7 +765,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
         const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
         const int2 k = pg_sees(a.bt, w.s, rr);
-        pt_slow_row<D, KIND>(a, w.b, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (w.h * G + rr - tk * G) * D, max(k.x, part0),
+        pt_slow_row<D, KIND>(a, w.b, w.s.row0, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (w.h * G + rr - tk * G) * D, max(k.x, part0),
                              min(k.y, part1), a.scale < 0.f ? -sc : sc, shift, f, out_row(i), direct ? nullptr : slot + (int64_t)i * D, c0, c1);
       };
       // The parts of a row: its O_0 and O_1 with weights w0, w1 where the warpgroups had other tiles of the same rows (each then
@@ -937,6 +952,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 // ---- host -------------------------------------------------------------------------------------------------------------------
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
                               uint32_t box_rows);
+int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_rows);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16 && (c == 64 || c == 128); }
 
@@ -957,6 +973,12 @@ static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAtten
 
 int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s) {
   CUtensorMap km, vm;
+  if (kind == PG_ROWS) {
+    int rc = kch_make_tensor_map_rows(&km, a.k, a.bt.N, a.bt.n_kv, a.ld_k, a.c, PT_KT);
+    if (rc == KCH_OK) rc = kch_make_tensor_map_rows(&vm, a.v, a.bt.N, a.bt.n_kv, a.ld_v, a.c, PT_KT);
+    if (rc != KCH_OK) return rc;
+    return a.c == 64 ? pt_launch<64, PG_ROWS, 0>(km, vm, a, ctas, s) : pt_launch<128, PG_ROWS, 0>(km, vm, a, ctas, s);
+  }
   const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT;
   int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
   if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);

@@ -105,6 +105,18 @@ class PagedAttendArgs(C.Structure):
                 ("workspace", _vp), ("workspace_bytes", _i64)]
 
 
+class PromptAttendArgs(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("ld_q", _i64), ("ld_k", _i64), ("ld_v", _i64), ("cu_seqlens", _vp), ("B", _i), ("N", _i64),
+                ("dtype", _i), ("nh", _i), ("n_kv", _i), ("c", _i), ("scale", _f), ("sliding_window", _i), ("sink", _vp), ("sink_dtype", _i),
+                ("out", _vp), ("zero_rest", _i), ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("ld_q", _i64), ("ld_k", _i64), ("ld_q_out", _i64), ("ld_k_out", _i64),
+                ("N", _i64), ("nh", _i), ("n_kv", _i), ("c", _i), ("dtype", _i), ("positions", _vp), ("ld_positions", _i64), ("axes", _i),
+                ("sections", _i * 4), ("turns", _vp), ("rotary_dim", _i), ("neighbours", _i), ("inverse", _i)]
+
+
 # indices into a cache's device counters (include/kch_b200.h KCH_CTR_*)
 CTR_ACC_LEN, CTR_N_BLOCKS, CTR_RING_N, CTR_HAS_PREV, CTR_TOKENS, CTR_ARRIVALS, CTR_WORDS = 0, 1, 2, 3, 4, 5, 8
 STATUS_CACHE_CAPACITY = 64
@@ -167,6 +179,9 @@ PROTOTYPES = {
     "kch_paged_read": (_i, [C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _i64, _vp, _i64, _i, _i, _vp]),
     "kch_paged_attend_workspace_bytes": (_i64, [C.POINTER(PagedAttendArgs)]),
     "kch_paged_attend": (_i, [C.POINTER(PagedAttendArgs), _vp]),
+    "kch_prompt_attend_workspace_bytes": (_i64, [C.POINTER(PromptAttendArgs)]),
+    "kch_prompt_attend": (_i, [C.POINTER(PromptAttendArgs), _vp]),
+    "kch_rotary": (_i, [C.POINTER(RotaryArgs), _vp]),
     "kch_cache_append_prompt_workspace_bytes": (_i64, [C.POINTER(CacheAppendArgs), _i64]),
     "kch_cache_append_prompt": (_i, [C.POINTER(CacheAppendArgs), _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "kch_csa_layer_workspace_bytes": (_i64, [C.POINTER(CsaLayerArgs)]),
