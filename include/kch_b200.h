@@ -7,7 +7,7 @@
  *    no state between calls other than a cache of TMA descriptors and one device status word.
  *  - `stream` is a cudaStream_t passed as void*.  Calls are asynchronous on that stream.
  *  - dtype tags: KCH_F32, KCH_BF16 for activations / weights; KCH_FP8_E4M3, KCH_INT8 only for
- *    block-scaled compressed rows (one fp32 scale per 64 elements).
+ *    block-scaled compressed rows (one fp32 scale per 64 elements) and pages, KCH_INT4 only for pages.
  *  - Return value: KCH_OK (0); KCH_ERR_INVALID (<0) for a rejected argument — the message
  *    (kch_last_error) names the offending parameter the way the reference's ValueError does;
  *    KCH_ERR_CUDA (>0) for a CUDA failure.  Device-side bounded waits that expire set a status word
@@ -31,6 +31,7 @@ extern "C" {
 #define KCH_BF16 1
 #define KCH_FP8_E4M3 2
 #define KCH_INT8 3
+#define KCH_INT4 4
 
 #define KCH_ACT_SILU 1
 #define KCH_ACT_SIGMOID 2
@@ -417,10 +418,12 @@ int kch_quantize_rows(const void* x, int64_t ld, void* payload, float* scales, f
 /* No counterpart in the reference, whose caches hold one batch in lock step.  Keys and values of many sequences in a pool of
  * pages: k, v [num_pages, n_kv, page_size, c], 16-byte aligned, in the activations' type (`kind` = KCH_F32 / KCH_BF16) or in
  * 8 bits (KCH_FP8_E4M3, KCH_INT8) with one fp32 scale a row, [num_pages, n_kv, page_size].  c: a multiple of 8 up to 256;
- * page_size: a power of two from 8 to 256. */
+ * page_size: a power of two from 8 to 256.  KCH_INT4: k, v [num_pages, n_kv, page_size, c / 2] bytes of two channels, the even one in the
+ * low half, as code + 8; a bf16 scale for 32 channels, [num_pages, n_kv, page_size, c / 32], of 5 significant bits, up to 2^122 or NaN
+ * (kch_paged_append writes no others; of a scale with more bits the attention's products are rounded once more); c a multiple of 32. */
 typedef struct kch_paged_cache {
   void *k, *v;
-  float *k_scales, *v_scales;  /* 8-bit kinds only */
+  void *k_scales, *v_scales;   /* float *; KCH_INT4: bf16 */
   int kind;
   int64_t num_pages;
   int page_size, n_kv, c;
@@ -445,7 +448,9 @@ typedef struct kch_paged_batch {
 
 /* Writes the packed rows k, v [N, n_kv, c] (tokens ld_k / ld_v elements apart) into their pages.  8-bit kinds: s = max |x| / 448
  * (e4m3) or / 127 (int8) over the row of a key head, 1 for a row of zeros; stored round(x / s), ties to even.  A row that is not
- * finite gets the scale NaN and reads back as NaN; codes of NaN are never written (but read as what they are).  What a position that occurs twice in a batch holds is undefined. */
+ * finite gets the scale NaN and reads back as NaN; codes of NaN are never written (but read as what they are).  KCH_INT4: s is the smallest
+ * number of 5 significant bits (2^-126 at least) with 7 s >= max |x| over 32 channels, 1 for zeros; stored round(x / s) + 8, ties to even; 32
+ * channels that are not finite, or of which one is above 7 * 2^122, read back as NaN.  What a position that occurs twice in a batch holds is undefined. */
 int kch_paged_append(const kch_paged_cache* cache, const kch_paged_batch* batch, const void* k, int64_t ld_k, const void* v,
                      int64_t ld_v, int dtype, void* stream);
 /* Reads the rows of those positions back as packed rows in `dtype`: stored value times scale, rounded once.  Rows of no sequence:

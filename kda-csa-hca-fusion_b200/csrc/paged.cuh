@@ -286,7 +286,7 @@ int kch_paged_join(const PgJoinArgs& a, int ctas, cudaStream_t s);
 
 struct PgAttend {                      // what both attention kernels get
   PgBatch bt;
-  const void *q, *k, *v; const float *ks, *vs;
+  const void *q, *k, *v, *ks, *vs;      // (ks, vs: scales; float, in 4 bits bf16)
   void* out;
   int64_t ld_q, ld_k, ld_v;             // (ld_k, ld_v: of packed rows)
   int c, page, zero_rest, slot_rows;

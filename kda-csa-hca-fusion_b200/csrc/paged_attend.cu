@@ -58,6 +58,21 @@ struct PgStored {
   }
 };
 
+// 8 values in 4 bits: a word
+struct PgInt4 { uint8_t two; };
+template <>
+struct PgStored<PgInt4> {
+  uint32_t w;
+  __device__ __forceinline__ void load(const void* base, int64_t i) { w = __ldg((const uint32_t*)((const uint8_t*)base + i / 2)); }
+  __device__ __forceinline__ void none() { w = 0x88888888u; }
+  __device__ __forceinline__ float value(int e) const { return (float)((int)((w >> (4 * e)) & 15u) - 8); }
+  __device__ __forceinline__ void put(float* to, float f) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      reinterpret_cast<float4*>(to)[k] = make_float4(value(4 * k) * f, value(4 * k + 1) * f, value(4 * k + 2) * f, value(4 * k + 3) * f);
+  }
+};
+
 // a weight of -0: nothing is seen there (a weight that is merely too small is 0, and 0 times a NaN is one)
 __device__ __forceinline__ bool pa_none(float weight) { return __float_as_uint(weight) == 0x80000000u; }
 
@@ -127,7 +142,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
             const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));
             kw[k].load(a.k, row * c + d);
             vw[k].load(a.v, row * c + d);
-            if (sizeof(P) == 1) { fk[k] = __ldg(a.ks + row); fv[k] = __ldg(a.vs + row); }
+            if constexpr (std::is_same<P, PgInt4>::value) {
+              fk[k] = __bfloat162float(((const bf16*)a.ks)[row * (c / 32) + d / 32]);
+              fv[k] = __bfloat162float(((const bf16*)a.vs)[row * (c / 32) + d / 32]);
+            } else if constexpr (sizeof(P) == 1) {
+              fk[k] = __ldg((const float*)a.ks + row);
+              fv[k] = __ldg((const float*)a.vs + row);
+            }
           }
         }
       }
@@ -500,6 +521,7 @@ static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   const int64_t rows = N * G;                            // of a key head
   if (!kch_paged_attend_tc5_supported(dtype, c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
   else if (rows > 32 * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
+  else if (kind == KCH_INT4) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
   else if (kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
@@ -542,6 +564,7 @@ static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, 
   } while (0)
   if (kind == KCH_FP8_E4M3) { if (dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
   else if (kind == KCH_INT8) { if (dtype == KCH_F32) PA_ROWS(float, int8_t); else PA_ROWS(bf16, int8_t); }
+  else if (kind == KCH_INT4) { if (dtype == KCH_F32) PA_ROWS(float, PgInt4); else PA_ROWS(bf16, PgInt4); }
   else if (dtype == KCH_F32) PA_ROWS(float, float);
   else PA_ROWS(bf16, bf16);
   KCH_LAUNCH_OK();

@@ -198,7 +198,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const int r0 = key & (a.page - 1);
         if (scales) {
           if (there)
-            bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (values ? a.vs : a.ks) + ((int64_t)id * n_kv + w.h) * a.page + r0, box * 4,
+            bulk_copy_g2s((values ? sm.vs[st] : sm.ks[st]) + lane * box, (const float*)(values ? a.vs : a.ks) + ((int64_t)id * n_kv + w.h) * a.page + r0, box * 4,
                           &sm.full[st]);
         } else if (mine) {
           pm_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * D, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
@@ -486,7 +486,7 @@ paged_attend_mma_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
-                              uint32_t box_rows);
+                              uint32_t box_rows, bool plain = false);
 
 template <int D, int KIND, int R>
 static int pm_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {

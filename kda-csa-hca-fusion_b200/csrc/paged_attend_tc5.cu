@@ -59,17 +59,19 @@
 template <int D, int KIND, int FEW>
 struct PtCfg {
   static constexpr int R = FEW ? FEW : 256, TWO = FEW ? FEW : 128, COPIES = FEW ? 128 / FEW : 1;
-  static constexpr bool Q8 = KIND == KCH_FP8_E4M3 || KIND == KCH_INT8, ROWS = KIND == PG_ROWS;
-  static constexpr bool APART = FEW && !Q8;              // keys' and values' pages are copied by a warp each
-  static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = PT_KT * D;
-  static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8), RAWS = Q8 ? (D == 128 ? 3 : 6) : 0;
+  static constexpr bool ROWS = KIND == PG_ROWS, Q4 = KIND == KCH_INT4, Q8 = KIND == KCH_FP8_E4M3 || KIND == KCH_INT8;
+  static constexpr bool CODES = Q8 || Q4;                // pages hold codes, which a warpgroup turns into tiles
+  static constexpr bool APART = FEW && !CODES;           // keys' and values' pages are copied by a warp each
+  static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = Q4 ? PT_KT * D / 2 : PT_KT * D, GROUPS = D / 32;      // (GROUPS: scales of a row, Q4)
+  static constexpr int RAW_ALL = RAW + (Q4 ? PT_KT * GROUPS * 2 : 0);      // with 4 bits' scales behind them
+  static constexpr int STAGES = Q8 ? (D == 128 ? 3 : 6) : Q4 ? (D == 128 ? 4 : 7) : (D == 128 ? 5 : 8), RAWS = CODES ? (D == 128 ? 3 : 6) : 0;
   // of 4 pairs: how many powers are FMAs' and not the special-function unit's
-  static constexpr int POLY = D == 64 && !FEW && !Q8 ? 1 : 0;
+  static constexpr int POLY = D == 64 && !FEW && !CODES ? 1 : 0;
   static constexpr int SCALES = 4;                       // key tiles whose scales are held
-  static constexpr int THREADS = Q8 ? 512 : 384;         // 8-bit pages: a warpgroup that turns them into tiles
+  static constexpr int THREADS = CODES ? 512 : 384;
   // registers of the warpgroups, and of a thread at launch
-  static constexpr int REG_FEED = Q8 ? 80 : 88, REG_SOFT = Q8 ? 168 : 208, REG_CONV = 88, REG_LAUNCH = 65536 / THREADS / 8 * 8;
-  static_assert(128 * (REG_FEED + 2 * REG_SOFT + (Q8 ? REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
+  static constexpr int REG_FEED = CODES ? 80 : 88, REG_SOFT = CODES ? 168 : 208, REG_CONV = 88, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(128 * (REG_FEED + 2 * REG_SOFT + (CODES ? REG_CONV : 0)) <= THREADS * REG_LAUNCH, "register split");
 };
 
 // 32 bytes of a row.  (The lanes' rows are as many lines, one a cycle: half of 16 bytes' stores.)
@@ -88,7 +90,7 @@ struct PtSmem {
   typedef PtCfg<D, KIND, FEW> C;
   alignas(1024) uint8_t q[2][128 * D * 2];
   alignas(1024) uint8_t kv[C::STAGES][C::TILE];
-  alignas(C::Q8 ? 1024 : 16) uint8_t raw[C::RAWS ? C::RAWS : 1][C::RAWS ? C::RAW : 16];
+  alignas(C::CODES ? 1024 : 16) uint8_t raw[C::RAWS ? C::RAWS : 1][C::RAWS ? C::RAW_ALL : 16];
   alignas(16) float scale[C::Q8 ? C::SCALES : 1][2][C::Q8 ? PT_KT : 4];
   float ml[2][256];                                      // maxima and sums of the parts of an item's keys
   float factor[2][32];                                   // of its rows: 1 / the denominator
@@ -100,7 +102,7 @@ struct PtSmem {
   uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
-static_assert(sizeof(PtSmem<128, KCH_BF16, 0>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, 0>) <= 232448, "shared memory of the paged attention");
+static_assert(sizeof(PtSmem<128, KCH_BF16, 0>) <= 232448 && sizeof(PtSmem<128, KCH_INT8, 0>) <= 232448 && sizeof(PtSmem<128, KCH_INT4, 0>) <= 232448, "shared memory of the paged attention");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 4 * 16384, "the plan lies in the ring of tiles");
 
 __device__ __forceinline__ void pt_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -215,6 +217,16 @@ __device__ __forceinline__ void pt_codes4(uint32_t w, uint32_t& lo, uint32_t& hi
   }
 }
 
+// 8 channels in bf16 from a word of 4-bit codes, times their scale: the code's place in the mantissa of 16 makes 16 + u of it, and
+// (16 + u) s - 24 s = (u - 8) s has at most 8 bits where s has 5: exact.  s, s24: pairs of the scale and -24 times it.
+__device__ __forceinline__ void pt_nibbles8(uint32_t w, uint32_t s, uint32_t s24, uint4& x) {
+  const uint32_t even = w << 3, odd = w >> 1;            // (of each byte the lower and the upper code, in its bits 3 .. 6)
+  x.x = pt_bf16_fma((__byte_perm(even, odd, 0x4400) & 0x00780078u) | 0x41804180u, s, s24);
+  x.y = pt_bf16_fma((__byte_perm(even, odd, 0x5511) & 0x00780078u) | 0x41804180u, s, s24);
+  x.z = pt_bf16_fma((__byte_perm(even, odd, 0x6622) & 0x00780078u) | 0x41804180u, s, s24);
+  x.w = pt_bf16_fma((__byte_perm(even, odd, 0x7733) & 0x00780078u) | 0x41804180u, s, s24);
+}
+
 // Is there a code of NaN (0x7F, 0xFF) among the keys [from, to) of a sequence, or their values?  A warp's.
 template <int D>
 __device__ __noinline__ bool pt_nan_among(const PgAttend& a, int b, int h, int from, int to) {
@@ -236,15 +248,18 @@ __device__ __noinline__ bool pt_nan_among(const PgAttend& a, int b, int h, int f
 }
 
 // One row on one warp over the keys [from, to), reading only those: sum_j round(p_j) v_j, p_j = 2^(s_j sc - shift); columns
-// c0 .. c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).  16 keys at a time, a lane with D / 32 channels of each; their pages
-// are asked for 16 keys ahead, and the sums of the lanes are halved over and over until lane l has that of key l mod 16: 0.15 us a key on
+// c0 .. c1 of it go to `dst` (fp32, a part) or `out` (times f, rounded).  16 keys at a time (4 bits, whose scales take
+// registers too: 8), a lane with D / 32 channels of each; their pages are asked for as many keys ahead, and the sums of the lanes are halved
+// over and over until lane l has that of key l mod 16: 0.15 us a key on
 // all warps.  (With each key's page asked for where it is needed, and a sum of its own, 0.5 us.)
 template <int D, int KIND>
 __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int h, const bf16* q, int from, int to, float sc, float shift,
                                          float f, bf16* out, float* dst, int c0, int c1) {
-  constexpr bool Q8 = PtCfg<D, KIND, 0>::Q8, ROWS = PtCfg<D, KIND, 0>::ROWS;
-  constexpr int E = D / 32, ES = Q8 ? 1 : 2, BYTES = E * ES, U = 16;       // channels and bytes of a lane, keys in flight
-  typedef typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type Raw;
+  typedef PtCfg<D, KIND, 0> C;
+  constexpr bool Q8 = C::Q8, Q4 = C::Q4, ROWS = C::ROWS;
+  constexpr int E = D / 32, BYTES = Q4 ? E / 2 : Q8 ? E : 2 * E, U = Q4 ? 8 : 16;      // channels and bytes of a lane, keys in flight
+  typedef typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t,
+          typename std::conditional<BYTES == 2, uint16_t, uint8_t>::type>::type>::type Raw;
   const int lane = threadIdx.x & 31, own = lane & (U - 1);
   float qv[E], o[E];
 #pragma unroll
@@ -253,7 +268,8 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
     uint32_t w;
     if constexpr (BYTES == 8) w = e < 2 ? x.x : x.y;
     else w = x;
-    if constexpr (!Q8) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+    if constexpr (Q4) return (float)((int)(w >> (4 * e) & 15u) - 8);
+    if constexpr (!C::CODES) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
     const uint8_t code = (uint8_t)(w >> (8 * e));
     if constexpr (KIND == KCH_INT8) return (float)(int8_t)code;
     __nv_fp8_e4m3 v;
@@ -266,6 +282,7 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
   for (int j0 = from; j0 < to; j0 += U) {
     const int next = ask(j0 + U);
     Raw k[U], v[U];
+    uint32_t sf[Q4 ? U : 1];                             // 4 bits: the scales of the lane's channels, the key's and the value's
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int pg = __shfl_sync(0xffffffffu, page, u), j = min(j0 + u, to - 1);
@@ -276,6 +293,13 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
       } else {
         at_k = at_v = ((((int64_t)max(pg, 0) * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * 32 + lane) * BYTES;
       }
+      if constexpr (Q4) {
+        sf[u] = 0u;
+        if (pg >= 0) {
+          const int64_t at = (((int64_t)pg * a.bt.n_kv + h) * a.page + (j & (a.page - 1))) * C::GROUPS + lane * E / 32;
+          sf[u] = __ldg((const uint16_t*)a.ks + at) | (uint32_t)__ldg((const uint16_t*)a.vs + at) << 16;
+        }
+      }
       k[u] = v[u] = Raw{};                               // (a page that is missing: zeros)
       if (pg >= 0) {
         k[u] = __ldg(reinterpret_cast<const Raw*>((const uint8_t*)a.k + at_k));
@@ -285,15 +309,15 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
     float ks = 1.f, vs = 1.f;
     if (Q8 && page >= 0) {
       const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (min(j0 + own, to - 1) & (a.page - 1));
-      ks = __ldg(a.ks + row);
-      vs = __ldg(a.vs + row);
+      ks = __ldg((const float*)a.ks + row);
+      vs = __ldg((const float*)a.vs + row);
     }
     float s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       s[u] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[u] = fmaf(qv[e], value(k[u], e), s[u]);
+      for (int e = 0; e < E; ++e) s[u] = fmaf(qv[e], Q4 ? value(k[u], e) * __uint_as_float(sf[Q4 ? u : 0] << 16) : value(k[u], e), s[u]);
     }
 #pragma unroll
     for (int n = U / 2; n > 0; n >>= 1) {
@@ -303,14 +327,15 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
         s[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
       }
     }
-    s[0] += __shfl_xor_sync(0xffffffffu, s[0], 16);
+#pragma unroll
+    for (int n = U; n < 32; n <<= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], n);
     const float p = round_to<bf16>(ex2_fast(fmaf(s[0] * ks, sc, -shift)) * vs);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float pu = __shfl_sync(0xffffffffu, p, u);
       if (j0 + u < to) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(pu, value(v[u], e), o[e]);
+        for (int e = 0; e < E; ++e) o[e] = fmaf(pu, Q4 ? value(v[u], e) * __uint_as_float(sf[Q4 ? u : 0] & 0xFFFF0000u) : value(v[u], e), o[e]);
       }
     }
     page = next;
@@ -336,7 +361,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::Q8 ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
+    for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::CODES ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
     mbarrier_init(&sm.q_full, C::APART ? 1 : 2);
@@ -374,11 +399,11 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // that a prompt of 8192 tokens was 6 % slower).
       // A warp that comes to fill a place of the ring has filled one at most three places back, so everything N before that has
       // been used, and a barrier's parity cannot be that of two uses ago.
-      const int box = min(a.page, PT_KT), boxes = PT_KT / box, panels = C::Q8 ? 1 : C::PANELS;
+      const int box = min(a.page, PT_KT), boxes = PT_KT / box, panels = C::CODES ? 1 : C::PANELS;
       const int mybox = lane / panels, mypanel = lane % panels;
       const bool mine = lane < boxes * panels;
-      constexpr int N = C::Q8 ? C::RAWS : C::STAGES;
-      uint64_t *fb = C::Q8 ? sm.raw_full : sm.full, *eb = C::Q8 ? sm.raw_empty : sm.empty;
+      constexpr int N = C::CODES ? C::RAWS : C::STAGES;
+      uint64_t *fb = C::CODES ? sm.raw_full : sm.full, *eb = C::CODES ? sm.raw_empty : sm.empty;
       int g = 0;
       bool ok = true;
       for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
@@ -401,17 +426,33 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           bool fine = g < N || wait(eb + st, g / N - 1);
           fine = __all_sync(0xffffffffu, fine);
           if (!fine) return false;
-          if (lane == 0) mbarrier_expect_tx(fb + st, C::Q8 ? C::RAW : C::TILE);
+          const bool there = mine && (unsigned)id < (unsigned)a.bt.num_pages;
+          uint8_t* scales = sm.raw[C::Q4 ? st : 0] + C::RAW + mybox * box * (2 * C::GROUPS);      // 4 bits: of this lane's box
+          uint32_t bytes = C::CODES ? C::RAW : C::TILE;
+          if constexpr (C::Q4) {
+            bytes += __popc(__ballot_sync(0xffffffffu, there)) * box * (2 * C::GROUPS);
+            if (mine && !there) {                        // zeros, by hand
+              for (int i = 0; i < box * (2 * C::GROUPS); i += 16) *reinterpret_cast<uint4*>(scales + i) = make_uint4(0u, 0u, 0u, 0u);
+              t5_fence_async_smem();                     // (a copy writes there next)
+            }
+            __syncwarp();
+          }
+          if (lane == 0) mbarrier_expect_tx(fb + st, bytes);
           __syncwarp();
           if (C::ROWS && mine) {
             // (a tile of which no row sees a key: zeros.  The rows behind a sequence's end are the next one's: masked, their values cleared below.)
             pt_tma_3d(sm.kv[st] + mypanel * (PT_KT * 128), v ? &vmap : &kmap, mypanel * 64, w.h, needed(tile, key) ? w.s.row0 + key : a.bt.N, fb + st);
           } else if (mine) {
-            if ((unsigned)id >= (unsigned)a.bt.num_pages) {            // out of range: zeros
+            if (!there) {                                // out of range: zeros
               if (needed(tile, key)) pg_bad(a.bt);
               id = (int)a.bt.num_pages;
             }
-            uint8_t* dst = C::Q8 ? sm.raw[C::Q8 ? st : 0] + mybox * box * D : sm.kv[C::Q8 ? 0 : st] + mypanel * (PT_KT * 128) + mybox * box * 128;
+            if constexpr (C::Q4)
+              if (there)
+                bulk_copy_g2s(scales, (const bf16*)(v ? a.vs : a.ks) + (((int64_t)id * n_kv + w.h) * a.page + (key & (a.page - 1))) * C::GROUPS,
+                              box * (2 * C::GROUPS), fb + st);
+            uint8_t* dst = C::CODES ? sm.raw[C::CODES ? st : 0] + mybox * box * (C::RAW / PT_KT)
+                                    : sm.kv[C::CODES ? 0 : st] + mypanel * (PT_KT * 128) + mybox * box * 128;
             pt_tma_4d(dst, v ? &vmap : &kmap, mypanel * 64, key & (a.page - 1), w.h, id, fb + st);
           }
           ++g;
@@ -438,8 +479,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         }
       }
       // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones)
-      for (int i = 1, n = C::Q8 ? C::RAWS : C::STAGES; i <= n && i <= g; ++i)
-        wait(C::Q8 ? &sm.raw_full[C::Q8 ? (g - i) % n : 0] : &sm.full[C::Q8 ? 0 : (g - i) % n], (g - i) / n);
+      for (int i = 1, n = C::CODES ? C::RAWS : C::STAGES; i <= n && i <= g; ++i)
+        wait(C::CODES ? &sm.raw_full[C::CODES ? (g - i) % n : 0] : &sm.full[C::CODES ? 0 : (g - i) % n], (g - i) / n);
     } else if (warp == 1) {
       // ------------------------------ MMA issuer --------------------------------------------------------------------------
       if (t5_elect()) {
@@ -562,9 +603,9 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               const int64_t at = there ? ((int64_t)id * n_kv + w.h) * a.page + (key & (a.page - 1)) : 0;
               const int bytes = there ? 4 : 0;           // (none: 4 bytes of zeros)
               asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-                           ::"r"(smem_addr_u32(&sm.scale[slot][0][t + 64 * i])), "l"(a.ks + at), "r"(bytes) : "memory");
+                           ::"r"(smem_addr_u32(&sm.scale[slot][0][t + 64 * i])), "l"((const float*)a.ks + at), "r"(bytes) : "memory");
               asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-                           ::"r"(smem_addr_u32(&sm.scale[slot][1][t + 64 * i])), "l"(a.vs + at), "r"(bytes) : "memory");
+                           ::"r"(smem_addr_u32(&sm.scale[slot][1][t + 64 * i])), "l"((const float*)a.vs + at), "r"(bytes) : "memory");
             }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr_u32(&sm.sc_full[slot])) : "memory");
             id0 = n0;
@@ -722,8 +763,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           pt_unpack(sum2, la, lb);
           l += la + lb;
         }
-        if (!C::Q8 && w.s.kv > key0 && w.s.kv < key0 + PT_KT) {
-          // (payloads of 8 bits are numbers by now, and the scales there are 0)
+        if (!C::CODES && w.s.kv > key0 && w.s.kv < key0 + PT_KT) {
+          // (codes are numbers by now, or the scales there are 0)
           const int at = pair ? ring + 1 + 2 * s : ring + 2 + 4 * s + (s + 1 < w.count ? 2 : 1) * x;      // of the tile's values in the ring
           if (ok) ok = wait(&sm.full[at % C::STAGES], at / C::STAGES);
           ok = __all_sync(0xffffffffu, ok);
@@ -894,44 +935,72 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
     if (tid == 128 && !part) a.records[blockIdx.x].valid = 0;
   } else {
-    // ------------------------------ 8-bit pages: payloads to bf16 tiles, scales ------------------------------------------------
-    if constexpr (C::Q8) {
+    // ------------------------------ codes to bf16 tiles ------------------------------------------------------------------------
+    if constexpr (C::CODES) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_CONV));
       const int t = tid - 384;
       bool ok = true;
       int g = 0;
       for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
-        const int tiles = 2 * w.count * (paired(w) ? 1 : 2);       // of keys and values
+        const bool pair = paired(w);
+        const int tiles = 2 * w.count * (pair ? 1 : 2);            // of keys and values
         for (int i = 0; i < tiles && ok; ++i, ++g) {
           ok = wait(&sm.raw_full[g % C::RAWS], g / C::RAWS);
           if (ok && g >= C::STAGES) ok = wait(&sm.empty[g % C::STAGES], g / C::STAGES - 1);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          // 16 codes each: 2 words of a tile's row, 4 such pieces a row and panel.  8 threads that meet in the banks have 4 pieces of
-          // two rows: one of an even and one of an odd number (whose words lie apart in the tile), and where the codes are
-          // swizzled too, numbers that differ in bit 2 as well (5 = 101b: their pieces lie apart there).  A thread's place in
-          // both swizzles is the same in every round.
-          constexpr int ROWS = D == 128 ? 16 : 32, ROUNDS = PT_KT / ROWS;      // rows between two rounds
-          const int k = lane & 3, wq = t >> 5;
-          const int row = D == 128 ? (wq >> 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : wq * 8 + (lane >> 2), panel = D == 128 ? wq & 1 : 0;
-          const uint8_t* src = sm.raw[g % C::RAWS] + row * D + ((D == 128 ? (panel * 4 + k) ^ (row & 7) : k ^ ((row >> 1) & 3)) << 4);
-          uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
-          uint32_t most = 0u;
-          uint8_t *to0 = line + (((2 * k) ^ (row & 7)) << 4), *to1 = line + (((2 * k + 1) ^ (row & 7)) << 4);
+          if constexpr (C::Q4) {
+            // 32 codes and their scale a thread, a quarter (half) of a row: a warp reads 512 bytes in a row.  The words of 8 channels go to
+            // their places two and two about in the second panel, so that 8 threads meet in no bank.  Keys that no row sees, and
+            // what lies behind the sequence's end, are zeros (a scale there may be NaN).
+            const int piece = t % C::GROUPS, panel = piece >> 1, turn = D == 128 ? 2 * panel : 0;
+            const int turns = (i - 2) / 4, rest = (i - 2) % 4;
+            const int tile = pair ? w.first + i / 2
+                                  : 2 * w.first + (i < 2 ? i : turns == w.count - 1 ? 2 * turns + rest : 2 * turns + (rest & 1) * 2 + (rest >> 1));
+            const int key0 = w.x.first_key + tile * PT_KT;
+#pragma unroll 1
+            for (int row = t / C::GROUPS; row < PT_KT; row += 128 / C::GROUPS) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sm.raw[g % C::RAWS] + row * (D / 2) + piece * 16);
+              uint32_t s = *reinterpret_cast<const uint16_t*>(sm.raw[g % C::RAWS] + C::RAW + (row * C::GROUPS + piece) * 2);
+              const int key = key0 + row;
+              s = key >= w.x.lo && key < w.s.kv ? s | s << 16 : 0u;
+              const uint32_t s24 = pt_bf16_fma(s, 0xC1C0C1C0u, 0u);      // -24 s
+              uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
+              const uint32_t w4[4] = {turn ? u.z : u.x, turn ? u.w : u.y, turn ? u.x : u.z, turn ? u.y : u.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4 x;
+                pt_nibbles8(w4[j], s, s24, x);
+                *reinterpret_cast<uint4*>(line + (((((piece & 1) << 2) + (j ^ turn)) ^ (row & 7)) << 4)) = x;
+              }
+            }
+          } else {
+            // 16 codes each: 2 words of a tile's row, 4 such pieces a row and panel.  8 threads that meet in the banks have 4 pieces of
+            // two rows: one of an even and one of an odd number (whose words lie apart in the tile), and where the codes are
+            // swizzled too, numbers that differ in bit 2 as well (5 = 101b: their pieces lie apart there).  A thread's place in
+            // both swizzles is the same in every round.
+            constexpr int ROWS = D == 128 ? 16 : 32, ROUNDS = PT_KT / ROWS;      // rows between two rounds
+            const int k = lane & 3, wq = t >> 5;
+            const int row = D == 128 ? (wq >> 1) * 8 + ((lane >> 3) ^ ((lane >> 2) & 1) * 5) : wq * 8 + (lane >> 2), panel = D == 128 ? wq & 1 : 0;
+            const uint8_t* src = sm.raw[g % C::RAWS] + row * D + ((D == 128 ? (panel * 4 + k) ^ (row & 7) : k ^ ((row >> 1) & 3)) << 4);
+            uint8_t* line = sm.kv[g % C::STAGES] + panel * (PT_KT * 128) + row * 128;
+            uint32_t most = 0u;
+            uint8_t *to0 = line + (((2 * k) ^ (row & 7)) << 4), *to1 = line + (((2 * k + 1) ^ (row & 7)) << 4);
 #pragma unroll 4
-          for (int n = 0; n < ROUNDS; ++n) {
-            const uint4 u = *reinterpret_cast<const uint4*>(src + n * (ROWS * D));
-            uint4 lo, hi;
-            pt_codes4<KIND>(u.x, lo.x, lo.y, most);
-            pt_codes4<KIND>(u.y, lo.z, lo.w, most);
-            pt_codes4<KIND>(u.z, hi.x, hi.y, most);
-            pt_codes4<KIND>(u.w, hi.z, hi.w, most);
-            *reinterpret_cast<uint4*>(to0 + n * (ROWS * 128)) = lo;
-            *reinterpret_cast<uint4*>(to1 + n * (ROWS * 128)) = hi;
+            for (int n = 0; n < ROUNDS; ++n) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + n * (ROWS * D));
+              uint4 lo, hi;
+              pt_codes4<KIND>(u.x, lo.x, lo.y, most);
+              pt_codes4<KIND>(u.y, lo.z, lo.w, most);
+              pt_codes4<KIND>(u.z, hi.x, hi.y, most);
+              pt_codes4<KIND>(u.w, hi.z, hi.w, most);
+              *reinterpret_cast<uint4*>(to0 + n * (ROWS * 128)) = lo;
+              *reinterpret_cast<uint4*>(to1 + n * (ROWS * 128)) = hi;
+            }
+            // a code of NaN (an append writes none): at the ends of items from here on it is looked for among what the sequences have
+            if (KIND == KCH_FP8_E4M3 && (most >= 0x07F00000u || (most & 0xFFFFu) >= 0x07F0u))
+              *(volatile uint32_t*)&sm.nan_code = 1u;
           }
-          // a code of NaN (an append writes none): at the ends of items from here on it is looked for among what the sequences have
-          if (KIND == KCH_FP8_E4M3 && (most >= 0x07F00000u || (most & 0xFFFFu) >= 0x07F0u))
-            *(volatile uint32_t*)&sm.nan_code = 1u;
           t5_fence_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -951,7 +1020,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
-                              uint32_t box_rows);
+                              uint32_t box_rows, bool plain = false);
 int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_rows);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16 && (c == 64 || c == 128); }
@@ -979,13 +1048,14 @@ int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaSt
     if (rc != KCH_OK) return rc;
     return a.c == 64 ? pt_launch<64, PG_ROWS, 0>(km, vm, a, ctas, s) : pt_launch<128, PG_ROWS, 0>(km, vm, a, ctas, s);
   }
-  const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT;
-  int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
-  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c, box);
+  const bool q4 = kind == KCH_INT4;
+  const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT, wide = q4 ? a.c / 2 : a.c;
+  int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, wide, box, q4);
+  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, wide, box, q4);
   if (rc != KCH_OK) return rc;
 #define PT_GO(D_, K_, F_) pt_launch<D_, K_, F_>(km, vm, a, ctas, s)
 #define PT_KIND(D_)                                                                            \
-  (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, 0) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, 0)  \
+  (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, 0) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, 0) : q4 ? PT_GO(D_, KCH_INT4, 0) \
    : rows == 16 ? PT_GO(D_, KCH_BF16, 16) : rows == 32 ? PT_GO(D_, KCH_BF16, 32) : PT_GO(D_, KCH_BF16, 0))
   return a.c == 64 ? PT_KIND(64) : PT_KIND(128);
 #undef PT_KIND

@@ -15,9 +15,10 @@
 
 int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtype, const char* fn) {
   KCH_REQUIRE(dtype == KCH_F32 || dtype == KCH_BF16, "%s: unsupported dtype tag %d", fn, dtype);
-  KCH_REQUIRE(p->kind == dtype || p->kind == KCH_FP8_E4M3 || p->kind == KCH_INT8,
-              "%s: kind=%d: pages hold the activations' type (%d) or one of the 8-bit kinds", fn, p->kind, dtype);
+  KCH_REQUIRE(p->kind == dtype || p->kind == KCH_FP8_E4M3 || p->kind == KCH_INT8 || p->kind == KCH_INT4,
+              "%s: kind=%d: pages hold the activations' type (%d) or one of the 8- and 4-bit kinds", fn, p->kind, dtype);
   KCH_REQUIRE(p->c >= 8 && p->c <= 256 && p->c % 8 == 0, "%s: c=%d must be a multiple of 8 from 8 to 256", fn, p->c);
+  KCH_REQUIRE(p->kind != KCH_INT4 || p->c % 32 == 0, "%s: c=%d must be a multiple of 32, the channels of a scale in 4 bits", fn, p->c);
   KCH_REQUIRE(p->page_size >= 8 && p->page_size <= 256 && (p->page_size & (p->page_size - 1)) == 0,
               "%s: page_size=%d must be a power of two from 8 to 256", fn, p->page_size);
   KCH_REQUIRE(p->n_kv >= 1, "%s: n_kv=%d must be >= 1", fn, p->n_kv);
@@ -29,7 +30,7 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
   KCH_REQUIRE(b->table && b->t0 && b->cu_seqlens, "%s: null table, t0 or cu_seqlens", fn);
   KCH_REQUIRE(p->k && p->v && (((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0, "%s: pages must be 16-byte aligned", fn);
   KCH_REQUIRE(p->kind < KCH_FP8_E4M3 || (p->k_scales && p->v_scales && (((uintptr_t)p->k_scales | (uintptr_t)p->v_scales) & 15) == 0),
-              "%s: 8-bit pages need their scales, 16-byte aligned", fn);
+              "%s: 8- and 4-bit pages need their scales, 16-byte aligned", fn);
   return KCH_OK;
 }
 
@@ -50,7 +51,7 @@ PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b) {
 struct PgRows {
   PgBatch bt;
   void *x[2]; int64_t ld[2];           // packed rows of k and v, tokens ld elements apart
-  void* pages[2]; float* scales[2];
+  void* pages[2]; void* scales[2];
   int n_kv, c, page, kind, zero_rest;
   int tokens;                          // of a warp at a time: 1 or 2
   int parts;                           // warps that share a token's rows
@@ -83,6 +84,28 @@ __device__ __forceinline__ uint32_t pc_codes2(float x0, float x1, float s, float
   if (a0 != pc_int8(q0 * hi)) a0 = pc_int8(pc_quotient(x0, s));
   if (a1 != pc_int8(q1 * hi)) a1 = pc_int8(pc_quotient(x1, s));
   return ((uint32_t)a0 & 0xFFu) | (((uint32_t)a1 & 0xFFu) << 8);
+}
+
+// 4 bits, of 32 channels (4 threads'): the smallest number of 5 bits, 7 times which is `top` or more (top > 0, as bits; 7 s is exact in 32
+// bits), and the codes of 8 values as a word, the first in its lowest bits.
+#define PC_MOST4 0x7DE00000u           // 7 * 2^122: 24 s, which the attention adds in bf16, stays a number
+__device__ __forceinline__ float pc_scale4(uint32_t top) {
+  const float most = __uint_as_float(top);
+  uint32_t b = (__float_as_uint(most / 7.f) + 0x7FFFFu) & 0xFFF80000u;
+  if (7.f * __uint_as_float(b) < most) b += 0x80000u;    // (the quotient was rounded down onto a number of 5 bits)
+  return fmaxf(__uint_as_float(b), 1.17549435e-38f);
+}
+__device__ __forceinline__ uint32_t pc_codes4(const float (&x)[8], float s) {
+  const float lo = 1.f - 4.76837158203125e-07f, hi = 1.f + 4.76837158203125e-07f, inv = 1.f / s;      // 2^-21
+  uint32_t w = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = x[e] * inv;
+    int code = (int)rintf(q * lo);
+    if (code != (int)rintf(q * hi)) code = (int)rintf(pc_quotient(x[e], s));
+    w |= (uint32_t)(code + 8) << (4 * e);
+  }
+  return w;
 }
 
 // where packed row t lies: its sequence by bisection of cu_seqlens, then page and row.  Rows (page * n_kv * page_size + row) of the
@@ -137,9 +160,9 @@ __device__ __forceinline__ PcWords<T> pc_words(const void* p) {
 
 // A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
 // looked up once a token, and four rows a thread are in flight.  Where tokens are few, several warps share one's rows.  READ: pages
-// -> packed rows, else packed rows -> pages.
+// -> packed rows, else packed rows -> pages.  BITS of what is stored: 8, 4, or 0: the rows as they are.
 #define PC_FLIGHT 4
-template <typename T, int GROUP, bool READ, bool Q8>
+template <typename T, int GROUP, bool READ, int BITS>
 __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_constant__ PgRows a) {
   __shared__ int32_t scu[PC_SMEM_B + 1];
   const int32_t* cu = a.bt.cu;
@@ -159,7 +182,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
     // (k and v of a head one after the other: row 2 h + kv)
     auto packed = [&](int row) { return (T*)a.x[row & 1] + t * a.ld[row & 1] + (int64_t)(row >> 1) * a.c + d; };
     auto pool_row = [&](int row) { return site + (int64_t)(row >> 1) * a.page; };
-    if constexpr (!Q8) {
+    if constexpr (BITS == 0) {
       if ((READ ? t >= a.bt.N : site < 0) || !in_row) continue;
       if (READ && site == -1 && !a.zero_rest) continue;
       for (int r = row0; r < rows; r += step * PC_FLIGHT) {
@@ -178,7 +201,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
           for (int k = 0; k < (int)sizeof(T) / 2; ++k) to[k] = x[i].w[k];
         }
       }
-    } else if constexpr (READ) {
+    } else if constexpr (READ && BITS == 8) {
       if (t >= a.bt.N || !in_row || (site == -1 && !a.zero_rest)) continue;
       for (int r = row0; r < rows; r += step * PC_FLIGHT) {
         uint2 u[PC_FLIGHT] = {};
@@ -189,7 +212,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
           f[i] = 0.f;
           if (row < rows && site >= 0) {
             u[i] = __ldg((const uint2*)((const uint8_t*)a.pages[row & 1] + pool_row(row) * a.c + d));
-            f[i] = __ldg(a.scales[row & 1] + pool_row(row));
+            f[i] = __ldg((const float*)a.scales[row & 1] + pool_row(row));
           }
         }
 #pragma unroll
@@ -204,6 +227,35 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
             __nv_fp8_e4m3 v;
             v.__x = code;
             x[e] = (a.kind == KCH_FP8_E4M3 ? float(v) : (float)(int8_t)code) * f[i];
+          }
+          pc_store(packed(row), x);
+        }
+      }
+    } else if constexpr (READ) {
+      if (t >= a.bt.N || !in_row || (site == -1 && !a.zero_rest)) continue;
+      for (int r = row0; r < rows; r += step * PC_FLIGHT) {
+        uint32_t u[PC_FLIGHT];
+        float f[PC_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          u[i] = 0u;
+          f[i] = 0.f;
+          if (row < rows && site >= 0) {
+            u[i] = __ldg((const uint32_t*)((const uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2));
+            f[i] = __bfloat162float(((const bf16*)a.scales[row & 1])[pool_row(row) * (a.c / 32) + d / 32]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PC_FLIGHT; ++i) {
+          const int row = r + i * step;
+          if (row >= rows) break;
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = (float)((int)((u[i] >> (4 * e)) & 15u) - 8) * f[i];
+          if (site < 0) {                                // (0 * -8 is -0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
           }
           pc_store(packed(row), x);
         }
@@ -225,8 +277,15 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
 #pragma unroll
           for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
 #pragma unroll
-          for (int o = GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int o = BITS == 4 ? 2 : GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           if (!here || row >= rows) continue;
+          if constexpr (BITS == 4) {
+            const bool number = top <= PC_MOST4;         // (what is not reads as NaN)
+            const float s = top && number ? pc_scale4(top) : 1.f;
+            *(uint32_t*)((uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2) = number ? pc_codes4(x[i], s) : 0x88888888u;
+            if (d % 32 == 0) ((uint16_t*)a.scales[row & 1])[pool_row(row) * (a.c / 32) + d / 32] = number ? (uint16_t)(__float_as_uint(s) >> 16) : 0x7FC0u;
+            continue;
+          }
           const bool finite = top < 0x7F800000u;
           float s = top ? fmaxf(__uint_as_float(top) / (a.kind == KCH_FP8_E4M3 ? 448.f : 127.f), 1.17549435e-38f) : 1.f;
           const float inv = 1.f / s;
@@ -236,7 +295,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
             w[e] = finite ? pc_codes2(x[i][4 * e], x[i][4 * e + 1], s, inv, a.kind) | pc_codes2(x[i][4 * e + 2], x[i][4 * e + 3], s, inv, a.kind) << 16 : 0u;
           if (!finite) s = __uint_as_float(0x7FC00000u); // a row that is not finite reads as NaN, whichever the kind
           *(uint2*)((uint8_t*)a.pages[row & 1] + pool_row(row) * a.c + d) = make_uint2(w[0], w[1]);
-          if (d == 0) a.scales[row & 1][pool_row(row)] = s;
+          if (d == 0) ((float*)a.scales[row & 1])[pool_row(row)] = s;
         }
       }
     }
@@ -246,16 +305,16 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
 // 8-bit pages: one wave of blocks, whose warps walk the tokens; more of them would only wait for the others' end (32768 tokens of 8 heads
 // of 128 read from e4m3: 38 us, 42 with 8 to an SM).  Rows that are copied: 8 to an SM, of which it holds 6 (28708 such tokens written
 // as bf16: 41 us, 44 in one wave, where an SM that is behind stays so).
-template <typename T, int GROUP, bool READ, bool Q8>
+template <typename T, int GROUP, bool READ, int BITS>
 static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
   static const int resident = [] {
     int n = 0;
-    if (!Q8) return 8;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, Q8>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
+    if (BITS == 0) return 8;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, BITS>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
   }();
   const int64_t wave = (int64_t)resident * KCH_SMS / a.parts;
   const dim3 grid((unsigned)(blocks < wave ? blocks : wave), (unsigned)a.parts);
-  paged_rows_kernel<T, GROUP, READ, Q8><<<grid, PC_THREADS, 0, s>>>(a);
+  paged_rows_kernel<T, GROUP, READ, BITS><<<grid, PC_THREADS, 0, s>>>(a);
 }
 
 static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k, int64_t ld_k, void* v, int64_t ld_v, int dtype,
@@ -298,8 +357,9 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   } while (0)
 #define PC_KIND(T_)                                                                                                      \
   do {                                                                                                                   \
-    if (p->kind < KCH_FP8_E4M3) PC_WIDTH(T_, false);                                                                     \
-    else PC_WIDTH(T_, true);                                                                                             \
+    if (p->kind < KCH_FP8_E4M3) PC_WIDTH(T_, 0);                                                                         \
+    else if (p->kind == KCH_INT4) PC_WIDTH(T_, 4);                                                                       \
+    else PC_WIDTH(T_, 8);                                                                                                \
   } while (0)
   if (dtype == KCH_BF16) PC_KIND(bf16);
   else PC_KIND(float);

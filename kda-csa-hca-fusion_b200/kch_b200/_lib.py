@@ -10,7 +10,7 @@ import os
 
 import torch
 
-KCH_F32, KCH_BF16, KCH_FP8_E4M3, KCH_INT8 = 0, 1, 2, 3
+KCH_F32, KCH_BF16, KCH_FP8_E4M3, KCH_INT8, KCH_INT4 = 0, 1, 2, 3, 4
 ACT_SILU, ACT_SIGMOID, ACT_NEG_SOFTPLUS, ACT_SILU_L2NORM = 1, 2, 3, 4
 
 _HERE = os.path.dirname(os.path.abspath(__file__))

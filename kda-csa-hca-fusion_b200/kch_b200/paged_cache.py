@@ -4,7 +4,8 @@ Not in the reference, whose decode caches hold one batch that advances in lock s
 Here sequences of any lengths share a pool of pages and a call: some bring a chunk of a prompt, some one token.  The
 caller assigns pages (a block table per batch); everything the kernels need of the lengths stays on the device, so a
 captured CUDA graph replays with other lengths and tables.  ``kv_quant='fp8'|'int8'`` stores rows in 8 bits with one fp32
-scale a row and key head, quantised as they are written.  Forward only.
+scale a row and key head, ``kv_quant='int4'`` in 4 bits with a bf16 scale for 32 channels, quantised as they are written.  Forward
+only.
 """
 from __future__ import annotations
 
@@ -13,7 +14,8 @@ import torch
 from . import _lib
 from .decoding_cache import _QUANT, _validate_cache_dtype
 
-_PAYLOAD = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
+_PAYLOAD = {"fp8": torch.float8_e4m3fn, "int8": torch.int8, "int4": torch.uint8}
+_KINDS = {**_QUANT, "int4": _lib.KCH_INT4}
 
 
 def _int_at_least(name, v, least):
@@ -42,8 +44,9 @@ class PagedKVCache:
     """``num_pages`` pages of ``page_size`` tokens for ``n_kv`` key heads of width ``c``.
 
     ``k_pages``, ``v_pages`` ``[num_pages, n_kv, page_size, c]`` in ``dtype`` (fp32 or bf16), or with ``kv_quant`` in e4m3 /
-    int8 beside ``k_scales``, ``v_scales`` fp32 ``[num_pages, n_kv, page_size]``.  ``storage``: those four tensors of a pool
-    that exists already (the scales None without ``kv_quant``).
+    int8 beside ``k_scales``, ``v_scales`` fp32 ``[num_pages, n_kv, page_size]``; ``'int4'`` (c a multiple of 32): bytes ``[.., c // 2]``, channel
+    2 i in the low half of byte i and channel 2 i + 1 in the high one, as code + 8, beside bf16 scales ``[.., c // 32]`` of 5 significant bits.
+    ``storage``: those four tensors of a pool that exists already (the scales None without ``kv_quant``).
 
     Every method takes a ragged batch of B sequences (at most 4096): ``table`` int32 ``[B, max_pages]``, ``t0`` int32 ``[B]``
     (tokens of a sequence before this call's) and ``cu_seqlens`` int32 ``[B + 1]``: rows ``cu_seqlens[b] .. cu_seqlens[b+1]`` of
@@ -64,23 +67,28 @@ class PagedKVCache:
         if c > 256 or c % 8:
             raise ValueError(f"PagedKVCache: c={c} must be a multiple of 8 from 8 to 256")
         _validate_cache_dtype(dtype)
-        if kv_quant not in _QUANT:
-            raise ValueError(f"kv_quant={kv_quant!r} must be one of {list(_QUANT)}")
+        if kv_quant not in _KINDS:
+            raise ValueError(f"kv_quant={kv_quant!r} must be one of {list(_KINDS)}")
+        if kv_quant == "int4" and c % 32:
+            raise ValueError(f"PagedKVCache: c={c} must be a multiple of 32, the channels of a scale in 4 bits")
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError(f"PagedKVCache: backend 'b200' requires a CUDA device, got {device}")
         self.num_pages, self.page_size, self.n_kv, self.c = num_pages, page_size, n_kv, c
         self.dtype, self.kv_quant = dtype, kv_quant
-        shape = (num_pages, n_kv, page_size, c)
+        shape, scales = (num_pages, n_kv, page_size, c), (num_pages, n_kv, page_size)
         payload = dtype if kv_quant is None else _PAYLOAD[kv_quant]
+        scale = None if kv_quant is None else torch.float32
+        if kv_quant == "int4":
+            shape, scales, scale = (*scales, c // 2), (*scales, c // 32), torch.bfloat16
         if storage is None:
-            k, v = (torch.zeros(shape, dtype=torch.uint8 if kv_quant else dtype, device=device) for _ in range(2))
-            ks, vs = (torch.ones(shape[:3], dtype=torch.float32, device=device) if kv_quant else None for _ in range(2))
+            zero = 0x88 if kv_quant == "int4" else 0
+            k, v = (torch.full(shape, zero, dtype=torch.uint8 if kv_quant else dtype, device=device) for _ in range(2))
+            ks, vs = (torch.ones(scales, dtype=scale, device=device) if kv_quant else None for _ in range(2))
             storage = (k.view(payload), v.view(payload), ks, vs)
         if not isinstance(storage, (tuple, list)) or len(storage) != 4:
             raise ValueError("PagedKVCache: storage must be (k_pages, v_pages, k_scales, v_scales)")
-        scale = None if kv_quant is None else torch.float32
-        for name, t, want, dt in zip(("k_pages", "v_pages", "k_scales", "v_scales"), storage, (shape, shape, shape[:3], shape[:3]),
+        for name, t, want, dt in zip(("k_pages", "v_pages", "k_scales", "v_scales"), storage, (shape, shape, scales, scales),
                                      (payload, payload, scale, scale)):
             if dt is None and t is not None:
                 raise ValueError(f"PagedKVCache: {name} goes with kv_quant")
@@ -100,7 +108,7 @@ class PagedKVCache:
         self._byte = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._tag, self._index, self._lib = _lib.dtype_tag(dtype), self.k_pages.get_device(), _lib.load()
         self._c = _lib.PagedCache(self.k_pages.data_ptr(), self.v_pages.data_ptr(), _lib.ptr(self.k_scales), _lib.ptr(self.v_scales),
-                                  self._tag if kv_quant is None else _QUANT[kv_quant], num_pages, page_size, n_kv, c)
+                                  self._tag if kv_quant is None else _KINDS[kv_quant], num_pages, page_size, n_kv, c)
 
     # (not to be set: the kernels have their addresses)
     k_pages = property(lambda self: self._storage[0])
