@@ -501,6 +501,7 @@ PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 bool kch_paged_attend_tc5_supported(int dtype, int c);
 int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
+int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s);
 
 // How a call is run: the kernel, its rows an item, CTAs, rows of a slot of the workspace.  The host knows the rows of a call and its
 // sequences, not who has them: what a sequence has on average decides, and every form takes every batch.  Either side, us, few rows /
@@ -521,7 +522,6 @@ static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   const int64_t rows = N * G;                            // of a key head
   if (!kch_paged_attend_tc5_supported(dtype, c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
   else if (rows > 32 * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
-  else if (kind == KCH_INT4) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
   else if (kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
@@ -542,7 +542,9 @@ static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, 
   const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
   const PgJoinArgs j = {a.out, dtype, nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
   if (x.form != PA_SIMT) {
-    const int rc5 = x.form == PA_MMA ? kch_paged_attend_mma(a, kind, x.rows, x.ctas, s) : kch_paged_attend_tc5(a, kind, x.rows, x.ctas, s);
+    const int rc5 = x.form == PA_TC5 || x.form == PA_TC5_FEW ? kch_paged_attend_tc5(a, kind, x.rows, x.ctas, s)
+                    : kind == KCH_INT4                       ? kch_paged_attend_int4(a, x.rows, x.ctas, s)
+                                                             : kch_paged_attend_mma(a, kind, x.rows, x.ctas, s);
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);

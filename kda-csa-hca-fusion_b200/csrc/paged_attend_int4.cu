@@ -1,0 +1,500 @@
+// Attention of few new tokens a sequence over pages in 4 bits (bf16 activations, heads of 64 or 128).
+// Mathematics and division of the work: paged_attend.cu, paged.cuh.  A stored value is (u - 8) s, u a code of 4 bits, s the scale of 32 channels.
+//
+// A step is bound by the pages' bytes, 72 a row of 128 channels, and next to them by the operations that make numbers of the codes: a
+// shift, a mask and an FMA for two.  Codes are converted once, in the registers of the warp that multiplies them, whose products
+// (mma.sync) take keys, and channels of the values, as their 16 rows and the queries as their 8 columns: half the products that the
+// queries as rows would take (paged_attend_mma.cu), and 4 or 8 queries waste nothing.
+//   S^T = K Q^T:  a key's code in the mantissa of 16 is 16 + u, and (16 + u) s - 24 s, which is exact (s has 5 bits), an element of the
+//     operand.  The order of the contraction is free: thread (g, t) of a fragment has 32 (16) consecutive channels of keys g and g + 8, which
+//     are one group's, and the queries' fragments lie in the same order.
+//   O^T += V^T P^T:  thread (g, t) has 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9, again one group's; two keys' halves
+//     of a word meet by a byte permutation.  P^T comes from S^T by the transposition of 8 x 8 values that the warp has an instruction for.
+// A row's maximum is held by the 8 lanes that have its column, who only meet when one of them exceeds it by 2^8; sums stay apart until the end.
+// P is rounded to bf16.  Up to 4 rows: the other 4 columns are the same queries again, and multiply what the rounding has left.
+// A key lies in the fragments at rho(key): both products' words then come without meeting in the banks.
+//
+// A scale of NaN (32 channels that were not finite) reaches what sees it: a key's through its logit; a value's is taken for 0 and looked for
+// when the item ends, for 0 times it would reach everyone.
+#include <cuda.h>
+#include <math.h>
+
+#include <atomic>
+
+#include "paged.cuh"
+#include "tc5_utils.cuh"
+
+#define P4_KT 128
+#define P4_SPIN (1u << 26)
+
+// R rows an item: 8, 16 or 32, by what a sequence has.
+template <int R>
+struct P4Cfg {
+  static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;       // that compute; the first warpgroup copies
+  static constexpr int NT = R / 8;                                  // columns, in eights
+  static constexpr int SLICE = R == 32 ? 16 : 32, SHARE = P4_KT / SLICE, BLOCKS = SLICE / 16;      // a warp's keys of a tile; warps of a tile
+  static constexpr int REG_FEED = 56, REG_WORK = 224, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
+};
+template <int D, int R>
+struct P4Smem {
+  typedef P4Cfg<R> C;
+  static constexpr int STAGES = D == 128 ? 9 : 16, ROW = D / 2, GROUPS = D / 32;      // bytes and scales of a row
+  alignas(1024) uint8_t k[STAGES][P4_KT * ROW], v[STAGES][P4_KT * ROW];
+  alignas(16) uint16_t ks[STAGES][P4_KT * GROUPS], vs[STAGES][P4_KT * GROUPS];
+  alignas(16) float stage[C::WARPS][8 * D];
+  alignas(16) uint2 q[D / 16][C::NT][32];                // fragments of the queries: contraction step, columns, lane
+  float ml[2][C::WARPS][R];
+  uint32_t nan_scale, nan[R][GROUPS];                    // a value's scale of NaN among the item's tiles; the groups that it makes NaN, by row
+  alignas(8) uint64_t full[STAGES], empty[STAGES];
+};
+static_assert(sizeof(P4Smem<128, 32>) <= 232448 && sizeof(P4Smem<64, 32>) <= 232448, "shared memory of the paged attention over 4 bits");
+static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 9 * P4_KT * 32, "the plan lies in the ring of tiles");
+
+__device__ __forceinline__ void p4_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_addr_u32(dst)), "l"(map), "r"(smem_addr_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// code J of either half of w, as values: J is 0 .. 3, s the scales of both halves, s24 -24 times them
+template <int J>
+__device__ __forceinline__ uint32_t p4_pair(uint32_t w, uint32_t s, uint32_t s24) {
+  const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);
+  return p4_fma((x & 0x00780078u) | 0x41804180u, s, s24);
+}
+__device__ __forceinline__ uint32_t p4_s24(uint32_t s) { return p4_fma(s, 0xC1C0C1C0u, 0u); }
+__device__ __forceinline__ void p4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t p4_trans(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// where in its eight a key of the fragments lies in the tile
+template <int D>
+__device__ __forceinline__ int p4_rho(int key) { return D == 128 ? key ^ (key >> 1 & 1) : key ^ (key >> 2 & 1); }
+// byte of the tile at which 16-byte word c of row r lies (D = 128: swizzled by pairs of rows)
+template <int D>
+__device__ __forceinline__ int p4_word(int r, int c) { return r * (D / 2) + (D == 128 ? c ^ (r >> 1 & 3) : c) * 16; }
+__device__ __forceinline__ bool p4_nan(uint32_t s) { return (s & 0x7FFFu) > 0x7F80u; }
+
+// Scales of NaN among the values of the keys [from, to) of a sequence: which rows of the item see one, by groups.  Of `threads` threads.
+template <int D>
+__device__ __noinline__ void p4_find_nan(const PgAttend& a, int b, int h, int row0, int rows, PgSeq s, int from, int to, uint32_t (*nan)[D / 32], int tid,
+                                         int threads) {
+  constexpr int GROUPS = D / 32;
+  for (int64_t i = tid; i < (int64_t)(to - from) * GROUPS; i += threads) {
+    const int key = from + (int)(i / GROUPS), group = (int)(i % GROUPS), page = __ldg(a.bt.table + b * a.bt.ld_table + (key >> a.bt.shift));
+    if ((unsigned)page >= (unsigned)a.bt.num_pages) continue;
+    const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (key & (a.page - 1));
+    if (!p4_nan(__ldg((const uint16_t*)a.vs + row * GROUPS + group))) continue;
+    for (int r = 0; r < rows; ++r) {
+      const int2 keys = pg_sees(a.bt, s, row0 + r);
+      if (key >= keys.x && key < keys.y) *(volatile uint32_t*)&nan[r][group] = 1u;
+    }
+  }
+}
+
+template <int D, int R>
+__global__ void __launch_bounds__(P4Cfg<R>::THREADS, 1)
+paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
+  typedef P4Smem<D, R> S;
+  typedef P4Cfg<R> C;
+  typedef PgWalk<R, P4_KT, 0> Walk;
+  extern __shared__ __align__(1024) uint8_t p4_raw[];
+  S& sm = *reinterpret_cast<S*>(p4_raw);
+  if (smem_addr_u32(p4_raw) & 1023) {                    // (every block begins its memory there)
+    if (threadIdx.x == 0) atomicCAS(a.bt.status, 0u, (unsigned)KCH_STATUS_PAGED_ATTEND);
+    return;
+  }
+  const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
+  if (tid == 0) {
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::SHARE); }
+    sm.nan_scale = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
+  const PgPlace place = pg_plan<R, P4_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
+  pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
+  t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
+  __syncthreads();
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, P4_SPIN, a.bt.status); };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
+    // ------------------------------ pages into the ring: keys, values and the scales of either a warp, a box each lane ------------
+    const int box = min(a.page, P4_KT), boxes = P4_KT / box;
+    const bool mine = lane < boxes, scales = warp >= 2, values = warp & 1;
+    int g = 0;
+    bool ok = true;
+    for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
+      const int end = w.first + w.count;
+      const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
+      // a box of which some row may see a key: not before the first window, not behind the sequence's end
+      auto needed = [&](int tile, int key) { return mine && tile < w.x.tiles && key + box > w.x.lo && key < w.s.kv; };
+      // asked for a tile ahead; -1 where it is not needed
+      auto ask = [&](int tile) -> int {
+        const int key = w.x.first_key + tile * P4_KT + lane * box;
+        return tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
+      };
+      int id = ask(w.first);
+      for (int tile = w.first; tile < end && ok; ++tile, ++g) {
+        const int next = ask(tile + 1), st = g % S::STAGES, key = w.x.first_key + tile * P4_KT + lane * box;
+        ok = g < S::STAGES || wait(&sm.empty[st], g / S::STAGES - 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const bool there = mine && (unsigned)id < (unsigned)a.bt.num_pages;
+        const unsigned some = __ballot_sync(0xffffffffu, there);
+        uint16_t* to = (values ? sm.vs[st] : sm.ks[st]) + lane * box * S::GROUPS;
+        if (mine && !there) {                            // codes by a coordinate out of range, scales of 0 by hand
+          if (needed(tile, key)) pg_bad(a.bt);
+          if (scales) {
+            for (int i = 0; i < box * S::GROUPS / 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(0u, 0u, 0u, 0u);
+            t5_fence_async_smem();                       // (a copy writes there next)
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbarrier_expect_tx(&sm.full[st], scales ? __popc(some) * box * (2 * S::GROUPS) : P4_KT * S::ROW);
+        __syncwarp();
+        const int r0 = key & (a.page - 1);
+        if (scales) {
+          if (there)
+            bulk_copy_g2s(to, (const uint16_t*)(values ? a.vs : a.ks) + (((int64_t)id * n_kv + w.h) * a.page + r0) * S::GROUPS, box * (2 * S::GROUPS),
+                          &sm.full[st]);
+        } else if (mine) {
+          p4_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * S::ROW, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
+        }
+        id = next;
+      }
+    }
+    // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones)
+    for (int i = 1; i <= S::STAGES && i <= g; ++i) wait(&sm.full[(g - i) % S::STAGES], (g - i) / S::STAGES);
+    return;
+  }
+
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_WORK));
+  // ------------------------------ the warps that compute ---------------------------------------------------------------------------------
+  constexpr int KS = D / 16, MT = D / 16, RUN = D / 4, NT = C::NT, BL = C::BLOCKS;      // contraction steps; channels in 16s; channels of a key a thread has
+  const int g = lane >> 2, t = lane & 3, cw = warp - 4, ct = tid - 128;      // (counted from the first of them)
+  const int rho = p4_rho<D>(g);
+  const float sc = fmaxf(fabsf(a.scale), 1e-30f);        // (not 0: a masked logit is -inf)
+  const float raise = 8.f / sc;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;      // the sign goes to the queries: a maximum stays one
+  const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::WARPS) : "memory"); };
+  int n = 0;                                             // tiles of the ring
+  bool ok = true, part = false;
+  for (Walk w(a.bt, place); w.valid(); w.next()) {
+    const bool twice = R == 8 && w.x.rows <= 4;          // columns 4 .. 7 are the rows again
+    // queries: of step i the lane (g, t) has channels d, d + 4 and d + 1, d + 5 of row g, d = RUN t + 8 (i / 2) + 2 (i % 2)
+    for (int i = ct; i < KS * NT * 32; i += 32 * C::WARPS) {
+      const int ln = i & 31, nt = (i >> 5) % NT, step = (i >> 5) / NT, d = RUN * (ln & 3) + 8 * (step >> 1) + 2 * (step & 1);
+      const int r = 8 * nt + (twice ? (ln >> 2) & 3 : ln >> 2), row = w.block * R + r, tok = pg_token(a.bt, row);
+      uint2 u = make_uint2(0u, 0u);
+      if (r < w.x.rows) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>((const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + d);
+        const uint32_t x = __ldg(src) ^ flip, y = __ldg(src + 2) ^ flip;      // channels d, d + 1; d + 4, d + 5
+        u = make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+      }
+      sm.q[step][nt][ln] = u;
+    }
+    sync();
+    const int2 k0 = pg_sees(a.bt, w.s, w.block * R), k1 = pg_sees(a.bt, w.s, w.block * R + w.x.rows - 1);      // first and last row's
+    // value e of an accumulator: row 8 nt + 2 t + e % 2 of the item (key or channel g, + 8 from e = 2 on)
+    float m[NT][2], l[NT][2], o[MT][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) { m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f; }
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int e = 0; e < NT * 4; ++e) o[j][e / 4][e % 4] = 0.f;
+    for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
+      if (n % (C::WARPS / C::SHARE) != cw / C::SHARE) continue;
+      const int st = n % S::STAGES, base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + tile * P4_KT + base;      // the warp's keys
+      if (ok) ok = wait(&sm.full[st], n / S::STAGES);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
+        float s[BL][NT][4] = {};
+        {
+          uint32_t kw[BL][2][RUN / 8], ks[BL][2], k24[BL][2];
+#pragma unroll
+          for (int x = 0; x < 2 * BL; ++x) {
+            const int r = base + 8 * x + rho;
+            uint32_t (&to)[RUN / 8] = kw[x >> 1][x & 1];
+            if constexpr (D == 128) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sm.k[st] + p4_word<D>(r, t));
+              to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(sm.k[st] + r * S::ROW + 8 * t);
+              to[0] = u.x; to[1] = u.y;
+            }
+            const uint32_t f = sm.ks[st][r * S::GROUPS + (D == 128 ? t : t >> 1)];
+            ks[x >> 1][x & 1] = f | f << 16;
+            k24[x >> 1][x & 1] = p4_s24(f | f << 16);
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            uint2 q[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) q[nt] = sm.q[i][nt][lane];
+#pragma unroll
+            for (int b = 0; b < BL; ++b) {
+              const uint32_t x = kw[b][0][i >> 1], y = kw[b][1][i >> 1], fx = ks[b][0], fy = ks[b][1], gx = k24[b][0], gy = k24[b][1];
+              uint32_t a0, a1, a2, a3;
+              if (i & 1) {
+                a0 = p4_pair<2>(x, fx, gx); a1 = p4_pair<2>(y, fy, gy); a2 = p4_pair<3>(x, fx, gx); a3 = p4_pair<3>(y, fy, gy);
+              } else {
+                a0 = p4_pair<0>(x, fx, gx); a1 = p4_pair<0>(y, fy, gy); a2 = p4_pair<1>(x, fx, gx); a3 = p4_pair<1>(y, fy, gy);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) p4_mma(s[b][nt], a0, a1, a2, a3, q[nt].x, q[nt].y);
+            }
+          }
+        }
+        // what a row does not see is -inf
+        if (!(key0 >= k1.x && key0 + C::SLICE <= k0.y)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = 8 * nt + 2 * t + e, row = twice ? r & 3 : r;
+              const int2 keys = row < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + row) : make_int2(0, 0);
+#pragma unroll
+              for (int b = 0; b < BL; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int key = key0 + 16 * b + 8 * h + rho;
+                  if (!(key >= keys.x && key < keys.y)) s[b][nt][2 * h + e] = -INFINITY;
+                }
+            }
+        }
+        // a row's maximum is raised only when it is exceeded by 2^8
+        float top[NT][2];
+        bool any = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+            for (int b = 1; b < BL; ++b) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[b][nt][e], s[b][nt][2 + e]));
+            any = any || (m[nt][e] == -INFINITY ? top[nt][e] > m[nt][e] : top[nt][e] > m[nt][e] + raise);
+          }
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = top[nt][e];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              const bool up = m[nt][e] == -INFINITY ? x > m[nt][e] : x > m[nt][e] + raise;
+              const float f = up ? ex2_fast((m[nt][e] - x) * sc) : 1.f;
+              if (up) m[nt][e] = x;
+              l[nt][e] *= f;
+#pragma unroll
+              for (int j = 0; j < MT; ++j) { o[j][nt][e] *= f; o[j][nt][2 + e] *= f; }
+            }
+        }
+        uint32_t p[BL][NT][2];                           // P^T: keys 2t, 2t + 1 (and + 8) of row g
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float shift0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] * sc, shift1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] * sc;
+#pragma unroll
+          for (int b = 0; b < BL; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = ex2_fast(fmaf(s[b][nt][2 * h], sc, -shift0)), y = ex2_fast(fmaf(s[b][nt][2 * h + 1], sc, -shift1));
+              l[nt][0] += x;
+              l[nt][1] += y;
+              uint32_t u = pack2_bf16(x, y);
+              if (R == 8 && twice && t >= 2) u = pack2_bf16(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u));
+              p[b][nt][h] = p4_trans(u);
+            }
+        }
+        // of the values the lane has channels 16 g .. (8 g ..) of keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+        for (int b = 0; b < BL; ++b) {
+          uint32_t vw[4][D / 64], f[2], f24[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t two[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = base + 16 * b + 8 * h + p4_rho<D>(2 * t + e);
+              if constexpr (D == 128) {
+                const uint2 u = *reinterpret_cast<const uint2*>(sm.v[st] + p4_word<D>(r, g >> 1) + 8 * (g & 1));
+                vw[2 * h + e][0] = u.x; vw[2 * h + e][1] = u.y;
+              } else {
+                vw[2 * h + e][0] = *reinterpret_cast<const uint32_t*>(sm.v[st] + r * S::ROW + 4 * g);
+              }
+              two[e] = sm.vs[st][r * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
+            }
+            if (p4_nan(two[0]) || p4_nan(two[1])) {
+              *(volatile uint32_t*)&sm.nan_scale = 1u;
+              if (p4_nan(two[0])) two[0] = 0u;
+              if (p4_nan(two[1])) two[1] = 0u;
+            }
+            f[h] = two[0] | two[1] << 16;
+            f24[h] = p4_s24(f[h]);
+          }
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            const uint32_t x0 = __byte_perm(vw[0][i], vw[1][i], 0x5410), x1 = __byte_perm(vw[0][i], vw[1][i], 0x7632);      // channels 0 .. 3, 4 .. 7 of both keys
+            const uint32_t y0 = __byte_perm(vw[2][i], vw[3][i], 0x5410), y1 = __byte_perm(vw[2][i], vw[3][i], 0x7632);
+#define P4_PV(J_)                                                                                                                        \
+  {                                                                                                                                      \
+    const uint32_t a0 = p4_pair<J_>(x0, f[0], f24[0]), a1 = p4_pair<J_>(x1, f[0], f24[0]), a2 = p4_pair<J_>(y0, f[1], f24[1]),           \
+                   a3 = p4_pair<J_>(y1, f[1], f24[1]);                                                                                   \
+    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) p4_mma(o[4 * i + J_][nt], a0, a1, a2, a3, p[b][nt][0], p[b][nt][1]);               \
+  }
+            P4_PV(0) P4_PV(1) P4_PV(2) P4_PV(3)
+#undef P4_PV
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&sm.empty[st]);
+    }
+    if (twice) {                                         // (lane t has rows 2 t, 2 t + 1, lane t + 2 what their rounding left)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][0][e] += __shfl_xor_sync(0xffffffffu, o[j][0][e], 2);
+    }
+    // ---- the item's end: the warps' parts of its rows ---------------------------------------------------------------------------
+    const bool direct = w.starts() && w.ends();
+    float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(a.slot_rows, D);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float& x = l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g == 0) {
+          sm.ml[0][cw][8 * nt + 2 * t + e] = m[nt][e];
+          sm.ml[1][cw][8 * nt + 2 * t + e] = x;
+        }
+      }
+    sync();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (8 * nt >= w.x.rows) break;                     // (the same for all warps)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 2 * t + e;
+        float mm = sm.ml[0][0][8 * nt + r];
+#pragma unroll
+        for (int k = 1; k < C::WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][8 * nt + r]);
+        const bool none = m[nt][e] == -INFINITY;         // (a part without a key)
+        const float own = none ? 0.f : ex2_fast((m[nt][e] - mm) * sc);
+        float4* to = reinterpret_cast<float4*>(sm.stage[cw]) + r * (D / 4);
+        // channels 16 g + 8 i + 4 h .. + 3; words swizzled by the row, so that the lanes of a column do not meet in the banks
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            to[(D / 32 * g + 2 * i + h) ^ t] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                    : make_float4(o[4 * i][nt][2 * h + e] * own, o[4 * i + 1][nt][2 * h + e] * own,
+                                                                  o[4 * i + 2][nt][2 * h + e] * own, o[4 * i + 3][nt][2 * h + e] * own);
+      }
+      sync();
+      for (int k = ct; k < 8 * (D / 4); k += 32 * C::WARPS) {
+        const int r = k / (D / 4), c = k % (D / 4), row = 8 * nt + r;
+        if (row >= w.x.rows || !ok) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int at = r * (D / 4) + (c ^ (r >> 1));
+#pragma unroll
+        for (int i2 = 0; i2 < C::WARPS; ++i2) {
+          const float4 y = reinterpret_cast<const float4*>(sm.stage[i2])[at];
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+        float top = sm.ml[0][0][row], sum = 0.f;
+#pragma unroll
+        for (int i2 = 1; i2 < C::WARPS; ++i2) top = fmaxf(top, sm.ml[0][i2][row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i2 = 0; i2 < C::WARPS; ++i2) sum += sm.ml[1][i2][row] * ex2_fast((sm.ml[0][i2][row] - ref) * sc);      // (a NaN stays one)
+        if (direct) {
+          const int rr = w.block * R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
+          float below = sum;
+          if (a.sink && sum > 0.f) below += ex2_fast(ld_any(a.sink, head, a.sink_dtype) * PG_LOG2E - ref * sc);
+          const float f = sum == 0.f ? 0.f : 1.f / below;
+          *reinterpret_cast<uint2*>((bf16*)a.out + ((int64_t)(w.s.row0 + tok) * (n_kv * G) + head) * D + 4 * c) =
+              make_uint2(pack2_bf16(x.x * f, x.y * f), pack2_bf16(x.z * f, x.w * f));
+        } else {
+          *reinterpret_cast<float4*>(slot + (int64_t)row * D + 4 * c) = x;
+          if (c == 0) {
+            slot[(int64_t)a.slot_rows * D + row] = top * sc;
+            slot[(int64_t)a.slot_rows * D + a.slot_rows + row] = sum;
+          }
+        }
+      }
+      sync();
+    }
+    // scales of NaN among the values: the groups of the rows that see one
+    if (*(volatile uint32_t*)&sm.nan_scale != 0u) {
+      sync();                                            // (all have read the word)
+      if (ct == 0) *(volatile uint32_t*)&sm.nan_scale = 0u;
+      for (int i = ct; i < R * S::GROUPS; i += 32 * C::WARPS) sm.nan[i / S::GROUPS][i % S::GROUPS] = 0u;
+      sync();
+      const int part0 = w.x.first_key + w.first * P4_KT;
+      p4_find_nan<D>(a, w.b, w.h, w.block * R, w.x.rows, w.s, max(part0, w.x.lo), min(part0 + w.count * P4_KT, w.s.kv), sm.nan, ct, 32 * C::WARPS);
+      sync();
+      for (int i = ct; i < w.x.rows * D && ok; i += 32 * C::WARPS) {
+        const int row = i / D, d = i % D, rr = w.block * R + row, tok = pg_token(a.bt, rr), head = w.h * G + rr - tok * G;
+        if (!sm.nan[row][d / 32]) continue;
+        if (direct) ((uint16_t*)a.out)[((int64_t)(w.s.row0 + tok) * (n_kv * G) + head) * D + d] = 0x7FC0u;
+        else slot[(int64_t)row * D + d] = __uint_as_float(0x7FC00000u);
+      }
+    }
+    if (w.starts() && !w.ends()) {
+      part = true;
+      if (ct == 0)
+        a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
+                                 w.x.rows, w.s.row0};
+    }
+  }
+  if (ct == 0 && !part) a.records[blockIdx.x].valid = 0;
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
+                              uint32_t box_rows, bool plain = false);
+
+template <int D, int R>
+static int p4_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
+  const int smem = (int)sizeof(P4Smem<D, R>);
+  static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
+  int dev = 0;
+  KCH_CUDA_OK(cudaGetDevice(&dev));
+  if (dev > 63 || !((done.load(std::memory_order_relaxed) >> dev) & 1)) {
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_int4_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
+  }
+  paged_attend_int4_kernel<D, R><<<ctas, P4Cfg<R>::THREADS, smem, s>>>(km, vm, a);
+  KCH_LAUNCH_OK();
+  return KCH_OK;
+}
+
+int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const int box = a.page < P4_KT ? a.page : P4_KT;
+  int rc = kch_make_tensor_map_pages(&km, a.k, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c / 2, box, a.c == 64);
+  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c / 2, box, a.c == 64);
+  if (rc != KCH_OK) return rc;
+#define P4_ROWS(D_) (rows == 8 ? p4_launch<D_, 8>(km, vm, a, ctas, s) : rows == 16 ? p4_launch<D_, 16>(km, vm, a, ctas, s) : p4_launch<D_, 32>(km, vm, a, ctas, s))
+  return a.c == 64 ? P4_ROWS(64) : P4_ROWS(128);
+#undef P4_ROWS
+}
