@@ -14,9 +14,14 @@
 // P is rounded to bf16.  Up to 4 rows: the other 4 columns are the same queries again, and multiply what the rounding has left.
 // A key lies in the fragments at rho(key): both products' words then come without meeting in the banks.
 //
+// Measured, 64 sequences, 16 heads of 128 on 4: 8192 tokens in pages of 64 86 us (3.5 TB/s of pages; 89 in pages of 16, 111 of 8), 500 to
+// 16000 tokens in pages of 32 98; on two key heads 50, on one 41, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
+// the instructions that convert: 730 for 32 keys of a warp, 340 of them at half rate, on two warps a scheduler that keep it 56 % busy.
+// Tried: 12 warps of 152 registers 86 and 102; a tile's values multiplied while the next one's scores are 92 (registers move); shifts as
+// products with powers of two, on the other pipe, 93.  Pages by tensor maps of 64-byte rows: a copy engine's 5 clocks a row are 1280 for a tile.
+//
 // A scale of NaN (32 channels that were not finite) reaches what sees it: a key's through its logit; a value's is taken for 0 and looked for
 // when the item ends, for 0 times it would reach everyone.
-#include <cuda.h>
 #include <math.h>
 
 #include <atomic>
@@ -25,7 +30,7 @@
 #include "tc5_utils.cuh"
 
 #define P4_KT 128
-#define P4_SPIN (1u << 26)
+#define P4_WAIT 4000000000ull          // ns until a wait gives up
 
 // R rows an item: 8, 16 or 32, by what a sequence has.
 template <int R>
@@ -33,13 +38,14 @@ struct P4Cfg {
   static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;       // that compute; the first warpgroup copies
   static constexpr int NT = R / 8;                                  // columns, in eights
   static constexpr int SLICE = R == 32 ? 16 : 32, SHARE = P4_KT / SLICE, BLOCKS = SLICE / 16;      // a warp's keys of a tile; warps of a tile
-  static constexpr int REG_FEED = 56, REG_WORK = 224, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static constexpr int TEAMS = WARPS / SHARE;                       // each takes every TEAMS'th tile
+  static constexpr int REG_FEED = R == 32 ? 56 : 88, REG_WORK = R == 32 ? 224 : 208, REG_LAUNCH = 65536 / THREADS / 8 * 8;
   static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
 };
 template <int D, int R>
 struct P4Smem {
   typedef P4Cfg<R> C;
-  static constexpr int STAGES = D == 128 ? 9 : 16, ROW = D / 2, GROUPS = D / 32;      // bytes and scales of a row
+  static constexpr int STAGES = D == 128 ? 8 : 12, ROW = D / 2, GROUPS = D / 32;      // bytes and scales of a row
   alignas(1024) uint8_t k[STAGES][P4_KT * ROW], v[STAGES][P4_KT * ROW];
   alignas(16) uint16_t ks[STAGES][P4_KT * GROUPS], vs[STAGES][P4_KT * GROUPS];
   alignas(16) float stage[C::WARPS][8 * D];
@@ -49,23 +55,43 @@ struct P4Smem {
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
 static_assert(sizeof(P4Smem<128, 32>) <= 232448 && sizeof(P4Smem<64, 32>) <= 232448, "shared memory of the paged attention over 4 bits");
-static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 9 * P4_KT * 32, "the plan lies in the ring of tiles");
+static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 12 * P4_KT * 32, "the plan lies in the ring of tiles");
 
-__device__ __forceinline__ void p4_tma_4d(void* dst, const void* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+// A bounded wait that sleeps: a poll returns when the phase is complete, or after 10 us.  (Polls that return at once were an eighth of all
+// instructions, on the schedulers that the others compute with.)
+__device__ __forceinline__ bool p4_poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(smem_addr_u32(dst)), "l"(map), "r"(smem_addr_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok;
+}
+__device__ __noinline__ bool p4_wait_long(uint32_t bar, uint32_t parity, unsigned int* status, unsigned sleep) {
+  uint64_t since, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(since));
+  do {
+    if (p4_poll(bar, parity)) return true;
+    if (*(volatile unsigned int*)status != 0u) return false;
+    if (sleep) __nanosleep(sleep);
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+  } while (now - since < P4_WAIT);
+  atomicCAS(status, 0u, (unsigned)KCH_STATUS_PAGED_ATTEND);
+  return false;
 }
 __device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// code J of either half of w, as values: J is 0 .. 3, s the scales of both halves, s24 -24 times them
+// code J of either half of w, as values: J is 0 .. 3, s the scales of both halves, s24 -24 times them; sixteen: 16 in either half, a register
+// whose value the compiler does not know (with two constants it makes two operations of this one: 287 of them for 32 keys, 120 -> 100 us)
 template <int J>
-__device__ __forceinline__ uint32_t p4_pair(uint32_t w, uint32_t s, uint32_t s24) {
-  const uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);
-  return p4_fma((x & 0x00780078u) | 0x41804180u, s, s24);
+__device__ __forceinline__ uint32_t p4_pair(uint32_t w, uint32_t s, uint32_t s24, uint32_t sixteen) {
+  uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);
+  asm("lop3.b32 %0, %1, 0x00780078, %2, 0xEA;" : "=r"(x) : "r"(x), "r"(sixteen));
+  return p4_fma(x, s, s24);
 }
 __device__ __forceinline__ uint32_t p4_s24(uint32_t s) { return p4_fma(s, 0xC1C0C1C0u, 0u); }
 __device__ __forceinline__ void p4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -79,11 +105,7 @@ __device__ __forceinline__ uint32_t p4_trans(uint32_t x) {
   return r;
 }
 // where in its eight a key of the fragments lies in the tile
-template <int D>
-__device__ __forceinline__ int p4_rho(int key) { return D == 128 ? key ^ (key >> 1 & 1) : key ^ (key >> 2 & 1); }
-// byte of the tile at which 16-byte word c of row r lies (D = 128: swizzled by pairs of rows)
-template <int D>
-__device__ __forceinline__ int p4_word(int r, int c) { return r * (D / 2) + (D == 128 ? c ^ (r >> 1 & 3) : c) * 16; }
+__device__ __forceinline__ int p4_rho(int key) { return key ^ (key >> 2 & 1); }
 __device__ __forceinline__ bool p4_nan(uint32_t s) { return (s & 0x7FFFu) > 0x7F80u; }
 
 // Scales of NaN among the values of the keys [from, to) of a sequence: which rows of the item see one, by groups.  Of `threads` threads.
@@ -105,7 +127,7 @@ __device__ __noinline__ void p4_find_nan(const PgAttend& a, int b, int h, int ro
 
 template <int D, int R>
 __global__ void __launch_bounds__(P4Cfg<R>::THREADS, 1)
-paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
+paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
   typedef P4Smem<D, R> S;
   typedef P4Cfg<R> C;
   typedef PgWalk<R, P4_KT, 0> Walk;
@@ -117,67 +139,82 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv;
   if (tid == 0) {
-    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 4); mbarrier_init(&sm.empty[i], C::SHARE); }
+    for (int i = 0; i < S::STAGES; ++i) { mbarrier_init(&sm.full[i], 2); mbarrier_init(&sm.empty[i], C::SHARE); }
     sm.nan_scale = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
   const PgPlace place = pg_plan<R, P4_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   __syncthreads();
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, P4_SPIN, a.bt.status); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return p4_poll(smem_addr_u32(bar), parity & 1) || p4_wait_long(smem_addr_u32(bar), parity & 1, a.bt.status, warp < 4 ? 300u : 0u);
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_FEED));
-    // ------------------------------ pages into the ring: keys, values and the scales of either a warp, a box each lane ------------
-    const int box = min(a.page, P4_KT), boxes = P4_KT / box;
-    const bool mine = lane < boxes, scales = warp >= 2, values = warp & 1;
-    int g = 0;
+    // ------------------------------ pages into the ring: keys and values of the even and of the odd tiles a warp each, a lane a box of
+    // codes (0 .. 15) or of scales (16 .. 31).  (A tile is about a hundred instructions in a row, 1000 cycles beside warps that compute: two
+    // warps for all tiles held everyone up.) ------------------------------------------------------------------------------------------------
+    const int box = min(a.page, P4_KT), boxes = P4_KT / box, at = lane & 15;
+    const bool mine = at < boxes, scales = lane >= 16, values = warp & 1;
+    // of this lane's kind: where it lies in the pool, where it goes to (a stage on from there), bytes of a row
+    const uint8_t* from = (const uint8_t*)(scales ? (values ? a.vs : a.ks) : values ? a.v : a.k);
+    const int bytes = scales ? 2 * S::GROUPS : S::ROW;
+    uint8_t* first = (scales ? (uint8_t*)(values ? sm.vs : sm.ks) : (uint8_t*)(values ? sm.v : sm.k)) + at * box * bytes;
+    int ahead = warp >> 1, st = ahead, turn = 0, g = 0;  // tiles until this warp's next; its place in the ring, and how often that has been filled; tiles so far
     bool ok = true;
     for (Walk w(a.bt, place); w.valid() && ok; w.next()) {
-      const int end = w.first + w.count;
       const int32_t* pages = a.bt.table + (int64_t)w.b * a.bt.ld_table;
       // a box of which some row may see a key: not before the first window, not behind the sequence's end
-      auto needed = [&](int tile, int key) { return mine && tile < w.x.tiles && key + box > w.x.lo && key < w.s.kv; };
-      // asked for a tile ahead; -1 where it is not needed
-      auto ask = [&](int tile) -> int {
-        const int key = w.x.first_key + tile * P4_KT + lane * box;
-        return tile < end && needed(tile, key) ? __ldg(pages + (key >> a.bt.shift)) : -1;
+      int key0 = w.x.first_key + (w.first + ahead) * P4_KT;
+      const int last = min(w.s.kv, w.x.first_key + min(w.first + w.count, w.x.tiles) * P4_KT);
+      auto needed = [&](int k) { return mine && k + box > w.x.lo && k < last; };
+      // The table is asked for 32 pages at once (those of 2 to 32 tiles), and as many ahead: a page asked for a tile ahead came after 1400 cycles,
+      // later than the tile was used up.
+      int page0 = key0 >> a.bt.shift;
+      auto ask = [&](int from) {
+        const int i = from + lane;
+        return i >= w.x.lo >> a.bt.shift && i <= (last - 1) >> a.bt.shift ? __ldg(pages + i) : -1;
       };
-      int id = ask(w.first);
-      for (int tile = w.first; tile < end && ok; ++tile, ++g) {
-        const int next = ask(tile + 1), st = g % S::STAGES, key = w.x.first_key + tile * P4_KT + lane * box;
-        ok = g < S::STAGES || wait(&sm.empty[st], g / S::STAGES - 1);
+      int here = ask(page0), then = ask(page0 + 32);
+      for (; ahead < w.count && ok; ahead += 2, ++g, key0 += 2 * P4_KT) {
+        if ((key0 >> a.bt.shift) - page0 >= 32) {
+          page0 += 32;
+          here = then;
+          then = ask(page0 + 32);
+        }
+        const int key = key0 + at * box, id = __shfl_sync(0xffffffffu, here, ((key >> a.bt.shift) - page0) & 31);
+        ok = turn == 0 || wait(&sm.empty[st], turn - 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const bool there = mine && (unsigned)id < (unsigned)a.bt.num_pages;
-        const unsigned some = __ballot_sync(0xffffffffu, there);
-        uint16_t* to = (values ? sm.vs[st] : sm.ks[st]) + lane * box * S::GROUPS;
-        if (mine && !there) {                            // codes by a coordinate out of range, scales of 0 by hand
-          if (needed(tile, key)) pg_bad(a.bt);
+        const bool there = needed(key) && (unsigned)id < (unsigned)a.bt.num_pages;
+        const unsigned some = __ballot_sync(0xffffffffu, there) >> 16;
+        uint8_t* to = first + st * (P4_KT * bytes);
+        if (mine && !there) {                            // zeros: scales of 0, whatever the codes
+          if (needed(key)) pg_bad(a.bt);
           if (scales) {
-            for (int i = 0; i < box * S::GROUPS / 8; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < box * bytes; j += 16) *reinterpret_cast<uint4*>(to + j) = make_uint4(0u, 0u, 0u, 0u);
             t5_fence_async_smem();                       // (a copy writes there next)
           }
         }
         __syncwarp();
-        if (lane == 0) mbarrier_expect_tx(&sm.full[st], scales ? __popc(some) * box * (2 * S::GROUPS) : P4_KT * S::ROW);
+        if (lane == 0) mbarrier_expect_tx(&sm.full[st], __popc(some) * box * (2 * S::GROUPS + S::ROW));
         __syncwarp();
-        const int r0 = key & (a.page - 1);
-        if (scales) {
-          if (there)
-            bulk_copy_g2s(to, (const uint16_t*)(values ? a.vs : a.ks) + (((int64_t)id * n_kv + w.h) * a.page + r0) * S::GROUPS, box * (2 * S::GROUPS),
-                          &sm.full[st]);
-        } else if (mine) {
-          p4_tma_4d((values ? sm.v[st] : sm.k[st]) + lane * box * S::ROW, values ? &vmap : &kmap, 0, r0, w.h, there ? id : (int)a.bt.num_pages, &sm.full[st]);
-        }
-        id = next;
+        if (there) bulk_copy_g2s(to, from + (((int64_t)id * n_kv + w.h) * a.page + (key & (a.page - 1))) * bytes, box * bytes, &sm.full[st]);
+        st += 2;
+        if (st >= S::STAGES) { st -= S::STAGES; ++turn; }
       }
+      ahead -= w.count;
     }
-    // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones)
-    for (int i = 1; i <= S::STAGES && i <= g; ++i) wait(&sm.full[(g - i) % S::STAGES], (g - i) / S::STAGES);
+    // no copy is in flight when the block ends (after a wait that ran out nobody else may have waited for the last ones; every other stage
+    // is this warp's alone)
+    static_assert(S::STAGES % 2 == 0, "stages of two pairs of warps");
+    for (int i = 0; i < g && i < S::STAGES / 2; ++i) {
+      st -= 2;
+      if (st < 0) { st += S::STAGES; --turn; }
+      wait(&sm.full[st], turn);
+    }
     return;
   }
 
@@ -185,12 +222,14 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
   // ------------------------------ the warps that compute ---------------------------------------------------------------------------------
   constexpr int KS = D / 16, MT = D / 16, RUN = D / 4, NT = C::NT, BL = C::BLOCKS;      // contraction steps; channels in 16s; channels of a key a thread has
   const int g = lane >> 2, t = lane & 3, cw = warp - 4, ct = tid - 128;      // (counted from the first of them)
-  const int rho = p4_rho<D>(g);
+  const int rho = p4_rho(g);
+  uint32_t sixteen;
+  asm volatile("mov.b32 %0, 0x41804180;" : "=r"(sixteen));
   const float sc = fmaxf(fabsf(a.scale), 1e-30f);        // (not 0: a masked logit is -inf)
   const float raise = 8.f / sc;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;      // the sign goes to the queries: a maximum stays one
   const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::WARPS) : "memory"); };
-  int n = 0;                                             // tiles of the ring
+  int ahead = cw / C::SHARE, st = ahead, turn = 0;       // tiles until this team's next; its place in the ring (TEAMS < STAGES), and how often that has been filled
   bool ok = true, part = false;
   for (Walk w(a.bt, place); w.valid(); w.next()) {
     const bool twice = R == 8 && w.x.rows <= 4;          // columns 4 .. 7 are the rows again
@@ -216,10 +255,15 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int e = 0; e < NT * 4; ++e) o[j][e / 4][e % 4] = 0.f;
-    for (int tile = w.first; tile < w.first + w.count; ++tile, ++n) {
-      if (n % (C::WARPS / C::SHARE) != cw / C::SHARE) continue;
-      const int st = n % S::STAGES, base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + tile * P4_KT + base;      // the warp's keys
-      if (ok) ok = wait(&sm.full[st], n / S::STAGES);
+    const uint2* queries = &sm.q[0][0][lane];
+    uint2 own[NT == 1 ? KS : 1];                          // (eight rows' stay in registers)
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) own[i] = queries[32 * i];
+    }
+    for (; ahead < w.count; ahead += C::TEAMS) {
+      const int base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + (w.first + ahead) * P4_KT + base;      // the warp's keys
+      if (ok) ok = wait(&sm.full[st], turn);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
         float s[BL][NT][4] = {};
@@ -230,7 +274,7 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
             const int r = base + 8 * x + rho;
             uint32_t (&to)[RUN / 8] = kw[x >> 1][x & 1];
             if constexpr (D == 128) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sm.k[st] + p4_word<D>(r, t));
+              const uint4 u = *reinterpret_cast<const uint4*>(sm.k[st] + r * S::ROW + 16 * t);
               to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
             } else {
               const uint2 u = *reinterpret_cast<const uint2*>(sm.k[st] + r * S::ROW + 8 * t);
@@ -244,15 +288,18 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
           for (int i = 0; i < KS; ++i) {
             uint2 q[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) q[nt] = sm.q[i][nt][lane];
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (NT == 1) q[nt] = own[i];
+              else q[nt] = queries[32 * (NT * i + nt)];
+            }
 #pragma unroll
             for (int b = 0; b < BL; ++b) {
               const uint32_t x = kw[b][0][i >> 1], y = kw[b][1][i >> 1], fx = ks[b][0], fy = ks[b][1], gx = k24[b][0], gy = k24[b][1];
               uint32_t a0, a1, a2, a3;
               if (i & 1) {
-                a0 = p4_pair<2>(x, fx, gx); a1 = p4_pair<2>(y, fy, gy); a2 = p4_pair<3>(x, fx, gx); a3 = p4_pair<3>(y, fy, gy);
+                a0 = p4_pair<2>(x, fx, gx, sixteen); a1 = p4_pair<2>(y, fy, gy, sixteen); a2 = p4_pair<3>(x, fx, gx, sixteen); a3 = p4_pair<3>(y, fy, gy, sixteen);
               } else {
-                a0 = p4_pair<0>(x, fx, gx); a1 = p4_pair<0>(y, fy, gy); a2 = p4_pair<1>(x, fx, gx); a3 = p4_pair<1>(y, fy, gy);
+                a0 = p4_pair<0>(x, fx, gx, sixteen); a1 = p4_pair<0>(y, fy, gy, sixteen); a2 = p4_pair<1>(x, fx, gx, sixteen); a3 = p4_pair<1>(y, fy, gy, sixteen);
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) p4_mma(s[b][nt], a0, a1, a2, a3, q[nt].x, q[nt].y);
@@ -322,39 +369,42 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
             }
         }
         // of the values the lane has channels 16 g .. (8 g ..) of keys 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t f[BL][4], most = 0u;                    // their scales
+#pragma unroll
+        for (int i = 0; i < 4 * BL; ++i) {
+          f[i >> 2][i & 3] = sm.vs[st][(base + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
+          most = max(most, f[i >> 2][i & 3]);
+        }
+        if (most > 0x7F80u) {                            // (NaN, or below 0, which an append writes none of)
+#pragma unroll
+          for (int i = 0; i < 4 * BL; ++i)
+            if (p4_nan(f[i >> 2][i & 3])) {
+              f[i >> 2][i & 3] = 0u;
+              *(volatile uint32_t*)&sm.nan_scale = 1u;
+            }
+        }
 #pragma unroll
         for (int b = 0; b < BL; ++b) {
-          uint32_t vw[4][D / 64], f[2], f24[2];
+          uint32_t vw[4][D / 64];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t two[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = base + 16 * b + 8 * h + p4_rho<D>(2 * t + e);
-              if constexpr (D == 128) {
-                const uint2 u = *reinterpret_cast<const uint2*>(sm.v[st] + p4_word<D>(r, g >> 1) + 8 * (g & 1));
-                vw[2 * h + e][0] = u.x; vw[2 * h + e][1] = u.y;
-              } else {
-                vw[2 * h + e][0] = *reinterpret_cast<const uint32_t*>(sm.v[st] + r * S::ROW + 4 * g);
-              }
-              two[e] = sm.vs[st][r * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* from = sm.v[st] + (base + 16 * b + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::ROW + D / 16 * g;
+            if constexpr (D == 128) {
+              const uint2 u = *reinterpret_cast<const uint2*>(from);
+              vw[i][0] = u.x; vw[i][1] = u.y;
+            } else {
+              vw[i][0] = *reinterpret_cast<const uint32_t*>(from);
             }
-            if (p4_nan(two[0]) || p4_nan(two[1])) {
-              *(volatile uint32_t*)&sm.nan_scale = 1u;
-              if (p4_nan(two[0])) two[0] = 0u;
-              if (p4_nan(two[1])) two[1] = 0u;
-            }
-            f[h] = two[0] | two[1] << 16;
-            f24[h] = p4_s24(f[h]);
           }
+          const uint32_t fx = f[b][0] | f[b][1] << 16, fy = f[b][2] | f[b][3] << 16, gx = p4_s24(fx), gy = p4_s24(fy);
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) {
             const uint32_t x0 = __byte_perm(vw[0][i], vw[1][i], 0x5410), x1 = __byte_perm(vw[0][i], vw[1][i], 0x7632);      // channels 0 .. 3, 4 .. 7 of both keys
             const uint32_t y0 = __byte_perm(vw[2][i], vw[3][i], 0x5410), y1 = __byte_perm(vw[2][i], vw[3][i], 0x7632);
 #define P4_PV(J_)                                                                                                                        \
   {                                                                                                                                      \
-    const uint32_t a0 = p4_pair<J_>(x0, f[0], f24[0]), a1 = p4_pair<J_>(x1, f[0], f24[0]), a2 = p4_pair<J_>(y0, f[1], f24[1]),           \
-                   a3 = p4_pair<J_>(y1, f[1], f24[1]);                                                                                   \
+    const uint32_t a0 = p4_pair<J_>(x0, fx, gx, sixteen), a1 = p4_pair<J_>(x1, fx, gx, sixteen), a2 = p4_pair<J_>(y0, fy, gy, sixteen),           \
+                   a3 = p4_pair<J_>(y1, fy, gy, sixteen);                                                                                   \
     _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) p4_mma(o[4 * i + J_][nt], a0, a1, a2, a3, p[b][nt][0], p[b][nt][1]);               \
   }
             P4_PV(0) P4_PV(1) P4_PV(2) P4_PV(3)
@@ -364,7 +414,10 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
       }
       __syncwarp();
       if (lane == 0) mbarrier_arrive(&sm.empty[st]);
+      st += C::TEAMS;
+      if (st >= S::STAGES) { st -= S::STAGES; ++turn; }
     }
+    ahead -= w.count;
     if (twice) {                                         // (lane t has rows 2 t, 2 t + 1, lane t + 2 what their rounding left)
 #pragma unroll
       for (int j = 0; j < MT; ++j)
@@ -398,7 +451,7 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
 #pragma unroll
         for (int k = 1; k < C::WARPS; ++k) mm = fmaxf(mm, sm.ml[0][k][8 * nt + r]);
         const bool none = m[nt][e] == -INFINITY;         // (a part without a key)
-        const float own = none ? 0.f : ex2_fast((m[nt][e] - mm) * sc);
+        const float f = none ? 0.f : ex2_fast((m[nt][e] - mm) * sc);
         float4* to = reinterpret_cast<float4*>(sm.stage[cw]) + r * (D / 4);
         // channels 16 g + 8 i + 4 h .. + 3; words swizzled by the row, so that the lanes of a column do not meet in the banks
 #pragma unroll
@@ -406,8 +459,8 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             to[(D / 32 * g + 2 * i + h) ^ t] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                    : make_float4(o[4 * i][nt][2 * h + e] * own, o[4 * i + 1][nt][2 * h + e] * own,
-                                                                  o[4 * i + 2][nt][2 * h + e] * own, o[4 * i + 3][nt][2 * h + e] * own);
+                                                    : make_float4(o[4 * i][nt][2 * h + e] * f, o[4 * i + 1][nt][2 * h + e] * f,
+                                                                  o[4 * i + 2][nt][2 * h + e] * f, o[4 * i + 3][nt][2 * h + e] * f);
       }
       sync();
       for (int k = ct; k < 8 * (D / 4); k += 32 * C::WARPS) {
@@ -470,11 +523,8 @@ paged_attend_int4_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
-int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
-                              uint32_t box_rows, bool plain = false);
-
 template <int D, int R>
-static int p4_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
+static int p4_launch(const PgAttend& a, int ctas, cudaStream_t s) {
   const int smem = (int)sizeof(P4Smem<D, R>);
   static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
   int dev = 0;
@@ -483,18 +533,13 @@ static int p4_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAtten
     KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_int4_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
   }
-  paged_attend_int4_kernel<D, R><<<ctas, P4Cfg<R>::THREADS, smem, s>>>(km, vm, a);
+  paged_attend_int4_kernel<D, R><<<ctas, P4Cfg<R>::THREADS, smem, s>>>(a);
   KCH_LAUNCH_OK();
   return KCH_OK;
 }
 
 int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s) {
-  CUtensorMap km, vm;
-  const int box = a.page < P4_KT ? a.page : P4_KT;
-  int rc = kch_make_tensor_map_pages(&km, a.k, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c / 2, box, a.c == 64);
-  if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, 1, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, a.c / 2, box, a.c == 64);
-  if (rc != KCH_OK) return rc;
-#define P4_ROWS(D_) (rows == 8 ? p4_launch<D_, 8>(km, vm, a, ctas, s) : rows == 16 ? p4_launch<D_, 16>(km, vm, a, ctas, s) : p4_launch<D_, 32>(km, vm, a, ctas, s))
+#define P4_ROWS(D_) (rows == 8 ? p4_launch<D_, 8>(a, ctas, s) : rows == 16 ? p4_launch<D_, 16>(a, ctas, s) : p4_launch<D_, 32>(a, ctas, s))
   return a.c == 64 ? P4_ROWS(64) : P4_ROWS(128);
 #undef P4_ROWS
 }
