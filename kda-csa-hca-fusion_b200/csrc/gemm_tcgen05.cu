@@ -795,13 +795,15 @@ int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes
   return KCH_OK;
 }
 
-// Packed rows [rows, heads, c] in bf16, tokens ld elements apart: boxes of 64 channels of a head and `box_rows` tokens, 128-byte swizzle.
-int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_rows) {
+// Packed rows [rows, heads, c] in bf16, tokens ld elements apart: boxes of 64 channels of `box_heads` heads and `box_rows` tokens, 128-byte
+// swizzle.
+int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_heads,
+                             uint32_t box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode_fn();
   if (!enc) { kch_set_error("cuTensorMapEncodeTiled is not available from the driver"); return KCH_ERR_CUDA; }
   cuuint64_t gdim[3] = {c, heads, rows};
   cuuint64_t gstr[2] = {(cuuint64_t)c * 2, (cuuint64_t)ld * 2};
-  cuuint32_t box[3] = {64, 1, box_rows};
+  cuuint32_t box[3] = {64, box_heads, box_rows};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -27,6 +27,7 @@ struct PgBatch {
   int shift;                           // log2(page_size)
   unsigned int* status;                // [0]: of expired waits, which ends the others; [1]: of tables, which ends none
   int n_kv, G, window;                 // key heads, query heads of one, window (attention only)
+  int rows, extra;                     // rows of an item, where the kernel leaves that open; places of the line before an item's steps
   uint32_t g_mul; int g_shift;         // n / G = n * g_mul >> 32 + g_shift for n < 2^31; g_mul 0: n >> g_shift
 };
 // With s = floor(log2 G) and M = floor(2^(32 + s) / G) + 1, M G exceeds 2^(32 + s) by at most G < 2^(s + 1): exact below 2^31.
@@ -64,22 +65,25 @@ __device__ __forceinline__ int pg_page(const PgBatch& a, int b, int index) {
 // One block of rows of a sequence: which keys its rows see together.
 // tiles of KT keys from first_key (a multiple of KT) on; the keys before `lo` no row sees: their pages need not be there any more
 struct PgSpan { int rows, lo, first_key, tiles, steps; };
-// R rows a block, KT keys a tile.  TWO: blocks of at most TWO rows take two tiles a step.
+// R rows a block (0: a.rows), KT keys a tile.  TWO: blocks of at most TWO rows (R 0: of half of them) take two tiles a step.
 template <int R, int KT, int TWO>
 __device__ __forceinline__ PgSpan pg_span(const PgBatch& a, const PgSeq& s, int block) {
   PgSpan x;
-  const int r0 = block * R, r1 = min(r0 + R, s.len * a.G);
+  const int all = R ? R : a.rows, two = R ? TWO : a.rows / 2;
+  const int r0 = block * all, r1 = min(r0 + all, s.len * a.G);
   x.rows = r1 - r0;
   const int64_t first = (int64_t)s.t0 + pg_token(a, r0), last = (int64_t)s.t0 + pg_token(a, r1 - 1);      // positions of the first and the last query
   const int hi = (int)min(last + 1, (int64_t)s.kv);
   x.lo = a.window > 0 ? (int)min(max(first - a.window + 1, (int64_t)0), (int64_t)s.kv) : 0;
   x.first_key = x.lo / KT * KT;
   x.tiles = hi > x.first_key ? (hi - x.first_key + KT - 1) / KT : 0;
-  x.steps = max(x.rows <= TWO ? (x.tiles + 1) / 2 : x.tiles, 1);            // (a row without keys is stored all the same)
+  x.steps = max(x.rows <= two ? (x.tiles + 1) / 2 : x.tiles, 1);            // (a row without keys is stored all the same)
   return x;
 }
 template <int R>
-__device__ __forceinline__ int pg_blocks(const PgBatch& a, const PgSeq& s) { return (s.len * a.G + R - 1) / R; }
+__device__ __forceinline__ int pg_blocks(const PgBatch& a, const PgSeq& s) {
+  return R ? (s.len * a.G + R - 1) / (R ? R : 1) : (int)((unsigned)(s.len * a.G + a.rows - 1) / (unsigned)a.rows);
+}
 // the keys [x, y) that row `row` (token * G + head of the group) of a sequence sees
 __device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int row) {
   const int64_t pos = (int64_t)s.t0 + pg_token(a, row);
@@ -88,8 +92,8 @@ __device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int ro
 
 // Where a CTA's range of steps begins.  (Steps are counted in 32 bits: the host refuses a call that could have 2^31 - 1.)
 struct PgPlace {
-  int per, left;                       // steps of a CTA; steps of this one
-  int b, h, block, step;
+  int per, left;                       // places of the line of a CTA; of this one
+  int b, h, block, step;               // step: place in the item (its steps come behind `extra` others)
   PgSeq s;                             // of b
   PgSpan x;                            // of the block
 };
@@ -99,7 +103,7 @@ struct PgPlace {
 template <int R, int KT, int TWO>
 __device__ __forceinline__ int pg_steps(const PgBatch& a, const PgSeq& s) {
   const int lane = threadIdx.x & 31, blocks = pg_blocks<R>(a, s);
-  int mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps : 0;
+  int mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps + a.extra : 0;
   for (unsigned many = __ballot_sync(0xffffffffu, blocks > 1); many; many &= many - 1) {
     const int from = __ffs(many) - 1;
     PgSeq t;
@@ -110,7 +114,7 @@ __device__ __forceinline__ int pg_steps(const PgBatch& a, const PgSeq& s) {
     const int nb = pg_blocks<R>(a, t);
     int sum = 0;
 #pragma unroll 1
-    for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps;
+    for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps + a.extra;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == from) mine = sum;
@@ -156,7 +160,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     return p.left > 0 ? (int)start : 0x7FFFFFFF;
   };
   int start;
-  if (a.B <= 32) {                     // every warp by itself: no memory, no barrier
+  if (a.B == 1 || (a.B <= 32 && (int64_t)a.N * a.G <= (int64_t)(R ? R : a.rows) * a.B)) {      // every warp by itself: no memory, no barrier
     const PgSeq s = pg_seq_or_none(a, lane);
     const int x = pg_steps<R, KT, TWO>(a, s), upto = pg_scan(x);
     total = __shfl_sync(0xffffffffu, upto, 31);
@@ -173,10 +177,12 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
   } else {
     int* base = reinterpret_cast<int*>(mem);                // [B + 1] steps before sequence b
     int* found = base + a.B + 1;
+    // (dealt out over the warps: one that has 32 sequences of several blocks takes 10 000 clocks for them)
+    const int deal = min((a.B + warps - 1) / warps, 32);
 #pragma unroll 1
-    for (int b0 = warp * 32; b0 < a.B; b0 += warps * 32) {
-      const int x = pg_steps<R, KT, TWO>(a, pg_seq_or_none(a, b0 + lane));
-      if (b0 + lane < a.B) base[b0 + lane + 1] = x;
+    for (int b0 = warp * deal; b0 < a.B; b0 += warps * deal) {
+      const int x = pg_steps<R, KT, TWO>(a, pg_seq_or_none(a, lane < deal ? b0 + lane : a.B));
+      if (lane < deal && b0 + lane < a.B) base[b0 + lane + 1] = x;
     }
     if (tid == 0) base[0] = 0;
     __syncthreads();
@@ -214,7 +220,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     if (blocks > 1) {
 #pragma unroll 1
       for (int i0 = 0; i0 < blocks; i0 += 32) {
-        const int i = i0 + lane, n = i < blocks ? pg_span<R, KT, TWO>(a, p.s, i).steps : 0, x = pg_scan(n);
+        const int i = i0 + lane, n = i < blocks ? pg_span<R, KT, TWO>(a, p.s, i).steps + a.extra : 0, x = pg_scan(n);
         const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
         if (hit) {
           const int at = __ffs(hit) - 1;
@@ -239,23 +245,28 @@ struct PgWalk {
   int first, count;                    // its steps that belong to this CTA
   PgSeq s;
   PgSpan x;
-  int left;                            // steps of the CTA behind them
+  int left;                            // places of the CTA's range behind them
+  int from, taken;                     // places of the item that are in it
   __device__ __forceinline__ PgWalk(const PgBatch& a_, const PgPlace& p)
-      : a(a_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), s(p.s), x(p.x), left(p.left) {
+      : a(a_), b(p.b), h(p.h), block(p.block), first(0), count(0), s(p.s), x(p.x), left(p.left), from(p.step), taken(0) {
     if (left > 0) take();
   }
-  __device__ __forceinline__ bool valid() const { return count > 0; }
+  __device__ __forceinline__ bool valid() const { return count > 0; }      // (a range that ends before an item's first step has no more of it)
   __device__ __forceinline__ bool starts() const { return first == 0; }
   __device__ __forceinline__ bool ends() const { return first + count == x.steps; }
+  // the CTA that has the end of an item which starts in this one's range and is its last
+  __device__ __forceinline__ int last(const PgPlace& p, int cta) const {
+    return (int)(((int64_t)p.per * cta + (p.left - taken) - from + a.extra + x.steps - 1) / p.per);
+  }
   __device__ __forceinline__ void next() {
-    first = 0;
+    from = 0;
     count = 0;
     if (left <= 0) return;
     if (++block == pg_blocks<R>(a, s)) {
       block = 0;
       if (++h == a.n_kv) {
         h = 0;
-        do { s = pg_seq(a, ++b); } while (s.len == 0);       // (steps are left, so a sequence with rows follows)
+        do { s = pg_seq(a, ++b); } while (s.len == 0);       // (places are left, so a sequence with rows follows)
       }
     }
     x = pg_span<R, KT, TWO>(a, s, block);
@@ -264,8 +275,10 @@ struct PgWalk {
 
  private:
   __device__ __forceinline__ void take() {
-    count = min(x.steps - first, left);
-    left -= count;
+    taken = min(x.steps + a.extra - from, left);
+    left -= taken;
+    first = max(from - a.extra, 0);
+    count = max(from + taken - a.extra, 0) - first;
   }
 };
 
@@ -289,7 +302,7 @@ struct PgAttend {                      // what both attention kernels get
   const void *q, *k, *v, *ks, *vs;      // (ks, vs: scales; float, in 4 bits bf16)
   void* out;
   int64_t ld_q, ld_k, ld_v;             // (ld_k, ld_v: of packed rows)
-  int c, page, zero_rest, slot_rows;
+  int c, page, zero_rest, slot_rows, q_map;      // q_map: queries are fetched by a tensor map
   float scale;                         // times log2(e)
   const void* sink; int sink_dtype;
   PgRecord* records; float* slots;

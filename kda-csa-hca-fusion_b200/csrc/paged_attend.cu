@@ -81,7 +81,7 @@ __device__ __forceinline__ bool pa_none(float weight) { return __float_as_uint(w
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
 // steps that a call can have at most, whatever the lengths on the device (of which no two share a row)
-static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1); }
+static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1 + a.extra); }
 
 static constexpr int pa_smem(int ROWS, int DMAX) { return (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4; }
 static_assert(pa_smem(64, 256) <= 232448 && PG_PLAN_BYTES(PG_MAX_B) <= pa_smem(16, 64), "shared memory; the plan lies in the tiles' memory");
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
     }
     if (w.starts() && !w.ends()) {
       rec.valid = 1; rec.b = w.b; rec.h = w.h; rec.block = w.block; rec.rows = w.x.rows; rec.row0 = w.s.row0;
-      rec.last = (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per);   // (it is the last of the range)
+      rec.last = w.last(place, blockIdx.x);                    // (it is the last of the range)
     }
   }
   if (tid == 0) a.records[blockIdx.x] = rec;
@@ -499,7 +499,7 @@ int kch_paged_check(const kch_paged_cache* p, const kch_paged_batch* b, int dtyp
 PgBatch kch_paged_batch_of(const kch_paged_cache* p, const kch_paged_batch* b);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c);
-int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
+int kch_paged_attend_tc5(PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 int kch_paged_attend_mma(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s);
 int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s);
 
@@ -524,6 +524,8 @@ static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   else if (rows > 32 * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
   else if (kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
+  // Prompts and 4-bit pages: blocks of whole tokens, so that a copy of a tensor map fetches their queries.
+  if (x.form == PA_TC5 && (kind == PG_ROWS || kind == KCH_INT4) && G <= 128) x.rows = 128 / G * G * 2;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
   return x;
 }
@@ -531,6 +533,11 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
   return pa_plan(p->batch.B, p->batch.N, p->nh / p->cache.n_kv, p->cache.kind, p->dtype, p->cache.c);
 }
 static PaPlan pa_plan(const kch_prompt_attend_args* p) { return pa_plan(p->B, p->N, p->nh / p->n_kv, PG_ROWS, p->dtype, p->c); }
+
+static void pa_line(PgBatch& a, const PaPlan& x, int kind) {
+  a.rows = x.rows;
+  a.extra = x.form != PA_SIMT && (kind == PG_ROWS || kind == KCH_INT4) ? 2 : 0;
+}
 
 // The launches of a call whose arguments are in order: the attention, and the joining of the items that are in parts.
 static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, void* workspace, cudaStream_t s) {
@@ -608,6 +615,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
+  pa_line(a.bt, x, p->cache.kind);
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
   // (an item's queries may be read again while its rows are stored)
@@ -666,6 +674,7 @@ extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) 
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
+  pa_line(a.bt, x, PG_ROWS);
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
   KCH_REQUIRE(a.bt.status != nullptr, "%s: cannot resolve the device status word", fn);
   return pa_launch(a, x, PG_ROWS, p->dtype, p->nh, p->workspace, kch_stream(stream));

@@ -514,9 +514,7 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
     }
     if (w.starts() && !w.ends()) {
       part = true;
-      if (ct == 0)
-        a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
-                                 w.x.rows, w.s.row0};
+      if (ct == 0) a.records[blockIdx.x] = {1, w.b, w.h, w.block, w.last(place, blockIdx.x), w.x.rows, w.s.row0};
     }
   }
   if (ct == 0 && !part) a.records[blockIdx.x].valid = 0;

@@ -60,6 +60,7 @@ template <int D, int KIND, int FEW>
 struct PtCfg {
   static constexpr int R = FEW ? FEW : 256, TWO = FEW ? FEW : 128, COPIES = FEW ? 128 / FEW : 1;
   static constexpr bool ROWS = KIND == PG_ROWS, Q4 = KIND == KCH_INT4, Q8 = KIND == KCH_FP8_E4M3 || KIND == KCH_INT8;
+  static constexpr bool OPEN = ROWS || Q4;               // blocks of whole tokens (a.bt.rows), whose queries a tensor map's copies fetch
   static constexpr bool CODES = Q8 || Q4;                // pages hold codes, which a warpgroup turns into tiles
   static constexpr bool APART = FEW && !CODES;           // keys' and values' pages are copied by a warp each
   static constexpr int PANELS = D / 64, TILE = PT_KT * D * 2, RAW = Q4 ? PT_KT * D / 2 : PT_KT * D, GROUPS = D / 32;      // (GROUPS: scales of a row, Q4)
@@ -350,9 +351,10 @@ __device__ __noinline__ void pt_slow_row(const PgAttend& a, int b, int row0, int
 
 template <int D, int KIND, int FEW>
 __global__ void __launch_bounds__(PtCfg<D, KIND, FEW>::THREADS, 1)
-paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PgAttend a) {
+paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
+                        const __grid_constant__ PgAttend a) {
   typedef PtCfg<D, KIND, FEW> C;
-  typedef PgWalk<C::R, PT_KT, C::TWO> Walk;
+  typedef PgWalk<C::OPEN ? 0 : C::R, PT_KT, C::TWO> Walk;
   extern __shared__ __align__(1024) uint8_t pt_raw[];    // (no room to align it by hand; every block begins its memory there)
   PtSmem<D, KIND, FEW>& sm = *reinterpret_cast<PtSmem<D, KIND, FEW>*>(pt_raw);
   if (smem_addr_u32(pt_raw) & 1023) {
@@ -360,23 +362,25 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     return;
   }
   const int tid = threadIdx.x, warp = t5_warp_index(), lane = tid & 31, G = a.bt.G, n_kv = a.bt.n_kv, slot_rows = a.slot_rows;
+  const int R = C::OPEN ? a.bt.rows : C::R, TWO = C::OPEN ? a.bt.rows / 2 : C::TWO;      // rows of an item, and of either warpgroup
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbarrier_init(&sm.full[i], C::CODES ? 4 : 1); mbarrier_init(&sm.empty[i], 1); }
     for (int i = 0; i < C::RAWS; ++i) { mbarrier_init(&sm.raw_full[i], 1); mbarrier_init(&sm.raw_empty[i], 4); }
     for (int i = 0; i < C::SCALES; ++i) { mbarrier_init(&sm.sc_full[i], 64); mbarrier_init(&sm.sc_empty[i], 8); }
-    mbarrier_init(&sm.q_full, C::APART ? 1 : 2);
+    mbarrier_init(&sm.q_full, C::APART || (C::OPEN && a.q_map) ? 1 : 2);
     mbarrier_init(&sm.q_empty, 1);
     sm.odd[0] = sm.odd[1] = sm.nan_code = 0u;
     for (int i = 0; i < 2; ++i) { mbarrier_init(&sm.s_full[i], 1); mbarrier_init(&sm.p_full[i], 4); mbarrier_init(&sm.pv_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    if (C::OPEN && a.q_map) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr_u32(&sm.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const PgPlace place = pg_plan<C::R, PT_KT, C::TWO>(a.bt, sm.kv, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<C::OPEN ? 0 : C::R, PT_KT, C::TWO>(a.bt, sm.kv, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   t5_fence_before();
@@ -385,7 +389,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   const uint32_t tmem = sm.tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbarrier_wait_bounded(bar, parity & 1, KCH_STATUS_PAGED_ATTEND, PT_SPIN, a.bt.status); };
   // do the warpgroups have rows of their own, or the same rows and every other tile?
-  auto paired = [](const Walk& w) { return !FEW && w.x.rows > C::TWO; };
+  auto paired = [&](const Walk& w) { return !FEW && w.x.rows > TWO; };
   // The ring holds an item's tiles in the order in which they are used.  Rows of both: K0, then V0 K1, V1 K2, ..; rows of one: K0 K1,
   // then V0 K2 V1 K3, V2 K4 V3 K5, ..
 
@@ -539,7 +543,27 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const int t = tid - (128 - FETCH);
       int c = 0, kt = 0;
       bool ok = true;
-      for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
+      if (C::OPEN && a.q_map) {
+        // whole tokens: their heads of this key head, 64 channels a copy, for either warpgroup's tile.  (The rows behind a sequence's last
+        // token are the next one's, or zeros: no row of the item.)
+        if (warp == 2) {
+          const int tokens = TWO / G, bytes = TWO * 128 * C::PANELS;
+          for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
+            if (c) ok = wait(&sm.q_empty, c - 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const bool both = paired(w);
+            if (lane == 0) mbarrier_expect_tx(&sm.q_full, both ? 2 * bytes : bytes);
+            __syncwarp();
+            if (lane < (both ? 2 : 1) * C::PANELS) {
+              const int x = lane / C::PANELS, panel = lane % C::PANELS;
+              pt_tma_3d(sm.q[x] + panel * (128 * 128), &qmap, panel * 64, w.h * G, w.s.row0 + (w.block * 2 + x) * tokens, &sm.q_full);
+            }
+          }
+          if (c) wait(&sm.q_full, c - 1);                // (no copy is in flight when the block ends)
+        }
+      }
+      if (!(C::OPEN && a.q_map)) for (Walk w(a.bt, place); w.valid() && ok; w.next(), ++c) {
         if (c) ok = wait(&sm.q_empty, c - 1);
         if (!ok) break;
         constexpr int CHUNKS = D / 8, STEP = FETCH / CHUNKS;       // 16 bytes a thread
@@ -549,7 +573,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         // Every STEP'th row is a thread's.  Head, source and place in the swizzle are counted on from row to row: computed
         // anew for each they made 256 rows 13000 cycles, more than what is left of an item once its last scores are there.
         const int r0 = t / CHUNKS, skip = pg_token(a.bt, STEP), turn = STEP - skip * G;
-        const int row0 = w.block * C::R + r0, tok0 = pg_token(a.bt, row0);
+        const int row0 = w.block * R + r0, tok0 = pg_token(a.bt, row0);
         int g = row0 - tok0 * G;
         const bf16* src = (const bf16*)a.q + (w.s.row0 + tok0) * a.ld_q + (w.h * G + g) * D + k * 8;
         const int64_t ahead = skip * a.ld_q + turn * D, over = a.ld_q - (int64_t)G * D;
@@ -557,11 +581,15 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const uint32_t at = ((k & 7) ^ (r0 & 7)) << 4;
 #pragma unroll 1
         for (int r = r0; r < rows; r += 4 * STEP, to += 4 * STEP * 128) {
-          if (!FEW && r == 128 + r0) to += 128 * D * 2 - 128 * 128;      // the second tile
+          if (!FEW && !C::OPEN && r == 128 + r0) to += 128 * D * 2 - 128 * 128;      // the second tile
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (r + j * STEP >= rows) break;
-            const uint32_t dst = to + j * (STEP * 128) + (at ^ ((j * STEP & 7) << 4));
+            uint32_t dst = to + j * (STEP * 128) + (at ^ ((j * STEP & 7) << 4));
+            if constexpr (C::OPEN) {                     // (tiles of TWO rows, which may be no multiple of STEP)
+              const int x = r + j * STEP >= TWO ? 1 : 0, i = r + j * STEP - x * TWO;
+              dst = smem_addr_u32(sm.q[x]) + (k >> 3) * (128 * 128) + i * 128 + (((k & 7) ^ (i & 7)) << 4);
+            }
             if (flip) {
               uint4 u = __ldg(reinterpret_cast<const uint4*>(src));
               u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
@@ -629,9 +657,9 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     for (Walk w(a.bt, place); w.valid(); w.next()) {
       const bool pair = paired(w);
       constexpr int APART = 128 / C::COPIES;
-      const int ri = pair ? x * 128 + r : r % APART, sub = FEW ? r >> 5 : 0;      // row of the item, part of a tile's keys
-      const bool live = ri < w.x.rows;
-      const int2 keys = pg_sees(a.bt, w.s, w.block * C::R + ri);           // those of the row
+      const int ri = pair ? x * TWO + r : r % APART, sub = FEW ? r >> 5 : 0;      // row of the item, part of a tile's keys
+      const bool live = ri < w.x.rows && (!C::OPEN || r < TWO);
+      const int2 keys = pg_sees(a.bt, w.s, w.block * R + ri);           // those of the row
       float m = -INFINITY, l = 0.f;
       for (int s = 0; s < w.count; ++s, ++n) {
         const int tile = pair ? w.first + s : 2 * (w.first + s) + x;
@@ -671,6 +699,8 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (!whole) {
 #pragma unroll
               for (int k = 0; k < N; k += 32) {
+                // (a chunk's edge lies in one 32 of a tile, or two)
+                if (C::OPEN && __all_sync(0xffffffffu, !live || (lo <= col + k && hi >= col + k + 32))) continue;
                 const uint32_t mk = pt_range(lo - col - k, hi - col - k);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) sv[k + e] = mk & (1u << e) ? sv[k + e] : 0xFF800000u;
@@ -790,21 +820,21 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       const bool direct = w.starts() && w.ends();
       float* slot = a.slots + (2 * (int64_t)blockIdx.x + (w.starts() ? 1 : 0)) * pg_slot_floats(slot_rows, D);
       auto out_row = [&](int i) {                        // of the item's row i
-        const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
+        const int rr = w.block * R + i, tk = pg_token(a.bt, rr);
         return (bf16*)a.out + ((int64_t)(w.s.row0 + tk) * (n_kv * G) + w.h * G + rr - tk * G) * D;
       };
       auto factor = [&](int i, float l, float shift) {   // 1 / the row's denominator
         if (!direct) return 1.f;
         float below = l;
         if (a.sink && l > 0.f) {
-          const int rr = w.block * C::R + i;
+          const int rr = w.block * R + i;
           below += ex2_fast(ld_any(a.sink, w.h * G + rr - pg_token(a.bt, rr) * G, a.sink_dtype) * PG_LOG2E - shift);
         }
         return l == 0.f ? 0.f : 1.f / below;
       };
       auto redo = [&](int i, float shift, float f, int c0, int c1) {     // a row that is not finite, key by key, on the warp
         const int span = PT_KT * (pair ? 1 : 2), part0 = w.x.first_key + w.first * span, part1 = part0 + w.count * span;
-        const int rr = w.block * C::R + i, tk = pg_token(a.bt, rr);
+        const int rr = w.block * R + i, tk = pg_token(a.bt, rr);
         const int2 k = pg_sees(a.bt, w.s, rr);
         pt_slow_row<D, KIND>(a, w.b, w.s.row0, w.h, (const bf16*)a.q + (w.s.row0 + tk) * a.ld_q + (w.h * G + rr - tk * G) * D, max(k.x, part0),
                              min(k.y, part1), a.scale < 0.f ? -sc : sc, shift, f, out_row(i), direct ? nullptr : slot + (int64_t)i * D, c0, c1);
@@ -928,9 +958,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       ring += (pair ? 2 : 4) * w.count;
       if (w.starts() && !w.ends()) {
         part = true;
-        if (tid == 128)
-          a.records[blockIdx.x] = {1, w.b, w.h, w.block, (int)(((int64_t)place.per * blockIdx.x + (place.left - w.count) + w.x.steps - 1) / place.per),
-                                   w.x.rows, w.s.row0};
+        if (tid == 128) a.records[blockIdx.x] = {1, w.b, w.h, w.block, w.last(place, blockIdx.x), w.x.rows, w.s.row0};
       }
     }
     if (tid == 128 && !part) a.records[blockIdx.x].valid = 0;
@@ -1021,12 +1049,12 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 // ---- host -------------------------------------------------------------------------------------------------------------------
 int kch_make_tensor_map_pages(CUtensorMap* map, const void* base, int elem_bytes, uint64_t pages, uint32_t n_kv, uint32_t page_size, uint32_t c,
                               uint32_t box_rows, bool plain = false);
-int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_rows);
+int kch_make_tensor_map_rows(CUtensorMap* map, const void* base, uint64_t rows, uint32_t heads, uint64_t ld, uint32_t c, uint32_t box_heads, uint32_t box_rows);
 
 bool kch_paged_attend_tc5_supported(int dtype, int c) { return dtype == KCH_BF16 && (c == 64 || c == 128); }
 
 template <int D, int KIND, int FEW>
-static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAttend& a, int ctas, cudaStream_t s) {
+static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, const PgAttend& a, int ctas, cudaStream_t s) {
   const int smem = (int)sizeof(PtSmem<D, KIND, FEW>);
   static std::atomic<uint64_t> done{0};                  // devices on which the kernel has its shared memory
   int dev = 0;
@@ -1035,25 +1063,31 @@ static int pt_launch(const CUtensorMap& km, const CUtensorMap& vm, const PgAtten
     KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_tc5_kernel<D, KIND, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev <= 63) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
   }
-  paged_attend_tc5_kernel<D, KIND, FEW><<<ctas, PtCfg<D, KIND, FEW>::THREADS, smem, s>>>(km, vm, a);
+  paged_attend_tc5_kernel<D, KIND, FEW><<<ctas, PtCfg<D, KIND, FEW>::THREADS, smem, s>>>(km, vm, qm, a);
   KCH_LAUNCH_OK();
   return KCH_OK;
 }
 
-int kch_paged_attend_tc5(const PgAttend& a, int kind, int rows, int ctas, cudaStream_t s) {
-  CUtensorMap km, vm;
-  if (kind == PG_ROWS) {
-    int rc = kch_make_tensor_map_rows(&km, a.k, a.bt.N, a.bt.n_kv, a.ld_k, a.c, PT_KT);
-    if (rc == KCH_OK) rc = kch_make_tensor_map_rows(&vm, a.v, a.bt.N, a.bt.n_kv, a.ld_v, a.c, PT_KT);
+int kch_paged_attend_tc5(PgAttend& a, int kind, int rows, int ctas, cudaStream_t s) {
+  CUtensorMap km, vm, qm = {};
+  // (a negative scale's sign goes to the queries on their way: no plain copies)
+  a.q_map = (kind == PG_ROWS || kind == KCH_INT4) && a.bt.G <= 128 && a.scale >= 0.f;
+  if (a.q_map) {
+    const int rc = kch_make_tensor_map_rows(&qm, a.q, a.bt.N, (uint32_t)a.bt.n_kv * a.bt.G, a.ld_q, a.c, a.bt.G, a.bt.rows / 2 / a.bt.G);
     if (rc != KCH_OK) return rc;
-    return a.c == 64 ? pt_launch<64, PG_ROWS, 0>(km, vm, a, ctas, s) : pt_launch<128, PG_ROWS, 0>(km, vm, a, ctas, s);
+  }
+  if (kind == PG_ROWS) {
+    int rc = kch_make_tensor_map_rows(&km, a.k, a.bt.N, a.bt.n_kv, a.ld_k, a.c, 1, PT_KT);
+    if (rc == KCH_OK) rc = kch_make_tensor_map_rows(&vm, a.v, a.bt.N, a.bt.n_kv, a.ld_v, a.c, 1, PT_KT);
+    if (rc != KCH_OK) return rc;
+    return a.c == 64 ? pt_launch<64, PG_ROWS, 0>(km, vm, qm, a, ctas, s) : pt_launch<128, PG_ROWS, 0>(km, vm, qm, a, ctas, s);
   }
   const bool q4 = kind == KCH_INT4;
   const int es = kind == KCH_BF16 ? 2 : 1, box = a.page < PT_KT ? a.page : PT_KT, wide = q4 ? a.c / 2 : a.c;
   int rc = kch_make_tensor_map_pages(&km, a.k, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, wide, box, q4);
   if (rc == KCH_OK) rc = kch_make_tensor_map_pages(&vm, a.v, es, (uint64_t)a.bt.num_pages, a.bt.n_kv, a.page, wide, box, q4);
   if (rc != KCH_OK) return rc;
-#define PT_GO(D_, K_, F_) pt_launch<D_, K_, F_>(km, vm, a, ctas, s)
+#define PT_GO(D_, K_, F_) pt_launch<D_, K_, F_>(km, vm, qm, a, ctas, s)
 #define PT_KIND(D_)                                                                            \
   (kind == KCH_FP8_E4M3 ? PT_GO(D_, KCH_FP8_E4M3, 0) : kind == KCH_INT8 ? PT_GO(D_, KCH_INT8, 0) : q4 ? PT_GO(D_, KCH_INT4, 0) \
    : rows == 16 ? PT_GO(D_, KCH_BF16, 16) : rows == 32 ? PT_GO(D_, KCH_BF16, 32) : PT_GO(D_, KCH_BF16, 0))
