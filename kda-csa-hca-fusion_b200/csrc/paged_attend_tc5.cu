@@ -715,13 +715,18 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               t1 = fmaxf(t1, fmaxf(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])));
             }
           };
+          int begin = 0, end = PT_KT;                    // without the half of a tile of which no row of the warp sees a key
+          if (C::OPEN && !whole) {
+            if (__all_sync(0xffffffffu, !live || hi <= 64)) end = 64;
+            else if (__all_sync(0xffffffffu, !live || lo >= 64)) begin = 64;
+          }
           uint32_t few[32];                              // (FEW: 32 keys a warp, which stay)
           if constexpr (FEW != 0) {
             fetch(few, from);
             highest(few);
           } else {
 #pragma unroll 1
-            for (int col = 0; col < PT_KT; col += 64) {
+            for (int col = begin; col < end; col += 64) {
               uint32_t sv[64];
               fetch(sv, col);
               highest(sv);
@@ -783,10 +788,14 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             weigh(few, from);
           } else {
 #pragma unroll 1
-            for (int col = 0; col < PT_KT; col += 64) {
+            for (int col = begin; col < end; col += 64) {
               uint32_t sv[64];
               fetch(sv, col);
               weigh(sv, col);
+            }
+            if (C::OPEN && end - begin < PT_KT) {
+              const uint32_t zero[32] = {};
+              pt_st(tS + (begin ? 0u : 32u), zero);
             }
           }
           float la, lb;
