@@ -86,26 +86,42 @@ __device__ __forceinline__ uint32_t pc_codes2(float x0, float x1, float s, float
   return ((uint32_t)a0 & 0xFFu) | (((uint32_t)a1 & 0xFFu) << 8);
 }
 
-// 4 bits, of 32 channels (4 threads'): the smallest number of 5 bits, 7 times which is `top` or more (top > 0, as bits; 7 s is exact in 32
-// bits), and the codes of 8 values as a word, the first in its lowest bits.
+// 4 bits, of 32 channels (4 threads'): the smallest number of 5 bits, 7 times which is `top` or more (top > 0, as bits).  7 s is exact in 32 bits,
+// so that the two comparisons are: whether the product with 1 / 7 was rounded up or down does not matter.
 #define PC_MOST4 0x7DE00000u           // 7 * 2^122: 24 s, which the attention adds in bf16, stays a number
 __device__ __forceinline__ float pc_scale4(uint32_t top) {
   const float most = __uint_as_float(top);
-  uint32_t b = (__float_as_uint(most / 7.f) + 0x7FFFFu) & 0xFFF80000u;
-  if (7.f * __uint_as_float(b) < most) b += 0x80000u;    // (the quotient was rounded down onto a number of 5 bits)
+  uint32_t b = (__float_as_uint(most * 0.142857142857142857f) + 0x7FFFFu) & 0xFFF80000u;
+  if (7.f * __uint_as_float(b - 0x80000u) >= most) b -= 0x80000u;
+  if (7.f * __uint_as_float(b) < most) b += 0x80000u;
   return fmaxf(__uint_as_float(b), 1.17549435e-38f);
 }
+// The codes of 8 values as a word, the first in its lowest bits: x / s by one step from x times the reciprocal, plus 1.5 * 2^23 + 8, whose lowest bits
+// are then the nearest whole number to the quotient, and 8, ties to even.  A quotient in the middle between two codes comes out exactly;
+// bf16 values have no other that is nearer to it than 10^-3 (x has 8 bits, s 5), values in 32 bits have: there the true quotient decides.
+template <typename T>
 __device__ __forceinline__ uint32_t pc_codes4(const float (&x)[8], float s) {
-  const float lo = 1.f - 4.76837158203125e-07f, hi = 1.f + 4.76837158203125e-07f, inv = 1.f / s;      // 2^-21
+  const float inv = 1.f / s;
   uint32_t w = 0u;
+  float near = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float q = x[e] * inv;
-    int code = (int)rintf(q * lo);
-    if (code != (int)rintf(q * hi)) code = (int)rintf(pc_quotient(x[e], s));
-    w |= (uint32_t)(code + 8) << (4 * e);
+  for (int e = 7; e >= 0; --e) {
+    float q = x[e] * inv;
+    q = fmaf(fmaf(-q, s, x[e]), inv, q);
+    const float t = q + 12582920.f;
+    if constexpr (sizeof(T) == 4) near = fmaxf(near, fabsf(q - (t - 12582920.f)));
+    w = w * 16u + __float_as_uint(t);                    // (of 12582912's bits 0x4B400000 is left, shifted: taken off below)
   }
-  return w;
+  if constexpr (sizeof(T) == 4) {
+    if (near > 0.49999f) {
+      w = 0u;
+#pragma unroll
+      for (int e = 7; e >= 0; --e) w = w * 16u + (uint32_t)((int)rintf(pc_quotient(x[e], s)) + 8);
+      return w;
+    }
+  }
+  constexpr uint32_t left = 0x4B400000u * 0x11111111u;
+  return w - left;
 }
 
 // where packed row t lies: its sequence by bisection of cu_seqlens, then page and row.  Rows (page * n_kv * page_size + row) of the
@@ -156,6 +172,20 @@ __device__ __forceinline__ PcWords<T> pc_words(const void* p) {
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.w[i] = __ldg((const uint4*)p + i);
   return x;
+}
+
+// 8 values of 4 bits in bf16, rounded once: 16 + u by the code's place in the mantissa of 16, less 24, times s.
+__device__ __forceinline__ uint32_t pc_fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint4 pc_values4(uint32_t w, uint32_t s) {
+  const uint32_t even = w << 3, odd = w >> 1, ss = s | s << 16;      // (of each byte the lower and the upper code, in its bits 3 .. 6)
+  uint32_t x[4] = {__byte_perm(even, odd, 0x4400), __byte_perm(even, odd, 0x5511), __byte_perm(even, odd, 0x6622), __byte_perm(even, odd, 0x7733)};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = pc_fma2(pc_fma2((x[e] & 0x00780078u) | 0x41804180u, 0x3F803F80u, 0xC1C0C1C0u), ss, 0u);
+  return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
@@ -250,13 +280,13 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
         for (int i = 0; i < PC_FLIGHT; ++i) {
           const int row = r + i * step;
           if (row >= rows) break;
+          if constexpr (sizeof(T) == 2) {                // (0 is +0, where there is no page too)
+            *(uint4*)packed(row) = pc_values4(u[i], __float_as_uint(f[i]) >> 16);
+            continue;
+          }
           float x[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = (float)((int)((u[i] >> (4 * e)) & 15u) - 8) * f[i];
-          if (site < 0) {                                // (0 * -8 is -0)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-          }
+          for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((int)((u[i] >> (4 * e)) & 15u) - 8), f[i], 0.f);
           pc_store(packed(row), x);
         }
       }
@@ -282,7 +312,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
           if constexpr (BITS == 4) {
             const bool number = top <= PC_MOST4;         // (what is not reads as NaN)
             const float s = top && number ? pc_scale4(top) : 1.f;
-            *(uint32_t*)((uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2) = number ? pc_codes4(x[i], s) : 0x88888888u;
+            *(uint32_t*)((uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2) = number ? pc_codes4<T>(x[i], s) : 0x88888888u;
             if (d % 32 == 0) ((uint16_t*)a.scales[row & 1])[pool_row(row) * (a.c / 32) + d / 32] = number ? (uint16_t)(__float_as_uint(s) >> 16) : 0x7FC0u;
             continue;
           }
