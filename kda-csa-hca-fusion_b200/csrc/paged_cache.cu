@@ -101,7 +101,8 @@ __device__ __forceinline__ float pc_scale4(uint32_t top) {
 // bf16 values have no other that is nearer to it than 10^-3 (x has 8 bits, s 5), values in 32 bits have: there the true quotient decides.
 template <typename T>
 __device__ __forceinline__ uint32_t pc_codes4(const float (&x)[8], float s) {
-  const float inv = 1.f / s;
+  float inv;                                             // (within a unit of its last place, which the step makes up for)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   uint32_t w = 0u;
   float near = 0.f;
 #pragma unroll
@@ -190,9 +191,9 @@ __device__ __forceinline__ uint4 pc_values4(uint32_t w, uint32_t s) {
 
 // A warp has one token, or two where it has lanes for them; GROUP threads a row (key head, k or v) of it.  The page is
 // looked up once a token, and four rows a thread are in flight.  Where tokens are few, several warps share one's rows.  READ: pages
-// -> packed rows, else packed rows -> pages.  BITS of what is stored: 8, 4, or 0: the rows as they are.
+// -> packed rows, else packed rows -> pages.
 #define PC_FLIGHT 4
-template <typename T, int GROUP, bool READ, int BITS>
+template <typename T, int GROUP, bool READ, bool Q8>
 __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_constant__ PgRows a) {
   __shared__ int32_t scu[PC_SMEM_B + 1];
   const int32_t* cu = a.bt.cu;
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
     // (k and v of a head one after the other: row 2 h + kv)
     auto packed = [&](int row) { return (T*)a.x[row & 1] + t * a.ld[row & 1] + (int64_t)(row >> 1) * a.c + d; };
     auto pool_row = [&](int row) { return site + (int64_t)(row >> 1) * a.page; };
-    if constexpr (BITS == 0) {
+    if constexpr (!Q8) {
       if ((READ ? t >= a.bt.N : site < 0) || !in_row) continue;
       if (READ && site == -1 && !a.zero_rest) continue;
       for (int r = row0; r < rows; r += step * PC_FLIGHT) {
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
           for (int k = 0; k < (int)sizeof(T) / 2; ++k) to[k] = x[i].w[k];
         }
       }
-    } else if constexpr (READ && BITS == 8) {
+    } else if constexpr (READ) {
       if (t >= a.bt.N || !in_row || (site == -1 && !a.zero_rest)) continue;
       for (int r = row0; r < rows; r += step * PC_FLIGHT) {
         uint2 u[PC_FLIGHT] = {};
@@ -261,35 +262,6 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
           pc_store(packed(row), x);
         }
       }
-    } else if constexpr (READ) {
-      if (t >= a.bt.N || !in_row || (site == -1 && !a.zero_rest)) continue;
-      for (int r = row0; r < rows; r += step * PC_FLIGHT) {
-        uint32_t u[PC_FLIGHT];
-        float f[PC_FLIGHT];
-#pragma unroll
-        for (int i = 0; i < PC_FLIGHT; ++i) {
-          const int row = r + i * step;
-          u[i] = 0u;
-          f[i] = 0.f;
-          if (row < rows && site >= 0) {
-            u[i] = __ldg((const uint32_t*)((const uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2));
-            f[i] = __bfloat162float(((const bf16*)a.scales[row & 1])[pool_row(row) * (a.c / 32) + d / 32]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < PC_FLIGHT; ++i) {
-          const int row = r + i * step;
-          if (row >= rows) break;
-          if constexpr (sizeof(T) == 2) {                // (0 is +0, where there is no page too)
-            *(uint4*)packed(row) = pc_values4(u[i], __float_as_uint(f[i]) >> 16);
-            continue;
-          }
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((int)((u[i] >> (4 * e)) & 15u) - 8), f[i], 0.f);
-          pc_store(packed(row), x);
-        }
-      }
     } else {
       const bool here = site >= 0 && in_row;
       // (all lanes of the warp take the same rounds: a row's maximum is found by shuffles)
@@ -307,15 +279,8 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
 #pragma unroll
           for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
 #pragma unroll
-          for (int o = BITS == 4 ? 2 : GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int o = GROUP / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           if (!here || row >= rows) continue;
-          if constexpr (BITS == 4) {
-            const bool number = top <= PC_MOST4;         // (what is not reads as NaN)
-            const float s = top && number ? pc_scale4(top) : 1.f;
-            *(uint32_t*)((uint8_t*)a.pages[row & 1] + (pool_row(row) * a.c + d) / 2) = number ? pc_codes4<T>(x[i], s) : 0x88888888u;
-            if (d % 32 == 0) ((uint16_t*)a.scales[row & 1])[pool_row(row) * (a.c / 32) + d / 32] = number ? (uint16_t)(__float_as_uint(s) >> 16) : 0x7FC0u;
-            continue;
-          }
           const bool finite = top < 0x7F800000u;
           float s = top ? fmaxf(__uint_as_float(top) / (a.kind == KCH_FP8_E4M3 ? 448.f : 127.f), 1.17549435e-38f) : 1.f;
           const float inv = 1.f / s;
@@ -335,16 +300,157 @@ __global__ void __launch_bounds__(PC_THREADS) paged_rows_kernel(const __grid_con
 // 8-bit pages: one wave of blocks, whose warps walk the tokens; more of them would only wait for the others' end (32768 tokens of 8 heads
 // of 128 read from e4m3: 38 us, 42 with 8 to an SM).  Rows that are copied: 8 to an SM, of which it holds 6 (28708 such tokens written
 // as bf16: 41 us, 44 in one wave, where an SM that is behind stays so).
-template <typename T, int GROUP, bool READ, int BITS>
+template <typename T, int GROUP, bool READ, bool Q8>
 static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
   static const int resident = [] {
     int n = 0;
-    if (BITS == 0) return 8;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, BITS>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
+    if (!Q8) return 8;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows_kernel<T, GROUP, READ, Q8>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
   }();
   const int64_t wave = (int64_t)resident * KCH_SMS / a.parts;
   const dim3 grid((unsigned)(blocks < wave ? blocks : wave), (unsigned)a.parts);
-  paged_rows_kernel<T, GROUP, READ, BITS><<<grid, PC_THREADS, 0, s>>>(a);
+  paged_rows_kernel<T, GROUP, READ, Q8><<<grid, PC_THREADS, 0, s>>>(a);
+}
+
+
+// 4 bits.  16 values a thread, so that two of them share a scale; the rows of a batch of two rounds are asked for before the page is looked up, or
+// the next token's page after the rows of this one.  (With 8 values a thread and each waited for after the other, 26 096 tokens of 8 key heads of
+// 128 were written in 65 us and read in 36.5.)
+template <typename T> struct Pc16 { uint4 w[sizeof(T)]; };
+template <typename T, int GROUP, bool READ>
+__global__ void __launch_bounds__(PC_THREADS) paged_rows4_kernel(const __grid_constant__ PgRows a) {
+  constexpr int FLIGHT = READ ? 4 : 2;                   // rows of a thread in flight
+  __shared__ int32_t scu[PC_SMEM_B + 1];
+  const int32_t* cu = a.bt.cu;
+  if (a.bt.B <= PC_SMEM_B) {
+    for (int i = threadIdx.x; i <= a.bt.B; i += PC_THREADS) scu[i] = __ldg(a.bt.cu + i);
+    __syncthreads();
+    cu = scu;
+  }
+  const int lane = threadIdx.x & 31, each = 32 / a.tokens, mine = lane & (each - 1);      // lanes of a token, this one among them
+  const int d = (mine & (GROUP - 1)) * 16, rows = 2 * a.n_kv, step = each / GROUP * a.parts, row0 = mine / GROUP + each / GROUP * blockIdx.y;
+  const bool in_row = d < a.c;
+  const int64_t stride = (int64_t)gridDim.x * (PC_THREADS / 32) * a.tokens;
+  int64_t t = ((int64_t)blockIdx.x * (PC_THREADS / 32) + (threadIdx.x >> 5)) * a.tokens + lane / each;
+  auto site_of = [&](int64_t t) { return t < a.bt.N ? pc_site(a, cu, (int)t) : -1; };
+  int64_t site = READ ? site_of(t) : -1;
+  for (; t - lane / each < a.bt.N; t += stride) {
+    // (k and v of a head one after the other: row 2 h + kv)
+    auto packed = [&](int row) { return (T*)a.x[row & 1] + t * a.ld[row & 1] + (int64_t)(row >> 1) * a.c + d; };
+    auto codes = [&](int row) { return (uint2*)((uint8_t*)a.pages[row & 1] + ((site + (int64_t)(row >> 1) * a.page) * a.c + d) / 2); };
+    auto mark = [&](int row) { return (uint16_t*)a.scales[row & 1] + (site + (int64_t)(row >> 1) * a.page) * (a.c / 32) + d / 32; };
+    if constexpr (READ) {
+      const bool fill = t < a.bt.N && in_row && (site != -1 || a.zero_rest);
+      int64_t next = -1;
+      for (int r = row0; r < rows; r += step * FLIGHT) {
+        uint2 u[FLIGHT];
+        uint32_t s[FLIGHT];
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int row = r + i * step;
+          u[i] = make_uint2(0x88888888u, 0x88888888u);
+          s[i] = 0u;
+          if (fill && row < rows && site >= 0) {
+            u[i] = __ldg(codes(row));
+            s[i] = __ldg(mark(row));
+          }
+        }
+        if (r == row0) next = site_of(t + stride);
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int row = r + i * step;
+          if (!fill || row >= rows) break;
+          if constexpr (sizeof(T) == 2) {
+            T* to = packed(row);
+            const uint4 x = pc_values4(u[i].x, s[i]), y = pc_values4(u[i].y, s[i]);
+            if (((uintptr_t)to & 31) == 0) {             // (in halves, every sector is written twice)
+              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w), "r"(y.x), "r"(y.y),
+                           "r"(y.z), "r"(y.w) : "memory");
+            } else {
+              *(uint4*)to = x;
+              *((uint4*)to + 1) = y;
+            }
+          } else {
+            const float f = __uint_as_float(s[i] << 16);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = h ? u[i].y : u[i].x;
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((int)((w >> (4 * e)) & 15u) - 8), f, 0.f);      // (0 is +0)
+              pc_store(packed(row) + 8 * h, x);
+            }
+          }
+        }
+      }
+      site = row0 < rows ? next : site_of(t + stride);
+    } else {
+      // (what belongs to no sequence is not read)
+      const bool there = t < a.bt.N && in_row && t >= cu[0] && t < cu[a.bt.B];
+      auto ask = [&](int r0, Pc16<T> (&x)[FLIGHT]) {
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int row = r0 + row0 + i * step;
+#pragma unroll
+          for (int k = 0; k < (int)sizeof(T); ++k) x[i].w[k] = there && row < rows ? __ldg((const uint4*)packed(row) + k) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      };
+      Pc16<T> x[FLIGHT], ahead[FLIGHT];
+      ask(0, x);
+      site = there ? site_of(t) : -1;
+      // (all lanes of the warp take the same rounds: a group's maximum is found by a shuffle)
+      for (int r0 = 0; r0 < rows; r0 += step * FLIGHT) {
+        if (r0 + step * FLIGHT < rows) ask(r0 + step * FLIGHT, ahead);
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) {
+          const int row = r0 + row0 + i * step;
+          float v[2][8];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if constexpr (sizeof(T) == 2) {
+              const uint32_t w[8] = {x[i].w[0].x, x[i].w[0].y, x[i].w[0].z, x[i].w[0].w, x[i].w[1].x, x[i].w[1].y, x[i].w[1].z, x[i].w[1].w};
+              v[e >> 3][e & 7] = __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+            } else {
+              const uint4 w = x[i].w[e >> 2];
+              v[e >> 3][e & 7] = __uint_as_float((e & 3) == 0 ? w.x : (e & 3) == 1 ? w.y : (e & 3) == 2 ? w.z : w.w);
+            }
+          }
+          uint32_t top = 0;                              // as bits: a NaN is above an infinity, which is above every number
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint4 w = x[i].w[k];
+              top = __vimax3_u16x2(top, w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu);
+              top = __vimax3_u16x2(top, w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu);
+            }
+            top = max(top & 0xFFFF0000u, top << 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[e >> 3][e & 7]) & 0x7FFFFFFFu);
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          if (site < 0 || row >= rows) continue;
+          const bool number = top <= PC_MOST4;           // (what is not reads as NaN)
+          const float s = top && number ? pc_scale4(top) : 1.f;
+          *codes(row) = number ? make_uint2(pc_codes4<T>(v[0], s), pc_codes4<T>(v[1], s)) : make_uint2(0x88888888u, 0x88888888u);
+          if (d % 32 == 0) *mark(row) = number ? (uint16_t)(__float_as_uint(s) >> 16) : (uint16_t)0x7FC0u;
+        }
+#pragma unroll
+        for (int i = 0; i < FLIGHT; ++i) x[i] = ahead[i];
+      }
+    }
+  }
+}
+
+template <typename T, int GROUP, bool READ>
+static void pc_launch4(const PgRows& a, int64_t blocks, cudaStream_t s) {
+  static const int resident = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_rows4_kernel<T, GROUP, READ>, PC_THREADS, 0) == cudaSuccess && n > 0 ? n : 4;
+  }();
+  const int64_t wave = (int64_t)resident * KCH_SMS / a.parts;
+  const dim3 grid((unsigned)(blocks < wave ? blocks : wave), (unsigned)a.parts);
+  paged_rows4_kernel<T, GROUP, READ><<<grid, PC_THREADS, 0, s>>>(a);
 }
 
 static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k, int64_t ld_k, void* v, int64_t ld_v, int dtype,
@@ -367,7 +473,8 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   a.pages[0] = p->k; a.pages[1] = p->v; a.scales[0] = p->k_scales; a.scales[1] = p->v_scales;
   a.n_kv = p->n_kv; a.c = p->c; a.page = p->page_size; a.kind = p->kind; a.zero_rest = zero_rest;
   cudaStream_t s = kch_stream(stream);
-  const int pieces = p->c / 8, group = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
+  const bool q4 = p->kind == KCH_INT4;
+  const int pieces = p->c / (q4 ? 16 : 8), least = q4 ? 4 : 8, group = pieces <= least ? least : pieces <= 2 * least ? 2 * least : 4 * least;
   a.tokens = 2 * p->n_kv * group <= 16 ? 2 : 1;
   const int64_t blocks = ceil_div64(b->N, PC_THREADS / 32 * a.tokens);
   // as many warps to a token as it has rounds of rows, while they are fewer than 16 to an SM
@@ -379,6 +486,17 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
     if (read) pc_launch<T_, G_, true, Q_>(a, blocks, s);                                                                 \
     else pc_launch<T_, G_, false, Q_>(a, blocks, s);                                                                     \
   } while (0)
+#define PC_GO4(T_, G_)                                                                                                   \
+  do {                                                                                                                   \
+    if (read) pc_launch4<T_, G_, true>(a, blocks, s);                                                                    \
+    else pc_launch4<T_, G_, false>(a, blocks, s);                                                                        \
+  } while (0)
+#define PC_WIDTH4(T_)                                                                                                    \
+  do {                                                                                                                   \
+    if (group == 4) PC_GO4(T_, 4);                                                                                       \
+    else if (group == 8) PC_GO4(T_, 8);                                                                                  \
+    else PC_GO4(T_, 16);                                                                                                 \
+  } while (0)
 #define PC_WIDTH(T_, Q_)                                                                                                 \
   do {                                                                                                                   \
     if (group == 8) PC_GO(T_, 8, Q_);                                                                                    \
@@ -387,14 +505,16 @@ static int rows_impl(const kch_paged_cache* p, const kch_paged_batch* b, void* k
   } while (0)
 #define PC_KIND(T_)                                                                                                      \
   do {                                                                                                                   \
-    if (p->kind < KCH_FP8_E4M3) PC_WIDTH(T_, 0);                                                                         \
-    else if (p->kind == KCH_INT4) PC_WIDTH(T_, 4);                                                                       \
-    else PC_WIDTH(T_, 8);                                                                                                \
+    if (q4) PC_WIDTH4(T_);                                                                                               \
+    else if (p->kind < KCH_FP8_E4M3) PC_WIDTH(T_, false);                                                                \
+    else PC_WIDTH(T_, true);                                                                                             \
   } while (0)
   if (dtype == KCH_BF16) PC_KIND(bf16);
   else PC_KIND(float);
 #undef PC_KIND
 #undef PC_WIDTH
+#undef PC_WIDTH4
+#undef PC_GO4
 #undef PC_GO
   KCH_LAUNCH_OK();
   return KCH_OK;
