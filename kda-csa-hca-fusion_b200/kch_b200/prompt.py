@@ -67,7 +67,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, sink_logits=None, slidi
         if not cu_seqlens.is_contiguous():
             cu_seqlens = cu_seqlens.contiguous()
         if out is None:
-            o = q.new_empty(shape)
+            o = torch.empty_strided(shape, (nh * c, c, 1), dtype=dtype, device=q.device)
         else:
             o = out
             if o.shape != shape or o.dtype is not dtype or o.get_device() != index or not o.is_contiguous() or o.data_ptr() % 16:
@@ -83,7 +83,7 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, sink_logits=None, slidi
             if len(_ws_bytes) > 4096:
                 _ws_bytes.clear()
             nbytes = _ws_bytes[sizes] = int(lib.kch_prompt_attend_workspace_bytes(a))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
         _lib.check(lib.kch_prompt_attend(a, _lib.stream()))
     return o

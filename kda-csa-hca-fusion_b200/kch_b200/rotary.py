@@ -116,9 +116,10 @@ class RotaryPositions:
             ld = axes
         with _lib.device(self.device):
             if out is None:
-                to_q, ld_to_q, to_k, ld_to_k = q.new_empty(shape), nh * c, None, n_kv * c
-                y = (to_q, None if k is None else k.new_empty(other))
-                to_q, to_k = to_q.data_ptr(), _lib.ptr(y[1])
+                ld_to_q, ld_to_k, to_k = nh * c, n_kv * c, None
+                y = (torch.empty_strided(shape, (ld_to_q, c, 1), dtype=dtype, device=self.device),
+                     None if k is None else torch.empty_strided(other, (ld_to_k, c, 1), dtype=dtype, device=self.device))
+                to_q, to_k = y[0].data_ptr(), _lib.ptr(y[1])
             else:
                 y = (out[0], out[1])
                 (to_q, ld_to_q), (to_k, ld_to_k) = self._own_out("q", y[0], q), self._own_out("k", y[1], k)
