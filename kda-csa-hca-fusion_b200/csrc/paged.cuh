@@ -14,20 +14,21 @@
 
 #define PG_MAX_B 4096                  // sequences of a call: their table of steps is kept in shared memory
 #define PG_LOG2E 1.4426950408889634f
+#define PG_EXTRA 2                     // places of the line before an item's steps (see above)
 #define PG_ROWS 16                     // kind of keys and values that are packed rows like the queries, and not in pages (beside the KCH_ types)
 
 unsigned int* kch_status_device_ptr();
 
 struct PgBatch {
-  const int32_t* table; int64_t ld_table;      // NULL: keys and values are packed rows
-  const int32_t *t0, *cu;              // t0 NULL: no sequence has earlier tokens
+  const int32_t* table; int64_t ld_table;      // (of pages)
+  const int32_t *t0, *cu;              // (t0: of pages)
   int B, N;                            // sequences; rows of the packed tensors
   int cap;                             // positions that a row of the table covers (below 2^31)
   int64_t num_pages;
   int shift;                           // log2(page_size)
   unsigned int* status;                // [0]: of expired waits, which ends the others; [1]: of tables, which ends none
   int n_kv, G, window;                 // key heads, query heads of one, window (attention only)
-  int rows, extra;                     // rows of an item, where the kernel leaves that open; places of the line before an item's steps
+  int rows;                            // of an item, where the kernel leaves that open
   uint32_t g_mul; int g_shift;         // n / G = n * g_mul >> 32 + g_shift for n < 2^31; g_mul 0: n >> g_shift
 };
 // With s = floor(log2 G) and M = floor(2^(32 + s) / G) + 1, M G exceeds 2^(32 + s) by at most G < 2^(s + 1): exact below 2^31.
@@ -44,11 +45,13 @@ __device__ __forceinline__ int pg_token(const PgBatch& a, int row) {          //
 struct PgSeq { int row0, len, t0, kv; };      // first packed row, new tokens, tokens before them, keys in all
 
 // (Whatever cu_seqlens and t0 hold, rows stay inside the packed tensors and keys inside the table.)
+// PACKED: keys and values are packed rows, and no sequence has earlier tokens.
+template <bool PACKED = false>
 __device__ __forceinline__ PgSeq pg_seq(const PgBatch& a, int b) {
   PgSeq s;
   s.row0 = min(max(__ldg(a.cu + b), 0), a.N);
   s.len = min(max(__ldg(a.cu + b + 1), s.row0), a.N) - s.row0;
-  const int t0 = a.t0 ? __ldg(a.t0 + b) : 0;
+  const int t0 = PACKED ? 0 : __ldg(a.t0 + b);
   s.t0 = max(t0, 0);
   s.kv = t0 < 0 ? 0 : (int)min((int64_t)t0 + s.len, (int64_t)a.cap);       // (positions before 0: no keys)
   return s;
@@ -93,17 +96,17 @@ __device__ __forceinline__ int2 pg_sees(const PgBatch& a, const PgSeq& s, int ro
 // Where a CTA's range of steps begins.  (Steps are counted in 32 bits: the host refuses a call that could have 2^31 - 1.)
 struct PgPlace {
   int per, left;                       // places of the line of a CTA; of this one
-  int b, h, block, step;               // step: place in the item (its steps come behind `extra` others)
+  int b, h, block, step;               // step: place in the item (its steps come behind EXTRA others)
   PgSeq s;                             // of b
   PgSpan x;                            // of the block
 };
 
 // steps of sequence b (0 behind the last) for each key head: by the lane where it is one block, as in a batch of single tokens, else
 // by the warp over its blocks
-template <int R, int KT, int TWO>
+template <int R, int KT, int TWO, int EXTRA>
 __device__ __forceinline__ int pg_steps(const PgBatch& a, const PgSeq& s) {
   const int lane = threadIdx.x & 31, blocks = pg_blocks<R>(a, s);
-  int mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps + a.extra : 0;
+  int mine = blocks == 1 ? pg_span<R, KT, TWO>(a, s, 0).steps + EXTRA : 0;
   for (unsigned many = __ballot_sync(0xffffffffu, blocks > 1); many; many &= many - 1) {
     const int from = __ffs(many) - 1;
     PgSeq t;
@@ -114,17 +117,18 @@ __device__ __forceinline__ int pg_steps(const PgBatch& a, const PgSeq& s) {
     const int nb = pg_blocks<R>(a, t);
     int sum = 0;
 #pragma unroll 1
-    for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps + a.extra;
+    for (int i = lane; i < nb; i += 32) sum += pg_span<R, KT, TWO>(a, t, i).steps + EXTRA;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == from) mine = sum;
   }
   return mine * a.n_kv;
 }
+template <bool PACKED>
 __device__ __forceinline__ PgSeq pg_seq_or_none(const PgBatch& a, int b) {
   PgSeq s = {0, 0, 0, 0};
   if (b < a.B) {
-    s = pg_seq(a, b);
+    s = pg_seq<PACKED>(a, b);
     if (s.len > 0 && s.kv - s.t0 < s.len) pg_bad(a);        // it begins before position 0, or the table ends before it does (without new tokens it needs no page)
   }
   return s;
@@ -142,7 +146,7 @@ __device__ __forceinline__ int pg_scan(int x) {             // sums over the lan
 
 // The whole block calls it; `mem`: PG_PLAN_BYTES(B) of shared memory, free again after the next __syncthreads().
 #define PG_PLAN_BYTES(B) (32 + 4 * ((B) + 1))
-template <int R, int KT, int TWO>
+template <int R, int KT, int TWO, int EXTRA = 0, bool PACKED = false>
 __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta, int ctas) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   PgPlace p = {};
@@ -160,9 +164,9 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     return p.left > 0 ? (int)start : 0x7FFFFFFF;
   };
   int start;
-  if (a.B == 1 || (a.B <= 32 && (int64_t)a.N * a.G <= (int64_t)(R ? R : a.rows) * a.B)) {      // every warp by itself: no memory, no barrier
-    const PgSeq s = pg_seq_or_none(a, lane);
-    const int x = pg_steps<R, KT, TWO>(a, s), upto = pg_scan(x);
+  if (a.B <= 8 || (a.B <= 32 && (int64_t)a.N * a.G <= (int64_t)(R ? R : a.rows) * a.B)) {      // every warp by itself: no memory, no barrier
+    const PgSeq s = pg_seq_or_none<PACKED>(a, lane);
+    const int x = pg_steps<R, KT, TWO, EXTRA>(a, s), upto = pg_scan(x);
     total = __shfl_sync(0xffffffffu, upto, 31);
     start = range();
     if (p.left > 0) {
@@ -181,7 +185,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     const int deal = min((a.B + warps - 1) / warps, 32);
 #pragma unroll 1
     for (int b0 = warp * deal; b0 < a.B; b0 += warps * deal) {
-      const int x = pg_steps<R, KT, TWO>(a, pg_seq_or_none(a, lane < deal ? b0 + lane : a.B));
+      const int x = pg_steps<R, KT, TWO, EXTRA>(a, pg_seq_or_none<PACKED>(a, lane < deal ? b0 + lane : a.B));
       if (lane < deal && b0 + lane < a.B) base[b0 + lane + 1] = x;
     }
     if (tid == 0) base[0] = 0;
@@ -206,7 +210,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
       p.b = found[0];
       before = base[p.b];
       mine = base[p.b + 1] - before;
-      p.s = pg_seq(a, p.b);
+      p.s = pg_seq<PACKED>(a, p.b);
     }
   }
   if (p.left > 0) {                    // the key head, then the block, by every warp
@@ -220,7 +224,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     if (blocks > 1) {
 #pragma unroll 1
       for (int i0 = 0; i0 < blocks; i0 += 32) {
-        const int i = i0 + lane, n = i < blocks ? pg_span<R, KT, TWO>(a, p.s, i).steps + a.extra : 0, x = pg_scan(n);
+        const int i = i0 + lane, n = i < blocks ? pg_span<R, KT, TWO>(a, p.s, i).steps + EXTRA : 0, x = pg_scan(n);
         const unsigned hit = __ballot_sync(0xffffffffu, i < blocks && x > rest);
         if (hit) {
           const int at = __ffs(hit) - 1;
@@ -238,7 +242,7 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
 }
 
 // The items of a CTA, one after the other; every role of a kernel walks them by itself.
-template <int R, int KT, int TWO>
+template <int R, int KT, int TWO, int EXTRA = 0, bool PACKED = false>
 struct PgWalk {
   const PgBatch& a;
   int b, h, block;                     // the item
@@ -248,7 +252,7 @@ struct PgWalk {
   int left;                            // places of the CTA's range behind them
   int from, taken;                     // places of the item that are in it
   __device__ __forceinline__ PgWalk(const PgBatch& a_, const PgPlace& p)
-      : a(a_), b(p.b), h(p.h), block(p.block), first(0), count(0), s(p.s), x(p.x), left(p.left), from(p.step), taken(0) {
+      : a(a_), b(p.b), h(p.h), block(p.block), first(p.step), count(0), s(p.s), x(p.x), left(p.left), from(p.step), taken(0) {
     if (left > 0) take();
   }
   __device__ __forceinline__ bool valid() const { return count > 0; }      // (a range that ends before an item's first step has no more of it)
@@ -256,17 +260,17 @@ struct PgWalk {
   __device__ __forceinline__ bool ends() const { return first + count == x.steps; }
   // the CTA that has the end of an item which starts in this one's range and is its last
   __device__ __forceinline__ int last(const PgPlace& p, int cta) const {
-    return (int)(((int64_t)p.per * cta + (p.left - taken) - from + a.extra + x.steps - 1) / p.per);
+    return (int)(((int64_t)p.per * cta + (p.left - (EXTRA ? taken : count)) - (EXTRA ? from : 0) + EXTRA + x.steps - 1) / p.per);
   }
   __device__ __forceinline__ void next() {
-    from = 0;
+    if (EXTRA) from = 0; else first = 0;
     count = 0;
     if (left <= 0) return;
     if (++block == pg_blocks<R>(a, s)) {
       block = 0;
       if (++h == a.n_kv) {
         h = 0;
-        do { s = pg_seq(a, ++b); } while (s.len == 0);       // (places are left, so a sequence with rows follows)
+        do { s = pg_seq<PACKED>(a, ++b); } while (s.len == 0);       // (places are left, so a sequence with rows follows)
       }
     }
     x = pg_span<R, KT, TWO>(a, s, block);
@@ -275,10 +279,15 @@ struct PgWalk {
 
  private:
   __device__ __forceinline__ void take() {
-    taken = min(x.steps + a.extra - from, left);
-    left -= taken;
-    first = max(from - a.extra, 0);
-    count = max(from + taken - a.extra, 0) - first;
+    if constexpr (EXTRA == 0) {
+      count = min(x.steps - first, left);
+      left -= count;
+    } else {
+      taken = min(x.steps + EXTRA - from, left);
+      left -= taken;
+      first = max(from - EXTRA, 0);
+      count = max(from + taken - EXTRA, 0) - first;
+    }
   }
 };
 

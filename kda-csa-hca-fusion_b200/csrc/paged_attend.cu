@@ -81,26 +81,27 @@ __device__ __forceinline__ bool pa_none(float weight) { return __float_as_uint(w
 #define PA_CTAS (2 * KCH_SMS)          // at most, of either attention kernel
 
 // steps that a call can have at most, whatever the lengths on the device (of which no two share a row)
-static int64_t pa_steps(const PgBatch& a, int rows, int tile) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1 + a.extra); }
+static int64_t pa_steps(const PgBatch& a, int rows, int tile, int extra) { return ((int64_t)a.N * a.G / rows + a.B) * a.n_kv * (a.cap / tile + 1 + extra); }
 
 static constexpr int pa_smem(int ROWS, int DMAX) { return (ROWS * (DMAX + 4) + 2 * PA_KT * (DMAX + 4) + ROWS * (PA_KT + 4) + 3 * ROWS) * 4; }
 static_assert(pa_smem(64, 256) <= 232448 && PG_PLAN_BYTES(PG_MAX_B) <= pa_smem(16, 64), "shared memory; the plan lies in the tiles' memory");
 
-// T: activations; P: stored values; DMAX: widths up to this (columns behind the width are 0)
-template <typename T, typename P, int ROWS, int DMAX>
+// T: activations; P: stored values; DMAX: widths up to this (columns behind the width are 0); PACKED: keys and values are packed rows (asked at run
+// time, pages took a fifth longer)
+template <typename T, typename P, int ROWS, int DMAX, bool PACKED>
 __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend a) {
   constexpr int LD = DMAX + 4, LS = PA_KT + 4, RT = ROWS / 16, CT = DMAX / 64;
   extern __shared__ float4 pa_mem[];
   float* sq = reinterpret_cast<float*>(pa_mem);
   float *sk = sq + ROWS * LD, *sv = sk + PA_KT * LD, *sp = sv + PA_KT * LD, *sm = sp + ROWS * LS, *sl = sm + ROWS, *sa = sl + ROWS;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, c = a.c, c8 = c >> 3;
-  const PgPlace place = pg_plan<ROWS, PA_KT, 0>(a.bt, pa_mem, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<ROWS, PA_KT, 0, 0, PACKED>(a.bt, pa_mem, blockIdx.x, gridDim.x);
   pg_zero_rest(a, sizeof(T), blockIdx.x, gridDim.x);
   __syncthreads();
   for (int i = tid; i < (ROWS + 2 * PA_KT) * LD; i += PA_THREADS) sq[i] = 0.f;      // columns c .. DMAX of all three stay 0
   PgRecord rec = {};
   const int G = a.bt.G, n_kv = a.bt.n_kv;
-  PgWalk<ROWS, PA_KT, 0> w(a.bt, place);
+  PgWalk<ROWS, PA_KT, 0, 0, PACKED> w(a.bt, place);
   for (; w.valid(); w.next()) {
     const int r0 = w.block * ROWS;                             // first (token, head) row of the block in its sequence
     __syncthreads();
@@ -132,13 +133,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attend_simt_kernel(PgAttend 
         vw[k].none();
         fk[k] = fv[k] = 1.f;
         if (j < PA_KT && pos >= w.x.lo && pos < w.s.kv) {
-          if (!a.bt.table) {                                   // packed rows
+          if constexpr (PACKED) {
             kw[k].load(a.k, (w.s.row0 + pos) * a.ld_k + (int64_t)w.h * c + d);
             vw[k].load(a.v, (w.s.row0 + pos) * a.ld_v + (int64_t)w.h * c + d);
-            continue;
-          }
-          const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift);
-          if (pg >= 0) {
+          } else if (const int64_t pg = pg_page(a.bt, w.b, pos >> a.bt.shift); pg >= 0) {
             const int64_t row = (pg * n_kv + w.h) * a.page + (pos & (a.page - 1));
             kw[k].load(a.k, row * c + d);
             vw[k].load(a.v, row * c + d);
@@ -534,17 +532,13 @@ static PaPlan pa_plan(const kch_paged_attend_args* p) {
 }
 static PaPlan pa_plan(const kch_prompt_attend_args* p) { return pa_plan(p->B, p->N, p->nh / p->n_kv, PG_ROWS, p->dtype, p->c); }
 
-static void pa_line(PgBatch& a, const PaPlan& x, int kind) {
-  a.rows = x.rows;
-  a.extra = x.form != PA_SIMT && (kind == PG_ROWS || kind == KCH_INT4) ? 2 : 0;
-}
-
 // The launches of a call whose arguments are in order: the attention, and the joining of the items that are in parts.
 static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, void* workspace, cudaStream_t s) {
   const int c = a.c;
   a.records = (PgRecord*)workspace;
   a.slots = (float*)((char*)workspace + pg_records_bytes(x.ctas));
   a.slot_rows = x.slot_rows;
+  a.bt.rows = x.rows;
   // Where no block of rows can have two steps, no item is in parts and there is nothing to join.
   const bool whole = a.bt.cap <= x.tile * (x.two && (x.form == PA_TC5_FEW || (int64_t)a.bt.N * a.bt.G <= x.rows / 2) ? 2 : 1);
   const PgJoinArgs j = {a.out, dtype, nh, a.bt.G, c, x.rows, x.slot_rows, a.sink, a.sink_dtype, a.records, a.slots};
@@ -555,23 +549,25 @@ static int pa_launch(PgAttend& a, const PaPlan& x, int kind, int dtype, int nh, 
     return rc5 != KCH_OK || whole ? rc5 : kch_paged_join(j, x.ctas, s);
   }
   const int rows = x.rows, dmax = c <= 64 ? 64 : c <= 128 ? 128 : 256, smem = pa_smem(rows, dmax);
-#define PA_GO(T_, P_, R_, D_)                                                                                                 \
+#define PA_GO(T_, P_, R_, D_, K_)                                                                                             \
   do {                                                                                                                        \
-    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
-    paged_attend_simt_kernel<T_, P_, R_, D_><<<x.ctas, PA_THREADS, smem, s>>>(a);                                            \
+    KCH_CUDA_OK(cudaFuncSetAttribute(paged_attend_simt_kernel<T_, P_, R_, D_, K_>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); \
+    paged_attend_simt_kernel<T_, P_, R_, D_, K_><<<x.ctas, PA_THREADS, smem, s>>>(a);                                        \
   } while (0)
-#define PA_WIDTH(T_, P_, R_)                                                                                                  \
+#define PA_WIDTH(T_, P_, R_, K_)                                                                                              \
   do {                                                                                                                        \
-    if (dmax == 64) PA_GO(T_, P_, R_, 64);                                                                                    \
-    else if (dmax == 128) PA_GO(T_, P_, R_, 128);                                                                             \
-    else PA_GO(T_, P_, R_, 256);                                                                                              \
+    if (dmax == 64) PA_GO(T_, P_, R_, 64, K_);                                                                                \
+    else if (dmax == 128) PA_GO(T_, P_, R_, 128, K_);                                                                         \
+    else PA_GO(T_, P_, R_, 256, K_);                                                                                          \
   } while (0)
-#define PA_ROWS(T_, P_)                                                                                                       \
+#define PA_FORM(T_, P_, K_)                                                                                                   \
   do {                                                                                                                        \
-    if (rows == 16) PA_WIDTH(T_, P_, 16);                                                                                     \
-    else PA_WIDTH(T_, P_, 64);                                                                                                \
+    if (rows == 16) PA_WIDTH(T_, P_, 16, K_);                                                                                 \
+    else PA_WIDTH(T_, P_, 64, K_);                                                                                            \
   } while (0)
-  if (kind == KCH_FP8_E4M3) { if (dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
+#define PA_ROWS(T_, P_) PA_FORM(T_, P_, false)
+  if (kind == PG_ROWS) { if (dtype == KCH_F32) PA_FORM(float, float, true); else PA_FORM(bf16, bf16, true); }
+  else if (kind == KCH_FP8_E4M3) { if (dtype == KCH_F32) PA_ROWS(float, __nv_fp8_e4m3); else PA_ROWS(bf16, __nv_fp8_e4m3); }
   else if (kind == KCH_INT8) { if (dtype == KCH_F32) PA_ROWS(float, int8_t); else PA_ROWS(bf16, int8_t); }
   else if (kind == KCH_INT4) { if (dtype == KCH_F32) PA_ROWS(float, PgInt4); else PA_ROWS(bf16, PgInt4); }
   else if (dtype == KCH_F32) PA_ROWS(float, float);
@@ -615,8 +611,8 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
-  pa_line(a.bt, x, p->cache.kind);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT && p->cache.kind == KCH_INT4 ? PG_EXTRA : 0) < PG_MOST,
+              "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
   // (an item's queries may be read again while its rows are stored)
   const uintptr_t q0 = (uintptr_t)p->q, q1 = q0 + ((p->batch.N - 1) * p->ld_q + (int64_t)p->nh * c) * es, o0 = (uintptr_t)p->out;
@@ -674,8 +670,7 @@ extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) 
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
-  pa_line(a.bt, x, PG_ROWS);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT ? PG_EXTRA : 0) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
   KCH_REQUIRE(a.bt.status != nullptr, "%s: cannot resolve the device status word", fn);
   return pa_launch(a, x, PG_ROWS, p->dtype, p->nh, p->workspace, kch_stream(stream));
 }

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(P4Cfg<R>::THREADS, 1)
 paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
   typedef P4Smem<D, R> S;
   typedef P4Cfg<R> C;
-  typedef PgWalk<R, P4_KT, 0> Walk;
+  typedef PgWalk<R, P4_KT, 0, PG_EXTRA> Walk;
   extern __shared__ __align__(1024) uint8_t p4_raw[];
   S& sm = *reinterpret_cast<S*>(p4_raw);
   if (smem_addr_u32(p4_raw) & 1023) {                    // (every block begins its memory there)
@@ -143,7 +143,7 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
     sm.nan_scale = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const PgPlace place = pg_plan<R, P4_KT, 0>(a.bt, sm.k, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<R, P4_KT, 0, PG_EXTRA>(a.bt, sm.k, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   __syncthreads();

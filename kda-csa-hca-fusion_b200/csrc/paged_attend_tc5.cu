@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(PtCfg<D, KIND, FEW>::THREADS, 1)
 paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
                         const __grid_constant__ PgAttend a) {
   typedef PtCfg<D, KIND, FEW> C;
-  typedef PgWalk<C::OPEN ? 0 : C::R, PT_KT, C::TWO> Walk;
+  typedef PgWalk<C::OPEN ? 0 : C::R, PT_KT, C::TWO, C::OPEN ? PG_EXTRA : 0, C::ROWS> Walk;
   extern __shared__ __align__(1024) uint8_t pt_raw[];    // (no room to align it by hand; every block begins its memory there)
   PtSmem<D, KIND, FEW>& sm = *reinterpret_cast<PtSmem<D, KIND, FEW>*>(pt_raw);
   if (smem_addr_u32(pt_raw) & 1023) {
@@ -380,7 +380,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr_u32(&sm.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const PgPlace place = pg_plan<C::OPEN ? 0 : C::R, PT_KT, C::TWO>(a.bt, sm.kv, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<C::OPEN ? 0 : C::R, PT_KT, C::TWO, C::OPEN ? PG_EXTRA : 0, C::ROWS>(a.bt, sm.kv, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   t5_fence_before();
