@@ -313,13 +313,14 @@ static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
 }
 
 
-// 4 bits.  16 values a thread, so that two of them share a scale; the rows of a batch of two rounds are asked for before the page is looked up, or
-// the next token's page after the rows of this one.  (With 8 values a thread and each waited for after the other, 26 096 tokens of 8 key heads of
-// 128 were written in 65 us and read in 36.5.)
+// 4 bits.  16 values a thread, so that two of them share a scale; the first rows of a token are asked for before its page is looked up and the next
+// ones while these are at work, or (READ) the next token's page behind the rows of this one.  26 096 tokens of 8 key heads of 128 are written in 39
+// us and read in 25; the memory's rate is 18 for either.  Writing is bound by its instructions, 180 for 16 values.  (With 8 values a thread and each
+// wait behind the other 65 and 36.5; two rows of a thread in flight, which leaves 24 warps an SM, 43.)
 template <typename T> struct Pc16 { uint4 w[sizeof(T)]; };
 template <typename T, int GROUP, bool READ>
-__global__ void __launch_bounds__(PC_THREADS) paged_rows4_kernel(const __grid_constant__ PgRows a) {
-  constexpr int FLIGHT = READ ? 4 : 2;                   // rows of a thread in flight
+__global__ void __launch_bounds__(PC_THREADS, (READ || sizeof(T) == 4) ? 1 : 4) paged_rows4_kernel(const __grid_constant__ PgRows a) {
+  constexpr int FLIGHT = READ ? 4 : 1;                   // rows of a thread at a time
   __shared__ int32_t scu[PC_SMEM_B + 1];
   const int32_t* cu = a.bt.cu;
   if (a.bt.B <= PC_SMEM_B) {
