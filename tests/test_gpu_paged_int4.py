@@ -296,6 +296,78 @@ def test_a_captured_step_replays_with_other_lengths(kch, dtype, c):
         assert torch.equal(out, m.cache.forward_step(q, m.table, t0, m.cu))
 
 
+@pytest.mark.parametrize("new,past", [([1, 3, 1], [300, 40, 129]), ([40, 200], [100, 64])])
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_a_pool_from_elsewhere_with_codes_of_0_and_scales_of_both_signs(kch, dtype, c, new, past):
+    """Code 0 stands for -8 scales, which no append writes; a scale below 0 turns its 32 channels over."""
+    m = Batch4(kch, new, past, dtype=dtype, c=c, page=16)
+    for x in ("k", "v"):
+        pages, scales = getattr(m.cache, x + "_pages"), getattr(m.cache, x + "_scales")
+        pages.copy_(torch.randint(0, 256, pages.shape, generator=m.g, device=DEV, dtype=torch.uint8))
+        scales.mul_(torch.where(torch.rand(scales.shape, generator=m.g, device=DEV) < 0.5, -1., 1.))
+    q = m.randn(m.N, 4, c)
+    want, tol = reference(m, q, window=200)
+    close(m.cache.forward_step(q, *m.args, sliding_window=200), want, tol)
+    got = m.cache.read_step(*m.args, n_rows=m.N)[0]
+    for b, (n, p) in enumerate(zip(new, past)):
+        rows = got[sum(new[:b]):sum(new[:b + 1])]
+        assert torch.equal(rows.double(), m.values("k", b, p + n)[:, p:].transpose(0, 1))
+
+
+@pytest.mark.parametrize("new,past", [([1, 1], [33, 700]), ([40, 300], [100, 900])])
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_strided_queries_and_outputs_and_rows_that_begin_on_16_bytes_and_no_more(kch, dtype, c, new, past):
+    m = Batch4(kch, new, past, dtype=dtype, c=c)
+    q = m.randn(m.N, 6, c)
+    want = m.cache.forward_step(q, *m.args)
+    ahead = 16 // want.element_size()
+    room = torch.full((ahead + want.numel() + ahead,), 7.0, dtype=dtype, device=DEV)
+    out = room[ahead:ahead + want.numel()].view(want.shape)
+    assert out.data_ptr() % 32 == 16
+    m.cache.forward_step(q, *m.args, out=out)
+    assert torch.equal(out, want) and (room[:ahead] == 7).all() and (room[-ahead:] == 7).all()
+    wide = torch.randn(m.N, 6 * c + 3 * ahead, device=DEV).to(dtype)
+    wide[:, ahead:ahead + 6 * c] = q.flatten(1)
+    assert torch.equal(m.cache.forward_step(wide[:, ahead:ahead + 6 * c].unflatten(1, (6, c)), *m.args), want)
+    rows = m.cache.read_step(*m.args, n_rows=m.N)
+    rooms = [torch.full((ahead + rows[0].numel() + ahead,), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    outs = tuple(r[ahead:ahead + rows[0].numel()].view(rows[0].shape) for r in rooms)
+    m.cache.read_step(*m.args, n_rows=m.N, out=outs)
+    for got, kept, r in zip(rows, outs, rooms):
+        assert torch.equal(got, kept) and (r[:ahead] == 7).all() and (r[-ahead:] == 7).all()
+
+
+@pytest.mark.parametrize("B,N,n_kv", [(4096, 4096, 16), (4096, 16400, 16), (32, 65536, 128)])
+def test_lengths_that_fall_and_rise_again_beyond_what_is_counted_do_nothing(kch, B, N, n_kv):
+    """Every other sequence has all rows: more steps in all than 32 bits hold, which the host, who sees N alone, cannot know."""
+    from kch_b200 import _lib
+    assert _lib.device_status() == 0
+    cache = kch.PagedKVCache(1, 256, n_kv, 64, DEV, torch.bfloat16, kv_quant="int4")
+    table = torch.zeros(B, 4096, dtype=torch.int32, device=DEV)
+    t0 = torch.full((B,), 4096 * 256 - N, dtype=torch.int32, device=DEV)
+    cu = (torch.arange(B + 1, device=DEV) % 2 * N).int()
+    q, out = torch.zeros(N, n_kv, 64, dtype=torch.bfloat16, device=DEV), torch.full((N, n_kv, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    cache.forward_step(q, table, t0, cu, out=out)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+    assert (out == 7).all()
+
+
+def test_calls_on_two_streams_at_once_and_again(kch):
+    a, b = (Batch4(kch, new, [97 * i for i in range(20)], n_kv=2, seed=s) for s, new in ((1, [1] * 20), (2, [1] * 10 + [50] * 10)))
+    qa, qb = a.randn(a.N, 16, 128), b.randn(b.N, 16, 128)
+    want = [a.cache.forward_step(qa, *a.args), b.cache.forward_step(qb, *b.args)]
+    torch.cuda.synchronize()
+    s, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, (m, q) in enumerate(((a, qa), (b, qb))):
+            with torch.cuda.stream(s[i]):
+                got[i].append(m.cache.forward_step(q, *m.args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
 def test_offsets_that_pass_32_bits(kch):
     """A pool whose rows lie beyond 2^32 bytes, and twice that in codes."""
     pages, page, c = 2 ** 32 // (64 * 64) + 40, 64, 128

@@ -190,6 +190,27 @@ def test_lengths_out_of_range_stay_in_the_tensors(kch):
     assert torch.equal(out, want) and (room[:100] == 5).all() and (room[200:] == 5).all()
 
 
+def test_lengths_that_fall_and_rise_again_beyond_what_is_counted_do_nothing(kch):
+    """Every other prompt has all rows: more steps in all than 32 bits hold, which the host, who sees N alone, cannot know."""
+    from kch_b200 import _lib
+    assert _lib.device_status() == 0
+    N, B, n_kv = 65536, 4096, 32
+    cu = (torch.arange(B + 1, device=DEV) % 2 * N).int()
+    q, out = torch.zeros(N, n_kv, 64, dtype=torch.bfloat16, device=DEV), torch.full((N, n_kv, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    kch.prompt_attention(q, q, q, cu, out=out)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == _lib.STATUS_PAGED_TABLE
+    assert (out == 7).all()
+
+
+def test_many_prompts_of_a_token_and_a_few(kch):
+    """More prompts than a block has threads; one key head and as many as there are query heads."""
+    for nh, n_kv in ((4, 1), (3, 3)):
+        m = Prompts([1 + i % 5 + (i % 97 == 0) * 200 for i in range(900)], nh=nh, n_kv=n_kv, c=64, seed=nh)
+        want, tol = reference(m, m.q)
+        close(kch.prompt_attention(*m.args), want, tol)
+
+
 def test_rows_beyond_32_bits_of_elements(kch):
     """Keys and values whose last rows lie behind 2^32 elements."""
     N, c = 2 ** 17, 128
