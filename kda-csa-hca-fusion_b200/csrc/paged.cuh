@@ -14,7 +14,8 @@
 
 #define PG_MAX_B 4096                  // sequences of a call: their table of steps is kept in shared memory
 #define PG_LOG2E 1.4426950408889634f
-#define PG_EXTRA 2                     // places of the line before an item's steps (see above)
+#define PG_EXTRA 2                     // places of the line before an item's steps (see above) on tcgen05
+#define PG_EXTRA_MOST 4                // of any form
 #define PG_ROWS 16                     // kind of keys and values that are packed rows like the queries, and not in pages (beside the KCH_ types)
 
 unsigned int* kch_status_device_ptr();

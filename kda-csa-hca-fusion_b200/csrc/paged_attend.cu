@@ -507,6 +507,8 @@ int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s)
 //   rows (tokens x heads of a key head) of a sequence: up to 32, an item of the forms for few rows; behind that they read the keys twice.
 //     bf16  8 heads: 1 token 55 / 58, 4 (32 rows) 57 / 60, 5 (40 rows) 100 / 61;  16 heads: 2 tokens 37 / 41, 3 (48 rows) 52 / 42
 //     e4m3  8 heads: 1 token 46 / 80, 4 68 / 81, 5 126 / 81;  16 heads: 2 tokens 42 / 47, 3 72 / 48;  int8: 47 / 74, 68 / 74, 125 / 75; 41 / 45, 72 / 46
+//     4 bits: up to 16 rows (their form converts codes once for 16 rows, and chunks convert them faster than the other kinds').  8 heads: 1 token 33 / 76,
+//           4 (32 rows, in an instance for 32 that has been taken out) 93 / 77;  16 heads: 1 token 29 / 47, 2 62 / 47
 //   tokens of a sequence: up to 4, so that a long chunk among single tokens cannot be most of a batch's work.  With 190 tokens in one sequence
 //     and one in each other (4 on average) 4 heads take 118 / 96 (bf16), 145 / 147 (e4m3), 146 / 141 (int8), 2 heads 191 / 174, 245 / 267, 254 / 254; with
 //     448 (8 on average) 127 / 100, 223 / 165, 222 / 156, and 246 / 182, 300 / 277, 302 / 265.  Alike ones would go on to 32 rows: 8 tokens of 4 heads
@@ -519,9 +521,9 @@ static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   PaPlan x;
   const int64_t rows = N * G;                            // of a key head
   if (!kch_paged_attend_tc5_supported(dtype, c)) x = {PA_SIMT, rows <= 16 * B ? 16 : 64, PA_KT, PA_CTAS, 0, false};
-  else if (rows > 32 * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
+  else if (rows > (kind == KCH_INT4 ? 16 : 32) * B || N > 4 * B || kind == PG_ROWS) x = {PA_TC5, 256, 128, KCH_SMS, 0, true};
   else if (kind == KCH_BF16) x = {PA_TC5_FEW, rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, true};
-  else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};
+  else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};      // (4 bits: 8 or 16)
   // Prompts and 4-bit pages: blocks of whole tokens, so that a copy of a tensor map fetches their queries.
   if (x.form == PA_TC5 && (kind == PG_ROWS || kind == KCH_INT4) && G <= 128) x.rows = 128 / G * G * 2;
   x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
@@ -611,7 +613,7 @@ extern "C" int kch_paged_attend(const kch_paged_attend_args* p, void* stream) {
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT && p->cache.kind == KCH_INT4 ? PG_EXTRA : 0) < PG_MOST,
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, p->cache.kind != KCH_INT4 || x.form == PA_SIMT ? 0 : PG_EXTRA_MOST) < PG_MOST,
               "kch_paged_attend: N=%lld rows against tables of %d pages are more than a call takes",
               (long long)p->batch.N, p->batch.max_pages);
   // (an item's queries may be read again while its rows are stored)
@@ -670,7 +672,7 @@ extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) 
   a.scale = p->scale * PG_LOG2E;
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
-  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT ? PG_EXTRA : 0) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
+  KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT ? PG_EXTRA_MOST : 0) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
   KCH_REQUIRE(a.bt.status != nullptr, "%s: cannot resolve the device status word", fn);
   return pa_launch(a, x, PG_ROWS, p->dtype, p->nh, p->workspace, kch_stream(stream));
 }

@@ -30,16 +30,17 @@
 #include "tc5_utils.cuh"
 
 #define P4_KT 128
+#define P4_EXTRA 4                     // places of the line before an item's tiles (paged.cuh): its ends take as long as four of them
 #define P4_WAIT 4000000000ull          // ns until a wait gives up
 
-// R rows an item: 8, 16 or 32, by what a sequence has.
+// R rows an item: 8 or 16, by what a sequence has.
 template <int R>
 struct P4Cfg {
   static constexpr int WARPS = 8, THREADS = 128 + 32 * WARPS;       // that compute; the first warpgroup copies
   static constexpr int NT = R / 8;                                  // columns, in eights
-  static constexpr int SLICE = R == 32 ? 16 : 32, SHARE = P4_KT / SLICE, BLOCKS = SLICE / 16;      // a warp's keys of a tile; warps of a tile
+  static constexpr int SLICE = 32, SHARE = P4_KT / SLICE, BLOCKS = SLICE / 16;      // a warp's keys of a tile; warps of a tile
   static constexpr int TEAMS = WARPS / SHARE;                       // each takes every TEAMS'th tile
-  static constexpr int REG_FEED = R == 32 ? 56 : 88, REG_WORK = R == 32 ? 224 : 208, REG_LAUNCH = 65536 / THREADS / 8 * 8;
+  static constexpr int REG_FEED = 88, REG_WORK = 208, REG_LAUNCH = 65536 / THREADS / 8 * 8;
   static_assert(128 * REG_FEED + 32 * WARPS * REG_WORK <= THREADS * REG_LAUNCH, "register split");
 };
 template <int D, int R>
@@ -54,7 +55,7 @@ struct P4Smem {
   uint32_t nan_scale, nan[R][GROUPS];                    // a value's scale of NaN among the item's tiles; the groups that it makes NaN, by row
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
-static_assert(sizeof(P4Smem<128, 32>) <= 232448 && sizeof(P4Smem<64, 32>) <= 232448, "shared memory of the paged attention over 4 bits");
+static_assert(sizeof(P4Smem<128, 16>) <= 232448 && sizeof(P4Smem<64, 16>) <= 232448, "shared memory of the paged attention over 4 bits");
 static_assert(PG_PLAN_BYTES(PG_MAX_B) <= 12 * P4_KT * 32, "the plan lies in the ring of tiles");
 
 // A bounded wait that sleeps: a poll returns when the phase is complete, or after 10 us.  (Polls that return at once were an eighth of all
@@ -68,7 +69,7 @@ __device__ __forceinline__ bool p4_poll(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
-__device__ __noinline__ bool p4_wait_long(uint32_t bar, uint32_t parity, unsigned int* status, unsigned sleep) {
+__device__ __forceinline__ bool p4_wait_long(uint32_t bar, uint32_t parity, unsigned int* status, unsigned sleep) {
   uint64_t since, now;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(since));
   do {
@@ -79,6 +80,11 @@ __device__ __noinline__ bool p4_wait_long(uint32_t bar, uint32_t parity, unsigne
   } while (now - since < P4_WAIT);
   atomicCAS(status, 0u, (unsigned)KCH_STATUS_PAGED_ATTEND);
   return false;
+}
+// As a call it keeps the loops short, but the compiler then leaves the registers as they were launched: 8 rows, which have enough of them,
+// call (64 sequences of 8192 tokens 86 us, 88 without), 16 do not (38 us where they do 41).
+__device__ __noinline__ bool p4_wait_call(uint32_t bar, uint32_t parity, unsigned int* status, unsigned sleep) {
+  return p4_wait_long(bar, parity, status, sleep);
 }
 __device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(P4Cfg<R>::THREADS, 1)
 paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
   typedef P4Smem<D, R> S;
   typedef P4Cfg<R> C;
-  typedef PgWalk<R, P4_KT, 0, PG_EXTRA> Walk;
+  typedef PgWalk<R, P4_KT, 0, P4_EXTRA> Walk;
   extern __shared__ __align__(1024) uint8_t p4_raw[];
   S& sm = *reinterpret_cast<S*>(p4_raw);
   if (smem_addr_u32(p4_raw) & 1023) {                    // (every block begins its memory there)
@@ -143,12 +149,14 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
     sm.nan_scale = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const PgPlace place = pg_plan<R, P4_KT, 0, PG_EXTRA>(a.bt, sm.k, blockIdx.x, gridDim.x);
+  const PgPlace place = pg_plan<R, P4_KT, 0, P4_EXTRA>(a.bt, sm.k, blockIdx.x, gridDim.x);
   pg_zero_rest(a, 2, blockIdx.x, gridDim.x);
   t5_fence_async_smem();                                 // (the plan was read from the ring's memory, which copies write next)
   __syncthreads();
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return p4_poll(smem_addr_u32(bar), parity & 1) || p4_wait_long(smem_addr_u32(bar), parity & 1, a.bt.status, warp < 4 ? 300u : 0u);
+    if (p4_poll(smem_addr_u32(bar), parity & 1)) return true;
+    return R == 8 ? p4_wait_call(smem_addr_u32(bar), parity & 1, a.bt.status, warp < 4 ? 300u : 0u)
+                  : p4_wait_long(smem_addr_u32(bar), parity & 1, a.bt.status, warp < 4 ? 300u : 0u);
   };
 
   if (warp < 4) {
@@ -537,7 +545,6 @@ static int p4_launch(const PgAttend& a, int ctas, cudaStream_t s) {
 }
 
 int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s) {
-#define P4_ROWS(D_) (rows == 8 ? p4_launch<D_, 8>(a, ctas, s) : rows == 16 ? p4_launch<D_, 16>(a, ctas, s) : p4_launch<D_, 32>(a, ctas, s))
-  return a.c == 64 ? P4_ROWS(64) : P4_ROWS(128);
-#undef P4_ROWS
+  if (a.c == 64) return rows == 8 ? p4_launch<64, 8>(a, ctas, s) : p4_launch<64, 16>(a, ctas, s);
+  return rows == 8 ? p4_launch<128, 8>(a, ctas, s) : p4_launch<128, 16>(a, ctas, s);
 }

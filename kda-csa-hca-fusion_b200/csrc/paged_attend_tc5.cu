@@ -431,7 +431,7 @@ paged_attend_tc5_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           fine = __all_sync(0xffffffffu, fine);
           if (!fine) return false;
           const bool there = mine && (unsigned)id < (unsigned)a.bt.num_pages;
-          uint8_t* scales = sm.raw[C::Q4 ? st : 0] + C::RAW + mybox * box * (2 * C::GROUPS);      // 4 bits: of this lane's box
+          uint8_t* scales = C::Q4 ? sm.raw[C::Q4 ? st : 0] + (C::Q4 ? C::RAW : 0) + mybox * box * (2 * C::GROUPS) : nullptr;      // 4 bits: of this lane's box
           uint32_t bytes = C::CODES ? C::RAW : C::TILE;
           if constexpr (C::Q4) {
             bytes += __popc(__ballot_sync(0xffffffffu, there)) * box * (2 * C::GROUPS);
