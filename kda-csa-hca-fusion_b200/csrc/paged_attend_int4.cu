@@ -12,12 +12,12 @@
 //     of a word meet by a byte permutation.  P^T comes from S^T by the transposition of 8 x 8 values that the warp has an instruction for.
 // A row's maximum is held by the 8 lanes that have its column, who only meet when one of them exceeds it by 2^8; sums stay apart until the end.
 // P is rounded to bf16.  Up to 4 rows: the other 4 columns are the same queries again, and multiply what the rounding has left.
-// A key lies in the fragments at rho(key): both products' words then come without meeting in the banks.
+// Fragment row g is key rho(g) of its eight, so that keys' words come without meeting in the banks (values' meet two and two).
 //
 // Measured, 64 sequences, 16 heads of 128 on 4: 8192 tokens in pages of 64 86 us (3.5 TB/s of pages; 89 in pages of 16, 111 of 8), 500 to
-// 16000 tokens in pages of 32 98; on two key heads 50, on one 41, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
+// 16000 tokens in pages of 32 91; on two key heads 51, on one 38, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
 // the instructions that convert: 730 for 32 keys of a warp, 340 of them at half rate, on two warps a scheduler that keep it 56 % busy.
-// Tried: 12 warps of 152 registers 86 and 102; a tile's values multiplied while the next one's scores are 92 (registers move); shifts as
+// Tried: 12 warps of 152 registers 86 (and 102 where 8 took 98); a tile's values multiplied while the next one's scores are 92 (registers move); shifts as
 // products with powers of two, on the other pipe, 93.  Pages by tensor maps of 64-byte rows: a copy engine's 5 clocks a row are 1280 for a tile.
 //
 // A scale of NaN (32 channels that were not finite) reaches what sees it: a key's through its logit; a value's is taken for 0 and looked for
@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 // code J of either half of w, as values: J is 0 .. 3, s the scales of both halves, s24 -24 times them; sixteen: 16 in either half, a register
-// whose value the compiler does not know (with two constants it makes two operations of this one: 287 of them for 32 keys, 120 -> 100 us)
+// whose value the compiler does not know (with two constants it makes two operations of this one, 287 of them for 32 keys: 64 sequences of 8192 tokens 113 us, 99 without)
 template <int J>
 __device__ __forceinline__ uint32_t p4_pair(uint32_t w, uint32_t s, uint32_t s24, uint32_t sixteen) {
   uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);
@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t p4_trans(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-// where in its eight a key of the fragments lies in the tile
+// which key of its eight a row of the fragments is
 __device__ __forceinline__ int p4_rho(int key) { return key ^ (key >> 2 & 1); }
 __device__ __forceinline__ bool p4_nan(uint32_t s) { return (s & 0x7FFFu) > 0x7F80u; }
 

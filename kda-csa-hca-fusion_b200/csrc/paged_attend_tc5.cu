@@ -1,4 +1,5 @@
-// Attention of new tokens over a paged cache on tcgen05 (bf16 activations, heads of 64 or 128; pages in bf16, e4m3 or int8).
+// Attention of new tokens over a paged cache on tcgen05 (bf16 activations, heads of 64 or 128; pages in bf16, e4m3, int8 or 4 bits), and
+// of whole prompts, whose keys and values are packed rows (KIND PG_ROWS).
 // Mathematics and division of the work: paged_attend.cu, paged.cuh.
 //
 // One persistent CTA an SM; two softmax warpgroups X = 0, 1 of a row per thread.  An item is a block of (token, head of the group)
@@ -20,6 +21,12 @@
 // 8-bit pages: four more warps turn the copied payloads into bf16 tiles (exactly: a payload has at most 7 bits of mantissa;
 // only e4m3's codes of NaN become 480, and where a tile has one the rows that may see it are summed again);
 // a row's scale multiplies its logit, or its probability before that is rounded to bf16.
+// 4-bit pages: the same warps make the values themselves, a scale for 32 channels included ((u - 8) s with s of 5 bits has 8 bits at most:
+// exact), so that the softmax has no scales to apply.  Packed rows: a tile is a box of a tensor map over tokens, and what follows a
+// sequence in it is the next one's: masked, its values cleared like those behind the end in a last page.
+// Both of these (OPEN) take blocks of whole tokens, 128 / G * G rows a warpgroup, whose queries are two or four copies of a tensor map (through two
+// warps they came 5000 clocks after the item before had been stored), count the ends of items in the division (paged.cuh), and leave out
+// masks, and halves of a tile, where a warp's rows have no edge.
 //
 // The running maximum of a row is raised, and O_X rescaled, only when a tile exceeds it by 2^8: probabilities up to 256 lose
 // nothing in bf16 or in the fp32 sums, and the accumulator makes its way through registers only a few times a row.
@@ -42,6 +49,10 @@
 // Short items cost their ends: 37 x 16 items of 256 rows and 9 tiles take 117 us, four to a CTA, of which steps are 75: 10000 clocks
 // until a CTA's first scores, as many for the first end (its code comes from memory), then 6000 an end and 3000 until the next item's
 // scores (its queries: 12000 clocks for two warps' copies, most of them behind the last softmax).
+// Prompts, 16 heads of 128 on 4 (OPEN; before the three measures above): one of 8192 tokens 257 us (351), 37 of 20 to 1500 184 (316), 64 of 512 147
+// (188); two of 8300 and 14001 on 2 key heads 1042 (1317), 1200 TFLOP/s in a burst.  An item's first scores are there 600 clocks after the one before it, its end
+// takes 5000 (900 until the last product, 3700 to store its rows); a step of a long prompt is 3430, a masked one up to 5000.  Chunks over 4-bit pages: 1024
+// tokens behind 15360 155 us, where bf16 pages take 142.
 #include <cuda.h>
 #include <math.h>
 

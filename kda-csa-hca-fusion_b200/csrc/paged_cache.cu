@@ -1,4 +1,5 @@
-// The paged key / value cache: rows written into their pages (as they are, or in 8 bits with a scale a row), and read back.
+// The paged key / value cache: rows written into their pages (as they are, in 8 bits with a scale a row, or in 4 with one for 32 channels), and
+// read back.
 //
 //   write   s = max_d |x_d| / Q   (Q = 448 for e4m3, 127 for int8; 1 for a row of zeros),   payload_d = round(x_d / s)
 //   read    x_d = payload_d * s
@@ -314,7 +315,7 @@ static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
 
 
 // 4 bits.  16 values a thread, so that two of them share a scale; the first rows of a token are asked for before its page is looked up and the next
-// ones while these are at work, or (READ) the next token's page behind the rows of this one.  26 096 tokens of 8 key heads of 128 are written in 39
+// ones while these are at work, or (READ) the next token's page behind the rows of this one.  25 609 tokens of 8 key heads of 128 are written in 39
 // us and read in 25; the memory's rate is 18 for either.  Writing is bound by its instructions, 180 for 16 values.  (With 8 values a thread and each
 // wait behind the other 65 and 36.5; two rows of a thread in flight, which leaves 24 warps an SM, 43.)
 template <typename T> struct Pc16 { uint4 w[sizeof(T)]; };
