@@ -21,7 +21,8 @@
 // products with powers of two, on the other pipe, 93.  Pages by tensor maps of 64-byte rows: a copy engine's 5 clocks a row are 1280 for a tile.
 //
 // A scale of NaN (32 channels that were not finite) reaches what sees it: a key's through its logit; a value's is taken for 0 and looked for
-// when the item ends, for 0 times it would reach everyone.
+// when the item ends, for 0 times it would reach everyone.  So are the scales above 2^123 that no append writes, of which 24 times may be no number:
+// what lies behind a sequence's end, or before its window, may hold any bits.
 #include <math.h>
 
 #include <atomic>
@@ -52,7 +53,7 @@ struct P4Smem {
   alignas(16) float stage[C::WARPS][8 * D];
   alignas(16) uint2 q[D / 16][C::NT][32];                // fragments of the queries: contraction step, columns, lane
   float ml[2][C::WARPS][R];
-  uint32_t nan_scale, nan[R][GROUPS];                    // a value's scale of NaN among the item's tiles; the groups that it makes NaN, by row
+  uint32_t nan_scale, nan[R][GROUPS];                    // a value's odd scale among the keys of the item; the groups that it makes NaN, by row
   alignas(8) uint64_t full[STAGES], empty[STAGES];
 };
 static_assert(sizeof(P4Smem<128, 16>) <= 232448 && sizeof(P4Smem<64, 16>) <= 232448, "shared memory of the paged attention over 4 bits");
@@ -112,9 +113,11 @@ __device__ __forceinline__ uint32_t p4_trans(uint32_t x) {
 }
 // which key of its eight a row of the fragments is
 __device__ __forceinline__ int p4_rho(int key) { return key ^ (key >> 2 & 1); }
-__device__ __forceinline__ bool p4_nan(uint32_t s) { return (s & 0x7FFFu) > 0x7F80u; }
+// a scale that no product can take: NaN, an infinity, or above 2^123, of which 24 times still fits bf16 (an append writes up to 2^122)
+#define P4_MOST 0x7D00u
+__device__ __forceinline__ bool p4_odd(uint32_t s) { return (s & 0x7FFFu) > P4_MOST; }
 
-// Scales of NaN among the values of the keys [from, to) of a sequence: which rows of the item see one, by groups.  Of `threads` threads.
+// Such scales among the values of the keys [from, to) of a sequence: which rows of the item see one, by groups.  Of `threads` threads.
 template <int D>
 __device__ __noinline__ void p4_find_nan(const PgAttend& a, int b, int h, int row0, int rows, PgSeq s, int from, int to, uint32_t (*nan)[D / 32], int tid,
                                          int threads) {
@@ -123,7 +126,7 @@ __device__ __noinline__ void p4_find_nan(const PgAttend& a, int b, int h, int ro
     const int key = from + (int)(i / GROUPS), group = (int)(i % GROUPS), page = __ldg(a.bt.table + b * a.bt.ld_table + (key >> a.bt.shift));
     if ((unsigned)page >= (unsigned)a.bt.num_pages) continue;
     const int64_t row = ((int64_t)page * a.bt.n_kv + h) * a.page + (key & (a.page - 1));
-    if (!p4_nan(__ldg((const uint16_t*)a.vs + row * GROUPS + group))) continue;
+    if (!p4_odd(__ldg((const uint16_t*)a.vs + row * GROUPS + group))) continue;
     for (int r = 0; r < rows; ++r) {
       const int2 keys = pg_sees(a.bt, s, row0 + r);
       if (key >= keys.x && key < keys.y) *(volatile uint32_t*)&nan[r][group] = 1u;
@@ -383,12 +386,13 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
           f[i >> 2][i & 3] = sm.vs[st][(base + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
           most = max(most, f[i >> 2][i & 3]);
         }
-        if (most > 0x7F80u) {                            // (NaN, or below 0, which an append writes none of)
+        if (most > P4_MOST) {                            // (or below 0, which an append writes none of)
 #pragma unroll
           for (int i = 0; i < 4 * BL; ++i)
-            if (p4_nan(f[i >> 2][i & 3])) {
+            if (p4_odd(f[i >> 2][i & 3])) {
+              const int key = key0 + 8 * (i >> 1) + p4_rho(2 * t + (i & 1));
               f[i >> 2][i & 3] = 0u;
-              *(volatile uint32_t*)&sm.nan_scale = 1u;
+              if (key >= w.x.lo && key < w.s.kv) *(volatile uint32_t*)&sm.nan_scale = 1u;      // (else no row sees it)
             }
         }
 #pragma unroll
@@ -504,7 +508,7 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
       }
       sync();
     }
-    // scales of NaN among the values: the groups of the rows that see one
+    // odd scales among the values: the groups of the rows that see one
     if (*(volatile uint32_t*)&sm.nan_scale != 0u) {
       sync();                                            // (all have read the word)
       if (ct == 0) *(volatile uint32_t*)&sm.nan_scale = 0u;
