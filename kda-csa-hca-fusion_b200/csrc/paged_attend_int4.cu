@@ -11,11 +11,12 @@
 //   O^T += V^T P^T:  thread (g, t) has 16 (8) consecutive channels of keys 2t, 2t + 1, 2t + 8, 2t + 9, again one group's; two keys' halves
 //     of a word meet by a byte permutation.  P^T comes from S^T by the transposition of 8 x 8 values that the warp has an instruction for.
 // A row's maximum is held by the 8 lanes that have its column, who only meet when one of them exceeds it by 2^8; sums stay apart until the end.
-// P is rounded to bf16.  Up to 4 rows: the other 4 columns are the same queries again, and multiply what the rounding has left.
+// P is rounded to bf16, and what the rounding leaves is multiplied as well, as in the other kinds' steps: up to 4 rows in the other 4 columns, which are the
+// same queries again, more rows by products of their own (7 % of the time with 8 rows, 10 % with 16).
 // Fragment row g is key rho(g) of its eight, so that keys' words come without meeting in the banks (values' meet two and two).
 //
 // Measured, 64 sequences, 16 heads of 128 on 4: 8192 tokens in pages of 64 86 us (3.5 TB/s of pages; 89 in pages of 16, 111 of 8), 500 to
-// 16000 tokens in pages of 32 91; on two key heads 51, on one 38, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
+// 16000 tokens in pages of 32 90; on two key heads 55, on one 42, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
 // the instructions that convert: 730 for 32 keys of a warp, 340 of them at half rate, on two warps a scheduler that keep it 56 % busy.
 // Tried: 12 warps of 152 registers 86 (and 102 where 8 took 98); a tile's values multiplied while the next one's scores are 92 (registers move); shifts as
 // products with powers of two, on the other pipe, 93.  Pages by tensor maps of 64-byte rows: a copy engine's 5 clocks a row are 1280 for a tile.
@@ -26,6 +27,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tc5_utils.cuh"
@@ -243,11 +245,11 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
   int ahead = cw / C::SHARE, st = ahead, turn = 0;       // tiles until this team's next; its place in the ring (TEAMS < STAGES), and how often that has been filled
   bool ok = true, part = false;
   for (Walk w(a.bt, place); w.valid(); w.next()) {
-    const bool twice = R == 8 && w.x.rows <= 4;          // columns 4 .. 7 are the rows again
+    const bool four = R == 8 && w.x.rows <= 4;           // columns 4 .. 7 are the rows again
     // queries: of step i the lane (g, t) has channels d, d + 4 and d + 1, d + 5 of row g, d = RUN t + 8 (i / 2) + 2 (i % 2)
     for (int i = ct; i < KS * NT * 32; i += 32 * C::WARPS) {
       const int ln = i & 31, nt = (i >> 5) % NT, step = (i >> 5) / NT, d = RUN * (ln & 3) + 8 * (step >> 1) + 2 * (step & 1);
-      const int r = 8 * nt + (twice ? (ln >> 2) & 3 : ln >> 2), row = w.block * R + r, tok = pg_token(a.bt, row);
+      const int r = 8 * nt + (four ? (ln >> 2) & 3 : ln >> 2), row = w.block * R + r, tok = pg_token(a.bt, row);
       uint2 u = make_uint2(0u, 0u);
       if (r < w.x.rows) {
         const uint32_t* src = reinterpret_cast<const uint32_t*>((const bf16*)a.q + (w.s.row0 + tok) * a.ld_q + (w.h * G + row - tok * G) * D + d);
@@ -267,170 +269,185 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
 #pragma unroll
       for (int e = 0; e < NT * 4; ++e) o[j][e / 4][e % 4] = 0.f;
     const uint2* queries = &sm.q[0][0][lane];
-    uint2 own[NT == 1 ? KS : 1];                          // (eight rows' stay in registers)
-    if constexpr (NT == 1) {
+    // The item's tiles, for four rows and for more apart: the same loop for both took the four 97 us where they have 90 (64 sequences of 500 to 16000
+    // tokens, 16 heads of 128 on 4).
+    auto tiles = [&](auto rows4) {
+      constexpr bool twice = decltype(rows4)::value;
+      uint2 own[twice ? KS : 1];                         // (four rows' stay in registers; of more, with the rest of P beside it, they would not fit)
+      if constexpr (twice) {
 #pragma unroll
-      for (int i = 0; i < KS; ++i) own[i] = queries[32 * i];
-    }
-    for (; ahead < w.count; ahead += C::TEAMS) {
-      const int base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + (w.first + ahead) * P4_KT + base;      // the warp's keys
-      if (ok) ok = wait(&sm.full[st], turn);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
-        float s[BL][NT][4] = {};
-        {
-          uint32_t kw[BL][2][RUN / 8], ks[BL][2], k24[BL][2];
+        for (int i = 0; i < KS; ++i) own[i] = queries[32 * i];
+      }
+      for (; ahead < w.count; ahead += C::TEAMS) {
+        const int base = C::SLICE * (cw % C::SHARE), key0 = w.x.first_key + (w.first + ahead) * P4_KT + base;      // the warp's keys
+        if (ok) ok = wait(&sm.full[st], turn);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && key0 < k1.y && key0 + C::SLICE > k0.x) {
+          float s[BL][NT][4] = {};
+          {
+            uint32_t kw[BL][2][RUN / 8], ks[BL][2], k24[BL][2];
 #pragma unroll
-          for (int x = 0; x < 2 * BL; ++x) {
-            const int r = base + 8 * x + rho;
-            uint32_t (&to)[RUN / 8] = kw[x >> 1][x & 1];
-            if constexpr (D == 128) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sm.k[st] + r * S::ROW + 16 * t);
-              to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
-            } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(sm.k[st] + r * S::ROW + 8 * t);
-              to[0] = u.x; to[1] = u.y;
-            }
-            const uint32_t f = sm.ks[st][r * S::GROUPS + (D == 128 ? t : t >> 1)];
-            ks[x >> 1][x & 1] = f | f << 16;
-            k24[x >> 1][x & 1] = p4_s24(f | f << 16);
-          }
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            uint2 q[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if constexpr (NT == 1) q[nt] = own[i];
-              else q[nt] = queries[32 * (NT * i + nt)];
-            }
-#pragma unroll
-            for (int b = 0; b < BL; ++b) {
-              const uint32_t x = kw[b][0][i >> 1], y = kw[b][1][i >> 1], fx = ks[b][0], fy = ks[b][1], gx = k24[b][0], gy = k24[b][1];
-              uint32_t a0, a1, a2, a3;
-              if (i & 1) {
-                a0 = p4_pair<2>(x, fx, gx, sixteen); a1 = p4_pair<2>(y, fy, gy, sixteen); a2 = p4_pair<3>(x, fx, gx, sixteen); a3 = p4_pair<3>(y, fy, gy, sixteen);
+            for (int x = 0; x < 2 * BL; ++x) {
+              const int r = base + 8 * x + rho;
+              uint32_t (&to)[RUN / 8] = kw[x >> 1][x & 1];
+              if constexpr (D == 128) {
+                const uint4 u = *reinterpret_cast<const uint4*>(sm.k[st] + r * S::ROW + 16 * t);
+                to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
               } else {
-                a0 = p4_pair<0>(x, fx, gx, sixteen); a1 = p4_pair<0>(y, fy, gy, sixteen); a2 = p4_pair<1>(x, fx, gx, sixteen); a3 = p4_pair<1>(y, fy, gy, sixteen);
+                const uint2 u = *reinterpret_cast<const uint2*>(sm.k[st] + r * S::ROW + 8 * t);
+                to[0] = u.x; to[1] = u.y;
+              }
+              const uint32_t f = sm.ks[st][r * S::GROUPS + (D == 128 ? t : t >> 1)];
+              ks[x >> 1][x & 1] = f | f << 16;
+              k24[x >> 1][x & 1] = p4_s24(f | f << 16);
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              uint2 q[NT];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (twice) q[nt] = own[i];
+                else q[nt] = queries[32 * (NT * i + nt)];
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) p4_mma(s[b][nt], a0, a1, a2, a3, q[nt].x, q[nt].y);
-            }
-          }
-        }
-        // what a row does not see is -inf
-        if (!(key0 >= k1.x && key0 + C::SLICE <= k0.y)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = 8 * nt + 2 * t + e, row = twice ? r & 3 : r;
-              const int2 keys = row < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + row) : make_int2(0, 0);
-#pragma unroll
-              for (int b = 0; b < BL; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const int key = key0 + 16 * b + 8 * h + rho;
-                  if (!(key >= keys.x && key < keys.y)) s[b][nt][2 * h + e] = -INFINITY;
+              for (int b = 0; b < BL; ++b) {
+                const uint32_t x = kw[b][0][i >> 1], y = kw[b][1][i >> 1], fx = ks[b][0], fy = ks[b][1], gx = k24[b][0], gy = k24[b][1];
+                uint32_t a0, a1, a2, a3;
+                if (i & 1) {
+                  a0 = p4_pair<2>(x, fx, gx, sixteen); a1 = p4_pair<2>(y, fy, gy, sixteen); a2 = p4_pair<3>(x, fx, gx, sixteen); a3 = p4_pair<3>(y, fy, gy, sixteen);
+                } else {
+                  a0 = p4_pair<0>(x, fx, gx, sixteen); a1 = p4_pair<0>(y, fy, gy, sixteen); a2 = p4_pair<1>(x, fx, gx, sixteen); a3 = p4_pair<1>(y, fy, gy, sixteen);
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) p4_mma(s[b][nt], a0, a1, a2, a3, q[nt].x, q[nt].y);
+              }
             }
-        }
-        // a row's maximum is raised only when it is exceeded by 2^8
-        float top[NT][2];
-        bool any = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
-#pragma unroll
-            for (int b = 1; b < BL; ++b) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[b][nt][e], s[b][nt][2 + e]));
-            any = any || (m[nt][e] == -INFINITY ? top[nt][e] > m[nt][e] : top[nt][e] > m[nt][e] + raise);
           }
-        if (__any_sync(0xffffffffu, any)) {
+          // what a row does not see is -inf
+          if (!(key0 >= k1.x && key0 + C::SLICE <= k0.y)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int r = 8 * nt + 2 * t + e, row = twice ? r & 3 : r;
+                const int2 keys = row < w.x.rows ? pg_sees(a.bt, w.s, w.block * R + row) : make_int2(0, 0);
+#pragma unroll
+                for (int b = 0; b < BL; ++b)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int key = key0 + 16 * b + 8 * h + rho;
+                    if (!(key >= keys.x && key < keys.y)) s[b][nt][2 * h + e] = -INFINITY;
+                  }
+              }
+          }
+          // a row's maximum is raised only when it is exceeded by 2^8
+          float top[NT][2];
+          bool any = false;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float& x = top[nt][e];
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              const bool up = m[nt][e] == -INFINITY ? x > m[nt][e] : x > m[nt][e] + raise;
-              const float f = up ? ex2_fast((m[nt][e] - x) * sc) : 1.f;
-              if (up) m[nt][e] = x;
-              l[nt][e] *= f;
+              top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-              for (int j = 0; j < MT; ++j) { o[j][nt][e] *= f; o[j][nt][2 + e] *= f; }
+              for (int b = 1; b < BL; ++b) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[b][nt][e], s[b][nt][2 + e]));
+              any = any || (m[nt][e] == -INFINITY ? top[nt][e] > m[nt][e] : top[nt][e] > m[nt][e] + raise);
             }
-        }
-        uint32_t p[BL][NT][2];                           // P^T: keys 2t, 2t + 1 (and + 8) of row g
+          if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float shift0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] * sc, shift1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] * sc;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int b = 0; b < BL; ++b)
+              for (int e = 0; e < 2; ++e) {
+                float& x = top[nt][e];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const bool up = m[nt][e] == -INFINITY ? x > m[nt][e] : x > m[nt][e] + raise;
+                const float f = up ? ex2_fast((m[nt][e] - x) * sc) : 1.f;
+                if (up) m[nt][e] = x;
+                l[nt][e] *= f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float x = ex2_fast(fmaf(s[b][nt][2 * h], sc, -shift0)), y = ex2_fast(fmaf(s[b][nt][2 * h + 1], sc, -shift1));
-              l[nt][0] += x;
-              l[nt][1] += y;
-              uint32_t u = pack2_bf16(x, y);
-              if (R == 8 && twice && t >= 2) u = pack2_bf16(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u));
-              p[b][nt][h] = p4_trans(u);
-            }
-        }
-        // of the values the lane has channels 16 g .. (8 g ..) of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t f[BL][4], most = 0u;                    // their scales
-#pragma unroll
-        for (int i = 0; i < 4 * BL; ++i) {
-          f[i >> 2][i & 3] = sm.vs[st][(base + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
-          most = max(most, f[i >> 2][i & 3]);
-        }
-        if (most > P4_MOST) {                            // (or below 0, which an append writes none of)
-#pragma unroll
-          for (int i = 0; i < 4 * BL; ++i)
-            if (p4_odd(f[i >> 2][i & 3])) {
-              const int key = key0 + 8 * (i >> 1) + p4_rho(2 * t + (i & 1));
-              f[i >> 2][i & 3] = 0u;
-              if (key >= w.x.lo && key < w.s.kv) *(volatile uint32_t*)&sm.nan_scale = 1u;      // (else no row sees it)
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < BL; ++b) {
-          uint32_t vw[4][D / 64];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint8_t* from = sm.v[st] + (base + 16 * b + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::ROW + D / 16 * g;
-            if constexpr (D == 128) {
-              const uint2 u = *reinterpret_cast<const uint2*>(from);
-              vw[i][0] = u.x; vw[i][1] = u.y;
-            } else {
-              vw[i][0] = *reinterpret_cast<const uint32_t*>(from);
-            }
+                for (int j = 0; j < MT; ++j) { o[j][nt][e] *= f; o[j][nt][2 + e] *= f; }
+              }
           }
-          const uint32_t fx = f[b][0] | f[b][1] << 16, fy = f[b][2] | f[b][3] << 16, gx = p4_s24(fx), gy = p4_s24(fy);
+          uint32_t p[BL][NT][2], rest[BL][NT][2];          // P^T: keys 2t, 2t + 1 (and + 8) of row g; what its rounding leaves
 #pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            const uint32_t x0 = __byte_perm(vw[0][i], vw[1][i], 0x5410), x1 = __byte_perm(vw[0][i], vw[1][i], 0x7632);      // channels 0 .. 3, 4 .. 7 of both keys
-            const uint32_t y0 = __byte_perm(vw[2][i], vw[3][i], 0x5410), y1 = __byte_perm(vw[2][i], vw[3][i], 0x7632);
+          for (int nt = 0; nt < NT; ++nt) {
+            const float shift0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] * sc, shift1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] * sc;
+#pragma unroll
+            for (int b = 0; b < BL; ++b)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float x = ex2_fast(fmaf(s[b][nt][2 * h], sc, -shift0)), y = ex2_fast(fmaf(s[b][nt][2 * h + 1], sc, -shift1));
+                l[nt][0] += x;
+                l[nt][1] += y;
+                uint32_t u = pack2_bf16(x, y);
+                if constexpr (!twice) rest[b][nt][h] = p4_trans(pack2_bf16(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
+                else if (t >= 2) u = pack2_bf16(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u));
+                p[b][nt][h] = p4_trans(u);
+              }
+          }
+          // of the values the lane has channels 16 g .. (8 g ..) of keys 2t, 2t + 1, 2t + 8, 2t + 9
+          uint32_t f[BL][4], most = 0u;                    // their scales
+#pragma unroll
+          for (int i = 0; i < 4 * BL; ++i) {
+            f[i >> 2][i & 3] = sm.vs[st][(base + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::GROUPS + (D == 128 ? g >> 1 : g >> 2)];
+            most = max(most, f[i >> 2][i & 3]);
+          }
+          if (most > P4_MOST) {                            // (or below 0, which an append writes none of)
+#pragma unroll
+            for (int i = 0; i < 4 * BL; ++i)
+              if (p4_odd(f[i >> 2][i & 3])) {
+                const int key = key0 + 8 * (i >> 1) + p4_rho(2 * t + (i & 1));
+                f[i >> 2][i & 3] = 0u;
+                if (key >= w.x.lo && key < w.s.kv) *(volatile uint32_t*)&sm.nan_scale = 1u;      // (else no row sees it)
+              }
+          }
+#pragma unroll
+          for (int b = 0; b < BL; ++b) {
+            uint32_t vw[4][D / 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint8_t* from = sm.v[st] + (base + 16 * b + 8 * (i >> 1) + p4_rho(2 * t + (i & 1))) * S::ROW + D / 16 * g;
+              if constexpr (D == 128) {
+                const uint2 u = *reinterpret_cast<const uint2*>(from);
+                vw[i][0] = u.x; vw[i][1] = u.y;
+              } else {
+                vw[i][0] = *reinterpret_cast<const uint32_t*>(from);
+              }
+            }
+            const uint32_t fx = f[b][0] | f[b][1] << 16, fy = f[b][2] | f[b][3] << 16, gx = p4_s24(fx), gy = p4_s24(fy);
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+              const uint32_t x0 = __byte_perm(vw[0][i], vw[1][i], 0x5410), x1 = __byte_perm(vw[0][i], vw[1][i], 0x7632);      // channels 0 .. 3, 4 .. 7 of both keys
+              const uint32_t y0 = __byte_perm(vw[2][i], vw[3][i], 0x5410), y1 = __byte_perm(vw[2][i], vw[3][i], 0x7632);
 #define P4_PV(J_)                                                                                                                        \
-  {                                                                                                                                      \
-    const uint32_t a0 = p4_pair<J_>(x0, fx, gx, sixteen), a1 = p4_pair<J_>(x1, fx, gx, sixteen), a2 = p4_pair<J_>(y0, fy, gy, sixteen),           \
-                   a3 = p4_pair<J_>(y1, fy, gy, sixteen);                                                                                   \
-    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) p4_mma(o[4 * i + J_][nt], a0, a1, a2, a3, p[b][nt][0], p[b][nt][1]);               \
-  }
-            P4_PV(0) P4_PV(1) P4_PV(2) P4_PV(3)
+    {                                                                                                                                    \
+      const uint32_t a0 = p4_pair<J_>(x0, fx, gx, sixteen), a1 = p4_pair<J_>(x1, fx, gx, sixteen), a2 = p4_pair<J_>(y0, fy, gy, sixteen),         \
+                     a3 = p4_pair<J_>(y1, fy, gy, sixteen);                                                                                 \
+      _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) {                                                                                \
+        p4_mma(o[4 * i + J_][nt], a0, a1, a2, a3, p[b][nt][0], p[b][nt][1]);                                                             \
+        if constexpr (!twice) p4_mma(o[4 * i + J_][nt], a0, a1, a2, a3, rest[b][nt][0], rest[b][nt][1]);                                 \
+      }                                                                                                                                  \
+    }
+              P4_PV(0) P4_PV(1) P4_PV(2) P4_PV(3)
 #undef P4_PV
+            }
           }
         }
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&sm.empty[st]);
+        st += C::TEAMS;
+        if (st >= S::STAGES) { st -= S::STAGES; ++turn; }
       }
-      __syncwarp();
-      if (lane == 0) mbarrier_arrive(&sm.empty[st]);
-      st += C::TEAMS;
-      if (st >= S::STAGES) { st -= S::STAGES; ++turn; }
+    };
+    if constexpr (R == 8) {
+      if (four) tiles(std::true_type{});
+      else tiles(std::false_type{});
+    } else {
+      tiles(std::false_type{});
     }
     ahead -= w.count;
-    if (twice) {                                         // (lane t has rows 2 t, 2 t + 1, lane t + 2 what their rounding left)
+    if (four) {                                          // (lane t has rows 2 t, 2 t + 1, lane t + 2 what their rounding left)
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
