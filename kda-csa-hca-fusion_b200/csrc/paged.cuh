@@ -167,7 +167,8 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
     return p.left > 0 ? (int)start : 0x7FFFFFFF;
   };
   int start;
-  if (a.B <= 8 || (a.B <= 32 && (int64_t)a.N * a.G <= (int64_t)(R ? R : a.rows) * a.B)) {      // every warp by itself: no memory, no barrier
+  const bool one = (int64_t)a.N * a.G <= (int64_t)(R ? R : a.rows) * a.B;       // a block a sequence, on average
+  if (a.B <= 8 || (a.B <= 32 && one)) {                     // every warp by itself: no memory, no barrier
     const PgSeq s = pg_seq_or_none<PACKED>(a, lane);
     const int x = pg_steps<R, KT, TWO, EXTRA>(a, s), upto = pg_scan(x);
     total = __shfl_sync(0xffffffffu, upto, 31);
@@ -184,8 +185,9 @@ __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta,
   } else {
     int* base = reinterpret_cast<int*>(mem);                // [B + 1] steps before sequence b
     int* found = base + a.B + 1;
-    // (dealt out over the warps: one that has 32 sequences of several blocks takes 10 000 clocks for them)
-    const int deal = min((a.B + warps - 1) / warps, 32);
+    // (Sequences of several blocks are dealt out over the warps: one that has 32 of them takes 10 000 clocks.  Of a block each, a lane has one, and few
+    // warps are sooner done: steps of 64 sequences 37.2 us, dealt out 37.8; 8-bit pages, 16 heads of 128 on 1.)
+    const int deal = one ? 32 : min((a.B + warps - 1) / warps, 32);
 #pragma unroll 1
     for (int b0 = warp * deal; b0 < a.B; b0 += warps * deal) {
       const int x = pg_steps<R, KT, TWO, EXTRA>(a, pg_seq_or_none<PACKED>(a, lane < deal ? b0 + lane : a.B));
