@@ -15,7 +15,7 @@
 #define PG_MAX_B 4096                  // sequences of a call: their table of steps is kept in shared memory
 #define PG_LOG2E 1.4426950408889634f
 #define PG_EXTRA 2                     // places of the line before an item's steps (see above) on tcgen05
-#define PG_EXTRA_MOST 4                // of any form
+#define PG_EXTRA_MOST 4                // of any form: what the host counts (pa_steps)
 #define PG_ROWS 16                     // kind of keys and values that are packed rows like the queries, and not in pages (beside the KCH_ types)
 
 unsigned int* kch_status_device_ptr();
@@ -151,6 +151,7 @@ __device__ __forceinline__ int pg_scan(int x) {             // sums over the lan
 #define PG_PLAN_BYTES(B) (32 + 4 * ((B) + 1))
 template <int R, int KT, int TWO, int EXTRA = 0, bool PACKED = false>
 __device__ __forceinline__ PgPlace pg_plan(const PgBatch& a, void* mem, int cta, int ctas) {
+  static_assert(EXTRA <= PG_EXTRA_MOST, "the host's bound on the places of a call counts fewer");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   PgPlace p = {};
   int total, before = 0, mine = 0;                          // steps: of all, before sequence p.b, of it
