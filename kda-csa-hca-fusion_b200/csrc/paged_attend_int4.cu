@@ -89,6 +89,10 @@ __device__ __forceinline__ bool p4_wait_long(uint32_t bar, uint32_t parity, unsi
 __device__ __noinline__ bool p4_wait_call(uint32_t bar, uint32_t parity, unsigned int* status, unsigned sleep) {
   return p4_wait_long(bar, parity, status, sleep);
 }
+// What a block that ends waits for: its own copies, whatever the status says (p4_wait_long gives up as soon as another wait has).  10 ms at most.
+__device__ __forceinline__ void p4_drain(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < 1000 && !p4_poll(bar, parity); ++i) {}
+}
 __device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -226,7 +230,7 @@ paged_attend_int4_kernel(const __grid_constant__ PgAttend a) {
     for (int i = 0; i < g && i < S::STAGES / 2; ++i) {
       st -= 2;
       if (st < 0) { st += S::STAGES; --turn; }
-      wait(&sm.full[st], turn);
+      p4_drain(smem_addr_u32(&sm.full[st]), turn & 1);
     }
     return;
   }
