@@ -265,6 +265,12 @@ def require_cuda(*tensors, fn="kch_b200"):
                                "there is no CPU fallback")
 
 
+def forward_only(fn):
+    """Raises for a call whose tensors require a gradient, while gradients are enabled: the outputs have none, and it would be lost without a word."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError(f"{fn}(b200): forward only, and a tensor requires a gradient; call under torch.no_grad() or with detached tensors")
+
+
 def device_status(reset=False) -> int:
     return int(load().kch_device_status(1 if reset else 0))
 

@@ -2,7 +2,7 @@
 
 Not in the reference.  What :class:`PagedKVCache` attends in its pages, with the keys and values still the activations that a projection
 has left: the prompt is then attended as it is, whatever kind of cache keeps it (its 8- or 4-bit rows serve the tokens that follow,
-``PagedKVCache.forward_step``).  Forward only.
+``PagedKVCache.forward_step``).  Forward only: tensors that require a gradient are refused while gradients are enabled.
 """
 from __future__ import annotations
 
@@ -46,6 +46,8 @@ def prompt_attention(q, k, v, cu_seqlens, *, scale=None, sink_logits=None, slidi
     its sequence up to itself, or the last ``sliding_window`` tokens of that.  ``scale``: ``c ** -0.5`` unless given; ``sink_logits [nh]`` adds
     ``exp(sink)`` to the denominator.  Rows of no sequence are zeros, and stay as they are in a tensor given as ``out``, which overlaps
     none of the others.  The lengths stay on the device: a captured call replays with other ones."""
+    if q.requires_grad or k.requires_grad or v.requires_grad or (sink_logits is not None and sink_logits.requires_grad):
+        _lib.forward_only("prompt_attention")
     shape, kv, index, dtype = q.shape, k.shape, q.get_device(), q.dtype
     tag = _lib.dtype_tag(dtype)
     if not (len(shape) == len(kv) == 3 and kv == v.shape and shape[0] == kv[0] and shape[2] == kv[2] and shape[1] > 0 and kv[1] > 0 and index >= 0

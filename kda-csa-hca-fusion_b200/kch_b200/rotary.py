@@ -96,8 +96,11 @@ class RotaryPositions:
 
     def rotate(self, q, k, positions, *, inverse=False, out=None):
         """``q [N, nh, c]`` and ``k [N, n_kv, c]`` (or None) turned by ``positions``, int32 ``[N, axes]`` (or ``[N]`` where there is
-        one axis) on the device: ``(q', k')``.  ``inverse`` turns back, which is the gradient too.  ``out=(q', k')``: tensors to
-        store to, which may be ``q`` and ``k`` themselves (column slices of a fused projection, say) and overlap nothing else."""
+        one axis) on the device: ``(q', k')``.  ``inverse`` turns back, which is the gradient too; the call itself records none, and refuses
+        tensors that require one while gradients are enabled.  ``out=(q', k')``: tensors to store to, which may be ``q`` and ``k`` themselves
+        (column slices of a fused projection, say) and overlap nothing else."""
+        if q.requires_grad or (k is not None and k.requires_grad):
+            _lib.forward_only("rotate")
         shape, index, axes, dtype, c = q.shape, self._index, self._axes, q.dtype, self.c
         tag = _lib.dtype_tag(dtype)
         at, n_kv = positions.shape, 0
