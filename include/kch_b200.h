@@ -488,7 +488,8 @@ int kch_paged_attend(const kch_paged_attend_args* args, void* stream);
 /* The same attention of whole prompts whose keys and values are packed rows like the queries: k, v [N, n_kv, c] (tokens ld_k, ld_v elements
  * apart), key j of sequence b in row cu_seqlens[b] + j, no earlier tokens.  All else as in kch_paged_attend_args: q, k, v and out 16-byte aligned,
  * out apart from all three.  The kernels count a call's tiles in 32 bits, and the host knows of the lengths only that they add up to N: with all
- * of it as one sequence there may be 2^31 of them, which limits a call to 2 million tokens of 16 bf16 heads of 128 (fp32: a quarter of that). */
+ * of it as one sequence there may be 2^31 of them, which limits a call of 16 heads of 128 on 4 key heads to 2 million tokens in bf16 and 741 000 in fp32
+ * (whose tiles are smaller). */
 typedef struct kch_prompt_attend_args {
   const void *q, *k, *v;
   int64_t ld_q, ld_k, ld_v;

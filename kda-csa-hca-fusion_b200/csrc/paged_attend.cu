@@ -658,9 +658,6 @@ extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) 
     KCH_REQUIRE((uintptr_t)t.x >= o1 || (uintptr_t)t.x + ((p->N - 1) * t.ld + t.width) * es <= o0, "%s: out overlaps %s", fn, t.name);
   }
   KCH_REQUIRE((o0 & 15) == 0, "%s: out must be 16-byte aligned", fn);
-  const int64_t need = kch_prompt_attend_workspace_bytes(p);
-  KCH_REQUIRE(p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= need,
-              "%s: workspace of %lld bytes (256-byte aligned) is too small: %lld needed", fn, (long long)p->workspace_bytes, (long long)need);
   PgAttend a = {};
   a.bt.cu = p->cu_seqlens;
   a.bt.B = p->B; a.bt.N = (int)p->N; a.bt.cap = (int)p->N;
@@ -673,6 +670,9 @@ extern "C" int kch_prompt_attend(const kch_prompt_attend_args* p, void* stream) 
   a.sink = p->sink; a.sink_dtype = p->sink_dtype;
   const PaPlan x = pa_plan(p);
   KCH_REQUIRE(pa_steps(a.bt, x.rows, x.tile, x.form != PA_SIMT ? PG_EXTRA_MOST : 0) < PG_MOST, "%s: N=%lld rows of %d heads are more than a call takes", fn, (long long)p->N, p->nh);
+  const int64_t need = kch_prompt_attend_workspace_bytes(p);
+  KCH_REQUIRE(p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= need,
+              "%s: workspace of %lld bytes (256-byte aligned) is too small: %lld needed", fn, (long long)p->workspace_bytes, (long long)need);
   KCH_REQUIRE(a.bt.status != nullptr, "%s: cannot resolve the device status word", fn);
   return pa_launch(a, x, PG_ROWS, p->dtype, p->nh, p->workspace, kch_stream(stream));
 }
