@@ -526,7 +526,9 @@ static PaPlan pa_plan(int64_t B, int64_t N, int G, int kind, int dtype, int c) {
   else x = {PA_MMA, rows <= 8 * B ? 8 : rows <= 16 * B ? 16 : 32, 128, KCH_SMS, 0, false};      // (4 bits: 8 or 16)
   // Prompts and 4-bit pages: blocks of whole tokens, so that a copy of a tensor map fetches their queries.
   if (x.form == PA_TC5 && (kind == PG_ROWS || kind == KCH_INT4) && G <= 128) x.rows = 128 / G * G * 2;
-  x.slot_rows = (int)(rows < x.rows ? (rows + 7) / 8 * 8 : x.rows);      // (slots are stored to in 16-byte words)
+  // (Slots are stored to in 32-byte words, of which c + 2 numbers a row make whole ones where the rows are a multiple of 8: blocks of whole tokens are 250 rows
+  // of 5 heads, say.)
+  x.slot_rows = (int)(((rows < x.rows ? rows : x.rows) + 7) / 8 * 8);
   return x;
 }
 static PaPlan pa_plan(const kch_paged_attend_args* p) {
