@@ -507,8 +507,8 @@ int kch_paged_attend_int4(const PgAttend& a, int rows, int ctas, cudaStream_t s)
 //   rows (tokens x heads of a key head) of a sequence: up to 32, an item of the forms for few rows; behind that they read the keys twice.
 //     bf16  8 heads: 1 token 55 / 58, 4 (32 rows) 57 / 60, 5 (40 rows) 100 / 61;  16 heads: 2 tokens 37 / 41, 3 (48 rows) 52 / 42
 //     e4m3  8 heads: 1 token 46 / 80, 4 68 / 81, 5 126 / 81;  16 heads: 2 tokens 42 / 47, 3 72 / 48;  int8: 47 / 74, 68 / 74, 125 / 75; 41 / 45, 72 / 46
-//     4 bits: up to 16 rows (their form converts codes once for 16 rows, and chunks convert them faster than the other kinds').  8 heads: 1 token 33 / 76,
-//           4 (32 rows, in an instance for 32 that has been taken out) 93 / 77;  16 heads: 1 token 29 / 47, 2 62 / 47
+//     4 bits: up to 16 rows (their form converts codes once for 16 rows, and chunks convert them faster than the other kinds').  8 heads: 1 token 31 / 75,
+//           2 (16 rows) 41 / 75, 4 (32 rows, in an instance for 32 that has been taken out) 93 / 75;  16 heads: 1 token 26 / 45, 2 62 / 45
 //   tokens of a sequence: up to 4, so that a long chunk among single tokens cannot be most of a batch's work.  With 190 tokens in one sequence
 //     and one in each other (4 on average) 4 heads take 118 / 96 (bf16), 145 / 147 (e4m3), 146 / 141 (int8), 2 heads 191 / 174, 245 / 267, 254 / 254; with
 //     448 (8 on average) 127 / 100, 223 / 165, 222 / 156, and 246 / 182, 300 / 277, 302 / 265.  Alike ones would go on to 32 rows: 8 tokens of 4 heads

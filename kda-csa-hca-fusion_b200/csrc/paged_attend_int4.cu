@@ -17,7 +17,8 @@
 //
 // Measured, 64 sequences, 16 heads of 128 on 4: 8192 tokens in pages of 64 86 us (3.5 TB/s of pages; 89 in pages of 16, 111 of 8), 500 to
 // 16000 tokens in pages of 32 90; on two key heads 55, on one 42, of which 20 are the launches, the plan, the first tile and the joining.  Bound by
-// the instructions that convert: 730 for 32 keys of a warp, 340 of them at half rate, on two warps a scheduler that keep it 56 % busy.
+// issue: by the counters 731 instructions for 32 keys of a warp (all roles), 344 of them the ALU's, which has half the rate and is 53 % busy, 260 the FMA
+// pipe's and 32 products, on two warps a scheduler that keep it 56 % busy.
 // Tried: 12 warps of 152 registers 86 (and 102 where 8 took 98); a tile's values multiplied while the next one's scores are 92 (registers move); shifts as
 // products with powers of two, on the other pipe, 93.  Pages by tensor maps of 64-byte rows: a copy engine's 5 clocks a row are 1280 for a tile.
 //
@@ -99,7 +100,7 @@ __device__ __forceinline__ uint32_t p4_fma(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 // code J of either half of w, as values: J is 0 .. 3, s the scales of both halves, s24 -24 times them; sixteen: 16 in either half, a register
-// whose value the compiler does not know (with two constants it makes two operations of this one, 287 of them for 32 keys: 64 sequences of 8192 tokens 113 us, 99 without)
+// whose value the compiler does not know (mask and 16 as constants: 64 sequences of 8192 tokens 113 us, 99 so)
 template <int J>
 __device__ __forceinline__ uint32_t p4_pair(uint32_t w, uint32_t s, uint32_t s24, uint32_t sixteen) {
   uint32_t x = J == 0 ? w << 3 : w >> (4 * J - 3);

@@ -97,7 +97,7 @@ __device__ __forceinline__ float pc_scale4(uint32_t top) {
   if (7.f * __uint_as_float(b) < most) b += 0x80000u;
   return fmaxf(__uint_as_float(b), 1.17549435e-38f);
 }
-// The codes of 8 values as a word, the first in its lowest bits: x / s by one step from x times the reciprocal, plus 1.5 * 2^23 + 8, whose lowest bits
+// The codes of 8 values as a word, the first in its lowest bits: x / s by one Newton step on the residual of x times the reciprocal, plus 1.5 * 2^23 + 8, whose lowest bits
 // are then the nearest whole number to the quotient, and 8, ties to even.  A quotient in the middle between two codes comes out exactly;
 // bf16 values have no other that is nearer to it than 10^-3 (x has 8 bits, s 5), values in 32 bits have: there the true quotient decides.
 template <typename T>
@@ -315,9 +315,10 @@ static void pc_launch(const PgRows& a, int64_t blocks, cudaStream_t s) {
 
 
 // 4 bits.  16 values a thread, so that two of them share a scale; the first rows of a token are asked for before its page is looked up and the next
-// ones while these are at work, or (READ) the next token's page behind the rows of this one.  25 609 tokens of 8 key heads of 128 are written in 39
-// us and read in 25; the memory's rate is 18 for either.  Writing is bound by its instructions, 180 for 16 values.  (With 8 values a thread and each
-// wait behind the other 65 and 36.5; two rows of a thread in flight, which leaves 24 warps an SM, 43.)
+// ones while these are at work, or (READ) the next token's page behind the rows of this one.  25 609 tokens of 8 key heads of 128, 134 MB either way, which are 20.5 us
+// at the copy rate: written in 36.6 us and read in 26.0, call after call; 41.9 and 31.7 with cold caches.  Writing is bound by issue: by the counters 270 instructions for
+// 16 values of a thread, look-ups among them, 68 % of the slots.  (With 8 values a thread and each wait behind the other 65 and 36.5 us; two rows of a
+// thread in flight, which leaves 24 warps an SM, a tenth more.)
 template <typename T> struct Pc16 { uint4 w[sizeof(T)]; };
 template <typename T, int GROUP, bool READ>
 __global__ void __launch_bounds__(PC_THREADS, (READ || sizeof(T) == 4) ? 1 : 4) paged_rows4_kernel(const __grid_constant__ PgRows a) {

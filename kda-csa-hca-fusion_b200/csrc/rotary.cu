@@ -10,7 +10,8 @@
 // Bound by the bytes of x and y.  A block takes a few tokens: sines and cosines once a token and pair into shared memory, for all heads of
 // queries and keys (each head's own would be 45 instructions a pair, more than the memory leaves time for), while the threads' first rows
 // are under way; then 8 pairs a thread and row, in 16-byte words, two rows at a time.  Measured: 27 290 tokens of 16 and 8 heads of 128 in bf16,
-// three axes, 54.5 us, 6.2 TB/s, 0.94 of the copy rate; 64 tokens 2.6 us.
+// three axes, 53.6 us, 6.3 TB/s, 0.95 of the copy rate; 64 tokens 1.7 us in a run of such calls.  Where r is no multiple of 16 a thread has a pair, in accesses
+// of 2 or 4 bytes: 9600 tokens of 16 and 4 heads of 64 in bf16 take 22 us with r = 24 and 30 with 40, 15 with 32 and 9 with 64 (fp32 26, 33, 23, 17).
 #include "kch_common.cuh"
 
 #define RO_THREADS 256
@@ -220,7 +221,9 @@ extern "C" int kch_rotary(const kch_rotary_args* p, void* stream) {
   const bool words = p->rotary_dim % 16 == 0;
   const int lanes = words ? a.pairs / 8 : a.pairs;
   while ((1 << a.width) < lanes) ++a.width;
-  // about 8 pieces a thread to a block, but two blocks to an SM where there are tokens for that
+  // About 8 pieces a thread to a block, but two blocks to an SM where there are tokens for that.  Either side, us, bf16 heads of 128: 27 290 tokens of 24 heads 4 pieces
+  // 52.4, 8 53.6, 16 54.7;  9600 of 20 heads 14.7, 17.1, 16.3;  4000 6.9, 8.1, 8.4;  one block an SM at least, two, eight: 4000 tokens 8.1, 8.1, 6.8;  1000
+  // 3.8, 3.0, 3.8;  fp32, 8 heads of 64, 1000 tokens 2.8, 2.3, 3.6;  9600 8.9, 8.9, 7.9.
   const int64_t pieces = (int64_t)a.rows << a.width;
   int64_t tokens = 8 * RO_THREADS / pieces;
   if (tokens > p->N / (2 * KCH_SMS)) tokens = p->N / (2 * KCH_SMS);
